@@ -292,6 +292,114 @@ int j4q_decode_plan_info(j4q_plan plan, j4q_decode_plan_desc *out);
 /* Waits for the device, then frees the graph and the plan's own buffers. 0 is a no-op. */
 int j4q_decode_plan_destroy(j4q_plan plan);
 
+/* ---- attention over an 8-bit key/value cache (engine-local; the reference has no attention) ---- */
+/* What a decoder does between q|k|v and o: rotary positions, a paged cache, attention. The results of
+ * quantMatvec / quantMatmul go in, o's activations come out.
+ *
+ * A cache holds, for `layers` layers and `sequences` sequences, keys and values as int8 codes with a 32-bit scale for
+ * every block of 16 tokens and kv head, in pages of page_tokens tokens that all layers have in common. Where new tokens
+ * begin a block its scale is max(amax / 127, 2^-64); a later token that does not fit doubles it until it does, and the
+ * block's codes are divided by as much (rounded to even, as every code is: an error below one step of the final
+ * scale). A block with a value that is not finite is NaN as a whole, and so is a row that sees it.
+ *
+ * A step: j4q_kv_extend names the sequences and how many tokens each gets; rows of q, k, v and out are these tokens in
+ * that order; then per layer j4q_kv_append and j4q_kv_attend. Pages and lengths are host state: a call that cannot be
+ * served changes nothing. Calls on one cache run in order, on whichever streams they are issued; under stream capture
+ * only append and attend may be called, the caller orders the graph's launches, and a launch serves the step
+ * that j4q_kv_extend or j4q_kv_begin have set up by then (of the sequences and tokens a sequence that it was captured
+ * with). */
+typedef uint64_t j4q_kv; /* 0 is never a valid handle */
+
+typedef struct j4q_kv_config {
+    int32_t layers, kv_heads;
+    int32_t head_dim;        /* 64, 96, 128, 192 or 256 */
+    int32_t page_tokens;     /* 16, 32 or 64 */
+    int64_t pages;           /* of the pool, for all sequences together */
+    int32_t sequences;       /* named 0 .. sequences - 1; all begin empty */
+    int32_t sequence_pages;  /* most pages of a sequence */
+} j4q_kv_config;
+
+typedef struct j4q_kv_desc {
+    j4q_kv_config config;
+    int64_t pages_free;
+    uint64_t bytes;          /* device memory of the cache: the pool, tables, and room for parts of results */
+    uint64_t page_bytes;     /* of a page in one layer */
+    int32_t step_sequences, step_rows;
+} j4q_kv_desc;
+
+/* Rotary positions: pair i of a head, channels (2i, 2i + 1) if interleaved, else (i, i + dims / 2), is turned by
+ * the angle whose cosine and sine are cos_table / sin_table[position][i] (device memory, fp32 [table_rows][dims / 2]);
+ * channels from dims on stay. positions (device memory, int32 [axes][rows]): row r's position of the axis
+ * pair_axis[i] (host memory, dims / 2 values; NULL: one axis), e.g. time, height and width. A position outside the
+ * tables gives NaN. */
+typedef struct j4q_rope {
+    const float *cos_table, *sin_table;
+    int64_t table_rows;
+    int32_t dims;            /* even, at most head_dim and 256 */
+    int32_t interleaved;
+    const int32_t *positions; /* NULL (append alone): a token's place in its sequence */
+    const uint8_t *pair_axis;
+} j4q_rope;
+
+/* Turns heads of x [rows][heads][head_dim] (J4Q_KIND_F32 or J4Q_KIND_BF16) into out, which is x itself or apart.
+ * Strides: values from a row to the next, 0 for heads * head_dim. Any even head_dim. */
+int j4q_rope_into(const void *x, void *out, int type, int64_t rows, int32_t heads, int32_t head_dim, int64_t x_stride, int64_t out_stride,
+                  const j4q_rope *rope, void *stream);
+
+int j4q_kv_create(const j4q_kv_config *config, j4q_kv *out);
+/* Waits for the device. 0 is a no-op. */
+int j4q_kv_destroy(j4q_kv kv);
+int j4q_kv_info(j4q_kv kv, j4q_kv_desc *out);
+/* Length of a sequence, and its pages in order (-1: evicted, and behind its last), up to `capacity`; either may be NULL. */
+int j4q_kv_sequence(j4q_kv kv, int32_t seq, int64_t *length, int32_t *pages, int32_t capacity);
+/* Begins a step: sequence seqs[i] (host memory; each at most once) gets tokens[i] >= 1 more tokens. Takes free pages, lowest
+ * first; a partly filled page that other sequences hold too is copied first. J4Q_ENOMEM where pages are short. */
+int j4q_kv_extend(j4q_kv kv, const int32_t *seqs, const int32_t *tokens, int32_t n, void *stream);
+/* Begins a step over the last tokens[i] tokens that seqs[i] has already. */
+int j4q_kv_begin(j4q_kv kv, const int32_t *seqs, const int32_t *tokens, int32_t n, void *stream);
+/* The empty sequence dst[i] becomes src[i]: sharing its pages (share != 0; a shared page is copied when one of its holders
+ * extends into it), or with copies of them. */
+int j4q_kv_fork(j4q_kv kv, const int32_t *src, const int32_t *dst, int32_t n, int share, void *stream);
+/* Cuts sequences to lengths[i] tokens (0 frees them whole); pages that no sequence holds any more are free. A step that
+ * one of them is part of ends. */
+int j4q_kv_truncate(j4q_kv kv, const int32_t *seqs, const int64_t *lengths, int32_t n);
+/* Frees the pages that no later token sees through this window and these first tokens; attend refuses masks that
+ * would show some of them. Positions stay what they are. */
+int j4q_kv_evict(j4q_kv kv, const int32_t *seqs, int32_t n, int32_t window, int32_t sinks, void *stream);
+/* Moves pages so that those in use are the pool's lowest; *moved (may be NULL): how many. */
+int j4q_kv_compact(j4q_kv kv, int64_t *moved, void *stream);
+
+typedef struct j4q_kv_append_args {
+    const void *k, *v;       /* [rows][kv_heads][head_dim], 16-byte aligned device memory */
+    int64_t kv_stride;       /* values from a row to the next, 0: dense; a multiple of 16 bytes */
+    int32_t type;            /* of k, v, q: J4Q_KIND_F32 or J4Q_KIND_BF16 */
+    int32_t heads;           /* of q */
+    const void *q;           /* NULL, or [rows][heads][head_dim]: turned as the keys are, into q_out (q itself or apart) */
+    void *q_out;
+    int64_t q_stride;        /* of q and q_out */
+    const j4q_rope *rope;    /* NULL: keys are stored as they are */
+} j4q_kv_append_args;
+/* Stores the step's keys (turned) and values in `layer`. The same call again stores the same. */
+int j4q_kv_append(j4q_kv kv, int32_t layer, const j4q_kv_append_args *args, void *stream);
+
+typedef struct j4q_kv_attend_args {
+    const void *q;           /* [rows][heads][head_dim], 16-byte aligned device memory */
+    void *out;               /* the same shape */
+    int64_t q_stride, out_stride; /* values from a row to the next, 0: dense; a multiple of 16 bytes */
+    int32_t q_type, out_type; /* J4Q_KIND_F32 or J4Q_KIND_BF16 */
+    int32_t heads;           /* a multiple of kv_heads: query head h reads kv head h / (heads / kv_heads) */
+    int32_t window;          /* 0: none */
+    int32_t sinks;
+    float scale;             /* 0: 1 / sqrt(head_dim) */
+} j4q_kv_attend_args;
+/* out = softmax(scale q k) v of every row of the step over the tokens j <= p of its sequence, p its own place, with
+ * j > p - window or j < sinks. Scores, weights and sums in at least fp32 precision where out is fp32; where it is bf16,
+ * steps of many rows take q and the weights in fp16. Bit for bit the same on every call with equal lengths. */
+int j4q_kv_attend(j4q_kv kv, int32_t layer, const j4q_kv_attend_args *args, void *stream);
+/* Tokens [first[i], first[i] + count) of seqs[i] in `layer` as the cache holds them: fp32 [n][count][kv_heads][head_dim],
+ * 16-byte aligned (either may be NULL); zeros where there is no token. */
+int j4q_kv_read(j4q_kv kv, int32_t layer, const int32_t *seqs, const int64_t *first, int64_t count, int32_t n, float *k, float *v, void *stream);
+
 /* ---- GGUF files (the step before uploadQuantized; engine-local) ---------------------- */
 /* The reference receives quantized blobs from an external caller (spi/QuantizedOps.java:24)
  * and knows the GGUF type ids (core/tensor/QuantType.java:3-13); this reader supplies them

@@ -103,6 +103,70 @@ class DecodePlanDesc(C.Structure):
     ]
 
 
+class KvConfig(C.Structure):
+    _fields_ = [
+        ("layers", C.c_int32),
+        ("kv_heads", C.c_int32),
+        ("head_dim", C.c_int32),
+        ("page_tokens", C.c_int32),
+        ("pages", C.c_int64),
+        ("sequences", C.c_int32),
+        ("sequence_pages", C.c_int32),
+    ]
+
+
+class KvDesc(C.Structure):
+    _fields_ = [
+        ("config", KvConfig),
+        ("pages_free", C.c_int64),
+        ("bytes", C.c_uint64),
+        ("page_bytes", C.c_uint64),
+        ("step_sequences", C.c_int32),
+        ("step_rows", C.c_int32),
+    ]
+
+
+class RopeArgs(C.Structure):
+    _fields_ = [
+        ("cos_table", C.c_void_p),
+        ("sin_table", C.c_void_p),
+        ("table_rows", C.c_int64),
+        ("dims", C.c_int32),
+        ("interleaved", C.c_int32),
+        ("positions", C.c_void_p),
+        ("pair_axis", C.c_void_p),
+    ]
+
+
+class KvAppendArgs(C.Structure):
+    _fields_ = [
+        ("k", C.c_void_p),
+        ("v", C.c_void_p),
+        ("kv_stride", C.c_int64),
+        ("type", C.c_int32),
+        ("heads", C.c_int32),
+        ("q", C.c_void_p),
+        ("q_out", C.c_void_p),
+        ("q_stride", C.c_int64),
+        ("rope", C.POINTER(RopeArgs)),
+    ]
+
+
+class KvAttendArgs(C.Structure):
+    _fields_ = [
+        ("q", C.c_void_p),
+        ("out", C.c_void_p),
+        ("q_stride", C.c_int64),
+        ("out_stride", C.c_int64),
+        ("q_type", C.c_int32),
+        ("out_type", C.c_int32),
+        ("heads", C.c_int32),
+        ("window", C.c_int32),
+        ("sinks", C.c_int32),
+        ("scale", C.c_float),
+    ]
+
+
 _i32, _i64, _u64, _vp = C.c_int32, C.c_int64, C.c_uint64, C.c_void_p
 _buf = C.c_uint64
 _pbuf = C.POINTER(C.c_uint64)
@@ -151,6 +215,20 @@ SIGNATURES = {
     "j4q_decode_plan_run": [_u64, _vp],
     "j4q_decode_plan_info": [_u64, C.POINTER(DecodePlanDesc)],
     "j4q_decode_plan_destroy": [_u64],
+    "j4q_rope_into": [_vp, _vp, C.c_int, _i64, _i32, _i32, _i64, _i64, C.POINTER(RopeArgs), _vp],
+    "j4q_kv_create": [C.POINTER(KvConfig), C.POINTER(_u64)],
+    "j4q_kv_destroy": [_u64],
+    "j4q_kv_info": [_u64, C.POINTER(KvDesc)],
+    "j4q_kv_sequence": [_u64, _i32, C.POINTER(_i64), C.POINTER(_i32), _i32],
+    "j4q_kv_extend": [_u64, C.POINTER(_i32), C.POINTER(_i32), _i32, _vp],
+    "j4q_kv_begin": [_u64, C.POINTER(_i32), C.POINTER(_i32), _i32, _vp],
+    "j4q_kv_fork": [_u64, C.POINTER(_i32), C.POINTER(_i32), _i32, C.c_int, _vp],
+    "j4q_kv_truncate": [_u64, C.POINTER(_i32), C.POINTER(_i64), _i32],
+    "j4q_kv_evict": [_u64, C.POINTER(_i32), _i32, _i32, _i32, _vp],
+    "j4q_kv_compact": [_u64, C.POINTER(_i64), _vp],
+    "j4q_kv_append": [_u64, _i32, C.POINTER(KvAppendArgs), _vp],
+    "j4q_kv_attend": [_u64, _i32, C.POINTER(KvAttendArgs), _vp],
+    "j4q_kv_read": [_u64, _i32, C.POINTER(_i32), C.POINTER(_i64), _i64, _i32, _vp, _vp, _vp],
     "j4q_gguf_open": [C.c_char_p, C.POINTER(_u64)],
     "j4q_gguf_close": [_u64],
     "j4q_gguf_file_info": [_u64, C.POINTER(GgufInfo)],

@@ -285,6 +285,14 @@ class Mi355xBackend:
             x_ptr, xq_ptr, xs_ptr, y_ptr, stream = _addresses(x_ptr, xq_ptr, xs_ptr, y_ptr, stream)
         check(self._lib().j4q_quant_matmul_into(weights.handle, x_ptr, m, v, xq_ptr, xs_ptr, y_ptr, stream), "quantMatmul_into")
 
+    def rope_into(self, x_ptr: int, out_ptr: int, rows: int, heads: int, head_dim: int, rope: "Rope", dtype: DType = DType.F32, x_stride: int = 0,
+                  out_stride: int = 0, stream: int = 0) -> None:
+        """Rotary positions (jax4j_amd.Rope, with its positions) on x [rows, heads, head_dim], F32 or BF16, into out (x itself
+        or apart), stream-ordered. Strides in values, 0: dense."""
+        kind = {DType.F32: N.KIND_F32, DType.BF16: N.KIND_BF16}.get(dtype, 0)
+        x, out, s = _addresses(x_ptr, out_ptr, stream)
+        check(self._lib().j4q_rope_into(x, out, kind, rows, heads, head_dim, x_stride, out_stride, C.byref(rope.args), s), "rope_into")
+
     def decode_plan(self, layers, head, batch: int, io: dict) -> "DecodePlan":
         """The quantized matmuls of a decode step as one replayable plan (engine-local).
 
