@@ -94,6 +94,7 @@ __host__ __device__ inline int kv_ranges(int tiles, const KvAttend &a) {
 }
 
 hipError_t launch_kv_decode(const KvAttend &a, hipStream_t s, hipEvent_t done);
+hipError_t launch_kv_prefill(const KvAttend &a, hipStream_t s, hipEvent_t done);
 // The parts of every row in one: out = sum of part * 2^(max - largest) / the same of the sums.
 hipError_t launch_kv_join(const KvAttend &a, hipStream_t s, hipEvent_t done);
 

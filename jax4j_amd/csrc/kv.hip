@@ -21,6 +21,8 @@ namespace {
 
 // Rows of partial results that a cache has room for: (D + 2) floats each.
 constexpr int64_t kPartRows = 65536;
+// Query rows (tokens x group) of a sequence and kv head up to which the kernel for few rows runs.
+constexpr int kFewRows = 16;
 
 struct Seq {
     int64_t len = 0;
@@ -720,20 +722,25 @@ int j4q_kv_attend(j4q_kv kv, int32_t layer, const j4q_kv_attend_args *args, void
     a.q_bf16 = g.q_type == J4Q_KIND_BF16;
     a.out_bf16 = g.out_type == J4Q_KIND_BF16;
     a.scale = (g.scale > 0.0f ? g.scale : 1.0f / sqrtf((float)k->c.head_dim)) * 1.4426950408889634f;
-    a.row_tile = a.max_rows <= 4 ? 4 : 8;
+    const bool many = a.max_rows > kFewRows;
+    a.row_tile = many ? 128 : a.max_rows <= 4 ? 4 : 8;
     if ((rc = abi::ready_locked())) return rc;
     Call c(*k, stream);
     // ranges of the tokens: enough workgroups to fill the chip, in pieces that are worth a workgroup
-    int64_t tiles = 0, most = 0;
-    for (int i = 0; i < n; i++) {
-        const int64_t len = k->seqs[(size_t)k->step_seq[(size_t)i]].len, t = k->step_tokens[(size_t)i];
-        const int64_t count = kv_tiles((int)(len - t), (int)(len - 1), a.window, a.sinks).count();
-        tiles += count * ((t * a.group + a.row_tile - 1) / a.row_tile);
-        most = std::max(most, count);
-    }
     const int64_t filled = 512;
+    int64_t tiles = 0, most = 0;
+    if ((int64_t)k->step_rows * a.group / a.row_tile * k->c.kv_heads < filled)
+        for (int i = 0; i < n; i++) {
+            const int64_t before = k->seqs[(size_t)k->step_seq[(size_t)i]].len - k->step_tokens[(size_t)i], rows = (int64_t)k->step_tokens[(size_t)i] * a.group;
+            for (int64_t r = 0; r < rows; r += a.row_tile) {
+                const int64_t last = std::min(rows, r + a.row_tile) - 1;
+                const int64_t count = kv_tiles((int)(before + r / a.group), (int)(before + last / a.group), a.window, a.sinks).count();
+                tiles += count;
+                most = std::max(most, count);
+            }
+        }
     a.split_tiles = (int32_t)std::max<int64_t>(4, (tiles * k->c.kv_heads + filled - 1) / filled);
-    if (c.captured) most = ((int64_t)k->c.sequence_pages * k->c.page_tokens + kKvTile - 1) / kKvTile;  // the graph's later runs
+    if (c.captured && most) most = ((int64_t)k->c.sequence_pages * k->c.page_tokens + kKvTile - 1) / kKvTile;  // the graph's later runs
     const int64_t room = kPartRows / ((int64_t)n * k->c.kv_heads * a.max_rows);
     a.splits = (int32_t)std::max<int64_t>(1, std::min<int64_t>({(most + a.split_tiles - 1) / a.split_tiles, room, 256}));
     if (a.splits > 1 && (most + a.split_tiles - 1) / a.split_tiles > a.splits && !c.captured)
@@ -742,7 +749,7 @@ int j4q_kv_attend(j4q_kv kv, int32_t layer, const j4q_kv_attend_args *args, void
     a.part_ml = k->part + kPartRows * k->c.head_dim;
     if ((int64_t)k->c.kv_heads * ((a.max_rows + a.row_tile - 1) / a.row_tile) > 65535 || n > 65535 || a.max_rows > INT_MAX / 2)
         return report_error(J4Q_EUNSUPPORTED, "kv attend: %d query rows of %d kv heads in %d sequences", a.max_rows, k->c.kv_heads, n);
-    if (c.e == hipSuccess) c.e = launch_kv_decode(a, c.s, c.event(true));
+    if (c.e == hipSuccess) c.e = many ? launch_kv_prefill(a, c.s, c.event(true)) : launch_kv_decode(a, c.s, c.event(true));
     return c.end("kv attend");
 }
 

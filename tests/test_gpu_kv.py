@@ -210,6 +210,7 @@ def test_values_that_are_not_finite(model, bad):
     assert np.isnan(k0.scale[1, 0]) and np.isnan(k0.scale).sum() == 1 and np.isnan(v1.scale[2, 1])
     for window in (0, 21, 18, 16):  # of the step of 30 tokens from place 23 on, those of later rows show nothing of block 1
         check_attend(m, rng, [0], [30], 4, window=window)
+        check_attend(m, rng, [0], [30], 4, window=window, okind="bf16")
     m.kv.begin([1], [3])  # behind the block of the value that is not finite is none
     check_attend(m, rng, [1], [3], 4)
 
@@ -240,7 +241,7 @@ def check_attend(m, rng, seqs, tokens, heads, window=0, sinks=0, scale=0.0, qkin
         with np.errstate(invalid="ignore", divide="ignore"):
             logs = np.abs(np.log2(v.scale[np.isfinite(v.scale)])).max()
             d = 2.0 ** -22 * (top + logs + 8)
-            if okind == "bf16" and max(tokens) * heads // m.c["kv_heads"] > 8:
+            if okind == "bf16" and max(tokens) * heads // m.c["kv_heads"] > 16:
                 d += 2.0 ** -11 * (products + 1)
             bar = 2 * d * np.nanmax(np.abs(v.values()))
         part = got[row:row + t]
@@ -288,6 +289,56 @@ def test_attend_few_rows_long(model, group, tokens):
     m.grow(rng, [0, 1, 2], [6000, tokens, 1500], 2.0)
     for window, sinks in ((0, 0), (1700, 4)):
         check_attend(m, rng, [0, 1, 2], [tokens] * 3, group, window=window, sinks=sinks, begin=True, size=2.0)
+
+
+@pytest.mark.parametrize("okind", ["bf16", "f32"])
+@pytest.mark.parametrize("dim,group,page", [(64, 1, 16), (96, 4, 32), (128, 4, 64), (128, 7, 16), (192, 2, 32), (256, 8, 16)])
+def test_attend_many_rows(model, dim, group, page, okind):
+    """Prompts whole and in chunks, rows that end all over a tile of them, sequences of uneven steps, windows."""
+    m = model(kv_heads=2, head_dim=dim, pages=400, page_tokens=page, sequences=5, sequence_pages=100)
+    rng = np.random.default_rng(dim + group)
+    for seqs, tokens in (([0, 1, 2, 3, 4], [1, 17, 64, 129, 300]), ([0, 4, 2], [200, 33, 1]), ([3], [70])):
+        m.grow(rng, seqs, tokens)
+        check_attend(m, rng, seqs, tokens, 2 * group, okind=okind)
+        check_attend(m, rng, seqs, tokens, 2 * group, okind=okind, window=50, sinks=3, qkind="bf16", pad=8, scale=0.3)
+        check_attend(m, rng, seqs, tokens, 2 * group, okind=okind, window=1)
+        check_attend(m, rng, seqs, tokens, 2 * group, okind=okind, window=130, sinks=66)
+
+
+@pytest.mark.parametrize("okind", ["bf16", "f32"])
+def test_attend_many_rows_long(model, okind):
+    """A chunk behind a long context: a row tile's tokens are several workgroups'."""
+    m = model(kv_heads=1, head_dim=128, pages=400, page_tokens=32, sequences=2, sequence_pages=300)
+    rng = np.random.default_rng(23)
+    m.grow(rng, [0, 1], [6000, 100], 2.0)
+    for window, sinks in ((0, 0), (1700, 4), (3000, 500)):
+        check_attend(m, rng, [0, 1], [41, 30], 4, window=window, sinks=sinks, begin=True, okind=okind)
+
+
+@pytest.mark.parametrize("okind", ["bf16", "f32"])
+def test_attend_many_rows_extremes(model, okind):
+    m = model(kv_heads=1, head_dim=128, pages=64, page_tokens=16, sequences=2, sequence_pages=40)
+    rng = np.random.default_rng(29)
+    m.kv.extend([0, 1], [400, 60])
+    k, v = rng.standard_normal((460, 1, 128)), rng.standard_normal((460, 1, 128))
+    k[100:104] *= 20
+    v[:16] *= 1e-3
+    v[200:240], k[300:320] = 0, 0
+    v[400:] *= 1e-12
+    k[400:] *= 1e12
+    m.write(0, [0, 1], [400, 60], k, v)
+    for size in (1e-20, 1.0, 3.0):
+        check_attend(m, rng, [0], [390], 4, size=size, begin=True, okind=okind)
+    check_attend(m, rng, [1], [50], 4, size=1e-12, begin=True, okind=okind)
+    q = rng.standard_normal((390, 4 * 128))
+    q[5, 130], q[100, 300] = np.nan, -np.inf
+    dq = dev(q.astype(np.float32))
+    out = dev_as(np.zeros((390, 512)), okind)[0]
+    m.kv.begin([0], [390])
+    torch.cuda.synchronize()
+    m.kv.attend(0, dq.data_ptr(), out.data_ptr(), 4, out_type=KIND[okind])
+    got = np.isnan(host(out, okind)).reshape(390, 4, 128)
+    assert got[5, 1].all() and got[100, 2].all() and got.sum() == 2 * 128
 
 
 def test_attend_extremes(model):
