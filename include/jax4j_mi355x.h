@@ -350,8 +350,9 @@ int j4q_kv_create(const j4q_kv_config *config, j4q_kv *out);
 /* Waits for the device. 0 is a no-op. */
 int j4q_kv_destroy(j4q_kv kv);
 int j4q_kv_info(j4q_kv kv, j4q_kv_desc *out);
-/* Length of a sequence, and its pages in order (-1: evicted, and behind its last), up to `capacity`; either may be NULL. */
-int j4q_kv_sequence(j4q_kv kv, int32_t seq, int64_t *length, int32_t *pages, int32_t capacity);
+/* Lengths of n sequences, and their pages in order, [n][capacity] (-1: evicted, and behind a sequence's last); either may be
+ * NULL. */
+int j4q_kv_tables(j4q_kv kv, const int32_t *seqs, int32_t n, int64_t *lengths, int32_t *pages, int32_t capacity);
 /* Begins a step: sequence seqs[i] (host memory; each at most once) gets tokens[i] >= 1 more tokens. Takes free pages, lowest
  * first; a partly filled page that other sequences hold too is copied first. J4Q_ENOMEM where pages are short. */
 int j4q_kv_extend(j4q_kv kv, const int32_t *seqs, const int32_t *tokens, int32_t n, void *stream);

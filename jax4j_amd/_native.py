@@ -219,16 +219,16 @@ SIGNATURES = {
     "j4q_kv_create": [C.POINTER(KvConfig), C.POINTER(_u64)],
     "j4q_kv_destroy": [_u64],
     "j4q_kv_info": [_u64, C.POINTER(KvDesc)],
-    "j4q_kv_sequence": [_u64, _i32, C.POINTER(_i64), C.POINTER(_i32), _i32],
-    "j4q_kv_extend": [_u64, C.POINTER(_i32), C.POINTER(_i32), _i32, _vp],
-    "j4q_kv_begin": [_u64, C.POINTER(_i32), C.POINTER(_i32), _i32, _vp],
-    "j4q_kv_fork": [_u64, C.POINTER(_i32), C.POINTER(_i32), _i32, C.c_int, _vp],
-    "j4q_kv_truncate": [_u64, C.POINTER(_i32), C.POINTER(_i64), _i32],
-    "j4q_kv_evict": [_u64, C.POINTER(_i32), _i32, _i32, _i32, _vp],
+    "j4q_kv_tables": [_u64, _vp, _i32, _vp, _vp, _i32],
+    "j4q_kv_extend": [_u64, _vp, _vp, _i32, _vp],
+    "j4q_kv_begin": [_u64, _vp, _vp, _i32, _vp],
+    "j4q_kv_fork": [_u64, _vp, _vp, _i32, C.c_int, _vp],
+    "j4q_kv_truncate": [_u64, _vp, _vp, _i32],
+    "j4q_kv_evict": [_u64, _vp, _i32, _i32, _i32, _vp],
     "j4q_kv_compact": [_u64, C.POINTER(_i64), _vp],
     "j4q_kv_append": [_u64, _i32, C.POINTER(KvAppendArgs), _vp],
     "j4q_kv_attend": [_u64, _i32, C.POINTER(KvAttendArgs), _vp],
-    "j4q_kv_read": [_u64, _i32, C.POINTER(_i32), C.POINTER(_i64), _i64, _i32, _vp, _vp, _vp],
+    "j4q_kv_read": [_u64, _i32, _vp, _vp, _i64, _i32, _vp, _vp, _vp],
     "j4q_gguf_open": [C.c_char_p, C.POINTER(_u64)],
     "j4q_gguf_close": [_u64],
     "j4q_gguf_file_info": [_u64, C.POINTER(GgufInfo)],

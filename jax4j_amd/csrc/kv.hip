@@ -388,16 +388,21 @@ int j4q_kv_info(j4q_kv kv, j4q_kv_desc *out) {
     return J4Q_OK;
 }
 
-int j4q_kv_sequence(j4q_kv kv, int32_t seq, int64_t *length, int32_t *pages, int32_t capacity) {
+int j4q_kv_tables(j4q_kv kv, const int32_t *seqs, int32_t n, int64_t *lengths, int32_t *pages, int32_t capacity) {
     std::lock_guard<std::mutex> lk(abi::lock());
     Kv *k;
-    int rc = get(kv, "kv sequence", &k);
+    int rc = get(kv, "kv tables", &k);
     if (rc) return rc;
-    if ((rc = check_seqs(*k, "kv sequence", &seq, 1, true))) return rc;
-    if (capacity > 0 && !pages) return report_error(J4Q_EINVAL, "kv sequence: pages is NULL");
-    const Seq &q = k->seqs[(size_t)seq];
-    if (length) *length = q.len;
-    for (int32_t i = 0; i < capacity; i++) pages[i] = (size_t)i < q.pages.size() ? q.pages[(size_t)i] : -1;
+    if ((rc = check_seqs(*k, "kv tables", seqs, n, false))) return rc;
+    if (capacity < 0 || (capacity > 0 && !pages)) return report_error(J4Q_EINVAL, "kv tables: room for %d pages", capacity);
+    for (int32_t i = 0; i < n; i++) {
+        const Seq &q = k->seqs[(size_t)seqs[i]];
+        if (lengths) lengths[i] = q.len;
+        const size_t have = std::min(q.pages.size(), (size_t)capacity);
+        int32_t *to = pages + (int64_t)i * capacity;
+        std::copy_n(q.pages.begin(), have, to);
+        std::fill(to + have, to + capacity, -1);
+    }
     return J4Q_OK;
 }
 
@@ -726,8 +731,10 @@ int j4q_kv_attend(j4q_kv kv, int32_t layer, const j4q_kv_attend_args *args, void
     a.row_tile = many ? 128 : a.max_rows <= 4 ? 4 : 8;
     if ((rc = abi::ready_locked())) return rc;
     Call c(*k, stream);
-    // ranges of the tokens: enough workgroups to fill the chip, in pieces that are worth a workgroup
-    const int64_t filled = 512;
+    // Ranges of the tokens where rows alone leave CUs idle: one workgroup of a CU's registers each. Joining them costs 4 to 5 us, a
+    // round of the 8 waves over a tile each 2.4 (one request, 8 kv heads of 128: 16 tiles 11.3 us in one range, 13.2 in two; 32
+    // tiles 16.2 and, in four, 13.7; 128 tiles 46 and, in sixteen, 14.1).
+    const int64_t filled = many ? 512 : 256, alone = many ? 4 : 16, least = many ? 4 : 8;
     int64_t tiles = 0, most = 0;
     if ((int64_t)k->step_rows * a.group / a.row_tile * k->c.kv_heads < filled)
         for (int i = 0; i < n; i++) {
@@ -739,7 +746,7 @@ int j4q_kv_attend(j4q_kv kv, int32_t layer, const j4q_kv_attend_args *args, void
                 most = std::max(most, count);
             }
         }
-    a.split_tiles = (int32_t)std::max<int64_t>(4, (tiles * k->c.kv_heads + filled - 1) / filled);
+    a.split_tiles = (int32_t)std::max<int64_t>(most <= alone ? alone : least, (tiles * k->c.kv_heads + filled - 1) / filled);
     if (c.captured && most) most = ((int64_t)k->c.sequence_pages * k->c.page_tokens + kKvTile - 1) / kKvTile;  // the graph's later runs
     const int64_t room = kPartRows / ((int64_t)n * k->c.kv_heads * a.max_rows);
     a.splits = (int32_t)std::max<int64_t>(1, std::min<int64_t>({(most + a.split_tiles - 1) / a.split_tiles, room, 256}));

@@ -29,7 +29,6 @@ typedef int v4i __attribute__((ext_vector_type(4)));
 
 constexpr float kHead = 4.0f;    // octaves that t may pass m by
 constexpr float kUnit = 26.0f;   // 2^26: the weight of t = m
-constexpr int kWaves = 4;
 constexpr int kFlushTiles = 1024;
 
 // v + the lanes' that are N to the right in their 16, round about.
@@ -78,8 +77,27 @@ __device__ __forceinline__ int pick(uint32_t a, uint32_t b, uint32_t c, uint32_t
     return (int)((__builtin_amdgcn_perm(b, a, low) | __builtin_amdgcn_perm(d, c, high)) ^ 0x80808080u);
 }
 
-__device__ __forceinline__ float value_at(const void *p, int64_t i, int bf16) {
-    return bf16 ? __builtin_bit_cast(float, (uint32_t)((const uint16_t *)p)[i] << 16) : ((const float *)p)[i];
+// 16 values from i on, 16-byte aligned.
+__device__ __forceinline__ void load16(const void *p, int64_t i, int bf16, float *x) {
+    if (bf16) {
+        const uint4 *from = (const uint4 *)((const uint16_t *)p + i);
+#pragma unroll
+        for (int j = 0; j < 2; j++) {
+            const uint4 t = from[j];
+            const uint32_t w[4] = {t.x, t.y, t.z, t.w};
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                x[8 * j + 2 * e] = __builtin_bit_cast(float, w[e] << 16);
+                x[8 * j + 2 * e + 1] = __builtin_bit_cast(float, w[e] & 0xffff0000u);
+            }
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            const float4 t = ((const float4 *)((const float *)p + i))[j];
+            x[4 * j] = t.x, x[4 * j + 1] = t.y, x[4 * j + 2] = t.z, x[4 * j + 3] = t.w;
+        }
+    }
 }
 __device__ __forceinline__ void store_out(void *p, int64_t i, int bf16, float f) {
     if (bf16) {
@@ -90,8 +108,12 @@ __device__ __forceinline__ void store_out(void *p, int64_t i, int bf16, float f)
     }
 }
 
+// Waves of a workgroup, each with its own tiles: two on a SIMD where their registers allow.
+constexpr int waves_of(int d) { return d > 128 ? 4 : 8; }
+
 template <int D, int R>
-__global__ void __launch_bounds__(256, D * R > 1024 ? 1 : 2) decode_kernel(KvAttend a) {
+__global__ void __launch_bounds__(64 * waves_of(D), waves_of(D) / 4) decode_kernel(KvAttend a) {
+    constexpr int kWaves = waves_of(D);
     constexpr int M = R / 4;                // matrix instructions for the four digits
     constexpr int S = (D + 63) / 64;        // steps of 64 channels
     constexpr int T = D / 16;               // tiles of 16 channels of the output
@@ -112,6 +134,48 @@ __global__ void __launch_bounds__(256, D * R > 1024 ? 1 : 2) decode_kernel(KvAtt
         if ((int)blockIdx.x + 1 < ranges) t1 = t0 + a.split_tiles;
     }
 
+    const int32_t *table = a.step.table + (int64_t)a.step.seq[i] * a.step.sequence_pages;
+    const int last_block = (len - 1) / kKvBlock, in_page = (1 << a.l.block_shift) - 1;
+    const uint32_t block_bytes = 2 * kKvBlock * D;
+
+    v4i kr[4][S], vr[T];
+    float2 sc;
+    // Pages of the lane's block of K and of V in a tile, looked up a tile ahead of the loads from them. A page that is not there
+    // gives bytes that weigh nothing.
+    int page_k, page_v;
+    auto look_up = [&](int tile) {
+        page_k = table[min(tile * 4 + (col >> 2), last_block) >> a.l.block_shift];
+        page_v = table[min(tile * 4 + quad, last_block) >> a.l.block_shift];
+    };
+    auto block_at = [&](int tile, int b, int page, int *in) -> const uint8_t * {
+        *in = (head << a.l.block_shift) + (min(tile * 4 + b, last_block) & in_page);
+        return a.l.base + (int64_t)max(page, 0) * a.l.page_bytes;
+    };
+    auto load_k = [&](int tile) {
+        int in;
+        const uint8_t *pg = block_at(tile, col >> 2, page_k, &in), *k = pg + in * block_bytes + (col & 3) * D + quad * 16;
+#pragma unroll
+        for (int s = 0; s < 4; s++)
+#pragma unroll
+            for (int c = 0; c < S; c++) kr[s][c] = *(const v4i *)(k + 4 * s * D + 64 * c);
+    };
+    auto load_v = [&](int tile) {
+        int in;
+        const uint8_t *pg = block_at(tile, quad, page_v, &in), *v = pg + in * block_bytes + kKvBlock * D + col * 16;
+        sc = *(const float2 *)(pg + a.l.scales + 8 * in);
+#pragma unroll
+        for (int t = 0; t < T; t++) vr[t] = *(const v4i *)(v + 256 * t);
+    };
+
+    // the wave's first tile, while the queries are made ready
+    if (t0 + wave < t1) {
+        const int tile = vis.tile(t0 + wave);
+        look_up(tile);
+        load_k(tile);
+        load_v(tile);
+        if (t0 + wave + kWaves < t1) look_up(vis.tile(t0 + wave + kWaves));
+    }
+
     const int rr = rg * R + col % R;
     const bool real = rr < tokens * a.group;
     const int p = len - tokens + (real ? rr / a.group : 0);  // the row's place
@@ -123,13 +187,19 @@ __global__ void __launch_bounds__(256, D * R > 1024 ? 1 : 2) decode_kernel(KvAtt
     {
         const int64_t at = (int64_t)(row0 + (real ? rr / a.group : 0)) * a.q_stride + (head * a.group + (real ? rr % a.group : 0)) * D;
         float x[S][16], most = 0.0f;
-        for (int s = 0; s < S; s++)
+        for (int s = 0; s < S; s++) {
+            const int d = s * 64 + quad * 16;
+            if (d < D) {
+                load16(a.q, at + d, a.q_bf16, x[s]);
+            } else {
+                for (int j = 0; j < 16; j++) x[s][j] = 0.0f;
+            }
             for (int j = 0; j < 16; j++) {
-                const int d = s * 64 + quad * 16 + j;
-                x[s][j] = d < D && real ? value_at(a.q, at + d, a.q_bf16) : 0.0f;
+                if (!real) x[s][j] = 0.0f;
                 const float m = fabsf(x[s][j]);
                 most = fmaxf(most, m < __builtin_inff() ? m : __builtin_inff());
             }
+        }
         most = max_column(most);
         // at least 2^-90, so that its reciprocal is finite
         const float unit = fmaxf(most, 0x1p-90f) * 0x1p-30f, inv = 1.0f / unit;
@@ -151,39 +221,10 @@ __global__ void __launch_bounds__(256, D * R > 1024 ? 1 : 2) decode_kernel(KvAtt
         for (int m = 0; m < M; m++) acc[m][t] = v4i{0, 0, 0, 0};
         for (int j = 0; j < 4; j++) o[t][j] = 0.0f;
     }
-    const int32_t *table = a.step.table + (int64_t)a.step.seq[i] * a.step.sequence_pages;
-    const int last_block = (len - 1) / kKvBlock, in_page = (1 << a.l.block_shift) - 1;
-    const uint32_t block_bytes = 2 * kKvBlock * D;
-
-    v4i kr[4][S], vr[T];
-    float2 sc;
-    // page and place of a block of the tile; a page that is not there gives bytes that weigh nothing
-    auto block_at = [&](int tile, int b, int *in) -> const uint8_t * {
-        const int blk = min(tile * 4 + b, last_block);
-        *in = (head << a.l.block_shift) + (blk & in_page);
-        return a.l.base + (int64_t)max(table[blk >> a.l.block_shift], 0) * a.l.page_bytes;
-    };
-    auto load_k = [&](int tile) {
-        int in;
-        const uint8_t *pg = block_at(tile, col >> 2, &in), *k = pg + in * block_bytes + (col & 3) * D + quad * 16;
-#pragma unroll
-        for (int s = 0; s < 4; s++)
-#pragma unroll
-            for (int c = 0; c < S; c++) kr[s][c] = *(const v4i *)(k + 4 * s * D + 64 * c);
-    };
-    auto load_v = [&](int tile) {
-        int in;
-        const uint8_t *pg = block_at(tile, quad, &in), *v = pg + in * block_bytes + kKvBlock * D + col * 16;
-        sc = *(const float2 *)(pg + a.l.scales + 8 * in);
-#pragma unroll
-        for (int t = 0; t < T; t++) vr[t] = *(const v4i *)(v + 256 * t);
-    };
-
     int since = 0;
     for (int u = t0 + wave; u < t1; u += kWaves) {
         const int tile = vis.tile(u);
-        load_k(tile);
-        load_v(tile);
+        const bool more = u + kWaves < t1;
         float t[16];
         float sk = sc.x, sv = fmaxf(sc.y, kKvMinScale);
         if (sc.y != sc.y) sv = sc.y;
@@ -208,6 +249,7 @@ __global__ void __launch_bounds__(256, D * R > 1024 ? 1 : 2) decode_kernel(KvAtt
                 t[4 * s + j] = __builtin_fmaf(sum_digits<R>(x), qk, lv);
             }
         }
+        if (more) load_k(vis.tile(u + kWaves));
         // tokens that not every row sees
         const int j0 = tile * kKvTile;
         if (j0 + kKvTile - 1 > q_first || (j0 <= q_last - a.window && j0 + kKvTile - 1 >= a.sinks)) {
@@ -254,6 +296,10 @@ __global__ void __launch_bounds__(256, D * R > 1024 ? 1 : 2) decode_kernel(KvAtt
 #pragma unroll
             for (int tt = 0; tt < T; tt++) acc[m][tt] = __builtin_amdgcn_mfma_i32_16x16x64_i8(vr[tt], b, acc[m][tt], 0, 0, 0);
         }
+        if (more) {
+            load_v(vis.tile(u + kWaves));
+            if (u + 2 * kWaves < t1) look_up(vis.tile(u + 2 * kWaves));
+        }
     }
 
     l_sum = sum_column(l_sum);
@@ -299,37 +345,81 @@ __global__ void __launch_bounds__(256, D * R > 1024 ? 1 : 2) decode_kernel(KvAtt
     }
 }
 
-// A row per workgroup.
+// A row per workgroup: D / 4 threads for four channels each, as many of these as 256 threads hold for ranges of their own, whose
+// first parts are on their way while the largest max is found. (One thread per channel that walked all ranges: 23 us for 64
+// ranges, a load's latency each.)
 __global__ void __launch_bounds__(256) join_kernel(KvAttend a) {
-    const int i = blockIdx.z, head = blockIdx.y, row = blockIdx.x, D = a.l.dim, d = threadIdx.x;
+    constexpr int kAhead = 8, kRanges = 256;
+    __shared__ float fs[kRanges], red[2][4];
+    __shared__ float4 sums[256];
+    const int i = blockIdx.z, head = blockIdx.y, row = blockIdx.x, D = a.l.dim, tid = threadIdx.x;
     const int row0 = a.step.row0[i], tokens = a.step.row0[i + 1] - row0;
-    if (row >= tokens * a.group || d >= D) return;
+    if (row >= tokens * a.group) return;
     const int64_t slot = (((int64_t)i * a.l.kv_heads + head) * a.max_rows + row) * a.splits;
     const int first = a.step.len[i] - tokens;
     const int t0 = row / a.row_tile * a.row_tile, t1 = min(tokens * a.group, t0 + a.row_tile) - 1;
     const int ranges = kv_ranges(kv_tiles(first + t0 / a.group, first + t1 / a.group, a.window, a.sinks).count(), a);
-    const float *ml = a.part_ml + 2 * slot;
-    float most = -__builtin_inff();
-    for (int s = 0; s < ranges; s++) most = fmaxf(most, ml[2 * s]);
-    float sum = 0.0f, total = 0.0f;
-    for (int s = 0; s < ranges; s++) {
-        const float f = most > -__builtin_inff() ? __builtin_amdgcn_exp2f(ml[2 * s] - most) : 1.0f;
-        sum = __builtin_fmaf(a.part[(slot + s) * D + d], f, sum);
-        total = __builtin_fmaf(ml[2 * s + 1], f, total);
+    const int width = D / 4, groups = 256 / width, group = tid / width, c = tid - group * width;
+    const float4 *part = (const float4 *)(a.part + slot * D) + c;
+    float4 ahead[kAhead];
+    const bool works = group < groups;
+#pragma unroll
+    for (int j = 0; j < kAhead; j++) {
+        const int s = group + j * groups;
+        if (works && s < ranges) ahead[j] = part[(int64_t)s * width];
     }
-    const int64_t to = (int64_t)(row0 + row / a.group) * a.out_stride + (head * a.group + row % a.group) * D + d;
-    store_out(a.out, to, a.out_bf16, total == 0.0f ? 0.0f : sum / total);
+    float m = -__builtin_inff(), l = 0.0f;
+    if (tid < ranges) {
+        const float2 ml = *(const float2 *)(a.part_ml + 2 * (slot + tid));
+        m = ml.x, l = ml.y;
+    }
+    float most = m;
+    for (int d = 32; d; d >>= 1) most = fmaxf(most, __shfl_xor(most, d));
+    if ((tid & 63) == 0) red[0][tid >> 6] = most;
+    __syncthreads();
+    most = fmaxf(fmaxf(red[0][0], red[0][1]), fmaxf(red[0][2], red[0][3]));
+    const float f = most > -__builtin_inff() ? __builtin_amdgcn_exp2f(m - most) : 1.0f;  // of no visible token: sums of 0, or NaN
+    fs[tid] = f;
+    l *= f;
+    if (tid >= ranges) l = 0.0f;
+    for (int d = 32; d; d >>= 1) l += __shfl_xor(l, d);
+    if ((tid & 63) == 0) red[1][tid >> 6] = l;
+    __syncthreads();
+    const float total = (red[1][0] + red[1][1]) + (red[1][2] + red[1][3]);
+    float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    auto add = [&](const float4 &p, float by) {
+        sum.x = __builtin_fmaf(p.x, by, sum.x), sum.y = __builtin_fmaf(p.y, by, sum.y);
+        sum.z = __builtin_fmaf(p.z, by, sum.z), sum.w = __builtin_fmaf(p.w, by, sum.w);
+    };
+    if (works) {
+#pragma unroll
+        for (int j = 0; j < kAhead; j++) {
+            const int s = group + j * groups;
+            if (s < ranges) add(ahead[j], fs[s]);
+        }
+        for (int s = group + kAhead * groups; s < ranges; s += groups) add(part[(int64_t)s * width], fs[s]);
+    }
+    sums[tid] = sum;
+    __syncthreads();
+    if (tid >= width) return;
+    for (int g = 1; g < groups; g++) add(sums[tid + g * width], 1.0f);
+    const int64_t to = (int64_t)(row0 + row / a.group) * a.out_stride + (head * a.group + row % a.group) * D + 4 * c;
+    const float by = total == 0.0f ? 0.0f : 1.0f / total;
+    store_out(a.out, to, a.out_bf16, sum.x * by);
+    store_out(a.out, to + 1, a.out_bf16, sum.y * by);
+    store_out(a.out, to + 2, a.out_bf16, sum.z * by);
+    store_out(a.out, to + 3, a.out_bf16, sum.w * by);
 }
 
 template <int R>
 hipError_t decode(const KvAttend &a, hipStream_t s, hipEvent_t done) {
     const dim3 grid((unsigned)a.splits, (unsigned)(a.l.kv_heads * ((a.max_rows + R - 1) / R)), (unsigned)a.step.n);
     switch (a.l.dim) {
-    case 64: return launch_with_event(decode_kernel<64, R>, grid, dim3(256), s, done, a);
-    case 96: return launch_with_event(decode_kernel<96, R>, grid, dim3(256), s, done, a);
-    case 128: return launch_with_event(decode_kernel<128, R>, grid, dim3(256), s, done, a);
-    case 192: return launch_with_event(decode_kernel<192, R>, grid, dim3(256), s, done, a);
-    case 256: return launch_with_event(decode_kernel<256, R>, grid, dim3(256), s, done, a);
+    case 64: return launch_with_event(decode_kernel<64, R>, grid, dim3(64 * waves_of(64)), s, done, a);
+    case 96: return launch_with_event(decode_kernel<96, R>, grid, dim3(64 * waves_of(96)), s, done, a);
+    case 128: return launch_with_event(decode_kernel<128, R>, grid, dim3(64 * waves_of(128)), s, done, a);
+    case 192: return launch_with_event(decode_kernel<192, R>, grid, dim3(64 * waves_of(192)), s, done, a);
+    case 256: return launch_with_event(decode_kernel<256, R>, grid, dim3(64 * waves_of(256)), s, done, a);
     }
     return hipErrorInvalidValue;
 }
@@ -344,7 +434,7 @@ hipError_t launch_kv_decode(const KvAttend &a, hipStream_t s, hipEvent_t done) {
 
 hipError_t launch_kv_join(const KvAttend &a, hipStream_t s, hipEvent_t done) {
     const dim3 grid((unsigned)a.max_rows, (unsigned)a.l.kv_heads, (unsigned)a.step.n);
-    return launch_with_event(join_kernel, grid, dim3((unsigned)(a.l.dim + 63) / 64 * 64), s, done, a);
+    return launch_with_event(join_kernel, grid, dim3(256), s, done, a);
 }
 
 }  // namespace j4q

@@ -16,6 +16,7 @@ Pointers are device addresses (integers); calls enqueue on ``stream`` (0: the en
 from __future__ import annotations
 
 import ctypes as C
+from array import array
 from operator import index
 
 import numpy as np
@@ -33,12 +34,23 @@ def _kind(dtype: DType) -> int:
     return _KINDS[dtype]
 
 
-def _ints(values, ctype=C.c_int32):
-    values = [index(v) for v in values]
-    bits = 8 * C.sizeof(ctype)
-    if any(not -(1 << bits - 1) <= v < 1 << bits - 1 for v in values):
-        raise IllegalArgumentException(f"a number does not fit {bits} bits")
-    return (ctype * len(values))(*values)
+def _ints(values, code="i") -> array:
+    """Whole numbers as the library reads them; an array of 64 takes 2 us, where a ctypes one takes 15."""
+    try:
+        return array(code, values)
+    except OverflowError:
+        raise IllegalArgumentException(f"a number does not fit {8 * array(code).itemsize} bits") from None
+
+
+def _int32(v) -> int:
+    v = index(v)
+    if not -0x80000000 <= v < 0x80000000:
+        raise IllegalArgumentException("a number does not fit 32 bits")
+    return v
+
+
+def _at(a: array) -> int:
+    return a.buffer_info()[0]
 
 
 def _equal(a, b, what: str) -> None:
@@ -80,7 +92,7 @@ class KvCache:
         self._be = backend
         self.handle = 0
         sequence_pages = pages if sequence_pages is None else sequence_pages
-        self._config = N.KvConfig(*_ints([layers, kv_heads, head_dim, page_tokens]), index(pages), *_ints([sequences, sequence_pages]))
+        self._config = N.KvConfig(*map(_int32, (layers, kv_heads, head_dim, page_tokens)), index(pages), *map(_int32, (sequences, sequence_pages)))
         out = C.c_uint64()
         check(backend._lib().j4q_kv_create(C.byref(self._config), C.byref(out)), "kv cache")
         self.handle = out.value
@@ -97,18 +109,20 @@ class KvCache:
         return {**{n: getattr(d.config, n) for n, _ in N.KvConfig._fields_}, **got}
 
     def length(self, seq: int) -> int:
-        n = C.c_int64()
-        check(N.load().j4q_kv_sequence(self.handle, *_ints([seq]), C.byref(n), None, 0), "kv sequence")
-        return n.value
+        return int(self.lengths([seq])[0])
+
+    def lengths(self, seqs) -> np.ndarray:
+        """Tokens of the sequences, int64 [n]."""
+        s = _ints(seqs)
+        out = np.empty(len(s), np.int64)
+        check(N.load().j4q_kv_tables(self.handle, _at(s), len(s), out.ctypes.data, None, 0), "kv tables")
+        return out
 
     def tables(self, seqs) -> np.ndarray:
         """Pages of the sequences, int32 [n, sequence_pages]; -1: evicted, and behind a sequence's last page."""
-        seqs, width = list(seqs), self._config.sequence_pages
-        out = np.empty((len(seqs), width), np.int32)
-        at = out.ctypes.data
-        for i, s in enumerate(_ints(seqs)):
-            row = C.cast(at + 4 * width * i, C.POINTER(C.c_int32))
-            check(N.load().j4q_kv_sequence(self.handle, s, None, row, width), "kv sequence")
+        s, width = _ints(seqs), self._config.sequence_pages
+        out = np.empty((len(s), width), np.int32)
+        check(N.load().j4q_kv_tables(self.handle, _at(s), len(s), None, out.ctypes.data, width), "kv tables")
         return out
 
     # ---- pages ---------------------------------------------------------------------------
@@ -116,30 +130,30 @@ class KvCache:
         """Begin a step: sequence seqs[i] gets tokens[i] more tokens (the step's rows, in this order)."""
         s, t = _ints(seqs), _ints(tokens)
         _equal(s, t, "counts of tokens")
-        check(self._be._lib().j4q_kv_extend(self.handle, s, t, len(s), *_addresses(stream)), "kv extend")
+        check(self._be._lib().j4q_kv_extend(self.handle, _at(s), _at(t), len(s), *_addresses(stream)), "kv extend")
 
     def begin(self, seqs, tokens, stream: int = 0) -> None:
         """Begin a step over the last tokens[i] tokens that sequence seqs[i] has already."""
         s, t = _ints(seqs), _ints(tokens)
         _equal(s, t, "counts of tokens")
-        check(self._be._lib().j4q_kv_begin(self.handle, s, t, len(s), *_addresses(stream)), "kv begin")
+        check(self._be._lib().j4q_kv_begin(self.handle, _at(s), _at(t), len(s), *_addresses(stream)), "kv begin")
 
     def fork(self, src, dst, share: bool = True, stream: int = 0) -> None:
         """The empty sequence dst[i] becomes src[i], sharing its pages or with copies of them."""
         s, d = _ints(src), _ints(dst)
         _equal(s, d, "forks")
-        check(self._be._lib().j4q_kv_fork(self.handle, s, d, len(s), int(bool(share)), *_addresses(stream)), "kv fork")
+        check(self._be._lib().j4q_kv_fork(self.handle, _at(s), _at(d), len(s), int(bool(share)), *_addresses(stream)), "kv fork")
 
     def truncate(self, seqs, lengths) -> None:
         """Cut sequences to lengths[i] tokens; 0 frees them."""
-        s, t = _ints(seqs), _ints(lengths, C.c_int64)
+        s, t = _ints(seqs), _ints(lengths, "q")
         _equal(s, t, "lengths")
-        check(self._be._lib().j4q_kv_truncate(self.handle, s, t, len(s)), "kv truncate")
+        check(self._be._lib().j4q_kv_truncate(self.handle, _at(s), _at(t), len(s)), "kv truncate")
 
     def evict(self, seqs, window: int, sinks: int = 0, stream: int = 0) -> None:
         """Free the pages that no later token sees through a window of so many tokens and so many first ones."""
         s = _ints(seqs)
-        check(self._be._lib().j4q_kv_evict(self.handle, s, len(s), *_ints([window, sinks]), *_addresses(stream)), "kv evict")
+        check(self._be._lib().j4q_kv_evict(self.handle, _at(s), len(s), _int32(window), _int32(sinks), *_addresses(stream)), "kv evict")
 
     def compact(self, stream: int = 0) -> int:
         """Move pages so that those in use are the pool's lowest; how many were moved."""
@@ -153,20 +167,20 @@ class KvCache:
         """Store the step's keys and values, [rows, kv_heads, head_dim] each, keys turned by ``rope``; with ``q_ptr`` the
         queries [rows, heads, head_dim] too are turned, into ``q_out_ptr`` (0: in place). Strides are in values, 0: dense."""
         k, v, q, qo, s = _addresses(k_ptr, v_ptr, q_ptr, q_out_ptr or q_ptr, stream)
-        a = N.KvAppendArgs(k, v, stride, _kind(dtype), *_ints([heads]), q or None, qo or None, q_stride, C.pointer(rope.args) if rope else None)
-        check(self._be._lib().j4q_kv_append(self.handle, *_ints([layer]), C.byref(a), s), "kv append")
+        a = N.KvAppendArgs(k, v, stride, _kind(dtype), _int32(heads), q or None, qo or None, q_stride, C.pointer(rope.args) if rope else None)
+        check(self._be._lib().j4q_kv_append(self.handle, _int32(layer), C.byref(a), s), "kv append")
 
     def attend(self, layer: int, q_ptr: int, out_ptr: int, heads: int, *, q_type: DType = DType.F32, out_type: DType = DType.F32, q_stride: int = 0,
                out_stride: int = 0, window: int = 0, sinks: int = 0, scale: float = 0.0, stream: int = 0) -> None:
         """Attention of the step's queries [rows, heads, head_dim] to the tokens j <= p of their sequence, p their own place,
         with j > p - window (0: no window) or j < sinks. ``scale`` 0: 1 / sqrt(head_dim)."""
         q, o, s = _addresses(q_ptr, out_ptr, stream)
-        a = N.KvAttendArgs(q, o, q_stride, out_stride, _kind(q_type), _kind(out_type), *_ints([heads, window, sinks]), scale)
-        check(self._be._lib().j4q_kv_attend(self.handle, *_ints([layer]), C.byref(a), s), "kv attend")
+        a = N.KvAttendArgs(q, o, q_stride, out_stride, _kind(q_type), _kind(out_type), _int32(heads), _int32(window), _int32(sinks), scale)
+        check(self._be._lib().j4q_kv_attend(self.handle, _int32(layer), C.byref(a), s), "kv attend")
 
     def read(self, layer: int, seqs, first, count: int, k_ptr: int, v_ptr: int, stream: int = 0) -> None:
         """Tokens [first[i], first[i] + count) of seqs[i] as fp32 [n, count, kv_heads, head_dim]; zeros where there is none."""
-        s, f = _ints(seqs), _ints(first, C.c_int64)
+        s, f = _ints(seqs), _ints(first, "q")
         _equal(s, f, "first tokens")
         k, v, st = _addresses(k_ptr, v_ptr, stream)
-        check(self._be._lib().j4q_kv_read(self.handle, *_ints([layer]), s, f, index(count), len(s), k or None, v or None, st), "kv read")
+        check(self._be._lib().j4q_kv_read(self.handle, _int32(layer), _at(s), _at(f), index(count), len(s), k or None, v or None, st), "kv read")
