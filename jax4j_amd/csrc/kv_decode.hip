@@ -255,8 +255,10 @@ __global__ void __launch_bounds__(64 * waves_of(D), waves_of(D) / 4) decode_kern
         if (j0 + kKvTile - 1 > q_first || (j0 <= q_last - a.window && j0 + kKvTile - 1 >= a.sinks)) {
             const int at = j0 + quad * kKvBlock;
 #pragma unroll
-            for (int j = 0; j < 16; j++)
-                if (!(at + j <= p && (at + j >= first_low || at + j < a.sinks))) t[j] = -__builtin_inff();
+            for (int j = 0; j < 16; j++) {
+                const bool seen = (at + j <= p) & ((at + j >= first_low) | (at + j < a.sinks));
+                t[j] = seen ? t[j] : -__builtin_inff();
+            }
         }
 #pragma unroll
         for (int j = 0; j < 16; j++) top = fmaxf(top, t[j]);

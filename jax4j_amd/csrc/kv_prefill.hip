@@ -38,6 +38,10 @@ __device__ __forceinline__ float max32(float v) {
     return fmaxf(t.a, t.b);
 }
 
+__device__ __forceinline__ float lane_of(float v, int lane) {
+    return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), lane));
+}
+
 // Four int8 codes as fp16: 1024 + 128 + code is exact in fp16, and so is the difference.
 __device__ __forceinline__ void codes_to_half(uint32_t c, uint32_t *out) {
     const uint32_t u = c ^ 0x80808080u;
@@ -54,15 +58,14 @@ __device__ __forceinline__ uint32_t bf16_bits(float f) {
     return f != f ? (u >> 16) | 0x40 : (u + 0x7fffu + ((u >> 16) & 1)) >> 16;
 }
 
-// NT: tiles of 32 rows of a wave. P: fp16 parts of q and w.
-template <int D, int NT, int P>
-__global__ void __launch_bounds__(256, NT == 1 && D <= 128 ? 2 : 1) prefill_kernel(KvAttend a) {
-    constexpr int kRows = 4 * NT * 32;
+// W: waves, of 32 rows each. P: fp16 parts of q and w.
+template <int D, int W, int P>
+__global__ void __launch_bounds__(64 * W, D <= 128 ? 2 : 1) prefill_kernel(KvAttend a) {
+    constexpr int kThreads = 64 * W, kRows = 32 * W;
     constexpr int KP = D + 8, VP = kKvTile + 8;            // row pitches in LDS: an odd number of 16 bytes, 16 rows on all banks
-    constexpr int N = (4 * D + 255) / 256;                 // 16-byte pieces of K, and of V, that a thread stages
+    constexpr int N = (4 * D + kThreads - 1) / kThreads;   // 16-byte pieces of K, and of V, that a thread stages
     __shared__ __align__(16) _Float16 ks[2][kKvTile][KP];
     __shared__ __align__(16) _Float16 vs[2][D][VP];
-    __shared__ __align__(16) float scales[2][3][4];        // K scale, log2 of V's, its reciprocal
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, col = lane & 31, half = lane >> 5;
     const int head = blockIdx.x % a.l.kv_heads, split = blockIdx.x / a.l.kv_heads, i = blockIdx.z;
     const int row0 = a.step.row0[i], tokens = a.step.row0[i + 1] - row0, len = a.step.len[i], rows = tokens * a.group;
@@ -79,17 +82,14 @@ __global__ void __launch_bounds__(256, NT == 1 && D <= 128 ? 2 : 1) prefill_kern
         t0 = split * a.split_tiles;
         if (split + 1 < ranges) t1 = t0 + a.split_tiles;
     }
-    // the wave's rows, and its places
-    const int w0 = r0 + wave * NT * 32, w1 = min(r1, w0 + NT * 32 - 1);
+    // the wave's rows, and its places; the lane's row
+    const int w0 = r0 + wave * 32, w1 = min(r1, w0 + 31);
     const int p_first = before + min(w0, r1) / a.group, p_last = before + w1 / a.group;
-    int place[NT];
-    v8h q[NT][P][D / 16];
-    float qk[NT];
-#pragma unroll
-    for (int n = 0; n < NT; n++) {
-        const int r = min(w0 + n * 32 + col, r1);
-        place[n] = before + r / a.group;
-        const int64_t at = (int64_t)(row0 + r / a.group) * a.q_stride + (head * a.group + r % a.group) * D + 8 * half;
+    const int row = min(w0 + col, r1), place = before + row / a.group;
+    v8h q[P][D / 16];
+    float qk;
+    {
+        const int64_t at = (int64_t)(row0 + row / a.group) * a.q_stride + (head * a.group + row % a.group) * D + 8 * half;
         float most = 0.0f;
         for (int s = 0; s < D / 16; s++)
             for (int j = 0; j < 8; j++) {
@@ -100,209 +100,218 @@ __global__ void __launch_bounds__(256, NT == 1 && D <= 128 ? 2 : 1) prefill_kern
         // to [2^13, 2^14), by a power of two (2^100 at most)
         const int e = max((int)(__builtin_bit_cast(uint32_t, most) >> 23) - 127 - 13, -100);
         const float up = __builtin_bit_cast(float, (uint32_t)(127 - e) << 23);
-        qk[n] = most < __builtin_inff() ? __builtin_bit_cast(float, (uint32_t)(127 + e) << 23) * a.scale : __builtin_nanf("");
+        qk = most < __builtin_inff() ? __builtin_bit_cast(float, (uint32_t)(127 + e) << 23) * a.scale : __builtin_nanf("");
         for (int s = 0; s < D / 16; s++)
             for (int j = 0; j < 8; j++) {
                 const float x = value_at(a.q, at + 16 * s + j, a.q_bf16) * up;
-                q[n][0][s][j] = (_Float16)x;
-                if constexpr (P == 2) q[n][1][s][j] = (_Float16)(x - (float)q[n][0][s][j]);
+                q[0][s][j] = (_Float16)x;
+                if constexpr (P == 2) q[1][s][j] = (_Float16)(x - (float)q[0][s][j]);
             }
     }
 
-    v16f o[NT][D / 32];
-    float m_at[NT], base[NT], lim[NT], l_sum[NT];
+    v16f o[D / 32];
 #pragma unroll
-    for (int n = 0; n < NT; n++) {
-        m_at[n] = -__builtin_inff();
-        base[n] = l_sum[n] = 0.0f;
-        lim[n] = -__builtin_inff();  // t (less m) that is too large
+    for (int d = 0; d < D / 32; d++)
 #pragma unroll
-        for (int d = 0; d < D / 32; d++)
-#pragma unroll
-            for (int r = 0; r < 16; r++) o[n][d][r] = 0.0f;
-    }
+        for (int r = 0; r < 16; r++) o[d][r] = 0.0f;
+    // lim: the t (less m) that is too large
+    float m_at = -__builtin_inff(), base = 0.0f, lim = -__builtin_inff(), l_sum = 0.0f;
 
     const int32_t *table = a.step.table + (int64_t)a.step.seq[i] * a.step.sequence_pages;
     const int last_block = (len - 1) / kKvBlock, in_mask = (1 << a.l.block_shift) - 1;
-    auto block_at = [&](int tile, int b, int *in) -> const uint8_t * {
-        const int blk = min(tile * 4 + b, last_block);
-        *in = (head << a.l.block_shift) + (blk & in_mask);
-        return a.l.base + (int64_t)max(table[blk >> a.l.block_shift], 0) * a.l.page_bytes;
-    };
+    // Piece c of K and of V lies 16 (c % D) bytes into that of block c / D, which is the same for a wave where 64 divides D. Pages
+    // are looked up a tile ahead of the loads from them, those a tile ahead of their conversion.
+    int page[N], scale_page;
     uint4 kraw[N], vraw[N];
-    float2 sraw = make_float2(0.0f, 0.0f);
+    // lane l of every wave: block l % 4's scale of K, log2 of V's and its reciprocal, of the next tile
+    float2 sraw;
+    float next_k, next_log, next_r;
+    auto block_of = [&](int j) { return D % 64 == 0 ? __builtin_amdgcn_readfirstlane((tid + kThreads * j) / D) : (tid + kThreads * j) / D; };
+    auto staged = [&](int j) { return 4 * D % kThreads == 0 || tid + kThreads * j < 4 * D; };
+    auto look_up = [&](int tile) {
+#pragma unroll
+        for (int j = 0; j < N; j++)
+            if (staged(j)) page[j] = table[min(tile * 4 + block_of(j), last_block) >> a.l.block_shift];
+        scale_page = table[min(tile * 4 + (lane & 3), last_block) >> a.l.block_shift];
+    };
     auto fetch = [&](int tile) {
 #pragma unroll
         for (int j = 0; j < N; j++) {
-            const int c = tid + 256 * j;
-            if (4 * D % 256 == 0 || c < 4 * D) {
-                int in;
-                const int token = c / (D / 16);
-                const uint8_t *pg = block_at(tile, token / kKvBlock, &in);
-                kraw[j] = *(const uint4 *)(pg + in * (2 * kKvBlock * D) + token % kKvBlock * D + c % (D / 16) * 16);
-                pg = block_at(tile, c / D, &in);
-                vraw[j] = *(const uint4 *)(pg + in * (2 * kKvBlock * D) + kKvBlock * D + c % D * 16);
-            }
+            if (!staged(j)) continue;
+            const int blk = min(tile * 4 + block_of(j), last_block), in = (head << a.l.block_shift) + (blk & in_mask);
+            const int pg = D % 64 == 0 ? __builtin_amdgcn_readfirstlane(page[j]) : page[j];
+            const uint8_t *k = a.l.base + (int64_t)max(pg, 0) * a.l.page_bytes + in * (2 * kKvBlock * D);
+            const int at = (tid + kThreads * j) % D * 16;
+            kraw[j] = *(const uint4 *)(k + at);
+            vraw[j] = *(const uint4 *)(k + kKvBlock * D + at);
         }
-        if (tid < 4) {
-            int in;
-            const uint8_t *pg = block_at(tile, tid, &in);
-            sraw = *(const float2 *)(pg + a.l.scales + 8 * in);
-            if (tile * 4 + tid > last_block) sraw = make_float2(0.0f, 1.0f);
-        }
+        const int blk = min(tile * 4 + (lane & 3), last_block), in = (head << a.l.block_shift) + (blk & in_mask);
+        sraw = *(const float2 *)(a.l.base + (int64_t)max(scale_page, 0) * a.l.page_bytes + a.l.scales + 8 * in);
     };
     auto stage = [&](int buf) {
 #pragma unroll
         for (int j = 0; j < N; j++) {
-            const int c = tid + 256 * j;
-            if (4 * D % 256 == 0 || c < 4 * D) {
-                uint32_t h[8];
-                codes_to_half(kraw[j].x, h), codes_to_half(kraw[j].y, h + 2), codes_to_half(kraw[j].z, h + 4), codes_to_half(kraw[j].w, h + 6);
-                uint4 *to = (uint4 *)&ks[buf][c / (D / 16)][c % (D / 16) * 16];
-                to[0] = make_uint4(h[0], h[1], h[2], h[3]);
-                to[1] = make_uint4(h[4], h[5], h[6], h[7]);
-                codes_to_half(vraw[j].x, h), codes_to_half(vraw[j].z, h + 2), codes_to_half(vraw[j].y, h + 4), codes_to_half(vraw[j].w, h + 6);
-                to = (uint4 *)&vs[buf][c % D][c / D * 16];
-                to[0] = make_uint4(h[0], h[1], h[2], h[3]);
-                to[1] = make_uint4(h[4], h[5], h[6], h[7]);
-            }
+            if (!staged(j)) continue;
+            const int c = tid + kThreads * j;
+            uint32_t h[8];
+            codes_to_half(kraw[j].x, h), codes_to_half(kraw[j].y, h + 2), codes_to_half(kraw[j].z, h + 4), codes_to_half(kraw[j].w, h + 6);
+            uint4 *to = (uint4 *)&ks[buf][c / (D / 16)][c % (D / 16) * 16];
+            to[0] = make_uint4(h[0], h[1], h[2], h[3]);
+            to[1] = make_uint4(h[4], h[5], h[6], h[7]);
+            codes_to_half(vraw[j].x, h), codes_to_half(vraw[j].z, h + 2), codes_to_half(vraw[j].y, h + 4), codes_to_half(vraw[j].w, h + 6);
+            to = (uint4 *)&vs[buf][c % D][c / D * 16];
+            to[0] = make_uint4(h[0], h[1], h[2], h[3]);
+            to[1] = make_uint4(h[4], h[5], h[6], h[7]);
         }
-        if (tid < 4) {
-            const float sv = sraw.y != sraw.y ? sraw.y : fmaxf(sraw.y, kKvMinScale);
-            scales[buf][0][tid] = sraw.x;
-            scales[buf][1][tid] = __builtin_amdgcn_logf(sv);
-            scales[buf][2][tid] = sv == sv ? 1.0f / sv : 1.0f;
-        }
+        // what lies behind the end is hidden, and must only not be NaN
+        const bool nan = sraw.y != sraw.y;
+        const float sv = nan ? 1.0f : fmaxf(sraw.y, kKvMinScale);
+        next_k = sraw.x;
+        next_log = nan ? sraw.y : __builtin_amdgcn_logf(sv);
+        next_r = __builtin_amdgcn_rcpf(sv);
     };
 
+    // behind the last tile the last one again, which nobody uses: no branch inside the round
+    auto tile_at = [&](int u) { return vis.tile(min(u, t1 - 1)); };
     if (t0 < t1) {
-        fetch(vis.tile(t0));
+        look_up(tile_at(t0));
+        fetch(tile_at(t0));
+        look_up(tile_at(t0 + 1));
         stage(0);
+        fetch(tile_at(t0 + 1));
+        look_up(tile_at(t0 + 2));
     }
     __syncthreads();
     for (int u = t0; u < t1; u++) {
         const int buf = (u - t0) & 1, tile = vis.tile(u), j0 = tile * kKvTile;
-        if (u + 1 < t1) fetch(vis.tile(u + 1));
-        // nothing of the tile that a row of the wave sees
-        const bool hidden = j0 > p_last || (j0 + kKvTile - 1 <= p_first - a.window && j0 >= a.sinks) || w0 > r1;
-        if (!hidden) {
-            float sk[4], lv[4], rsv[4];
+        const float scale_k = next_k, log_v = next_log, inv_v = next_r;
+        v16f s[2];
 #pragma unroll
-            for (int b = 0; b < 4; b++) sk[b] = scales[buf][0][b], lv[b] = scales[buf][1][b], rsv[b] = scales[buf][2][b];
-            const bool whole = j0 + kKvTile - 1 <= p_first && (j0 > p_last - a.window || j0 + kKvTile - 1 < a.sinks);
+        for (int r = 0; r < 16; r++) s[0][r] = s[1][r] = 0.0f;
+        v8h k[2][D / 16];
 #pragma unroll
-            for (int sub = 0; sub < 2; sub++) {
-                v16f s[NT];
+        for (int st = 0; st < D / 16; st++)
 #pragma unroll
-                for (int n = 0; n < NT; n++)
+            for (int sub = 0; sub < 2; sub++) k[sub][st] = *(const v8h *)&ks[buf][32 * sub + col][16 * st + 8 * half];
 #pragma unroll
-                    for (int r = 0; r < 16; r++) s[n][r] = 0.0f;
+        for (int st = 0; st < D / 16; st++)
 #pragma unroll
-                for (int st = 0; st < D / 16; st++) {
-                    const v8h k = *(const v8h *)&ks[buf][32 * sub + col][16 * st + 8 * half];
+            for (int p = 0; p < P; p++)
 #pragma unroll
-                    for (int n = 0; n < NT; n++)
+                for (int sub = 0; sub < 2; sub++) s[sub] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k[sub][st], q[p][st], s[sub], 0, 0, 0);
+        stage(buf ^ 1);
+        fetch(tile_at(u + 2));
+        look_up(tile_at(u + 3));
+        // operands some products ahead, and the next tile's conversion between the products
+        __builtin_amdgcn_sched_group_barrier(0x100, 8, 0);
 #pragma unroll
-                        for (int p = 0; p < P; p++) s[n] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k, q[n][p][st], s[n], 0, 0, 0);
+        for (int m = 0; m < P * D / 8; m++) {
+            __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+            if (m % P == 0) __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+            __builtin_amdgcn_sched_group_barrier(0x002, 5, 0);
+        }
+        {
+            float t[2][16], rsv[4], top = -__builtin_inff();
+#pragma unroll
+            for (int b = 0; b < 4; b++) {
+                const float f = qk * lane_of(scale_k, b), c = lane_of(log_v, b) + base;
+                rsv[b] = lane_of(inv_v, b);
+#pragma unroll
+                for (int r = 0; r < 8; r++) t[b / 2][b % 2 * 8 + r] = __builtin_fmaf(s[b / 2][b % 2 * 8 + r], f, c);
+            }
+            if (!(j0 + kKvTile - 1 <= p_first && (j0 > p_last - a.window || j0 + kKvTile - 1 < a.sinks))) {
+#pragma unroll
+                for (int r = 0; r < 32; r++) {
+                    const int at = j0 + 32 * (r / 16) + 8 * (r % 16 / 4) + 4 * half + r % 4;
+                    const bool seen = (at <= place) & ((at > place - a.window) | (at < a.sinks));
+                    t[r / 16][r % 16] = seen ? t[r / 16][r % 16] : -__builtin_inff();
                 }
-                v8h w[NT][P][2];
+            }
 #pragma unroll
-                for (int n = 0; n < NT; n++) {
-                    float t[16], top = -__builtin_inff();
+            for (int r = 0; r < 32; r++) top = fmaxf(top, t[r / 16][r % 16]);
+            if (__any(top > lim)) {
+                top = max32(top);
+                if (top > lim) {  // m moves up to the largest t: by `up` octaves
+                    const bool first = !(m_at > -__builtin_inff());
+                    const float up = first ? top : top - kUnit, f = first ? 0.0f : __builtin_amdgcn_exp2f(-up);
+                    m_at = first ? up : m_at + up;
+                    const float shift = kUnit - m_at - base;
+                    base = kUnit - m_at;
+                    lim = kUnit + kHead;
+                    l_sum *= f;
 #pragma unroll
-                    for (int r = 0; r < 16; r++) t[r] = __builtin_fmaf(s[n][r], qk[n] * sk[2 * sub + r / 8], lv[2 * sub + r / 8] + base[n]);
-                    if (!whole) {
+                    for (int r = 0; r < 32; r++) t[r / 16][r % 16] += shift;
 #pragma unroll
-                        for (int r = 0; r < 16; r++) {
-                            const int at = j0 + 32 * sub + 8 * (r / 4) + 4 * half + r % 4;
-                            if (!(at <= place[n] && (at > place[n] - a.window || at < a.sinks))) t[r] = -__builtin_inff();
-                        }
-                    }
+                    for (int d = 0; d < D / 32; d++)
 #pragma unroll
-                    for (int r = 0; r < 16; r++) top = fmaxf(top, t[r]);
-                    if (__any(top > lim[n])) {
-                        top = max32(top);
-                        if (top > lim[n]) {  // m moves up to the largest t: by `up` octaves
-                            const float up = top - (m_at[n] > -__builtin_inff() ? kUnit : 0.0f), f = m_at[n] > -__builtin_inff() ? __builtin_amdgcn_exp2f(-up) : 0.0f;
-                            m_at[n] = m_at[n] > -__builtin_inff() ? m_at[n] + up : up;
-                            const float shift = kUnit - m_at[n] - base[n];
-                            base[n] = kUnit - m_at[n];
-                            lim[n] = kUnit + kHead;
-                            l_sum[n] *= f;
-#pragma unroll
-                            for (int r = 0; r < 16; r++) t[r] += shift;
-#pragma unroll
-                            for (int d = 0; d < D / 32; d++)
-#pragma unroll
-                                for (int r = 0; r < 16; r++) o[n][d][r] *= f;
-                        }
-                    }
-#pragma unroll
-                    for (int r = 0; r < 16; r++) {
-                        const float e = __builtin_amdgcn_exp2f(t[r]);
-                        l_sum[n] = __builtin_fmaf(e, rsv[2 * sub + r / 8], l_sum[n]);
-                        w[n][0][r / 8][r % 8] = (_Float16)e;
-                        if constexpr (P == 2) w[n][1][r / 8][r % 8] = (_Float16)(e - (float)w[n][0][r / 8][r % 8]);
-                    }
+                        for (int r = 0; r < 16; r++) o[d][r] *= f;
                 }
+            }
 #pragma unroll
-                for (int d = 0; d < D / 32; d++)
+            for (int b = 0; b < 4; b++) {
+                // the sum is of the weights before they are rounded: where a block's value scale is far below others', its weights may
+                // fall below what fp16 holds, and count in the sum all the same
+                v8h w[P];
+                float sum = 0.0f;
 #pragma unroll
-                    for (int k = 0; k < 2; k++) {
-                        const v8h v = *(const v8h *)&vs[buf][32 * d + col][16 * (2 * sub + k) + 8 * half];
+                for (int r = 0; r < 8; r += 2) {
+                    const float e0 = __builtin_amdgcn_exp2f(t[b / 2][b % 2 * 8 + r]), e1 = __builtin_amdgcn_exp2f(t[b / 2][b % 2 * 8 + r + 1]);
+                    const v2h h = {(_Float16)e0, (_Float16)e1};
+                    w[0][r] = h[0], w[0][r + 1] = h[1];
+                    if constexpr (P == 2) w[1][r] = (_Float16)(e0 - (float)h[0]), w[1][r + 1] = (_Float16)(e1 - (float)h[1]);
+                    sum += e0 + e1;
+                }
+                l_sum = __builtin_fmaf(sum, rsv[b], l_sum);
 #pragma unroll
-                        for (int n = 0; n < NT; n++)
+                for (int d = 0; d < D / 32; d++) {
+                    const v8h v = *(const v8h *)&vs[buf][32 * d + col][16 * b + 8 * half];
 #pragma unroll
-                            for (int p = 0; p < P; p++) o[n][d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, w[n][p][k], o[n][d], 0, 0, 0);
-                    }
+                    for (int p = 0; p < P; p++) o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, w[p], o[d], 0, 0, 0);
+                }
             }
         }
-        if (u + 1 < t1) stage(buf ^ 1);
         __syncthreads();
     }
 
+    const int r = w0 + col;
+    const Two both = swap32(l_sum);
+    const float total = both.a + both.b;
+    if (r > r1) return;
+    if (a.splits > 1) {
+        const int64_t slot = (((int64_t)i * a.l.kv_heads + head) * a.max_rows + r) * a.splits + split;
 #pragma unroll
-    for (int n = 0; n < NT; n++) {
-        const int r = w0 + n * 32 + col;
-        const Two both = swap32(l_sum[n]);
-        const float total = both.a + both.b;
-        if (r > r1) continue;
-        if (a.splits > 1) {
-            const int64_t slot = (((int64_t)i * a.l.kv_heads + head) * a.max_rows + r) * a.splits + split;
+        for (int d = 0; d < D / 32; d++)
 #pragma unroll
-            for (int d = 0; d < D / 32; d++)
-#pragma unroll
-                for (int g = 0; g < 4; g++)
-                    *(float4 *)(a.part + slot * D + 32 * d + 8 * g + 4 * half) = make_float4(o[n][d][4 * g], o[n][d][4 * g + 1], o[n][d][4 * g + 2], o[n][d][4 * g + 3]);
-            if (half == 0) {
-                a.part_ml[2 * slot] = m_at[n];
-                a.part_ml[2 * slot + 1] = total;
-            }
-        } else {
-            const float f = total == 0.0f ? 0.0f : 1.0f / total;
-            const int64_t to = (int64_t)(row0 + r / a.group) * a.out_stride + (head * a.group + r % a.group) * D + 4 * half;
-#pragma unroll
-            for (int d = 0; d < D / 32; d++)
-#pragma unroll
-                for (int g = 0; g < 4; g++) {
-                    float4 x = make_float4(o[n][d][4 * g] * f, o[n][d][4 * g + 1] * f, o[n][d][4 * g + 2] * f, o[n][d][4 * g + 3] * f);
-                    const int64_t at = to + 32 * d + 8 * g;
-                    if (a.out_bf16) *(uint2 *)((uint16_t *)a.out + at) = make_uint2(bf16_bits(x.x) | bf16_bits(x.y) << 16, bf16_bits(x.z) | bf16_bits(x.w) << 16);
-                    else *(float4 *)((float *)a.out + at) = x;
-                }
+            for (int g = 0; g < 4; g++)
+                *(float4 *)(a.part + slot * D + 32 * d + 8 * g + 4 * half) = make_float4(o[d][4 * g], o[d][4 * g + 1], o[d][4 * g + 2], o[d][4 * g + 3]);
+        if (half == 0) {
+            a.part_ml[2 * slot] = m_at;
+            a.part_ml[2 * slot + 1] = total;
         }
+    } else {
+        const float f = total == 0.0f ? 0.0f : 1.0f / total;
+        const int64_t to = (int64_t)(row0 + r / a.group) * a.out_stride + (head * a.group + r % a.group) * D + 4 * half;
+#pragma unroll
+        for (int d = 0; d < D / 32; d++)
+#pragma unroll
+            for (int g = 0; g < 4; g++) {
+                const float4 x = make_float4(o[d][4 * g] * f, o[d][4 * g + 1] * f, o[d][4 * g + 2] * f, o[d][4 * g + 3] * f);
+                const int64_t at = to + 32 * d + 8 * g;
+                if (a.out_bf16) *(uint2 *)((uint16_t *)a.out + at) = make_uint2(bf16_bits(x.x) | bf16_bits(x.y) << 16, bf16_bits(x.z) | bf16_bits(x.w) << 16);
+                else *(float4 *)((float *)a.out + at) = x;
+            }
     }
 }
 
-template <int NT, int P>
+template <int W, int P>
 hipError_t prefill(const KvAttend &a, hipStream_t s, hipEvent_t done) {
-    const dim3 grid((unsigned)(a.l.kv_heads * a.splits), (unsigned)((a.max_rows + 128 * NT - 1) / (128 * NT)), (unsigned)a.step.n);
+    const dim3 grid((unsigned)(a.l.kv_heads * a.splits), (unsigned)((a.max_rows + 32 * W - 1) / (32 * W)), (unsigned)a.step.n);
     switch (a.l.dim) {
-    case 64: return launch_with_event(prefill_kernel<64, NT, P>, grid, dim3(256), s, done, a);
-    case 96: return launch_with_event(prefill_kernel<96, NT, P>, grid, dim3(256), s, done, a);
-    case 128: return launch_with_event(prefill_kernel<128, NT, P>, grid, dim3(256), s, done, a);
-    case 192: return launch_with_event(prefill_kernel<192, NT, P>, grid, dim3(256), s, done, a);
-    case 256: return launch_with_event(prefill_kernel<256, NT, P>, grid, dim3(256), s, done, a);
+    case 64: return launch_with_event(prefill_kernel<64, W, P>, grid, dim3(64 * W), s, done, a);
+    case 96: return launch_with_event(prefill_kernel<96, W, P>, grid, dim3(64 * W), s, done, a);
+    case 128: return launch_with_event(prefill_kernel<128, W, P>, grid, dim3(64 * W), s, done, a);
+    case 192: return launch_with_event(prefill_kernel<192, 4, P>, grid, dim3(256), s, done, a);
+    case 256: return launch_with_event(prefill_kernel<256, 4, P>, grid, dim3(256), s, done, a);
     }
     return hipErrorInvalidValue;
 }
@@ -311,7 +320,8 @@ hipError_t prefill(const KvAttend &a, hipStream_t s, hipEvent_t done) {
 
 hipError_t launch_kv_prefill(const KvAttend &a, hipStream_t s, hipEvent_t done) {
     hipEvent_t last = a.splits > 1 ? nullptr : done;
-    const hipError_t e = a.out_bf16 ? prefill<1, 1>(a, s, last) : prefill<1, 2>(a, s, last);
+    const bool wide = a.row_tile == 256;
+    const hipError_t e = a.out_bf16 ? wide ? prefill<8, 1>(a, s, last) : prefill<4, 1>(a, s, last) : wide ? prefill<8, 2>(a, s, last) : prefill<4, 2>(a, s, last);
     return e == hipSuccess && a.splits > 1 ? launch_kv_join(a, s, done) : e;
 }
 
