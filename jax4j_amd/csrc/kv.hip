@@ -728,7 +728,7 @@ int j4q_kv_attend(j4q_kv kv, int32_t layer, const j4q_kv_attend_args *args, void
     a.out_bf16 = g.out_type == J4Q_KIND_BF16;
     a.scale = (g.scale > 0.0f ? g.scale : 1.0f / sqrtf((float)k->c.head_dim)) * 1.4426950408889634f;
     const bool many = a.max_rows > kFewRows;
-    a.row_tile = many ? k->c.head_dim <= 128 && !getenv("EXP_4") ? 256 : 128 : a.max_rows <= 4 ? 4 : 8;
+    a.row_tile = many ? k->c.head_dim <= 128 ? 256 : 128 : a.max_rows <= 4 ? 4 : 8;
     if ((rc = abi::ready_locked())) return rc;
     Call c(*k, stream);
     // Ranges of the tokens where rows alone leave CUs idle: one workgroup of a CU's registers each. Joining them costs 4 to 5 us, a

@@ -11,7 +11,12 @@
 // q (scaled by a power of two per row) and w in fp16 round by 2^-11, which a bf16 result hides; for an fp32 result both are a sum
 // of two fp16 (22 bits), twice the matrix instructions.
 // m moves only when a t passes it by 7 octaves (w < 2^15 then), so the outputs are rescaled rarely.
+#include <type_traits>
+
 #include "kv.h"
+
+// Nothing is scheduled across.
+#define FENCE() __builtin_amdgcn_sched_barrier(0)
 
 namespace j4q {
 namespace {
@@ -38,10 +43,6 @@ __device__ __forceinline__ float max32(float v) {
     return fmaxf(t.a, t.b);
 }
 
-__device__ __forceinline__ float lane_of(float v, int lane) {
-    return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), lane));
-}
-
 // Four int8 codes as fp16: 1024 + 128 + code is exact in fp16, and so is the difference.
 __device__ __forceinline__ void codes_to_half(uint32_t c, uint32_t *out) {
     const uint32_t u = c ^ 0x80808080u;
@@ -66,6 +67,7 @@ __global__ void __launch_bounds__(64 * W, D <= 128 ? 2 : 1) prefill_kernel(KvAtt
     constexpr int N = (4 * D + kThreads - 1) / kThreads;   // 16-byte pieces of K, and of V, that a thread stages
     __shared__ __align__(16) _Float16 ks[2][kKvTile][KP];
     __shared__ __align__(16) _Float16 vs[2][D][VP];
+    __shared__ __align__(16) float scales[2][3][4];        // K scale, log2 of V's, its reciprocal
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, col = lane & 31, half = lane >> 5;
     const int head = blockIdx.x % a.l.kv_heads, split = blockIdx.x / a.l.kv_heads, i = blockIdx.z;
     const int row0 = a.step.row0[i], tokens = a.step.row0[i + 1] - row0, len = a.step.len[i], rows = tokens * a.group;
@@ -123,16 +125,14 @@ __global__ void __launch_bounds__(64 * W, D <= 128 ? 2 : 1) prefill_kernel(KvAtt
     // are looked up a tile ahead of the loads from them, those a tile ahead of their conversion.
     int page[N], scale_page;
     uint4 kraw[N], vraw[N];
-    // lane l of every wave: block l % 4's scale of K, log2 of V's and its reciprocal, of the next tile
-    float2 sraw;
-    float next_k, next_log, next_r;
+    float2 sraw = make_float2(0.0f, 0.0f);
     auto block_of = [&](int j) { return D % 64 == 0 ? __builtin_amdgcn_readfirstlane((tid + kThreads * j) / D) : (tid + kThreads * j) / D; };
     auto staged = [&](int j) { return 4 * D % kThreads == 0 || tid + kThreads * j < 4 * D; };
     auto look_up = [&](int tile) {
 #pragma unroll
         for (int j = 0; j < N; j++)
             if (staged(j)) page[j] = table[min(tile * 4 + block_of(j), last_block) >> a.l.block_shift];
-        scale_page = table[min(tile * 4 + (lane & 3), last_block) >> a.l.block_shift];
+        if (wave == 0) scale_page = table[min(tile * 4 + (lane & 3), last_block) >> a.l.block_shift];
     };
     auto fetch = [&](int tile) {
 #pragma unroll
@@ -145,30 +145,33 @@ __global__ void __launch_bounds__(64 * W, D <= 128 ? 2 : 1) prefill_kernel(KvAtt
             kraw[j] = *(const uint4 *)(k + at);
             vraw[j] = *(const uint4 *)(k + kKvBlock * D + at);
         }
+        if (wave != 0) return;
         const int blk = min(tile * 4 + (lane & 3), last_block), in = (head << a.l.block_shift) + (blk & in_mask);
         sraw = *(const float2 *)(a.l.base + (int64_t)max(scale_page, 0) * a.l.page_bytes + a.l.scales + 8 * in);
     };
-    auto stage = [&](int buf) {
-#pragma unroll
-        for (int j = 0; j < N; j++) {
-            if (!staged(j)) continue;
-            const int c = tid + kThreads * j;
-            uint32_t h[8];
-            codes_to_half(kraw[j].x, h), codes_to_half(kraw[j].y, h + 2), codes_to_half(kraw[j].z, h + 4), codes_to_half(kraw[j].w, h + 6);
-            uint4 *to = (uint4 *)&ks[buf][c / (D / 16)][c % (D / 16) * 16];
-            to[0] = make_uint4(h[0], h[1], h[2], h[3]);
-            to[1] = make_uint4(h[4], h[5], h[6], h[7]);
-            codes_to_half(vraw[j].x, h), codes_to_half(vraw[j].z, h + 2), codes_to_half(vraw[j].y, h + 4), codes_to_half(vraw[j].w, h + 6);
-            to = (uint4 *)&vs[buf][c % D][c / D * 16];
-            to[0] = make_uint4(h[0], h[1], h[2], h[3]);
-            to[1] = make_uint4(h[4], h[5], h[6], h[7]);
+    // a quarter of a pair of pieces: 8 codes of K (units 0, 1) or V (2, 3) to LDS
+    auto stage_unit = [&](int buf, int unit) {
+        const int j = unit / 4, c = tid + kThreads * j;
+        if (!staged(j)) return;
+        uint32_t h[4];
+        if (unit % 4 < 2) {
+            codes_to_half(unit % 2 ? kraw[j].z : kraw[j].x, h), codes_to_half(unit % 2 ? kraw[j].w : kraw[j].y, h + 2);
+            *(uint4 *)&ks[buf][c / (D / 16)][c % (D / 16) * 16 + unit % 2 * 8] = make_uint4(h[0], h[1], h[2], h[3]);
+        } else {
+            codes_to_half(unit % 2 ? vraw[j].y : vraw[j].x, h), codes_to_half(unit % 2 ? vraw[j].w : vraw[j].z, h + 2);
+            *(uint4 *)&vs[buf][c % D][c / D * 16 + unit % 2 * 8] = make_uint4(h[0], h[1], h[2], h[3]);
         }
+    };
+    auto stage_scales = [&](int buf) {
+        if (wave != 0) return;
         // what lies behind the end is hidden, and must only not be NaN
         const bool nan = sraw.y != sraw.y;
         const float sv = nan ? 1.0f : fmaxf(sraw.y, kKvMinScale);
-        next_k = sraw.x;
-        next_log = nan ? sraw.y : __builtin_amdgcn_logf(sv);
-        next_r = __builtin_amdgcn_rcpf(sv);
+        if (lane < 4) {
+            scales[buf][0][lane] = sraw.x;
+            scales[buf][1][lane] = nan ? sraw.y : __builtin_amdgcn_logf(sv);
+            scales[buf][2][lane] = __builtin_amdgcn_rcpf(sv);
+        }
     };
 
     // behind the last tile the last one again, which nobody uses: no branch inside the round
@@ -177,100 +180,134 @@ __global__ void __launch_bounds__(64 * W, D <= 128 ? 2 : 1) prefill_kernel(KvAtt
         look_up(tile_at(t0));
         fetch(tile_at(t0));
         look_up(tile_at(t0 + 1));
-        stage(0);
+        for (int unit = 0; unit < 4 * N; unit++) stage_unit(0, unit);
+        stage_scales(0);
         fetch(tile_at(t0 + 1));
         look_up(tile_at(t0 + 2));
     }
     __syncthreads();
-    for (int u = t0; u < t1; u++) {
-        const int buf = (u - t0) & 1, tile = vis.tile(u), j0 = tile * kKvTile;
-        const float scale_k = next_k, log_v = next_log, inv_v = next_r;
+    // One tile. The order is that of the source (the fences): each product goes with vector work that does not wait for it, the
+    // next tile's conversion beside the first half of the scores, their first half's scaling beside the second, and each
+    // block's weights beside the output products of the block before.
+    auto round = [&](int u, auto masked) {
+        constexpr int G = D / 16, E = D / 32, kAhead = 8, vAhead = 8;  // operands on their way from LDS
+        constexpr bool kMasked = decltype(masked)::value;
+        const int buf = (u - t0) & 1, j0 = vis.tile(u) * kKvTile;
         v16f s[2];
+        v8h k[kAhead], v[vAhead];
+        float t[2][16], top[2] = {-__builtin_inff(), -__builtin_inff()};
+        float f[4], c[4], rsv[4];
 #pragma unroll
         for (int r = 0; r < 16; r++) s[0][r] = s[1][r] = 0.0f;
-        v8h k[2][D / 16];
+        auto scores = [&](int sub, int st) {
 #pragma unroll
-        for (int st = 0; st < D / 16; st++)
+            for (int p = 0; p < P; p++) s[sub] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k[(sub * G + st) % kAhead], q[p][st], s[sub], 0, 0, 0);
+        };
+        auto scaled = [&](int sub, int r) {
+            float x = __builtin_fmaf(s[sub][r], f[2 * sub + r / 8], c[2 * sub + r / 8]);
+            if constexpr (kMasked) {
+                const int at = j0 + 32 * sub + 8 * (r / 4) + 4 * half + r % 4;
+                const bool seen = (at <= place) & ((at > place - a.window) | (at < a.sinks));
+                x = seen ? x : -__builtin_inff();
+            }
+            t[sub][r] = x;
+            top[sub] = fmaxf(top[sub], x);
+        };
+        auto read_k = [&](int n) {
+            if (n < 2 * G) k[n % kAhead] = *(const v8h *)&ks[buf][32 * (n / G) + col][16 * (n % G) + 8 * half];
+        };
+        auto read_v = [&](int n) {
+            if (n < 4 * E) v[n % vAhead] = *(const v8h *)&vs[buf][32 * (n % E) + col][16 * (n / E) + 8 * half];
+        };
+
 #pragma unroll
-            for (int sub = 0; sub < 2; sub++) k[sub][st] = *(const v8h *)&ks[buf][32 * sub + col][16 * st + 8 * half];
+        for (int n = 0; n < kAhead; n++) read_k(n);
+        FENCE();
 #pragma unroll
-        for (int st = 0; st < D / 16; st++)
+        for (int st = 0; st < G; st++) {
+            scores(0, st);
+            read_k(st + kAhead);
 #pragma unroll
-            for (int p = 0; p < P; p++)
-#pragma unroll
-                for (int sub = 0; sub < 2; sub++) s[sub] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k[sub][st], q[p][st], s[sub], 0, 0, 0);
-        stage(buf ^ 1);
-        fetch(tile_at(u + 2));
-        look_up(tile_at(u + 3));
-        // operands some products ahead, and the next tile's conversion between the products
-        __builtin_amdgcn_sched_group_barrier(0x100, 8, 0);
-#pragma unroll
-        for (int m = 0; m < P * D / 8; m++) {
-            __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
-            if (m % P == 0) __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
-            __builtin_amdgcn_sched_group_barrier(0x002, 5, 0);
+            for (int unit = st * 4 * N / G; unit < (st + 1) * 4 * N / G; unit++) stage_unit(buf ^ 1, unit);
+            FENCE();
         }
-        {
-            float t[2][16], rsv[4], top = -__builtin_inff();
+        stage_scales(buf ^ 1);
 #pragma unroll
-            for (int b = 0; b < 4; b++) {
-                const float f = qk * lane_of(scale_k, b), c = lane_of(log_v, b) + base;
-                rsv[b] = lane_of(inv_v, b);
+        for (int b = 0; b < 4; b++) f[b] = qk * scales[buf][0][b], c[b] = scales[buf][1][b] + base, rsv[b] = scales[buf][2][b];
+        fetch(tile_at(u + 2));
 #pragma unroll
-                for (int r = 0; r < 8; r++) t[b / 2][b % 2 * 8 + r] = __builtin_fmaf(s[b / 2][b % 2 * 8 + r], f, c);
+        for (int st = 0; st < G; st++) {
+            scores(1, st);
+            read_k(G + st + kAhead);
+#pragma unroll
+            for (int r = st * 16 / G; r < (st + 1) * 16 / G; r++) scaled(0, r);
+            if (st == G - 2) {
+#pragma unroll
+                for (int n = 0; n < vAhead; n++) read_v(n);
             }
-            if (!(j0 + kKvTile - 1 <= p_first && (j0 > p_last - a.window || j0 + kKvTile - 1 < a.sinks))) {
+            FENCE();
+        }
+        look_up(tile_at(u + 3));
 #pragma unroll
-                for (int r = 0; r < 32; r++) {
-                    const int at = j0 + 32 * (r / 16) + 8 * (r % 16 / 4) + 4 * half + r % 4;
-                    const bool seen = (at <= place) & ((at > place - a.window) | (at < a.sinks));
-                    t[r / 16][r % 16] = seen ? t[r / 16][r % 16] : -__builtin_inff();
-                }
+        for (int r = 0; r < 16; r++) scaled(1, r);
+        float most = fmaxf(top[0], top[1]);
+        if (__any(most > lim)) {
+            most = max32(most);
+            if (most > lim) {  // m moves up to the largest t: by `up` octaves
+                const bool first = !(m_at > -__builtin_inff());
+                const float up = first ? most : most - kUnit, shrink = first ? 0.0f : __builtin_amdgcn_exp2f(-up);
+                m_at = first ? up : m_at + up;
+                const float shift = kUnit - m_at - base;
+                base = kUnit - m_at;
+                lim = kUnit + kHead;
+                l_sum *= shrink;
+#pragma unroll
+                for (int r = 0; r < 32; r++) t[r / 16][r % 16] += shift;
+#pragma unroll
+                for (int d = 0; d < E; d++)
+#pragma unroll
+                    for (int r = 0; r < 16; r++) o[d][r] *= shrink;
             }
+        }
+        // The sum is of the weights before they are rounded: where a block's value scale is far below others', its weights may fall
+        // below what fp16 holds, and count in the sum all the same.
+        v8h w[2][P];
+        float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+        auto weights = [&](int b, int r) {
+            const float e0 = __builtin_amdgcn_exp2f(t[b / 2][b % 2 * 8 + r]), e1 = __builtin_amdgcn_exp2f(t[b / 2][b % 2 * 8 + r + 1]);
+            const v2h h = {(_Float16)e0, (_Float16)e1};
+            w[b % 2][0][r] = h[0], w[b % 2][0][r + 1] = h[1];
+            if constexpr (P == 2) w[b % 2][1][r] = (_Float16)(e0 - (float)h[0]), w[b % 2][1][r + 1] = (_Float16)(e1 - (float)h[1]);
+            sum[b] += e0 + e1;
+        };
 #pragma unroll
-            for (int r = 0; r < 32; r++) top = fmaxf(top, t[r / 16][r % 16]);
-            if (__any(top > lim)) {
-                top = max32(top);
-                if (top > lim) {  // m moves up to the largest t: by `up` octaves
-                    const bool first = !(m_at > -__builtin_inff());
-                    const float up = first ? top : top - kUnit, f = first ? 0.0f : __builtin_amdgcn_exp2f(-up);
-                    m_at = first ? up : m_at + up;
-                    const float shift = kUnit - m_at - base;
-                    base = kUnit - m_at;
-                    lim = kUnit + kHead;
-                    l_sum *= f;
+        for (int r = 0; r < 8; r += 2) weights(0, r);
+        FENCE();
 #pragma unroll
-                    for (int r = 0; r < 32; r++) t[r / 16][r % 16] += shift;
+        for (int b = 0; b < 4; b++) {
 #pragma unroll
-                    for (int d = 0; d < D / 32; d++)
+            for (int d = 0; d < E; d++) {
 #pragma unroll
-                        for (int r = 0; r < 16; r++) o[d][r] *= f;
+                for (int p = 0; p < P; p++) o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v[(b * E + d) % vAhead], w[b % 2][p], o[d], 0, 0, 0);
+                read_v(b * E + d + vAhead);
+                if (b < 3) {
+#pragma unroll
+                    for (int r = d * 4 / E; r < (d + 1) * 4 / E; r++) weights(b + 1, 2 * r);
                 }
+                FENCE();
             }
-#pragma unroll
-            for (int b = 0; b < 4; b++) {
-                // the sum is of the weights before they are rounded: where a block's value scale is far below others', its weights may
-                // fall below what fp16 holds, and count in the sum all the same
-                v8h w[P];
-                float sum = 0.0f;
-#pragma unroll
-                for (int r = 0; r < 8; r += 2) {
-                    const float e0 = __builtin_amdgcn_exp2f(t[b / 2][b % 2 * 8 + r]), e1 = __builtin_amdgcn_exp2f(t[b / 2][b % 2 * 8 + r + 1]);
-                    const v2h h = {(_Float16)e0, (_Float16)e1};
-                    w[0][r] = h[0], w[0][r + 1] = h[1];
-                    if constexpr (P == 2) w[1][r] = (_Float16)(e0 - (float)h[0]), w[1][r + 1] = (_Float16)(e1 - (float)h[1]);
-                    sum += e0 + e1;
-                }
-                l_sum = __builtin_fmaf(sum, rsv[b], l_sum);
-#pragma unroll
-                for (int d = 0; d < D / 32; d++) {
-                    const v8h v = *(const v8h *)&vs[buf][32 * d + col][16 * b + 8 * half];
-#pragma unroll
-                    for (int p = 0; p < P; p++) o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, w[p], o[d], 0, 0, 0);
-                }
-            }
+            l_sum = __builtin_fmaf(sum[b], rsv[b], l_sum);
         }
         __syncthreads();
+    };
+    // a tile of which every row of the wave sees every token
+    auto whole = [&](int u) {
+        const int j0 = vis.tile(u) * kKvTile, j1 = j0 + kKvTile - 1;
+        return j1 <= p_first && (j0 > p_last - a.window || j1 < a.sinks);
+    };
+    for (int u = t0; u < t1;) {
+        for (; u < t1 && whole(u); u++) round(u, std::false_type());
+        for (; u < t1 && !whole(u); u++) round(u, std::true_type());
     }
 
     const int r = w0 + col;
