@@ -105,6 +105,7 @@ struct KvAppend {
     void *q_out;
     int64_t kv_stride, q_stride;
     int32_t bf16, heads;  // heads: of q (0: no q)
+    int32_t heads_each;   // ... of a thread (the launcher's)
     int32_t max_blocks;   // workgroups (per kv head) for each sequence; 0: as many as it touches blocks (step.block0)
     int32_t items;        // ... of all sequences
     KvRope rope;

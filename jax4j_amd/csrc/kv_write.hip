@@ -26,16 +26,25 @@ __device__ __forceinline__ uint16_t to_bf16(float f) {
     return (uint16_t)((u + 0x7fffu + ((u >> 16) & 1)) >> 16);
 }
 
-// Cosine and sine of pair `pair` of row `row`, which is token `place` of its sequence.
-__device__ __forceinline__ void turn_of(const KvRope &r, int pair, int64_t row, int place, float *c, float *s) {
-    const int at = r.positions ? r.positions[(r.axes > 1 ? (int64_t)r.axis[pair] * r.rows : 0) + row] : place;
-    if (at < 0 || at >= r.table_rows) {  // no angle in the tables
-        *c = *s = __builtin_nanf("");
-        return;
+// Cosines and sines of pairs [pair, pair + V) of row `row`, which is token `place` of its sequence.
+template <int V>
+__device__ __forceinline__ void turns_of(const KvRope &r, int pair, int64_t row, int place, float *c, float *s) {
+    int at[V];
+    if (r.axes > 1) {
+#pragma unroll
+        for (int j = 0; j < V; j++) at[j] = r.positions[(int64_t)r.axis[pair + j] * r.rows + row];
+    } else {
+        const int one = r.positions ? r.positions[row] : place;
+#pragma unroll
+        for (int j = 0; j < V; j++) at[j] = one;
     }
-    const int64_t i = (int64_t)at * r.pairs + pair;
-    *c = r.cos[i];
-    *s = r.sin[i];
+#pragma unroll
+    for (int j = 0; j < V; j++) {
+        const bool there = at[j] >= 0 && at[j] < r.table_rows;  // else no angle in the tables
+        const int64_t i = (int64_t)(there ? at[j] : 0) * r.pairs + pair + j;
+        c[j] = there ? r.cos[i] : __builtin_nanf("");
+        s[j] = there ? r.sin[i] : __builtin_nanf("");
+    }
 }
 __device__ __forceinline__ void turn(float c, float s, float &u, float &w) {
 #pragma clang fp contract(off)
@@ -44,79 +53,86 @@ __device__ __forceinline__ void turn(float c, float s, float &u, float &w) {
     w = wc + us;
 }
 
-// V consecutive values.
+// V consecutive values, 4 of them or 8 bf16 in pieces of 16 (or 8) bytes.
 template <int V>
 __device__ __forceinline__ void load(const void *p, int64_t i, bool bf16, float *x) {
-    if constexpr (V == 4) {
-        if (bf16) {
-            const uint2 t = *(const uint2 *)((const uint16_t *)p + i);
-            x[0] = __builtin_bit_cast(float, t.x << 16);
-            x[1] = __builtin_bit_cast(float, t.x & 0xffff0000u);
-            x[2] = __builtin_bit_cast(float, t.y << 16);
-            x[3] = __builtin_bit_cast(float, t.y & 0xffff0000u);
-        } else {
-            const float4 t = *(const float4 *)((const float *)p + i);
-            x[0] = t.x, x[1] = t.y, x[2] = t.z, x[3] = t.w;
+    if constexpr (V == 1) {
+        x[0] = bf16 ? bf16_at(p, i) : ((const float *)p)[i];
+    } else if (bf16) {
+        uint32_t w[V / 2];
+        if constexpr (V == 8) *(uint4 *)w = *(const uint4 *)((const uint16_t *)p + i);
+        else *(uint2 *)w = *(const uint2 *)((const uint16_t *)p + i);
+#pragma unroll
+        for (int j = 0; j < V / 2; j++) {
+            x[2 * j] = __builtin_bit_cast(float, w[j] << 16);
+            x[2 * j + 1] = __builtin_bit_cast(float, w[j] & 0xffff0000u);
         }
     } else {
-        for (int j = 0; j < V; j++) x[j] = bf16 ? bf16_at(p, i + j) : ((const float *)p)[i + j];
+#pragma unroll
+        for (int j = 0; j < V; j += 4) *(float4 *)(x + j) = *(const float4 *)((const float *)p + i + j);
     }
 }
 template <int V>
 __device__ __forceinline__ void store(void *p, int64_t i, bool bf16, const float *x) {
-    if constexpr (V == 4) {
-        if (bf16) {
-            *(uint2 *)((uint16_t *)p + i) = make_uint2(to_bf16(x[0]) | (uint32_t)to_bf16(x[1]) << 16, to_bf16(x[2]) | (uint32_t)to_bf16(x[3]) << 16);
-        } else {
-            *(float4 *)((float *)p + i) = make_float4(x[0], x[1], x[2], x[3]);
-        }
+    if constexpr (V == 1) {
+        if (bf16) ((uint16_t *)p)[i] = to_bf16(x[0]);
+        else ((float *)p)[i] = x[0];
+    } else if (bf16) {
+        uint32_t w[V / 2];
+#pragma unroll
+        for (int j = 0; j < V / 2; j++) w[j] = to_bf16(x[2 * j]) | (uint32_t)to_bf16(x[2 * j + 1]) << 16;
+        if constexpr (V == 8) *(uint4 *)((uint16_t *)p + i) = *(const uint4 *)w;
+        else *(uint2 *)((uint16_t *)p + i) = *(const uint2 *)w;
     } else {
-        for (int j = 0; j < V; j++) {
-            if (bf16) ((uint16_t *)p)[i + j] = to_bf16(x[j]);
-            else ((float *)p)[i + j] = x[j];
-        }
+#pragma unroll
+        for (int j = 0; j < V; j += 4) *(float4 *)((float *)p + i + j) = *(const float4 *)(x + j);
     }
 }
 
-// 2 V channels of a row's heads [head0, head1): V pairs that are turned, or channels behind those, which are copied.
-// unit: which of the dim / (2 V). In place is fine: a thread reads what it writes.
-template <int V>
-__device__ __forceinline__ void rope_unit(const void *x, void *out, int64_t in_row, int64_t out_row, int head0, int head1, int dim, int unit,
-                                          bool bf16, const KvRope &r, int64_t row, int place) {
+// 2 V channels of H heads of a row from head0 on: V pairs that are turned, by the same cosines and sines for every head, or channels behind
+// those, which are copied. unit: which of the dim / (2 V). All loads go out before the first is used. In place is fine: a
+// thread reads what it writes.
+template <int V, int H>
+__device__ __forceinline__ void rope_unit(const void *x, void *out, int64_t in_row, int64_t out_row, int head0, int dim, int unit, bool bf16,
+                                          const KvRope &r, int64_t row, int place) {
     const int i = unit * V;
     const bool turned = i < r.pairs;
-    float c[V], s[V];
-    int at[2];
-    if (turned) {
-        for (int j = 0; j < V; j++) turn_of(r, i + j, row, place, &c[j], &s[j]);
-        at[0] = r.interleaved ? 2 * i : i;
-        at[1] = r.interleaved ? 2 * i + V : i + r.pairs;
-    } else {
-        at[0] = 2 * i;
-        at[1] = 2 * i + V;
+    const int at0 = turned && !r.interleaved ? i : 2 * i, at1 = turned && !r.interleaved ? i + r.pairs : 2 * i + V;
+    float a[H][2][V], c[V], s[V];
+#pragma unroll
+    for (int h = 0; h < H; h++) {
+        const int64_t from = in_row + (int64_t)(head0 + h) * dim;
+        load<V>(x, from + at0, bf16, a[h][0]);
+        load<V>(x, from + at1, bf16, a[h][1]);
     }
-    for (int h = head0; h < head1; h++) {
-        float a[2][V];
-        load<V>(x, in_row + (int64_t)h * dim + at[0], bf16, a[0]);
-        load<V>(x, in_row + (int64_t)h * dim + at[1], bf16, a[1]);
+    if (turned) turns_of<V>(r, i, row, place, c, s);
+#pragma unroll
+    for (int h = 0; h < H; h++) {
         if (turned) {
-            float *f = &a[0][0];
-            for (int j = 0; j < V; j++) turn(c[j], s[j], r.interleaved ? f[2 * j] : f[j], r.interleaved ? f[2 * j + 1] : f[V + j]);
+            float *f = &a[h][0][0];
+            if (r.interleaved) {
+#pragma unroll
+                for (int j = 0; j < V; j++) turn(c[j], s[j], f[2 * j], f[2 * j + 1]);
+            } else {
+#pragma unroll
+                for (int j = 0; j < V; j++) turn(c[j], s[j], f[j], f[V + j]);
+            }
         }
-        store<V>(out, out_row + (int64_t)h * dim + at[0], bf16, a[0]);
-        store<V>(out, out_row + (int64_t)h * dim + at[1], bf16, a[1]);
+        const int64_t to = out_row + (int64_t)(head0 + h) * dim;
+        store<V>(out, to + at0, bf16, a[h][0]);
+        store<V>(out, to + at1, bf16, a[h][1]);
     }
 }
 
-template <int V>
+template <int V, int H>
 __global__ void __launch_bounds__(256)
-rope_kernel(const void *x, void *out, int64_t rows, int heads, int heads_each, int dim, int64_t stride, int64_t out_stride, int bf16, KvRope r) {
-    const int units = dim / (2 * V), parts = (heads + heads_each - 1) / heads_each;
+rope_kernel(const void *x, void *out, int64_t rows, int heads, int dim, int64_t stride, int64_t out_stride, int bf16, KvRope r) {
+    const int units = dim / (2 * V), parts = heads / H;
     const int64_t t = (int64_t)blockIdx.x * 256 + threadIdx.x;
     const int64_t row = t / (units * parts);
     if (row >= rows) return;
-    const int rest = (int)(t - row * (units * parts)), part = rest / units, h0 = part * heads_each;
-    rope_unit<V>(x, out, row * stride, row * out_stride, h0, min(heads, h0 + heads_each), dim, rest - part * units, bf16 != 0, r, row, (int)row);
+    const int rest = (int)(t - row * (units * parts)), part = rest / units;
+    rope_unit<V, H>(x, out, row * stride, row * out_stride, part * H, dim, rest - part * units, bf16 != 0, r, row, (int)row);
 }
 
 __device__ __forceinline__ float block_max(float v, float *red) {
@@ -163,21 +179,24 @@ __global__ void __launch_bounds__(256) append_kernel(KvAppend a) {
     __shared__ float red[2][4];
     const int tid = threadIdx.x;
     const int items = a.items * a.l.kv_heads;
-    if ((int)blockIdx.x >= items) {  // 4 pairs of a query head a thread
-        const int units = D / 8;
-        const int64_t t = (int64_t)(blockIdx.x - items) * 256 + tid, row = t / (units * a.heads);
+    if ((int)blockIdx.x >= items) {  // 4 pairs of one or four query heads a thread
+        const int units = D / 8, parts = a.heads / a.heads_each;
+        const int64_t t = (int64_t)(blockIdx.x - items) * 256 + tid, row = t / (units * parts);
         if (row >= a.step.rows) return;
-        const int rest = (int)(t - row * (units * a.heads)), head = rest / units;
+        const int rest = (int)(t - row * (units * parts)), head = rest / units * a.heads_each, unit = rest % units;
         int place = 0;
         if (a.rope.pairs && !a.rope.positions) {
             const int i = sequence_of(a.step.row0, a.step.n, (int)row);
             place = a.step.len[i] - a.step.row0[i + 1] + (int)row;
         }
-        if (a.rope.pairs % 4 == 0) {
-            rope_unit<4>(a.q, a.q_out, row * a.q_stride, row * a.q_stride, head, head + 1, D, rest - head * units, a.bf16 != 0, a.rope, row, place);
-        } else {
+        const int64_t at = row * a.q_stride;
+        if (a.rope.pairs % 4 != 0) {
             for (int j = 0; j < 4; j++)
-                rope_unit<1>(a.q, a.q_out, row * a.q_stride, row * a.q_stride, head, head + 1, D, (rest - head * units) * 4 + j, a.bf16 != 0, a.rope, row, place);
+                for (int h = 0; h < a.heads_each; h++) rope_unit<1, 1>(a.q, a.q_out, at, at, head + h, D, unit * 4 + j, a.bf16 != 0, a.rope, row, place);
+        } else if (a.heads_each == 4) {
+            rope_unit<4, 4>(a.q, a.q_out, at, at, head, D, unit, a.bf16 != 0, a.rope, row, place);
+        } else {
+            rope_unit<4, 1>(a.q, a.q_out, at, at, head, D, unit, a.bf16 != 0, a.rope, row, place);
         }
         return;
     }
@@ -212,7 +231,7 @@ __global__ void __launch_bounds__(256) append_kernel(KvAppend a) {
         for (int t = tid; t < n * a.rope.pairs; t += 256) {
             const int r = t / a.rope.pairs, p = t - r * a.rope.pairs;
             float c, s;
-            turn_of(a.rope, p, row0 + lo - start + r, lo + r, &c, &s);
+            turns_of<1>(a.rope, p, row0 + lo - start + r, lo + r, &c, &s);
             float *u = a.rope.interleaved ? &xs[0][r][2 * p] : &xs[0][r][p], *w = a.rope.interleaved ? u + 1 : u + a.rope.pairs;
             turn(c, s, *u, *w);
         }
@@ -307,43 +326,48 @@ __global__ void __launch_bounds__(64) runs_kernel(KvRuns a) {
     for (int j = threadIdx.x; j < r.count; j += 64) a.words[r.at + j] = r.value + r.step * j;
 }
 
-// 16 KiB of a page per workgroup.
+// 16 KiB of a page per workgroup, four loads of a thread on their way before the first store.
 constexpr int kCopyBytes = 16384;
 __global__ void __launch_bounds__(256) copy_kernel(KvPairs a) {
     uint8_t *base = a.pool + (int64_t)blockIdx.z * a.layer_bytes;
     const uint4 *src = (const uint4 *)(base + (int64_t)a.src[blockIdx.y] * a.page_bytes);
     uint4 *dst = (uint4 *)(base + (int64_t)a.dst[blockIdx.y] * a.page_bytes);
-    const int n = (int)(a.page_bytes / 16), at = blockIdx.x * (kCopyBytes / 16) + threadIdx.x;
-    uint4 v[4];
-#pragma unroll
-    for (int j = 0; j < 4; j++)
-        if (at + 256 * j < n) v[j] = src[at + 256 * j];
-#pragma unroll
-    for (int j = 0; j < 4; j++)
-        if (at + 256 * j < n) dst[at + 256 * j] = v[j];
+    const int last = (int)(a.page_bytes / 16) - 1, at = blockIdx.x * (kCopyBytes / 16) + threadIdx.x;
+    // behind the page's end its last piece again
+    const int i0 = min(at, last), i1 = min(at + 256, last), i2 = min(at + 512, last), i3 = min(at + 768, last);
+    const uint4 v0 = src[i0], v1 = src[i1], v2 = src[i2], v3 = src[i3];
+    dst[i0] = v0;
+    dst[i1] = v1;
+    dst[i2] = v2;
+    dst[i3] = v3;
 }
 
 }  // namespace
 
 hipError_t launch_rope(const void *x, void *out, int64_t rows, int32_t heads, int32_t dim, int64_t stride, int64_t out_stride, bool bf16,
                        const KvRope &rope, hipStream_t s) {
-    const uintptr_t vec = bf16 ? 8 : 16, e = bf16 ? 2 : 4;
-    const bool wide = dim % 8 == 0 && rope.pairs % 4 == 0 && (uintptr_t)x % vec == 0 && (uintptr_t)out % vec == 0 && stride * e % vec == 0 &&
-                      out_stride * e % vec == 0;
-    const int v = wide ? 4 : 1;
-    // a thread's heads share its cosines and sines; few rows leave most of the chip to the heads
-    int each = 1;
-    while (each < 8 && rows * heads * (dim / (2 * v)) / (2 * each) >= 1 << 18) each *= 2;
-    const int64_t threads = rows * ((heads + each - 1) / each) * (dim / (2 * v));
-    const dim3 grid((unsigned)((threads + 255) / 256));
-    if (wide) rope_kernel<4><<<grid, 256, 0, s>>>(x, out, rows, heads, each, dim, stride, out_stride, bf16, rope);
-    else rope_kernel<1><<<grid, 256, 0, s>>>(x, out, rows, heads, each, dim, stride, out_stride, bf16, rope);
+    const uintptr_t e = bf16 ? 2 : 4;
+    const auto wide = [&](int v) {  // v values a load, of at most 16 bytes
+        const uintptr_t bytes = v * e < 16 ? v * e : 16;
+        return dim % (2 * v) == 0 && rope.pairs % v == 0 && (uintptr_t)x % bytes == 0 && (uintptr_t)out % bytes == 0 && stride * e % bytes == 0 &&
+               out_stride * e % bytes == 0;
+    };
+    const int v = bf16 && wide(8) ? 8 : wide(4) ? 4 : 1;
+    // four heads a thread share its cosines and sines, where that leaves threads for the chip
+    const int h = v > 1 && heads % 4 == 0 && rows * heads * (dim / (2 * v)) >= 1 << 18 ? 4 : 1;
+    const dim3 grid((unsigned)((rows * (heads / h) * (dim / (2 * v)) + 255) / 256));
+    const auto run = [&](auto kernel) { kernel<<<grid, 256, 0, s>>>(x, out, rows, heads, dim, stride, out_stride, bf16, rope); };
+    if (v == 8) h == 4 ? run(rope_kernel<8, 4>) : run(rope_kernel<8, 1>);
+    else if (v == 4) h == 4 ? run(rope_kernel<4, 4>) : run(rope_kernel<4, 1>);
+    else run(rope_kernel<1, 1>);
     return hipGetLastError();
 }
 
-hipError_t launch_kv_append(const KvAppend &a, hipStream_t s, hipEvent_t done) {
+hipError_t launch_kv_append(const KvAppend &args, hipStream_t s, hipEvent_t done) {
+    KvAppend a = args;
     const int64_t items = (int64_t)a.items * a.l.kv_heads;
-    const int64_t q = ((int64_t)a.step.rows * a.heads * (a.l.dim / 8) + 255) / 256;
+    a.heads_each = a.heads % 4 == 0 && (int64_t)a.step.rows * a.heads * (a.l.dim / 8) >= 1 << 18 ? 4 : 1;
+    const int64_t q = ((int64_t)a.step.rows * (a.heads / a.heads_each) * (a.l.dim / 8) + 255) / 256;
     const dim3 grid((unsigned)(items + q));
     switch (a.l.dim) {
     case 64: return launch_with_event(append_kernel<64>, grid, dim3(256), s, done, a);
