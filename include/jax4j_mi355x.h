@@ -342,7 +342,7 @@ typedef struct j4q_rope {
 } j4q_rope;
 
 /* Turns heads of x [rows][heads][head_dim] (J4Q_KIND_F32 or J4Q_KIND_BF16) into out, which is x itself or apart.
- * Strides: values from a row to the next, 0 for heads * head_dim. Any even head_dim. */
+ * Strides: values from a row to the next, 0 for heads * head_dim. Any even head_dim up to 2048. */
 int j4q_rope_into(const void *x, void *out, int type, int64_t rows, int32_t heads, int32_t head_dim, int64_t x_stride, int64_t out_stride,
                   const j4q_rope *rope, void *stream);
 

@@ -105,12 +105,13 @@ struct KvAppend {
     void *q_out;
     int64_t kv_stride, q_stride;
     int32_t bf16, heads;  // heads: of q (0: no q)
-    int32_t heads_each;   // ... of a thread (the launcher's)
+    int32_t rows_each, heads_each, wide;  // of a workgroup that turns queries (the launcher's)
     int32_t max_blocks;   // workgroups (per kv head) for each sequence; 0: as many as it touches blocks (step.block0)
     int32_t items;        // ... of all sequences
     KvRope rope;
 };
 hipError_t launch_kv_append(const KvAppend &a, hipStream_t s, hipEvent_t done);
+constexpr int kRopeMaxDim = 2048;
 hipError_t launch_rope(const void *x, void *out, int64_t rows, int32_t heads, int32_t dim, int64_t stride, int64_t out_stride, bool bf16,
                        const KvRope &rope, hipStream_t s);
 

@@ -673,7 +673,7 @@ int j4q_kv_append(j4q_kv kv, int32_t layer, const j4q_kv_append_args *args, void
     const int64_t even = (int64_t)k->step_most_blocks * (int64_t)k->step_seq.size();
     a.max_blocks = even <= 4ll * k->step_blocks ? k->step_most_blocks : 0;
     const int64_t items = a.max_blocks ? even : k->step_blocks;
-    if (items * k->c.kv_heads + ((int64_t)k->step_rows * a.heads * (k->c.head_dim / 8) + 255) / 256 > INT_MAX)
+    if (items * k->c.kv_heads + (int64_t)k->step_rows * a.heads > INT_MAX)
         return report_error(J4Q_EUNSUPPORTED, "kv append: %d tokens of %d heads in a call", k->step_rows, std::max(a.heads, k->c.kv_heads));
     a.items = (int32_t)items;
     if ((rc = abi::ready_locked())) return rc;
@@ -801,8 +801,8 @@ int j4q_rope_into(const void *x, void *out, int type, int64_t rows, int32_t head
                   const j4q_rope *rope, void *stream) {
     if (!x || !out || !rope) return report_error(J4Q_EINVAL, "rope_into: NULL argument");
     if (!dense_type(type)) return report_error(J4Q_EUNSUPPORTED, "rope_into: type %d (J4Q_KIND_F32 or J4Q_KIND_BF16)", type);
-    if (rows < 1 || rows > 1 << 30 || heads < 1 || heads > 65535 || head_dim < 2 || head_dim % 2 || head_dim > 65536)
-        return report_error(J4Q_EINVAL, "rope_into: %lld rows of %d heads of %d (an even number)", (long long)rows, heads, head_dim);
+    if (rows < 1 || rows > 1 << 30 || heads < 1 || heads > 65535 || head_dim < 2 || head_dim % 2 || head_dim > kRopeMaxDim)
+        return report_error(J4Q_EINVAL, "rope_into: %lld rows of %d heads of %d (an even number up to 2048)", (long long)rows, heads, head_dim);
     const int64_t width = (int64_t)heads * head_dim;
     if (!x_stride) x_stride = width;
     if (!out_stride) out_stride = width;
@@ -810,7 +810,7 @@ int j4q_rope_into(const void *x, void *out, int type, int64_t rows, int32_t head
         return report_error(J4Q_EINVAL, "rope_into: rows less than %lld values apart", (long long)width);
     const uintptr_t e = type == J4Q_KIND_BF16 ? 2 : 4;
     if (!aligned(x, e) || !aligned(out, e)) return report_error(J4Q_EINVAL, "rope_into: x and out must be aligned to their values");
-    if (rows > (INT64_MAX >> 20) / width || rows * width / 2 > (int64_t)INT_MAX * 256)
+    if (rows > (INT64_MAX >> 20) / width)
         return report_error(J4Q_EUNSUPPORTED, "rope_into: %lld rows of %lld values", (long long)rows, (long long)width);
     const uint8_t *a0 = (const uint8_t *)x, *b0 = (const uint8_t *)out;
     const uint8_t *a1 = a0 + ((rows - 1) * x_stride + width) * (int64_t)e, *b1 = b0 + ((rows - 1) * out_stride + width) * (int64_t)e;

@@ -14,6 +14,8 @@
 
 #include <float.h>
 
+#include <algorithm>
+
 namespace j4q {
 namespace {
 
@@ -26,25 +28,23 @@ __device__ __forceinline__ uint16_t to_bf16(float f) {
     return (uint16_t)((u + 0x7fffu + ((u >> 16) & 1)) >> 16);
 }
 
-// Cosines and sines of pairs [pair, pair + V) of row `row`, which is token `place` of its sequence.
-template <int V>
-__device__ __forceinline__ void turns_of(const KvRope &r, int pair, int64_t row, int place, float *c, float *s) {
-    int at[V];
-    if (r.axes > 1) {
-#pragma unroll
-        for (int j = 0; j < V; j++) at[j] = r.positions[(int64_t)r.axis[pair + j] * r.rows + row];
-    } else {
-        const int one = r.positions ? r.positions[row] : place;
-#pragma unroll
-        for (int j = 0; j < V; j++) at[j] = one;
+// The sequence i of n with first[i] <= at < first[i + 1].
+__device__ __forceinline__ int sequence_of(const int32_t *first, int n, int at) {
+    int lo = 0, hi = n - 1;
+    while (lo < hi) {
+        const int mid = (lo + hi + 1) / 2;
+        if (first[mid] <= at) lo = mid;
+        else hi = mid - 1;
     }
-#pragma unroll
-    for (int j = 0; j < V; j++) {
-        const bool there = at[j] >= 0 && at[j] < r.table_rows;  // else no angle in the tables
-        const int64_t i = (int64_t)(there ? at[j] : 0) * r.pairs + pair + j;
-        c[j] = there ? r.cos[i] : __builtin_nanf("");
-        s[j] = there ? r.sin[i] : __builtin_nanf("");
-    }
+    return lo;
+}
+
+// Cosine and sine of pair `pair` of row `row`, which is token `place` of its sequence.
+__device__ __forceinline__ float2 turn_of(const KvRope &r, int pair, int64_t row, int place) {
+    const int at = r.positions ? r.positions[(r.axes > 1 ? (int64_t)r.axis[pair] * r.rows : 0) + row] : place;
+    if (at < 0 || at >= r.table_rows) return make_float2(__builtin_nanf(""), __builtin_nanf(""));  // no angle in the tables
+    const int64_t i = (int64_t)at * r.pairs + pair;
+    return make_float2(r.cos[i], r.sin[i]);
 }
 __device__ __forceinline__ void turn(float c, float s, float &u, float &w) {
 #pragma clang fp contract(off)
@@ -89,50 +89,98 @@ __device__ __forceinline__ void store(void *p, int64_t i, bool bf16, const float
     }
 }
 
-// 2 V channels of H heads of a row from head0 on: V pairs that are turned, by the same cosines and sines for every head, or channels behind
-// those, which are copied. unit: which of the dim / (2 V). All loads go out before the first is used. In place is fine: a
-// thread reads what it writes.
-template <int V, int H>
-__device__ __forceinline__ void rope_unit(const void *x, void *out, int64_t in_row, int64_t out_row, int head0, int dim, int unit, bool bf16,
-                                          const KvRope &r, int64_t row, int place) {
-    const int i = unit * V;
-    const bool turned = i < r.pairs;
-    const int at0 = turned && !r.interleaved ? i : 2 * i, at1 = turned && !r.interleaved ? i + r.pairs : 2 * i + V;
-    float a[H][2][V], c[V], s[V];
+// A workgroup turns heads [head0, head0 + heads) of rows [row0, row0 + rows). An item is 2 V channels of a head: V pairs that are
+// turned, or channels behind those, which are copied. The rows' cosines and sines are looked up once, into LDS, whatever the number
+// of heads (looked up by every item they were three times as many loads as the values), while the items' values are on
+// their way. In place is fine: a thread reads what it writes.
+constexpr int kRopePairs = 1024;  // of a workgroup's rows together
+constexpr int kRopeItems = 4;     // of a thread
+static_assert(256 * kRopeItems >= kRopeMaxDim / 2, "a head is one workgroup's");
+struct RopeRows {
+    const void *x;
+    void *out;
+    int64_t stride, out_stride;  // of the rows
+    int32_t dim, bf16;
+};
+template <int V>
+__device__ __forceinline__ void rope_rows(const RopeRows &g, const KvRope &r, int64_t row0, int rows, int head0, int heads, const KvStep *step,
+                                          float2 *angles) {
+    const int units = g.dim / (2 * V), per_row = units * heads, count = rows * per_row;
+    float a[kRopeItems][2][V];
+    int row[kRopeItems], unit[kRopeItems], at0[kRopeItems], at1[kRopeItems];
+    int64_t head_at[kRopeItems];
 #pragma unroll
-    for (int h = 0; h < H; h++) {
-        const int64_t from = in_row + (int64_t)(head0 + h) * dim;
-        load<V>(x, from + at0, bf16, a[h][0]);
-        load<V>(x, from + at1, bf16, a[h][1]);
+    for (int j = 0; j < kRopeItems; j++) {
+        const int item = min((int)threadIdx.x + 256 * j, count - 1);
+        row[j] = item / per_row;
+        const int rest = item - row[j] * per_row, head = rest / units;
+        unit[j] = rest - head * units;
+        head_at[j] = (int64_t)(head0 + head) * g.dim;
+        const int i = unit[j] * V;
+        const bool halves = i < r.pairs && !r.interleaved;
+        at0[j] = halves ? i : 2 * i;
+        at1[j] = halves ? i + r.pairs : 2 * i + V;
+        if ((int)threadIdx.x + 256 * j < count) {
+            const int64_t from = (row0 + row[j]) * g.stride + head_at[j];
+            load<V>(g.x, from + at0[j], g.bf16, a[j][0]);
+            load<V>(g.x, from + at1[j], g.bf16, a[j][1]);
+        }
     }
-    if (turned) turns_of<V>(r, i, row, place, c, s);
+    if (r.pairs)
+        for (int t = threadIdx.x; t < rows * r.pairs; t += 256) {
+            const int k = t / r.pairs;
+            int place = 0;
+            if (step && !r.positions) {
+                const int i = sequence_of(step->row0, step->n, (int)row0 + k);
+                place = step->len[i] - step->row0[i + 1] + (int)row0 + k;
+            }
+            angles[t] = turn_of(r, t - k * r.pairs, row0 + k, place);
+        }
+    __syncthreads();
 #pragma unroll
-    for (int h = 0; h < H; h++) {
-        if (turned) {
-            float *f = &a[h][0][0];
+    for (int j = 0; j < kRopeItems; j++) {
+        if ((int)threadIdx.x + 256 * j >= count) break;
+        const int i = unit[j] * V;
+        if (i < r.pairs) {
+            float *f = &a[j][0][0];
+            const float2 *cs = angles + row[j] * r.pairs + i;
             if (r.interleaved) {
 #pragma unroll
-                for (int j = 0; j < V; j++) turn(c[j], s[j], f[2 * j], f[2 * j + 1]);
+                for (int e = 0; e < V; e++) turn(cs[e].x, cs[e].y, f[2 * e], f[2 * e + 1]);
             } else {
 #pragma unroll
-                for (int j = 0; j < V; j++) turn(c[j], s[j], f[j], f[V + j]);
+                for (int e = 0; e < V; e++) turn(cs[e].x, cs[e].y, f[e], f[V + e]);
             }
         }
-        const int64_t to = out_row + (int64_t)(head0 + h) * dim;
-        store<V>(out, to + at0, bf16, a[h][0]);
-        store<V>(out, to + at1, bf16, a[h][1]);
+        const int64_t to = (row0 + row[j]) * g.out_stride + head_at[j];
+        store<V>(g.out, to + at0[j], g.bf16, a[j][0]);
+        store<V>(g.out, to + at1[j], g.bf16, a[j][1]);
     }
 }
 
-template <int V, int H>
-__global__ void __launch_bounds__(256)
-rope_kernel(const void *x, void *out, int64_t rows, int heads, int dim, int64_t stride, int64_t out_stride, int bf16, KvRope r) {
-    const int units = dim / (2 * V), parts = heads / H;
-    const int64_t t = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    const int64_t row = t / (units * parts);
-    if (row >= rows) return;
-    const int rest = (int)(t - row * (units * parts)), part = rest / units;
-    rope_unit<V, H>(x, out, row * stride, row * out_stride, part * H, dim, rest - part * units, bf16 != 0, r, row, (int)row);
+// Rows and heads of a workgroup: about four items a thread where there are enough of them, else one.
+struct RopeGrid {
+    int rows, heads;
+    int64_t groups_x, groups_y;  // over rows, over heads
+};
+RopeGrid rope_grid(int64_t rows, int heads, int dim, int v, int pairs) {
+    const int units = dim / (2 * v);
+    const int64_t items = rows * heads * units;
+    const int most = 256 * kRopeItems, want = items >= (int64_t)most * 512 ? most : 256;
+    RopeGrid g;
+    g.heads = std::max(1, std::min(heads, std::max(want, units) / units));
+    g.rows = (int)std::max<int64_t>(1, std::min<int64_t>({rows, want / (units * g.heads), pairs ? kRopePairs / pairs : 1024}));
+    g.groups_x = (rows + g.rows - 1) / g.rows;
+    g.groups_y = (heads + g.heads - 1) / g.heads;
+    return g;
+}
+
+template <int V>
+__global__ void __launch_bounds__(256) rope_kernel(RopeRows g, int64_t rows, int heads, int rows_each, int heads_each, KvRope r) {
+    __shared__ float2 angles[kRopePairs];
+    const int64_t row0 = (int64_t)blockIdx.x * rows_each;
+    const int head0 = blockIdx.y * heads_each;
+    rope_rows<V>(g, r, row0, (int)min((int64_t)rows_each, rows - row0), head0, min(heads_each, heads - head0), nullptr, angles);
 }
 
 __device__ __forceinline__ float block_max(float v, float *red) {
@@ -160,17 +208,6 @@ __device__ __forceinline__ float next_scale(float amax, bool begun, float old, f
 __device__ __forceinline__ uint32_t code_of(float x, float r) { return (uint32_t)(int)rintf(x * r) & 0xffu; }
 __device__ __forceinline__ uint32_t shrink_of(uint32_t code, float f) { return (uint32_t)(int)rintf((float)(int8_t)code * f) & 0xffu; }
 
-// The sequence i of n with first[i] <= at < first[i + 1].
-__device__ __forceinline__ int sequence_of(const int32_t *first, int n, int at) {
-    int lo = 0, hi = n - 1;
-    while (lo < hi) {
-        const int mid = (lo + hi + 1) / 2;
-        if (first[mid] <= at) lo = mid;
-        else hi = mid - 1;
-    }
-    return lo;
-}
-
 // One block of 16 tokens of a kv head per workgroup, 256 threads; the workgroups behind them turn the queries.
 template <int D>
 __global__ void __launch_bounds__(256) append_kernel(KvAppend a) {
@@ -179,25 +216,14 @@ __global__ void __launch_bounds__(256) append_kernel(KvAppend a) {
     __shared__ float red[2][4];
     const int tid = threadIdx.x;
     const int items = a.items * a.l.kv_heads;
-    if ((int)blockIdx.x >= items) {  // 4 pairs of one or four query heads a thread
-        const int units = D / 8, parts = a.heads / a.heads_each;
-        const int64_t t = (int64_t)(blockIdx.x - items) * 256 + tid, row = t / (units * parts);
-        if (row >= a.step.rows) return;
-        const int rest = (int)(t - row * (units * parts)), head = rest / units * a.heads_each, unit = rest % units;
-        int place = 0;
-        if (a.rope.pairs && !a.rope.positions) {
-            const int i = sequence_of(a.step.row0, a.step.n, (int)row);
-            place = a.step.len[i] - a.step.row0[i + 1] + (int)row;
-        }
-        const int64_t at = row * a.q_stride;
-        if (a.rope.pairs % 4 != 0) {
-            for (int j = 0; j < 4; j++)
-                for (int h = 0; h < a.heads_each; h++) rope_unit<1, 1>(a.q, a.q_out, at, at, head + h, D, unit * 4 + j, a.bf16 != 0, a.rope, row, place);
-        } else if (a.heads_each == 4) {
-            rope_unit<4, 4>(a.q, a.q_out, at, at, head, D, unit, a.bf16 != 0, a.rope, row, place);
-        } else {
-            rope_unit<4, 1>(a.q, a.q_out, at, at, head, D, unit, a.bf16 != 0, a.rope, row, place);
-        }
+    if ((int)blockIdx.x >= items) {  // the queries
+        static_assert(sizeof xs >= kRopePairs * sizeof(float2));
+        const int at = blockIdx.x - items, rows = (a.step.rows + a.rows_each - 1) / a.rows_each;
+        const int row0 = at % rows * a.rows_each, head0 = at / rows * a.heads_each;
+        const RopeRows g{a.q, a.q_out, a.q_stride, a.q_stride, D, a.bf16};
+        const int n = min(a.rows_each, a.step.rows - row0), h = min(a.heads_each, a.heads - head0);
+        if (a.wide) rope_rows<4>(g, a.rope, row0, n, head0, h, &a.step, (float2 *)xs);
+        else rope_rows<1>(g, a.rope, row0, n, head0, h, &a.step, (float2 *)xs);
         return;
     }
     const int head = blockIdx.x % a.l.kv_heads;
@@ -230,10 +256,9 @@ __global__ void __launch_bounds__(256) append_kernel(KvAppend a) {
     if (a.rope.pairs) {
         for (int t = tid; t < n * a.rope.pairs; t += 256) {
             const int r = t / a.rope.pairs, p = t - r * a.rope.pairs;
-            float c, s;
-            turns_of<1>(a.rope, p, row0 + lo - start + r, lo + r, &c, &s);
+            const float2 cs = turn_of(a.rope, p, row0 + lo - start + r, lo + r);
             float *u = a.rope.interleaved ? &xs[0][r][2 * p] : &xs[0][r][p], *w = a.rope.interleaved ? u + 1 : u + a.rope.pairs;
-            turn(c, s, *u, *w);
+            turn(cs.x, cs.y, *u, *w);
         }
         __syncthreads();
     }
@@ -348,26 +373,33 @@ hipError_t launch_rope(const void *x, void *out, int64_t rows, int32_t heads, in
                        const KvRope &rope, hipStream_t s) {
     const uintptr_t e = bf16 ? 2 : 4;
     const auto wide = [&](int v) {  // v values a load, of at most 16 bytes
-        const uintptr_t bytes = v * e < 16 ? v * e : 16;
+        const uintptr_t bytes = v * e;
         return dim % (2 * v) == 0 && rope.pairs % v == 0 && (uintptr_t)x % bytes == 0 && (uintptr_t)out % bytes == 0 && stride * e % bytes == 0 &&
                out_stride * e % bytes == 0;
     };
     const int v = bf16 && wide(8) ? 8 : wide(4) ? 4 : 1;
-    // four heads a thread share its cosines and sines, where that leaves threads for the chip
-    const int h = v > 1 && heads % 4 == 0 && rows * heads * (dim / (2 * v)) >= 1 << 18 ? 4 : 1;
-    const dim3 grid((unsigned)((rows * (heads / h) * (dim / (2 * v)) + 255) / 256));
-    const auto run = [&](auto kernel) { kernel<<<grid, 256, 0, s>>>(x, out, rows, heads, dim, stride, out_stride, bf16, rope); };
-    if (v == 8) h == 4 ? run(rope_kernel<8, 4>) : run(rope_kernel<8, 1>);
-    else if (v == 4) h == 4 ? run(rope_kernel<4, 4>) : run(rope_kernel<4, 1>);
-    else run(rope_kernel<1, 1>);
+    const RopeGrid g = rope_grid(rows, heads, dim, v, rope.pairs);
+    if (g.groups_x > INT32_MAX || g.groups_y > 65535) return hipErrorInvalidValue;
+    const RopeRows r{x, out, stride, out_stride, dim, bf16};
+    const dim3 grid((unsigned)g.groups_x, (unsigned)g.groups_y);
+    if (v == 8) rope_kernel<8><<<grid, 256, 0, s>>>(r, rows, heads, g.rows, g.heads, rope);
+    else if (v == 4) rope_kernel<4><<<grid, 256, 0, s>>>(r, rows, heads, g.rows, g.heads, rope);
+    else rope_kernel<1><<<grid, 256, 0, s>>>(r, rows, heads, g.rows, g.heads, rope);
     return hipGetLastError();
 }
 
 hipError_t launch_kv_append(const KvAppend &args, hipStream_t s, hipEvent_t done) {
     KvAppend a = args;
     const int64_t items = (int64_t)a.items * a.l.kv_heads;
-    a.heads_each = a.heads % 4 == 0 && (int64_t)a.step.rows * a.heads * (a.l.dim / 8) >= 1 << 18 ? 4 : 1;
-    const int64_t q = ((int64_t)a.step.rows * (a.heads / a.heads_each) * (a.l.dim / 8) + 255) / 256;
+    int64_t q = 0;
+    if (a.heads) {
+        a.wide = a.rope.pairs % 4 == 0;
+        const RopeGrid g = rope_grid(a.step.rows, a.heads, a.l.dim, a.wide ? 4 : 1, a.rope.pairs);
+        a.rows_each = g.rows;
+        a.heads_each = g.heads;
+        q = g.groups_x * g.groups_y;
+    }
+    if (items + q > INT32_MAX) return hipErrorInvalidValue;
     const dim3 grid((unsigned)(items + q));
     switch (a.l.dim) {
     case 64: return launch_with_event(append_kernel<64>, grid, dim3(256), s, done, a);

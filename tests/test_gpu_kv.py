@@ -104,7 +104,8 @@ def model(backend):
 @pytest.mark.parametrize("kind", ["f32", "bf16"])
 @pytest.mark.parametrize("rows,heads,dim,rot,sections,interleaved", [
     (1, 1, 2, 2, None, False), (1, 40, 128, 128, None, True), (13, 3, 80, 80, (14, 13, 13), False), (7, 5, 96, 24, (4, 8), True),
-    (5, 3, 70, 14, (3, 4), False), (300, 9, 64, 64, (16, 8, 8), False), (2049, 33, 128, 64, None, True), (3, 2, 258, 256, None, False)])
+    (5, 3, 70, 14, (3, 4), False), (300, 9, 64, 64, (16, 8, 8), False), (2049, 33, 128, 64, None, True), (3, 2, 258, 256, None, False), (2, 3, 2048, 256, None, True),
+    (33, 1, 2046, 34, (17,), False), (70000, 1, 64, 64, None, False), (1, 700, 64, 32, None, True)])
 def test_rope_into(backend, kind, rows, heads, dim, rot, sections, interleaved):
     rng = np.random.default_rng(rows)
     cos, sin = R.tables(501, rot // 2)
