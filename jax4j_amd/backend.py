@@ -289,9 +289,10 @@ class Mi355xBackend:
                   out_stride: int = 0, stream: int = 0) -> None:
         """Rotary positions (jax4j_amd.Rope, with its positions) on x [rows, heads, head_dim], F32 or BF16, into out (x itself
         or apart), stream-ordered. Strides in values, 0: dense."""
-        kind = {DType.F32: N.KIND_F32, DType.BF16: N.KIND_BF16}.get(dtype, 0)
-        x, out, s = _addresses(x_ptr, out_ptr, stream)
-        check(self._lib().j4q_rope_into(x, out, kind, rows, heads, head_dim, x_stride, out_stride, C.byref(rope.args), s), "rope_into")
+        kind = N.KIND_F32 if dtype is DType.F32 else N.KIND_BF16 if dtype is DType.BF16 else 0
+        if not type(x_ptr) is type(out_ptr) is type(stream) is int:
+            x_ptr, out_ptr, stream = _addresses(x_ptr, out_ptr, stream)
+        check(self._lib().j4q_rope_into(x_ptr, out_ptr, kind, rows, heads, head_dim, x_stride, out_stride, rope.ref, stream), "rope_into")
 
     def decode_plan(self, layers, head, batch: int, io: dict) -> "DecodePlan":
         """The quantized matmuls of a decode step as one replayable plan (engine-local).

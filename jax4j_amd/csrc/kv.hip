@@ -117,8 +117,9 @@ int get(j4q_kv h, const char *op, Kv **out) {
 
 bool aligned(const void *p, uintptr_t a) { return ((uintptr_t)p & (a - 1)) == 0; }
 
-// One call's launches on its stream: behind the cache's last call where that was on another stream. Under capture the
-// caller orders the graph's launches.
+// One call's launches on its stream: behind the cache's last call where that was on another stream. That one's last launch has
+// completed k.done, but on the engine stream, which outlives the cache, where the event is recorded only when a call leaves it
+// (a launch with an event takes the host 1 to 2 us more). Under capture the caller orders the graph's launches.
 struct Call {
     Kv &k;
     hipStream_t s;
@@ -127,12 +128,15 @@ struct Call {
 
     Call(Kv &kv, void *stream) : k(kv), s(stream ? (hipStream_t)stream : abi::stream()) {
         captured = capturing(s);
-        if (!captured && k.used && k.last != s) e = hipStreamWaitEvent(s, k.done, 0);
+        if (captured || !k.used || k.last == s) return;
+        if (k.last == abi::stream()) e = hipEventRecord(k.done, k.last);
+        if (e == hipSuccess) e = hipStreamWaitEvent(s, k.done, 0);
     }
-    hipEvent_t event(bool last) const { return last && !captured ? k.done : nullptr; }
+    bool recorded() const { return !captured && s != abi::stream(); }
+    hipEvent_t event(bool last) const { return last && recorded() ? k.done : nullptr; }
     int end(const char *op) {
+        if (e != hipSuccess && recorded()) (void)hipEventRecord(k.done, s);
         if (!captured) {
-            if (e != hipSuccess) (void)hipEventRecord(k.done, s);
             k.last = s;
             k.used = true;
         }
@@ -325,7 +329,7 @@ int j4q_kv_create(const j4q_kv_config *config, j4q_kv *out) {
         r.words = k->words;
         r.n = 1;
         r.run[0] = KvRun{0, -1, 0, (int32_t)k->word_count()};
-        e = launch_kv_runs(r, abi::stream(), k->done);
+        e = launch_kv_runs(r, abi::stream(), nullptr);
     }
     if (e != hipSuccess) {
         (void)hipGetLastError();

@@ -25,13 +25,12 @@ from . import _native as N
 from .backend import Mi355xBackend, _addresses, check
 from .tensor import DType, IllegalArgumentException
 
-_KINDS = {DType.F32: N.KIND_F32, DType.BF16: N.KIND_BF16}
-
-
 def _kind(dtype: DType) -> int:
-    if dtype not in _KINDS:
-        raise IllegalArgumentException(f"values are F32 or BF16, not {dtype}")
-    return _KINDS[dtype]
+    if dtype is DType.F32:
+        return N.KIND_F32
+    if dtype is DType.BF16:
+        return N.KIND_BF16
+    raise IllegalArgumentException(f"values are F32 or BF16, not {dtype}")
 
 
 def _ints(values, code="i") -> array:
@@ -82,6 +81,7 @@ class Rope:
         self._axes = axes
         cos, sin, at = _addresses(cos_ptr, sin_ptr, positions)
         self.args = N.RopeArgs(cos, sin, rows, dims, int(interleaved), at or None, C.cast(axes, C.c_void_p) if axes else None)
+        self.ref = C.pointer(self.args)
 
 
 class KvCache:
@@ -166,21 +166,23 @@ class KvCache:
                q_out_ptr: int = 0, heads: int = 0, q_stride: int = 0, stream: int = 0) -> None:
         """Store the step's keys and values, [rows, kv_heads, head_dim] each, keys turned by ``rope``; with ``q_ptr`` the
         queries [rows, heads, head_dim] too are turned, into ``q_out_ptr`` (0: in place). Strides are in values, 0: dense."""
-        k, v, q, qo, s = _addresses(k_ptr, v_ptr, q_ptr, q_out_ptr or q_ptr, stream)
-        a = N.KvAppendArgs(k, v, stride, _kind(dtype), _int32(heads), q or None, qo or None, q_stride, C.pointer(rope.args) if rope else None)
-        check(self._be._lib().j4q_kv_append(self.handle, _int32(layer), C.byref(a), s), "kv append")
+        if not type(k_ptr) is type(v_ptr) is type(q_ptr) is type(q_out_ptr) is type(stream) is int:
+            k_ptr, v_ptr, q_ptr, q_out_ptr, stream = _addresses(k_ptr, v_ptr, q_ptr, q_out_ptr, stream)
+        a = N.KvAppendArgs(k_ptr, v_ptr, stride, _kind(dtype), _int32(heads), q_ptr, q_out_ptr or q_ptr, q_stride, rope.ref if rope else None)
+        check(self._be._lib().j4q_kv_append(self.handle, _int32(layer), C.byref(a), stream), "kv append")
 
     def attend(self, layer: int, q_ptr: int, out_ptr: int, heads: int, *, q_type: DType = DType.F32, out_type: DType = DType.F32, q_stride: int = 0,
                out_stride: int = 0, window: int = 0, sinks: int = 0, scale: float = 0.0, stream: int = 0) -> None:
         """Attention of the step's queries [rows, heads, head_dim] to the tokens j <= p of their sequence, p their own place,
         with j > p - window (0: no window) or j < sinks. ``scale`` 0: 1 / sqrt(head_dim)."""
-        q, o, s = _addresses(q_ptr, out_ptr, stream)
-        a = N.KvAttendArgs(q, o, q_stride, out_stride, _kind(q_type), _kind(out_type), _int32(heads), _int32(window), _int32(sinks), scale)
-        check(self._be._lib().j4q_kv_attend(self.handle, _int32(layer), C.byref(a), s), "kv attend")
+        if not type(q_ptr) is type(out_ptr) is type(stream) is int:
+            q_ptr, out_ptr, stream = _addresses(q_ptr, out_ptr, stream)
+        a = N.KvAttendArgs(q_ptr, out_ptr, q_stride, out_stride, _kind(q_type), _kind(out_type), _int32(heads), _int32(window), _int32(sinks), scale)
+        check(self._be._lib().j4q_kv_attend(self.handle, _int32(layer), C.byref(a), stream), "kv attend")
 
     def read(self, layer: int, seqs, first, count: int, k_ptr: int, v_ptr: int, stream: int = 0) -> None:
         """Tokens [first[i], first[i] + count) of seqs[i] as fp32 [n, count, kv_heads, head_dim]; zeros where there is none."""
         s, f = _ints(seqs), _ints(first, "q")
         _equal(s, f, "first tokens")
         k, v, st = _addresses(k_ptr, v_ptr, stream)
-        check(self._be._lib().j4q_kv_read(self.handle, _int32(layer), _at(s), _at(f), index(count), len(s), k or None, v or None, st), "kv read")
+        check(self._be._lib().j4q_kv_read(self.handle, _int32(layer), _at(s), _at(f), index(count), len(s), k, v, st), "kv read")
