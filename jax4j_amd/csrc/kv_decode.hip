@@ -185,8 +185,10 @@ __global__ void __launch_bounds__(64 * waves_of(D), waves_of(D) / 4) decode_kern
     float weight[M];
     float q_scale;
     {
+        // a column that is no row's has the first row's
         const int64_t at = (int64_t)(row0 + (real ? rr / a.group : 0)) * a.q_stride + (head * a.group + (real ? rr % a.group : 0)) * D;
-        float x[S][16], most = 0.0f;
+        float x[S][16], most = 0.0f, finite = 0.0f;
+#pragma unroll
         for (int s = 0; s < S; s++) {
             const int d = s * 64 + quad * 16;
             if (d < D) {
@@ -194,24 +196,25 @@ __global__ void __launch_bounds__(64 * waves_of(D), waves_of(D) / 4) decode_kern
             } else {
                 for (int j = 0; j < 16; j++) x[s][j] = 0.0f;
             }
+#pragma unroll
             for (int j = 0; j < 16; j++) {
-                if (!real) x[s][j] = 0.0f;
-                const float m = fabsf(x[s][j]);
-                most = fmaxf(most, m < __builtin_inff() ? m : __builtin_inff());
+                most = fmaxf(most, fabsf(x[s][j]));
+                finite = __builtin_fmaf(x[s][j], 0.0f, finite);  // else NaN
             }
         }
         most = max_column(most);
+        finite = sum_column(finite);
         // at least 2^-90, so that its reciprocal is finite
         const float unit = fmaxf(most, 0x1p-90f) * 0x1p-30f, inv = 1.0f / unit;
-        q_scale = most < __builtin_inff() ? unit * a.scale : __builtin_nanf("");
+        q_scale = unit * a.scale + finite;
         for (int m = 0; m < M; m++) {
             const uint32_t digit = (16 / R) * m + col / R;
             const uint32_t low = digit | (digit + 4) << 8 | 0x0c0c0000u, high = 0x0c0cu | digit << 16 | (digit + 4) << 24;
             weight[m] = __builtin_bit_cast(float, (127 + 8 * digit) << 23);
             for (int s = 0; s < S; s++)
                 for (int j = 0; j < 4; j++)
-                    qd[m][s][j] = pick(digits_of((int)rintf(x[s][4 * j] * inv)), digits_of((int)rintf(x[s][4 * j + 1] * inv)),
-                                       digits_of((int)rintf(x[s][4 * j + 2] * inv)), digits_of((int)rintf(x[s][4 * j + 3] * inv)), low, high);
+                    qd[m][s][j] = pick(digits_of((int)(x[s][4 * j] * inv)), digits_of((int)(x[s][4 * j + 1] * inv)),
+                                       digits_of((int)(x[s][4 * j + 2] * inv)), digits_of((int)(x[s][4 * j + 3] * inv)), low, high);
         }
     }
 
@@ -269,16 +272,18 @@ __global__ void __launch_bounds__(64 * waves_of(D), waves_of(D) / 4) decode_kern
             const float to = fmaxf(top > m_at + kHead ? top : m_at, m_at), f = to > m_at ? __builtin_amdgcn_exp2f(m_at - to) : 1.0f;
             m_at = to;
             l_sum *= f;
+            if (u >= t0 + kWaves) {  // before, there is nothing to scale
 #pragma unroll
-            for (int tt = 0; tt < T; tt++)
+                for (int tt = 0; tt < T; tt++)
 #pragma unroll
-                for (int j = 0; j < 4; j++) {
-                    float x = (float)acc[0][tt][j] * weight[0];
-                    if constexpr (M > 1) x = __builtin_fmaf((float)acc[1][tt][j], weight[1], x);
-                    o[tt][j] = (o[tt][j] + x) * f;
+                    for (int j = 0; j < 4; j++) {
+                        float x = (float)acc[0][tt][j] * weight[0];
+                        if constexpr (M > 1) x = __builtin_fmaf((float)acc[1][tt][j], weight[1], x);
+                        o[tt][j] = (o[tt][j] + x) * f;
 #pragma unroll
-                    for (int m = 0; m < M; m++) acc[m][tt][j] = 0;
-                }
+                        for (int m = 0; m < M; m++) acc[m][tt][j] = 0;
+                    }
+            }
         }
         const float base = m_at > -__builtin_inff() ? kUnit - m_at : 0.0f;
         uint32_t w[16];
