@@ -68,7 +68,7 @@ __global__ void __launch_bounds__(64 * W, D <= 128 ? 2 : 1) prefill_kernel(KvAtt
     __shared__ __align__(16) _Float16 ks[2][kKvTile][KP];
     __shared__ __align__(16) _Float16 vs[2][D][VP];
     __shared__ __align__(16) float scales[2][3][4];        // K scale, log2 of V's, its reciprocal
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, col = lane & 31, half = lane >> 5;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), col = lane & 31, half = lane >> 5;
     const int head = blockIdx.x % a.l.kv_heads, split = blockIdx.x / a.l.kv_heads, i = blockIdx.z;
     const int row0 = a.step.row0[i], tokens = a.step.row0[i + 1] - row0, len = a.step.len[i], rows = tokens * a.group;
     const int tile_count = (rows + kRows - 1) / kRows;
