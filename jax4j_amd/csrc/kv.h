@@ -64,6 +64,7 @@ struct KvAttend {
     int32_t window, sinks;         // window: INT32_MAX for none
     float scale;                   // of the scores, times log2(e)
     int32_t row_tile;              // rows of a workgroup
+    int32_t rows_from, rows_to;    // rows (tokens x group) of the sequences that the launch serves
     int32_t max_rows;              // most rows (tokens x group) of a sequence and kv head in the step
     int32_t splits;                // ranges of the visible tokens, one workgroup each
     int32_t split_tiles;           // tiles of a range, but for the last one, that takes what is left
@@ -93,6 +94,7 @@ __host__ __device__ inline int kv_ranges(int tiles, const KvAttend &a) {
     return n < a.splits ? n : a.splits;
 }
 
+constexpr int kKvSplits = 256;  // most ranges of a row's tokens
 hipError_t launch_kv_decode(const KvAttend &a, hipStream_t s, hipEvent_t done);
 hipError_t launch_kv_prefill(const KvAttend &a, hipStream_t s, hipEvent_t done);
 // The parts of every row in one: out = sum of part * 2^(max - largest) / the same of the sums.

@@ -287,6 +287,82 @@ int check_stride(const char *op, const char *what, const void *p, int type, int6
     return J4Q_OK;
 }
 
+// Tiles of 64 tokens that the workgroups of a call's sequences walk for one kv head: all of them, the longest walk's, and how many
+// workgroups and rows there are.
+struct Walks {
+    int64_t tiles = 0, most = 0, groups = 0, rows = 0;
+};
+Walks walks_of(const Kv &k, const KvAttend &a) {
+    Walks w;
+    for (size_t i = 0; i < k.step_seq.size(); i++) {
+        const int64_t before = k.seqs[(size_t)k.step_seq[i]].len - k.step_tokens[i], rows = (int64_t)k.step_tokens[i] * a.group;
+        if (rows < a.rows_from || rows > a.rows_to) continue;
+        w.rows += rows;
+        w.groups += (rows + a.row_tile - 1) / a.row_tile;
+        for (int64_t r = 0; r < rows; r += a.row_tile) {
+            const int64_t last = std::min(rows, r + a.row_tile) - 1;
+            const int64_t count = kv_tiles((int)(before + r / a.group), (int)(before + last / a.group), a.window, a.sinks).count();
+            w.tiles += count;
+            w.most = std::max(w.most, count);
+        }
+    }
+    return w;
+}
+// Cuts walks of up to `most` tiles into ranges of split_tiles, as far as there is room for their parts. A graph's later runs may
+// have longer ones.
+void set_splits(const Kv &k, bool captured, int64_t most, int64_t split_tiles, KvAttend *a) {
+    const int64_t room = kPartRows / ((int64_t)k.step_seq.size() * k.c.kv_heads * a->max_rows);
+    const int64_t longest = captured && most > 0 ? std::max(most, ((int64_t)k.c.sequence_pages * k.c.page_tokens + kKvTile - 1) / kKvTile) : most;
+    a->splits = (int32_t)std::max<int64_t>(1, std::min<int64_t>({(longest + split_tiles - 1) / split_tiles, room, kKvSplits}));
+    a->split_tiles = (int32_t)std::max(split_tiles, (most + a->splits - 1) / a->splits);
+}
+
+// Few rows: one workgroup of a CU's registers each, so ranges where the rows alone leave CUs idle. Joining them costs 4 to 5 us, a
+// round of the 8 waves over a tile each 2.4 (one request, 8 kv heads of 128: 16 tiles 11.3 us in one range, 13.2 in two; 32
+// tiles 16.2 and, in four, 13.7; 128 tiles 46 and, in sixteen, 14.1).
+void split_few(const Kv &k, bool captured, KvAttend *a) {
+    constexpr int64_t kFilled = 256, kAlone = 16, kLeast = 8;
+    a->row_tile = a->max_rows <= 4 ? 4 : 8;
+    const Walks w = walks_of(k, *a);
+    set_splits(k, captured, w.most, std::max(w.most <= kAlone ? kAlone : kLeast, (w.tiles * k.c.kv_heads + kFilled - 1) / kFilled), a);
+}
+
+// Many rows: workgroups of 256, whose conversion of a tile serves the most rows, or of 128, two to a CU, which fill the chip sooner:
+// 8 kv heads of 128 with 4 query heads each, a chunk of 512 tokens behind 3584 (64 workgroups of 256) 54 us and with 128 58, the
+// last 64 tokens of 4096 (8) 32 and 27; a prompt of 2048, whose workgroups walk 1 to 32 tiles (256) 68 and 62, one of 8192
+// (1024) 632 and 670.
+// Ranges by what they are estimated to cost: a tile takes a workgroup 1.3 us (of 128 rows), the chip's throughput has a floor,
+// and parts are written and read back, behind a launch. (The last 64 tokens of 4096, one kv head: 33.4 us in 4 ranges, 17.8 in 16.)
+void split_many(const Kv &k, bool captured, KvAttend *a) {
+    const double heads = k.c.kv_heads, width = k.c.head_dim / 128.0;
+    a->row_tile = 256;
+    int64_t groups = 0;
+    for (size_t i = 0; i < k.step_seq.size(); i++) {
+        const int64_t rows = (int64_t)k.step_tokens[i] * a->group;
+        if (rows >= a->rows_from && rows <= a->rows_to) groups += (rows + 255) / 256;
+    }
+    a->splits = 1;
+    a->split_tiles = INT_MAX / 2;
+    if (k.c.head_dim <= 128 && groups * k.c.kv_heads >= 448) return;
+    Walks w = walks_of(k, *a);
+    if (k.c.head_dim > 128 || groups * k.c.kv_heads < 64 || 4 * w.tiles < 3 * w.most * w.groups) {
+        a->row_tile = 128;
+        if (groups * k.c.kv_heads >= 448) return;
+        w = walks_of(k, *a);
+    }
+    const double tile_us = (a->row_tile == 256 ? 1.55 : 1.3) * width, all_us = (a->row_tile == 256 ? 1.9 : 0.9) * width * (double)w.tiles * heads / 256;
+    double best = 0;
+    int64_t ranges = 1;
+    for (int64_t s = 1; s <= 64 && s <= w.most; s++) {
+        const double walk = tile_us * (double)((w.most + s - 1) / s);
+        const double join = s == 1 ? 0 : (s > 16 ? 8 : 4) + (double)w.rows * heads * (double)s * 4 * k.c.head_dim / 4.5e6;
+        const double us = std::max(walk, all_us) + join;
+        if (s == 1 || us < best) best = us, ranges = s;
+    }
+    set_splits(k, captured, w.most, (w.most + ranges - 1) / ranges, a);
+    if (ranges == 1 && !captured) a->splits = 1;
+}
+
 }  // namespace
 }  // namespace j4q
 
@@ -713,17 +789,18 @@ int j4q_kv_attend(j4q_kv kv, int32_t layer, const j4q_kv_attend_args *args, void
     a.sinks = g.sinks;
     a.group = g.heads / k->c.kv_heads;
     const int n = (int)k->step_seq.size();
-    int64_t most_rows = 0;
+    int64_t few = 0, many = 0;  // most rows of a sequence and kv head that either kernel has
     for (int i = 0; i < n; i++) {
         const Seq &q = k->seqs[(size_t)k->step_seq[(size_t)i]];
-        const int64_t first = q.len - k->step_tokens[(size_t)i];
+        const int64_t first = q.len - k->step_tokens[(size_t)i], rows = (int64_t)k->step_tokens[(size_t)i] * a.group;
         if (q.gone1 > q.gone0 && (q.gone1 - 1 > first - a.window || q.gone0 < a.sinks))
             return report_error(J4Q_EINVAL, "kv attend: tokens [%lld, %lld) of sequence %d are evicted, and the mask shows some of them",
                                 (long long)q.gone0, (long long)q.gone1, k->step_seq[(size_t)i]);
-        most_rows = std::max(most_rows, (int64_t)k->step_tokens[(size_t)i] * a.group);
+        int64_t &most = rows > kFewRows ? many : few;
+        most = std::max(most, rows);
     }
-    if (most_rows > 1 << 30) return report_error(J4Q_EUNSUPPORTED, "kv attend: %lld query rows of a kv head", (long long)most_rows);
-    a.max_rows = (int32_t)most_rows;
+    if (many > 1 << 22 || n > 65535 || (few && (int64_t)k->c.kv_heads * ((few + 3) / 4) > 65535))
+        return report_error(J4Q_EUNSUPPORTED, "kv attend: %lld query rows of %d kv heads in %d sequences", (long long)std::max(few, many), k->c.kv_heads, n);
     a.l = k->layer(layer);
     a.step = k->step();
     a.q = g.q;
@@ -731,36 +808,21 @@ int j4q_kv_attend(j4q_kv kv, int32_t layer, const j4q_kv_attend_args *args, void
     a.q_bf16 = g.q_type == J4Q_KIND_BF16;
     a.out_bf16 = g.out_type == J4Q_KIND_BF16;
     a.scale = (g.scale > 0.0f ? g.scale : 1.0f / sqrtf((float)k->c.head_dim)) * 1.4426950408889634f;
-    const bool many = a.max_rows > kFewRows;
-    a.row_tile = many ? k->c.head_dim <= 128 ? 256 : 128 : a.max_rows <= 4 ? 4 : 8;
-    if ((rc = abi::ready_locked())) return rc;
-    Call c(*k, stream);
-    // Ranges of the tokens where rows alone leave CUs idle: one workgroup of a CU's registers each. Joining them costs 4 to 5 us, a
-    // round of the 8 waves over a tile each 2.4 (one request, 8 kv heads of 128: 16 tiles 11.3 us in one range, 13.2 in two; 32
-    // tiles 16.2 and, in four, 13.7; 128 tiles 46 and, in sixteen, 14.1).
-    const int64_t filled = many ? 512 : 256, alone = many ? 4 : 16, least = many ? 4 : 8;
-    int64_t tiles = 0, most = 0;
-    if ((int64_t)k->step_rows * a.group / a.row_tile * k->c.kv_heads < filled)
-        for (int i = 0; i < n; i++) {
-            const int64_t before = k->seqs[(size_t)k->step_seq[(size_t)i]].len - k->step_tokens[(size_t)i], rows = (int64_t)k->step_tokens[(size_t)i] * a.group;
-            for (int64_t r = 0; r < rows; r += a.row_tile) {
-                const int64_t last = std::min(rows, r + a.row_tile) - 1;
-                const int64_t count = kv_tiles((int)(before + r / a.group), (int)(before + last / a.group), a.window, a.sinks).count();
-                tiles += count;
-                most = std::max(most, count);
-            }
-        }
-    a.split_tiles = (int32_t)std::max<int64_t>(most <= alone ? alone : least, (tiles * k->c.kv_heads + filled - 1) / filled);
-    if (c.captured && most) most = ((int64_t)k->c.sequence_pages * k->c.page_tokens + kKvTile - 1) / kKvTile;  // the graph's later runs
-    const int64_t room = kPartRows / ((int64_t)n * k->c.kv_heads * a.max_rows);
-    a.splits = (int32_t)std::max<int64_t>(1, std::min<int64_t>({(most + a.split_tiles - 1) / a.split_tiles, room, 256}));
-    if (a.splits > 1 && (most + a.split_tiles - 1) / a.split_tiles > a.splits && !c.captured)
-        a.split_tiles = (int32_t)((most + a.splits - 1) / a.splits);
     a.part = k->part;
     a.part_ml = k->part + kPartRows * k->c.head_dim;
-    if ((int64_t)k->c.kv_heads * ((a.max_rows + a.row_tile - 1) / a.row_tile) > 65535 || n > 65535 || a.max_rows > INT_MAX / 2)
-        return report_error(J4Q_EUNSUPPORTED, "kv attend: %d query rows of %d kv heads in %d sequences", a.max_rows, k->c.kv_heads, n);
-    if (c.e == hipSuccess) c.e = many ? launch_kv_prefill(a, c.s, c.event(true)) : launch_kv_decode(a, c.s, c.event(true));
+    if ((rc = abi::ready_locked())) return rc;
+    Call c(*k, stream);
+    // sequences of few rows and of many, in a launch each
+    if (few && c.e == hipSuccess) {
+        a.rows_from = 1, a.rows_to = kFewRows, a.max_rows = (int32_t)few;
+        split_few(*k, c.captured, &a);
+        c.e = launch_kv_decode(a, c.s, c.event(!many));
+    }
+    if (many && c.e == hipSuccess) {
+        a.rows_from = kFewRows + 1, a.rows_to = INT_MAX, a.max_rows = (int32_t)many;
+        split_many(*k, c.captured, &a);
+        c.e = launch_kv_prefill(a, c.s, c.event(true));
+    }
     return c.end("kv attend");
 }
 

@@ -122,7 +122,7 @@ __global__ void __launch_bounds__(64 * waves_of(D), waves_of(D) / 4) decode_kern
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = lane & 15, quad = lane >> 4;
     const int i = blockIdx.z, head = blockIdx.y % a.l.kv_heads, rg = blockIdx.y / a.l.kv_heads;
     const int row0 = a.step.row0[i], tokens = a.step.row0[i + 1] - row0, len = a.step.len[i];
-    if (rg * R >= tokens * a.group) return;
+    if (rg * R >= tokens * a.group || tokens * a.group > a.rows_to) return;
     // tokens of this workgroup's rows
     const int q_first = len - tokens + rg * R / a.group, q_last = len - tokens + min(tokens * a.group - 1, rg * R + R - 1) / a.group;
     const KvTiles vis = kv_tiles(q_first, q_last, a.window, a.sinks);
@@ -356,12 +356,12 @@ __global__ void __launch_bounds__(64 * waves_of(D), waves_of(D) / 4) decode_kern
 // first parts are on their way while the largest max is found. (One thread per channel that walked all ranges: 23 us for 64
 // ranges, a load's latency each.)
 __global__ void __launch_bounds__(256) join_kernel(KvAttend a) {
-    constexpr int kAhead = 8, kRanges = 256;
+    constexpr int kAhead = 8, kRanges = kKvSplits;
     __shared__ float fs[kRanges], red[2][4];
     __shared__ float4 sums[256];
     const int i = blockIdx.z, head = blockIdx.y, row = blockIdx.x, D = a.l.dim, tid = threadIdx.x;
     const int row0 = a.step.row0[i], tokens = a.step.row0[i + 1] - row0;
-    if (row >= tokens * a.group) return;
+    if (row >= tokens * a.group || tokens * a.group < a.rows_from || tokens * a.group > a.rows_to) return;
     const int64_t slot = (((int64_t)i * a.l.kv_heads + head) * a.max_rows + row) * a.splits;
     const int first = a.step.len[i] - tokens;
     const int t0 = row / a.row_tile * a.row_tile, t1 = min(tokens * a.group, t0 + a.row_tile) - 1;
@@ -418,6 +418,46 @@ __global__ void __launch_bounds__(256) join_kernel(KvAttend a) {
     store_out(a.out, to + 3, a.out_bf16, sum.w * by);
 }
 
+// The same for at most kFewRanges ranges: D / 4 threads a row, all of whose parts are on their way at once.
+constexpr int kFewRanges = 16;
+__global__ void __launch_bounds__(256) join_few_kernel(KvAttend a) {
+    const int i = blockIdx.z, head = blockIdx.y, D = a.l.dim, width = D / 4, rows = 256 / width;
+    const int group = threadIdx.x / width, c = threadIdx.x - group * width, row = blockIdx.x * rows + group;
+    const int row0 = a.step.row0[i], tokens = a.step.row0[i + 1] - row0;
+    if (group >= rows || row >= tokens * a.group || tokens * a.group < a.rows_from || tokens * a.group > a.rows_to) return;
+    const int64_t slot = (((int64_t)i * a.l.kv_heads + head) * a.max_rows + row) * a.splits;
+    const int first = a.step.len[i] - tokens;
+    const int t0 = row / a.row_tile * a.row_tile, t1 = min(tokens * a.group, t0 + a.row_tile) - 1;
+    const int ranges = kv_ranges(kv_tiles(first + t0 / a.group, first + t1 / a.group, a.window, a.sinks).count(), a);
+    const float4 *part = (const float4 *)(a.part + slot * D) + c;
+    const float2 *ml = (const float2 *)(a.part_ml + 2 * slot);
+    float4 p[kFewRanges];
+    float2 m[kFewRanges];
+#pragma unroll
+    for (int s = 0; s < kFewRanges; s++)
+        if (s < ranges) p[s] = part[(int64_t)s * width], m[s] = ml[s];
+    float most = -__builtin_inff();
+#pragma unroll
+    for (int s = 0; s < kFewRanges; s++)
+        if (s < ranges) most = fmaxf(most, m[s].x);
+    float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    float total = 0.0f;
+#pragma unroll
+    for (int s = 0; s < kFewRanges; s++)
+        if (s < ranges) {
+            const float f = most > -__builtin_inff() ? __builtin_amdgcn_exp2f(m[s].x - most) : 1.0f;  // of no visible token: sums of 0, or NaN
+            total = __builtin_fmaf(m[s].y, f, total);
+            sum.x = __builtin_fmaf(p[s].x, f, sum.x), sum.y = __builtin_fmaf(p[s].y, f, sum.y);
+            sum.z = __builtin_fmaf(p[s].z, f, sum.z), sum.w = __builtin_fmaf(p[s].w, f, sum.w);
+        }
+    const int64_t to = (int64_t)(row0 + row / a.group) * a.out_stride + (head * a.group + row % a.group) * D + 4 * c;
+    const float by = total == 0.0f ? 0.0f : 1.0f / total;
+    store_out(a.out, to, a.out_bf16, sum.x * by);
+    store_out(a.out, to + 1, a.out_bf16, sum.y * by);
+    store_out(a.out, to + 2, a.out_bf16, sum.z * by);
+    store_out(a.out, to + 3, a.out_bf16, sum.w * by);
+}
+
 template <int R>
 hipError_t decode(const KvAttend &a, hipStream_t s, hipEvent_t done) {
     const dim3 grid((unsigned)a.splits, (unsigned)(a.l.kv_heads * ((a.max_rows + R - 1) / R)), (unsigned)a.step.n);
@@ -440,8 +480,11 @@ hipError_t launch_kv_decode(const KvAttend &a, hipStream_t s, hipEvent_t done) {
 }
 
 hipError_t launch_kv_join(const KvAttend &a, hipStream_t s, hipEvent_t done) {
-    const dim3 grid((unsigned)a.max_rows, (unsigned)a.l.kv_heads, (unsigned)a.step.n);
-    return launch_with_event(join_kernel, grid, dim3(256), s, done, a);
+    if (a.splits <= kFewRanges) {
+        const int rows = 256 / (a.l.dim / 4);
+        return launch_with_event(join_few_kernel, dim3((unsigned)((a.max_rows + rows - 1) / rows), (unsigned)a.l.kv_heads, (unsigned)a.step.n), dim3(256), s, done, a);
+    }
+    return launch_with_event(join_kernel, dim3((unsigned)a.max_rows, (unsigned)a.l.kv_heads, (unsigned)a.step.n), dim3(256), s, done, a);
 }
 
 }  // namespace j4q

@@ -23,6 +23,7 @@ namespace {
 
 typedef _Float16 v8h __attribute__((ext_vector_type(8)));
 typedef _Float16 v2h __attribute__((ext_vector_type(2)));
+typedef __bf16 v4b __attribute__((ext_vector_type(4)));
 typedef float v16f __attribute__((ext_vector_type(16)));
 
 constexpr float kUnit = 8.0f;  // the weight of t = m: 2^8
@@ -51,15 +52,23 @@ __device__ __forceinline__ void codes_to_half(uint32_t c, uint32_t *out) {
     out[1] = __builtin_bit_cast(uint32_t, __builtin_bit_cast(v2h, __builtin_amdgcn_perm(0x64646464u, u, 0x04030402u)) - bias);
 }
 
-__device__ __forceinline__ float value_at(const void *p, int64_t i, int bf16) {
-    return bf16 ? __builtin_bit_cast(float, (uint32_t)((const uint16_t *)p)[i] << 16) : ((const float *)p)[i];
+// 8 values from i on, 16-byte aligned.
+__device__ __forceinline__ void load8(const void *p, int64_t i, int bf16, float *x) {
+    if (bf16) {
+        const uint4 t = *(const uint4 *)((const uint16_t *)p + i);
+        const uint32_t w[4] = {t.x, t.y, t.z, t.w};
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            x[2 * j] = __builtin_bit_cast(float, w[j] << 16);
+            x[2 * j + 1] = __builtin_bit_cast(float, w[j] & 0xffff0000u);
+        }
+    } else {
+        const float4 *from = (const float4 *)((const float *)p + i);
+        const float4 t = from[0], u = from[1];
+        x[0] = t.x, x[1] = t.y, x[2] = t.z, x[3] = t.w, x[4] = u.x, x[5] = u.y, x[6] = u.z, x[7] = u.w;
+    }
 }
-__device__ __forceinline__ uint32_t bf16_bits(float f) {
-    const uint32_t u = __builtin_bit_cast(uint32_t, f);
-    return f != f ? (u >> 16) | 0x40 : (u + 0x7fffu + ((u >> 16) & 1)) >> 16;
-}
-
-// W: waves, of 32 rows each. P: fp16 parts of q and w.
+// W: waves, of 32 rows each. P: fp16 parts of q and w, 1 for a bf16 result, 2 for an fp32 one.
 template <int D, int W, int P>
 __global__ void __launch_bounds__(64 * W, D <= 128 ? 2 : 1) prefill_kernel(KvAttend a) {
     constexpr int kThreads = 64 * W, kRows = 32 * W;
@@ -72,7 +81,7 @@ __global__ void __launch_bounds__(64 * W, D <= 128 ? 2 : 1) prefill_kernel(KvAtt
     const int head = blockIdx.x % a.l.kv_heads, split = blockIdx.x / a.l.kv_heads, i = blockIdx.z;
     const int row0 = a.step.row0[i], tokens = a.step.row0[i + 1] - row0, len = a.step.len[i], rows = tokens * a.group;
     const int tile_count = (rows + kRows - 1) / kRows;
-    if ((int)blockIdx.y >= tile_count) return;
+    if ((int)blockIdx.y >= tile_count || rows < a.rows_from) return;
     const int r0 = (tile_count - 1 - (int)blockIdx.y) * kRows;  // the longest first
     const int r1 = min(rows, r0 + kRows) - 1;
     const int before = len - tokens;
@@ -92,22 +101,29 @@ __global__ void __launch_bounds__(64 * W, D <= 128 ? 2 : 1) prefill_kernel(KvAtt
     float qk;
     {
         const int64_t at = (int64_t)(row0 + row / a.group) * a.q_stride + (head * a.group + row % a.group) * D + 8 * half;
-        float most = 0.0f;
+        float x[D / 16][8], most = 0.0f, finite = 0.0f;
+#pragma unroll
+        for (int s = 0; s < D / 16; s++) load8(a.q, at + 16 * s, a.q_bf16, x[s]);
+#pragma unroll
         for (int s = 0; s < D / 16; s++)
+#pragma unroll
             for (int j = 0; j < 8; j++) {
-                const float m = fabsf(value_at(a.q, at + 16 * s + j, a.q_bf16));
-                most = fmaxf(most, m < __builtin_inff() ? m : __builtin_inff());
+                most = fmaxf(most, fabsf(x[s][j]));
+                finite = __builtin_fmaf(x[s][j], 0.0f, finite);  // else NaN
             }
         most = max32(most);
+        const Two both = swap32(finite);
         // to [2^13, 2^14), by a power of two (2^100 at most)
         const int e = max((int)(__builtin_bit_cast(uint32_t, most) >> 23) - 127 - 13, -100);
         const float up = __builtin_bit_cast(float, (uint32_t)(127 - e) << 23);
-        qk = most < __builtin_inff() ? __builtin_bit_cast(float, (uint32_t)(127 + e) << 23) * a.scale : __builtin_nanf("");
+        qk = __builtin_bit_cast(float, (uint32_t)(127 + e) << 23) * a.scale + (both.a + both.b);
+#pragma unroll
         for (int s = 0; s < D / 16; s++)
+#pragma unroll
             for (int j = 0; j < 8; j++) {
-                const float x = value_at(a.q, at + 16 * s + j, a.q_bf16) * up;
-                q[0][s][j] = (_Float16)x;
-                if constexpr (P == 2) q[1][s][j] = (_Float16)(x - (float)q[0][s][j]);
+                const float y = x[s][j] * up;
+                q[0][s][j] = (_Float16)y;
+                if constexpr (P == 2) q[1][s][j] = (_Float16)(y - (float)q[0][s][j]);
             }
     }
 
@@ -334,7 +350,7 @@ __global__ void __launch_bounds__(64 * W, D <= 128 ? 2 : 1) prefill_kernel(KvAtt
             for (int g = 0; g < 4; g++) {
                 const float4 x = make_float4(o[d][4 * g] * f, o[d][4 * g + 1] * f, o[d][4 * g + 2] * f, o[d][4 * g + 3] * f);
                 const int64_t at = to + 32 * d + 8 * g;
-                if (a.out_bf16) *(uint2 *)((uint16_t *)a.out + at) = make_uint2(bf16_bits(x.x) | bf16_bits(x.y) << 16, bf16_bits(x.z) | bf16_bits(x.w) << 16);
+                if constexpr (P == 1) *(v4b *)((uint16_t *)a.out + at) = v4b{(__bf16)x.x, (__bf16)x.y, (__bf16)x.z, (__bf16)x.w};
                 else *(float4 *)((float *)a.out + at) = x;
             }
     }

@@ -307,6 +307,18 @@ def test_attend_many_rows(model, dim, group, page, okind):
 
 
 @pytest.mark.parametrize("okind", ["bf16", "f32"])
+def test_attend_uneven_steps(model, okind):
+    """A chunk of a prompt beside sequences of one token and of a few, short and long."""
+    m = model(kv_heads=2, head_dim=128, pages=900, page_tokens=16, sequences=6, sequence_pages=400)
+    rng = np.random.default_rng(31)
+    seqs, tokens = [3, 0, 5, 1, 2, 4], [300, 1, 4, 5, 1, 17]
+    m.grow(rng, seqs, [50, 4000, 20, 700, 1, 100])
+    m.grow(rng, seqs, tokens)
+    for window, sinks in ((0, 0), (500, 4)):
+        check_attend(m, rng, seqs, tokens, 8, window=window, sinks=sinks, okind=okind)
+
+
+@pytest.mark.parametrize("okind", ["bf16", "f32"])
 def test_attend_many_rows_long(model, okind):
     """A chunk behind a long context: a row tile's tokens are several workgroups'."""
     m = model(kv_heads=1, head_dim=128, pages=400, page_tokens=32, sequences=2, sequence_pages=300)
