@@ -312,7 +312,8 @@ __global__ void __launch_bounds__(256) append_kernel(KvAppend a) {
 }
 
 // One block of 16 tokens of a kv head per workgroup.
-__global__ void __launch_bounds__(256) read_kernel(KvRead a, int blocks) {
+template <int N>
+__global__ void __launch_bounds__(256) read_kernel(KvReadOf<N> a, int blocks) {
     const int tid = threadIdx.x, D = a.l.dim, H = a.l.kv_heads;
     const int head = blockIdx.x % H, i = blockIdx.x / H / blocks;
     const int first = a.first[i], b = first / kKvBlock + blockIdx.x / H % blocks;
@@ -349,14 +350,16 @@ __global__ void __launch_bounds__(256) read_kernel(KvRead a, int blocks) {
 }
 
 // A wave per run.
-__global__ void __launch_bounds__(64) runs_kernel(KvRuns a) {
+template <int N>
+__global__ void __launch_bounds__(64) runs_kernel(KvRunsOf<N> a) {
     const KvRun r = a.run[blockIdx.x];
     for (int j = threadIdx.x; j < r.count; j += 64) a.words[r.at + j] = r.value + r.step * j;
 }
 
 // 16 KiB of a page per workgroup, four loads of a thread on their way before the first store.
 constexpr int kCopyBytes = 16384;
-__global__ void __launch_bounds__(256) copy_kernel(KvPairs a) {
+template <int N>
+__global__ void __launch_bounds__(256) copy_kernel(KvPairsOf<N> a) {
     uint8_t *base = a.pool + (int64_t)blockIdx.z * a.layer_bytes;
     const uint4 *src = (const uint4 *)(base + (int64_t)a.src[blockIdx.y] * a.page_bytes);
     uint4 *dst = (uint4 *)(base + (int64_t)a.dst[blockIdx.y] * a.page_bytes);
@@ -416,16 +419,30 @@ hipError_t launch_kv_append(const KvAppend &args, hipStream_t s, hipEvent_t done
 
 hipError_t launch_kv_read(const KvRead &r, hipStream_t s, hipEvent_t done) {
     const int blocks = (int)((r.count + 2 * kKvBlock - 2) / kKvBlock);
-    return launch_with_event(read_kernel, dim3((unsigned)(r.n * blocks * r.l.kv_heads)), dim3(256), s, done, r, blocks);
+    const dim3 grid((unsigned)(r.n * blocks * r.l.kv_heads));
+    if (r.n > 64) return launch_with_event(read_kernel<kKvReadSeqs>, grid, dim3(256), s, done, r, blocks);
+    KvReadOf<64> few{r.l, r.table, r.sequence_pages, r.n, r.count, r.k, r.v};
+    std::copy_n(r.seq, r.n, few.seq);
+    std::copy_n(r.first, r.n, few.first);
+    std::copy_n(r.len, r.n, few.len);
+    return launch_with_event(read_kernel<64>, grid, dim3(256), s, done, few, blocks);
 }
 
 hipError_t launch_kv_runs(const KvRuns &r, hipStream_t s, hipEvent_t done) {
-    return launch_with_event(runs_kernel, dim3((unsigned)r.n), dim3(64), s, done, r);
+    const dim3 grid((unsigned)r.n);
+    if (r.n > 24) return launch_with_event(runs_kernel<kKvRuns>, grid, dim3(64), s, done, r);
+    KvRunsOf<24> few{r.words, r.n};
+    std::copy_n(r.run, r.n, few.run);
+    return launch_with_event(runs_kernel<24>, grid, dim3(64), s, done, few);
 }
 
 hipError_t launch_kv_copy(const KvPairs &p, hipStream_t s, hipEvent_t done) {
     const dim3 grid((unsigned)((p.page_bytes + kCopyBytes - 1) / kCopyBytes), (unsigned)p.n, (unsigned)p.layers);
-    return launch_with_event(copy_kernel, grid, dim3(256), s, done, p);
+    if (p.n > 48) return launch_with_event(copy_kernel<kKvPairs>, grid, dim3(256), s, done, p);
+    KvPairsOf<48> few{p.pool, p.page_bytes, p.layer_bytes, p.layers, p.n};
+    std::copy_n(p.src, p.n, few.src);
+    std::copy_n(p.dst, p.n, few.dst);
+    return launch_with_event(copy_kernel<48>, grid, dim3(256), s, done, few);
 }
 
 }  // namespace j4q

@@ -36,7 +36,7 @@ def _kind(dtype: DType) -> int:
 def _ints(values, code="i") -> array:
     """Whole numbers as the library reads them; an array of 64 takes 2 us, where a ctypes one takes 15."""
     try:
-        return array(code, values)
+        return array(code, values if type(values) is list else list(values))
     except OverflowError:
         raise IllegalArgumentException(f"a number does not fit {8 * array(code).itemsize} bits") from None
 
