@@ -358,8 +358,8 @@ int j4q_kv_tables(j4q_kv kv, const int32_t *seqs, int32_t n, int64_t *lengths, i
 int j4q_kv_extend(j4q_kv kv, const int32_t *seqs, const int32_t *tokens, int32_t n, void *stream);
 /* Begins a step over the last tokens[i] tokens that seqs[i] has already. */
 int j4q_kv_begin(j4q_kv kv, const int32_t *seqs, const int32_t *tokens, int32_t n, void *stream);
-/* The empty sequence dst[i] becomes src[i]: sharing its pages (share != 0; a shared page is copied when one of its holders
- * extends into it), or with copies of them. */
+/* The empty sequence dst[i] becomes src[i], which is no dst of the same call: sharing its pages (share != 0; a shared
+ * page is copied when one of its holders extends into it), or with copies of them. */
 int j4q_kv_fork(j4q_kv kv, const int32_t *src, const int32_t *dst, int32_t n, int share, void *stream);
 /* Cuts sequences to lengths[i] tokens (0 frees them whole); pages that no sequence holds any more are free. A step that
  * one of them is part of ends. */

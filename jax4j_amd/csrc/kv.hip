@@ -4,11 +4,13 @@
 // Pages, lengths and reference counts live here, so a call that cannot be served (no page left, a table full, a mask that
 // would look at freed tokens) is refused before anything is enqueued or changed. The device has the tables and the current
 // step (which sequences, their lengths and rows), which a kernel with the changes in its arguments keeps up, in stream order.
-// A page is taken lowest first.
+// A page is taken lowest first. A call takes the host memory that it needs before it changes anything, so that one that finds
+// none leaves the cache as it was; a cache whose change the device did not get (a launch failed) is refused from then on.
 #include <limits.h>
 #include <math.h>
 
 #include <algorithm>
+#include <exception>
 #include <memory>
 #include <vector>
 
@@ -48,11 +50,12 @@ struct Kv {
     // the current step
     std::vector<int32_t> step_seq, step_tokens;
     int32_t step_rows = 0, step_blocks = 0, step_most_blocks = 0;
-    bool step_writable = false, step_checked = false;
+    bool step_checked = false;
     // calls on one stream after another
     hipEvent_t done = nullptr;
     hipStream_t last = nullptr;
     bool used = false;
+    bool lost = false;  // the device's words are not what is here
 
     int32_t at_seq() const { return c.sequences * c.sequence_pages; }
     int32_t at_len() const { return at_seq() + c.sequences; }
@@ -109,11 +112,15 @@ Kv *lookup(j4q_kv h) {
     return k->live && k->gen == (uint32_t)(h >> 32) ? k : nullptr;
 }
 
-int get(j4q_kv h, const char *op, Kv **out) {
+int get(j4q_kv h, const char *op, Kv **out, bool lost_too = false) {
     *out = lookup(h);
     if (!*out) return report_error(J4Q_EHANDLE, "%s: unknown or destroyed cache 0x%llx", op, (unsigned long long)h);
+    if ((*out)->lost && !lost_too) return report_error(J4Q_EHIP, "%s: an earlier call on this cache failed on the device", op);
     return J4Q_OK;
 }
+
+// What an entry point answers where host memory ran out in it.
+int no_memory(const char *op) { return report_error(J4Q_ENOMEM, "%s failed: out of host memory", op); }
 
 bool aligned(const void *p, uintptr_t a) { return ((uintptr_t)p & (a - 1)) == 0; }
 
@@ -134,6 +141,10 @@ struct Call {
     }
     bool recorded() const { return !captured && s != abi::stream(); }
     hipEvent_t event(bool last) const { return last && recorded() ? k.done : nullptr; }
+    int end_change(const char *op) {
+        k.lost |= e != hipSuccess;
+        return end(op);
+    }
     int end(const char *op) {
         if (e != hipSuccess && recorded()) (void)hipEventRecord(k.done, s);
         if (!captured) {
@@ -214,11 +225,11 @@ void end_step(Kv &k) {
 }
 bool in_step(const Kv &k, int32_t seq) { return std::find(k.step_seq.begin(), k.step_seq.end(), seq) != k.step_seq.end(); }
 
-// The last tokens[i] tokens of seqs[i] as the current step (lengths as they are now).
-void set_step(Kv &k, const int32_t *seqs, const int32_t *tokens, int32_t n, bool writable, Changes *ch) {
+// The last tokens[i] tokens of seqs[i] as the current step (lengths as they are now): at most step_changes(n) runs.
+size_t step_changes(int32_t n) { return 4 * (size_t)n + 2; }
+void set_step(Kv &k, const int32_t *seqs, const int32_t *tokens, int32_t n, Changes *ch) {
     k.step_seq.assign(seqs, seqs + n);
     k.step_tokens.assign(tokens, tokens + n);
-    k.step_writable = writable;
     k.step_checked = false;
     k.step_most_blocks = 0;
     for (int32_t i = 0; i < n; i++) ch->add(k.at_seq() + i, seqs[i]);
@@ -370,7 +381,7 @@ using namespace j4q;
 
 extern "C" {
 
-int j4q_kv_create(const j4q_kv_config *config, j4q_kv *out) {
+int j4q_kv_create(const j4q_kv_config *config, j4q_kv *out) try {
     if (!config || !out) return report_error(J4Q_EINVAL, "kv cache: NULL argument");
     const j4q_kv_config c = *config;
     if (c.layers < 1 || c.layers > 65535 || c.kv_heads < 1 || c.kv_heads > 1024)
@@ -390,6 +401,12 @@ int j4q_kv_create(const j4q_kv_config *config, j4q_kv *out) {
     if (rc) return rc;
     if ((rc = refuse_capture("kv cache", nullptr))) return rc;
     std::unique_ptr<Kv> k(new Kv);
+    g_kvs.reserve(g_kvs.size() + 1);
+    k->seqs.resize((size_t)c.sequences);
+    k->refs.assign((size_t)c.pages, 0);
+    k->free_bits.assign((size_t)((c.pages + 63) / 64), ~0ull);
+    k->step_seq.reserve((size_t)c.sequences);
+    k->step_tokens.reserve((size_t)c.sequences);
     k->c = c;
     k->page_bytes = page;
     k->layer_bytes = page * c.pages;
@@ -417,9 +434,6 @@ int j4q_kv_create(const j4q_kv_config *config, j4q_kv *out) {
     k->last = abi::stream();
     k->used = true;
     k->bytes = pool + words + part;
-    k->seqs.resize((size_t)c.sequences);
-    k->refs.assign((size_t)c.pages, 0);
-    k->free_bits.assign((size_t)((c.pages + 63) / 64), ~0ull);
     if (c.pages % 64) k->free_bits.back() = (1ull << (c.pages % 64)) - 1;
     k->free_pages = c.pages;
     k->live = true;
@@ -431,13 +445,15 @@ int j4q_kv_create(const j4q_kv_config *config, j4q_kv *out) {
     else g_kvs[slot] = std::move(k);
     *out = handle;
     return J4Q_OK;
+} catch (const std::exception &) {
+    return no_memory("kv cache");
 }
 
 int j4q_kv_destroy(j4q_kv kv) {
     if (kv == 0) return J4Q_OK;
     std::lock_guard<std::mutex> lk(abi::lock());
     Kv *k;
-    int rc = get(kv, "kv destroy", &k);
+    int rc = get(kv, "kv destroy", &k, true);
     if (rc) return rc;
     if ((rc = abi::ready_locked())) return rc;
     const hipError_t e = hipDeviceSynchronize();  // calls may still run on any stream
@@ -456,7 +472,7 @@ int j4q_kv_info(j4q_kv kv, j4q_kv_desc *out) {
     if (!out) return report_error(J4Q_EINVAL, "kv info: out is NULL");
     std::lock_guard<std::mutex> lk(abi::lock());
     Kv *k;
-    const int rc = get(kv, "kv info", &k);
+    const int rc = get(kv, "kv info", &k, true);
     if (rc) return rc;
     *out = j4q_kv_desc{};
     out->config = k->c;
@@ -468,7 +484,7 @@ int j4q_kv_info(j4q_kv kv, j4q_kv_desc *out) {
     return J4Q_OK;
 }
 
-int j4q_kv_tables(j4q_kv kv, const int32_t *seqs, int32_t n, int64_t *lengths, int32_t *pages, int32_t capacity) {
+int j4q_kv_tables(j4q_kv kv, const int32_t *seqs, int32_t n, int64_t *lengths, int32_t *pages, int32_t capacity) try {
     std::lock_guard<std::mutex> lk(abi::lock());
     Kv *k;
     int rc = get(kv, "kv tables", &k);
@@ -484,9 +500,11 @@ int j4q_kv_tables(j4q_kv kv, const int32_t *seqs, int32_t n, int64_t *lengths, i
         std::fill(to + have, to + capacity, -1);
     }
     return J4Q_OK;
+} catch (const std::exception &) {
+    return no_memory("kv tables");
 }
 
-int j4q_kv_extend(j4q_kv kv, const int32_t *seqs, const int32_t *tokens, int32_t n, void *stream) {
+int j4q_kv_extend(j4q_kv kv, const int32_t *seqs, const int32_t *tokens, int32_t n, void *stream) try {
     std::lock_guard<std::mutex> lk(abi::lock());
     Kv *k;
     int rc = get(kv, "kv extend", &k);
@@ -525,6 +543,13 @@ int j4q_kv_extend(j4q_kv kv, const int32_t *seqs, const int32_t *tokens, int32_t
     if ((rc = abi::ready_locked()) || (rc = refuse_capture("kv extend", stream))) return rc;
     Changes ch;
     Pairs pairs;
+    ch.runs.reserve((size_t)need + step_changes(n));
+    pairs.reserve(shared.empty() ? 0 : (size_t)n);
+    for (int32_t i = 0; i < n; i++) {
+        std::vector<int32_t> &pages = k->seqs[(size_t)seqs[i]].pages;
+        const size_t count = (size_t)((k->seqs[(size_t)seqs[i]].len + tokens[i] + per - 1) / per);
+        if (count > pages.capacity()) pages.reserve(std::max(count, std::min(2 * pages.capacity(), (size_t)k->c.sequence_pages)));
+    }
     for (int32_t i = 0; i < n; i++) {
         Seq &q = k->seqs[(size_t)seqs[i]];
         const int64_t table = (int64_t)seqs[i] * k->c.sequence_pages;
@@ -541,14 +566,16 @@ int j4q_kv_extend(j4q_kv kv, const int32_t *seqs, const int32_t *tokens, int32_t
             ch.add(table + (int64_t)q.pages.size() - 1, q.pages.back());
         }
     }
-    set_step(*k, seqs, tokens, n, true, &ch);
+    set_step(*k, seqs, tokens, n, &ch);
     Call c(*k, stream);
     copy_pages(c, pairs, false);
     ch.launch(c, true);
-    return c.end("kv extend");
+    return c.end_change("kv extend");
+} catch (const std::exception &) {
+    return no_memory("kv extend");
 }
 
-int j4q_kv_begin(j4q_kv kv, const int32_t *seqs, const int32_t *tokens, int32_t n, void *stream) {
+int j4q_kv_begin(j4q_kv kv, const int32_t *seqs, const int32_t *tokens, int32_t n, void *stream) try {
     std::lock_guard<std::mutex> lk(abi::lock());
     Kv *k;
     int rc = get(kv, "kv begin", &k);
@@ -560,33 +587,45 @@ int j4q_kv_begin(j4q_kv kv, const int32_t *seqs, const int32_t *tokens, int32_t 
             return report_error(J4Q_EINVAL, "kv begin: sequence %d has %lld tokens, not %d", seqs[i], (long long)k->seqs[(size_t)seqs[i]].len, tokens[i]);
     if ((rc = abi::ready_locked()) || (rc = refuse_capture("kv begin", stream))) return rc;
     Changes ch;
-    set_step(*k, seqs, tokens, n, true, &ch);
+    ch.runs.reserve(step_changes(n));
+    set_step(*k, seqs, tokens, n, &ch);
     Call c(*k, stream);
     ch.launch(c, true);
-    return c.end("kv begin");
+    return c.end_change("kv begin");
+} catch (const std::exception &) {
+    return no_memory("kv begin");
 }
 
-int j4q_kv_fork(j4q_kv kv, const int32_t *src, const int32_t *dst, int32_t n, int share, void *stream) {
+int j4q_kv_fork(j4q_kv kv, const int32_t *src, const int32_t *dst, int32_t n, int share, void *stream) try {
     std::lock_guard<std::mutex> lk(abi::lock());
     Kv *k;
     int rc = get(kv, "kv fork", &k);
     if (rc) return rc;
     if ((rc = check_seqs(*k, "kv fork", dst, n, true)) || (rc = check_seqs(*k, "kv fork", src, n, false))) return rc;
     int64_t need = 0;
+    size_t entries = 0;
+    std::vector<bool> made((size_t)k->c.sequences);
     for (int32_t i = 0; i < n; i++) {
         if (k->seqs[(size_t)dst[i]].len)
             return report_error(J4Q_EINVAL, "kv fork: sequence %d holds %lld tokens", dst[i], (long long)k->seqs[(size_t)dst[i]].len);
+        made[(size_t)dst[i]] = true;
+        entries += k->seqs[(size_t)src[i]].pages.size();
         if (!share)
             for (int32_t p : k->seqs[(size_t)src[i]].pages) need += p >= 0;
     }
+    for (int32_t i = 0; i < n; i++)
+        if (made[(size_t)src[i]]) return report_error(J4Q_EINVAL, "kv fork: sequence %d is made by this call and copied by it", src[i]);
     if (need > k->free_pages)
         return report_error(J4Q_ENOMEM, "kv fork failed: %lld pages needed, %lld free", (long long)need, (long long)k->free_pages);
     if ((rc = abi::ready_locked()) || (rc = refuse_capture("kv fork", stream))) return rc;
     Changes ch;
     Pairs pairs;
+    ch.runs.reserve(entries);
+    pairs.reserve((size_t)need);
+    for (int32_t i = 0; i < n; i++) k->seqs[(size_t)dst[i]].pages.reserve(k->seqs[(size_t)src[i]].pages.size());
     for (int32_t i = 0; i < n; i++) {
         Seq &d = k->seqs[(size_t)dst[i]];
-        d = k->seqs[(size_t)src[i]];  // a src that is a dst of this call was empty and stays so
+        d = k->seqs[(size_t)src[i]];
         for (size_t j = 0; j < d.pages.size(); j++) {
             if (d.pages[j] >= 0 && share) k->refs[(size_t)d.pages[j]]++;
             if (d.pages[j] >= 0 && !share) {
@@ -600,10 +639,12 @@ int j4q_kv_fork(j4q_kv kv, const int32_t *src, const int32_t *dst, int32_t n, in
     Call c(*k, stream);
     copy_pages(c, pairs, false);
     ch.launch(c, true);
-    return c.end("kv fork");
+    return c.end_change("kv fork");
+} catch (const std::exception &) {
+    return no_memory("kv fork");
 }
 
-int j4q_kv_truncate(j4q_kv kv, const int32_t *seqs, const int64_t *lengths, int32_t n) {
+int j4q_kv_truncate(j4q_kv kv, const int32_t *seqs, const int64_t *lengths, int32_t n) try {
     std::lock_guard<std::mutex> lk(abi::lock());
     Kv *k;
     int rc = get(kv, "kv truncate", &k);
@@ -631,9 +672,11 @@ int j4q_kv_truncate(j4q_kv kv, const int32_t *seqs, const int64_t *lengths, int3
         if (q.gone0 >= q.gone1) q.gone0 = q.gone1 = 0;
     }
     return J4Q_OK;
+} catch (const std::exception &) {
+    return no_memory("kv truncate");
 }
 
-int j4q_kv_evict(j4q_kv kv, const int32_t *seqs, int32_t n, int32_t window, int32_t sinks, void *stream) {
+int j4q_kv_evict(j4q_kv kv, const int32_t *seqs, int32_t n, int32_t window, int32_t sinks, void *stream) try {
     std::lock_guard<std::mutex> lk(abi::lock());
     Kv *k;
     int rc = get(kv, "kv evict", &k);
@@ -641,18 +684,22 @@ int j4q_kv_evict(j4q_kv kv, const int32_t *seqs, int32_t n, int32_t window, int3
     if (window < 1 || sinks < 0) return report_error(J4Q_EINVAL, "kv evict: a window of %d tokens, %d first ones (at least 1, 0)", window, sinks);
     if ((rc = check_seqs(*k, "kv evict", seqs, n, true))) return rc;
     if ((rc = abi::ready_locked()) || (rc = refuse_capture("kv evict", stream))) return rc;
-    const int64_t per = k->c.page_tokens;
+    const int64_t per = k->c.page_tokens, first = (sinks + per - 1) / per;
+    // the next token, at place len, sees j > len - window and j < sinks; an earlier one sees more
+    auto last = [&](const Seq &q) { return std::max<int64_t>(0, (q.len - window + 1) / per); };
     Changes ch;
     for (int32_t i = 0; i < n; i++) {
+        const Seq &q = k->seqs[(size_t)seqs[i]];
+        for (int64_t p = first, end = last(q); p < end; p++)
+            if (q.pages[(size_t)p] >= 0) ch.add((int64_t)seqs[i] * k->c.sequence_pages + p, -1);
+    }
+    for (int32_t i = 0; i < n; i++) {
         Seq &q = k->seqs[(size_t)seqs[i]];
-        // the next token, at place len, sees j > len - window and j < sinks; an earlier one sees more
-        const int64_t first = (sinks + per - 1) / per, end = std::max<int64_t>(0, (q.len - window + 1) / per);
+        const int64_t end = last(q);
         if (first >= end) continue;
         for (int64_t p = first; p < end; p++) {
-            if (q.pages[(size_t)p] < 0) continue;
             k->drop(q.pages[(size_t)p]);
             q.pages[(size_t)p] = -1;
-            ch.add((int64_t)seqs[i] * k->c.sequence_pages + p, -1);
         }
         q.gone0 = q.gone1 ? std::min(q.gone0, first * per) : first * per;
         q.gone1 = std::max(q.gone1, end * per);
@@ -660,10 +707,12 @@ int j4q_kv_evict(j4q_kv kv, const int32_t *seqs, int32_t n, int32_t window, int3
     k->step_checked = false;
     Call c(*k, stream);
     ch.launch(c, true);
-    return c.end("kv evict");
+    return c.end_change("kv evict");
+} catch (const std::exception &) {
+    return no_memory("kv evict");
 }
 
-int j4q_kv_compact(j4q_kv kv, int64_t *moved, void *stream) {
+int j4q_kv_compact(j4q_kv kv, int64_t *moved, void *stream) try {
     std::lock_guard<std::mutex> lk(abi::lock());
     Kv *k;
     int rc = get(kv, "kv compact", &k);
@@ -682,13 +731,15 @@ int j4q_kv_compact(j4q_kv kv, int64_t *moved, void *stream) {
     }
     Changes ch;
     if (!pairs.empty())
-        for (int32_t s = 0; s < k->c.sequences; s++)
-            for (size_t j = 0; j < k->seqs[(size_t)s].pages.size(); j++) {
-                int32_t &p = k->seqs[(size_t)s].pages[j];
-                if (p < 0 || to[(size_t)p] < 0) continue;
-                p = to[(size_t)p];
-                ch.add((int64_t)s * k->c.sequence_pages + (int64_t)j, p);
-            }
+        for (int32_t s = 0; s < k->c.sequences; s++) {
+            const Seq &q = k->seqs[(size_t)s];
+            for (size_t j = 0; j < q.pages.size(); j++)
+                if (q.pages[j] >= 0 && to[(size_t)q.pages[j]] >= 0) ch.add((int64_t)s * k->c.sequence_pages + (int64_t)j, to[(size_t)q.pages[j]]);
+        }
+    if (!pairs.empty())
+        for (Seq &q : k->seqs)
+            for (int32_t &p : q.pages)
+                if (p >= 0 && to[(size_t)p] >= 0) p = to[(size_t)p];
     for (const auto &[p, h] : pairs) {
         k->refs[(size_t)h] = k->refs[(size_t)p];
         k->refs[(size_t)p] = 0;
@@ -702,10 +753,12 @@ int j4q_kv_compact(j4q_kv kv, int64_t *moved, void *stream) {
     Call c(*k, stream);
     copy_pages(c, pairs, false);
     ch.launch(c, true);
-    return c.end("kv compact");
+    return c.end_change("kv compact");
+} catch (const std::exception &) {
+    return no_memory("kv compact");
 }
 
-int j4q_kv_append(j4q_kv kv, int32_t layer, const j4q_kv_append_args *args, void *stream) {
+int j4q_kv_append(j4q_kv kv, int32_t layer, const j4q_kv_append_args *args, void *stream) try {
     if (!args) return report_error(J4Q_EINVAL, "kv append: args is NULL");
     std::lock_guard<std::mutex> lk(abi::lock());
     Kv *k;
@@ -760,9 +813,11 @@ int j4q_kv_append(j4q_kv kv, int32_t layer, const j4q_kv_append_args *args, void
     Call c(*k, stream);
     if (c.e == hipSuccess) c.e = launch_kv_append(a, c.s, c.event(true));
     return c.end("kv append");
+} catch (const std::exception &) {
+    return no_memory("kv append");
 }
 
-int j4q_kv_attend(j4q_kv kv, int32_t layer, const j4q_kv_attend_args *args, void *stream) {
+int j4q_kv_attend(j4q_kv kv, int32_t layer, const j4q_kv_attend_args *args, void *stream) try {
     if (!args) return report_error(J4Q_EINVAL, "kv attend: args is NULL");
     std::lock_guard<std::mutex> lk(abi::lock());
     Kv *k;
@@ -824,9 +879,11 @@ int j4q_kv_attend(j4q_kv kv, int32_t layer, const j4q_kv_attend_args *args, void
         c.e = launch_kv_prefill(a, c.s, c.event(true));
     }
     return c.end("kv attend");
+} catch (const std::exception &) {
+    return no_memory("kv attend");
 }
 
-int j4q_kv_read(j4q_kv kv, int32_t layer, const int32_t *seqs, const int64_t *first, int64_t count, int32_t n, float *k_out, float *v_out, void *stream) {
+int j4q_kv_read(j4q_kv kv, int32_t layer, const int32_t *seqs, const int64_t *first, int64_t count, int32_t n, float *k_out, float *v_out, void *stream) try {
     std::lock_guard<std::mutex> lk(abi::lock());
     Kv *k;
     int rc = get(kv, "kv read", &k);
@@ -861,6 +918,8 @@ int j4q_kv_read(j4q_kv kv, int32_t layer, const int32_t *seqs, const int64_t *fi
         c.e = launch_kv_read(r, c.s, c.event(at + kKvReadSeqs >= n));
     }
     return c.end("kv read");
+} catch (const std::exception &) {
+    return no_memory("kv read");
 }
 
 int j4q_rope_into(const void *x, void *out, int type, int64_t rows, int32_t heads, int32_t head_dim, int64_t x_stride, int64_t out_stride,

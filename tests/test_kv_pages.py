@@ -247,6 +247,74 @@ def test_memory_of_a_cache_is_given_back(shim):
     """)
 
 
+def test_a_fork_of_what_the_call_itself_makes_is_refused(shim):
+    """Sequence 1 is empty when the call begins and would be a copy of 0 when it is copied: pages that nobody counted."""
+    run(shim, """
+        kv = cache(pages=8)
+        kv.extend([0], [4 * 16])
+        for share in (True, False):
+            assert refused(lambda: kv.fork([0, 1], [1, 2], share=share), "made by this call") == "IllegalArgumentException"
+            assert refused(lambda: kv.fork([3], [3], share=share), "made by this call") == "IllegalArgumentException"
+        assert kv.info()["pages_free"] == 4 and [kv.length(s) for s in range(4)] == [64, 0, 0, 0]
+    """)
+
+
+def test_no_host_memory(shim, monkeypatch):
+    """Every call that finds too little host memory for its lists says so, and leaves the cache as it was."""
+    monkeypatch.setenv("MALLOC_ARENA_MAX", "1")  # long lists neither from another thread's heap nor from what was freed
+    monkeypatch.setenv("MALLOC_MMAP_THRESHOLD_", str(1 << 17))
+    run(shim, """
+        import resource
+        be.upload_quantized(np.zeros(34, np.uint8), QuantType.Q8_0, (1, 32))
+        def limited(call, more=1 << 20):
+            used = int(open("/proc/self/statm").read().split()[0]) * resource.getpagesize()
+            resource.setrlimit(resource.RLIMIT_AS, (used + more, resource.RLIM_INFINITY))
+            try:
+                return refused(call, "failed", "out of host memory")
+            finally:
+                resource.setrlimit(resource.RLIMIT_AS, (resource.RLIM_INFINITY, resource.RLIM_INFINITY))
+        before = fake.fake_used()
+        assert limited(lambda: cache(pages=1 << 26), 64 << 20) == "RuntimeError"
+        assert fake.fake_used() == before
+        # pages of 1 KiB here: tables large against the pool
+        kv = cache(layers=1, kv_heads=1, pages=1 << 20, sequences=3, sequence_pages=1 << 20)
+        tokens = 1 << 23
+        def state():
+            return kv.info(), [kv.length(s) for s in range(3)]
+        def held(call):
+            was = state()
+            assert limited(call) == "RuntimeError"
+            assert state() == was
+            call()
+        held(lambda: kv.extend([0], [tokens]))
+        table = kv.tables([0]).tobytes()
+        assert limited(lambda: kv.fork([0], [1])) == "RuntimeError" and kv.tables([0]).tobytes() == table and kv.length(1) == 0
+        kv.extend([1], [16])
+        kv.truncate([0], [tokens // 2])
+        held(kv.compact)
+    """)
+
+
+def test_a_change_that_the_device_did_not_get(shim):
+    """Its tables are then not the host's: the cache is refused, and can be looked at and destroyed."""
+    run(shim, """
+        a = address(1 << 20)
+        for change in (lambda kv: kv.extend([1], [16]), lambda kv: kv.begin([0], [1]), lambda kv: kv.fork([0], [2]), lambda kv: kv.evict([0], 1),
+                       lambda kv: (kv.truncate([3], [0]), kv.compact())):
+            kv = cache()
+            kv.extend([3, 0], [20, 40])
+            kv.append(0, a, a)
+            fake.fake_fail_launches(1)
+            assert refused(lambda: kv.append(0, a, a), "kv append failed") == "RuntimeError"  # changes nothing here
+            assert refused(lambda: change(kv), "failed") == "RuntimeError"
+            fake.fake_fail_launches(0)
+            for call in (lambda: kv.extend([0], [1]), lambda: kv.append(0, a, a), lambda: kv.attend(0, a, a, 2), lambda: kv.read(0, [0], [0], 4, a, a)):
+                assert refused(call, "an earlier call") == "RuntimeError"
+            kv.info()
+            kv.destroy()
+    """)
+
+
 def test_binding_matches_the_header(tmp_path):
     import subprocess
     from pathlib import Path
