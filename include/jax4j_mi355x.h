@@ -375,7 +375,7 @@ typedef struct j4q_kv_append_args {
     int64_t kv_stride;       /* values from a row to the next, 0: dense; a multiple of 16 bytes */
     int32_t type;            /* of k, v, q: J4Q_KIND_F32 or J4Q_KIND_BF16 */
     int32_t heads;           /* of q */
-    const void *q;           /* NULL, or [rows][heads][head_dim]: turned as the keys are, into q_out (q itself or apart) */
+    const void *q;           /* NULL, or [rows][heads][head_dim]: turned as the keys are, into q_out (q itself or apart from all three) */
     void *q_out;
     int64_t q_stride;        /* of q and q_out */
     const j4q_rope *rope;    /* NULL: keys are stored as they are */
@@ -385,7 +385,7 @@ int j4q_kv_append(j4q_kv kv, int32_t layer, const j4q_kv_append_args *args, void
 
 typedef struct j4q_kv_attend_args {
     const void *q;           /* [rows][heads][head_dim], 16-byte aligned device memory */
-    void *out;               /* the same shape */
+    void *out;               /* the same shape: q itself, with its type and stride, or apart from it */
     int64_t q_stride, out_stride; /* values from a row to the next, 0: dense; a multiple of 16 bytes */
     int32_t q_type, out_type; /* J4Q_KIND_F32 or J4Q_KIND_BF16 */
     int32_t heads;           /* a multiple of kv_heads: query head h reads kv head h / (heads / kv_heads) */

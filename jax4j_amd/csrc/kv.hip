@@ -298,6 +298,15 @@ int check_stride(const char *op, const char *what, const void *p, int type, int6
     return J4Q_OK;
 }
 
+// Whether two tensors of rows `width` bytes wide share a byte.
+bool overlap(const void *a, int64_t a_stride, int64_t a_width, const void *b, int64_t b_stride, int64_t b_width, int64_t rows) {
+    const uintptr_t a0 = (uintptr_t)a, b0 = (uintptr_t)b;
+    if (a0 >= b0 + (rows - 1) * b_stride + b_width || b0 >= a0 + (rows - 1) * a_stride + a_width) return false;
+    if (a_stride != b_stride) return true;
+    const int64_t between = (int64_t)(b0 - a0) % a_stride, at = between < 0 ? between + a_stride : between;  // windows of the same rows
+    return at < a_width || at + b_width > a_stride;
+}
+
 // Tiles of 64 tokens that the workgroups of a call's sequences walk for one kv head: all of them, the longest walk's, and how many
 // workgroups and rows there are.
 struct Walks {
@@ -784,6 +793,11 @@ int j4q_kv_append(j4q_kv kv, int32_t layer, const j4q_kv_append_args *args, void
             return rc;
         a.heads = g.heads;
     }
+    const int64_t e = g.type == J4Q_KIND_BF16 ? 2 : 4, q_bytes = (int64_t)a.heads * k->c.head_dim * e;
+    if (g.q && ((g.q != g.q_out && overlap(g.q, a.q_stride * e, q_bytes, g.q_out, a.q_stride * e, q_bytes, k->step_rows)) ||
+                overlap(g.k, a.kv_stride * e, width * e, g.q_out, a.q_stride * e, q_bytes, k->step_rows) ||
+                overlap(g.v, a.kv_stride * e, width * e, g.q_out, a.q_stride * e, q_bytes, k->step_rows)))
+        return report_error(J4Q_EUNSUPPORTED, "kv append: q_out overlaps k, v, or q without being q itself");
     if ((rc = fill_rope("kv append", g.rope, k->c.head_dim, k->step_rows, false, &a.rope))) return rc;
     if (!k->step_checked) {
         for (size_t i = 0; i < k->step_seq.size(); i++) {
@@ -840,6 +854,10 @@ int j4q_kv_attend(j4q_kv kv, int32_t layer, const j4q_kv_attend_args *args, void
     if ((rc = check_stride("kv attend", "q", g.q, g.q_type, width, &a.q_stride)) ||
         (rc = check_stride("kv attend", "out", g.out, g.out_type, width, &a.out_stride)))
         return rc;
+    const int64_t qe = g.q_type == J4Q_KIND_BF16 ? 2 : 4, oe = g.out_type == J4Q_KIND_BF16 ? 2 : 4;
+    if ((g.q != g.out || g.q_type != g.out_type || a.q_stride != a.out_stride) &&
+        overlap(g.q, a.q_stride * qe, width * qe, g.out, a.out_stride * oe, width * oe, k->step_rows))
+        return report_error(J4Q_EUNSUPPORTED, "kv attend: out overlaps q without being q itself");
     a.window = g.window ? g.window : INT_MAX;
     a.sinks = g.sinks;
     a.group = g.heads / k->c.kv_heads;
@@ -937,9 +955,8 @@ int j4q_rope_into(const void *x, void *out, int type, int64_t rows, int32_t head
     if (!aligned(x, e) || !aligned(out, e)) return report_error(J4Q_EINVAL, "rope_into: x and out must be aligned to their values");
     if (rows > (INT64_MAX >> 20) / width)
         return report_error(J4Q_EUNSUPPORTED, "rope_into: %lld rows of %lld values", (long long)rows, (long long)width);
-    const uint8_t *a0 = (const uint8_t *)x, *b0 = (const uint8_t *)out;
-    const uint8_t *a1 = a0 + ((rows - 1) * x_stride + width) * (int64_t)e, *b1 = b0 + ((rows - 1) * out_stride + width) * (int64_t)e;
-    if (a0 < b1 && b0 < a1 && (a0 != b0 || x_stride != out_stride))
+    const int64_t b = (int64_t)e;
+    if ((x != out || x_stride != out_stride) && overlap(x, x_stride * b, width * b, out, out_stride * b, width * b, rows))
         return report_error(J4Q_EUNSUPPORTED, "rope_into: out overlaps x without being x itself");
     KvRope r;
     int rc = fill_rope("rope_into", rope, head_dim, rows, true, &r);

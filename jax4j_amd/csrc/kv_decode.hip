@@ -176,17 +176,15 @@ __global__ void __launch_bounds__(64 * waves_of(D), waves_of(D) / 4) decode_kern
         if (t0 + wave + kWaves < t1) look_up(vis.tile(t0 + wave + kWaves));
     }
 
-    const int rr = rg * R + col % R;
-    const bool real = rr < tokens * a.group;
-    const int p = len - tokens + (real ? rr / a.group : 0);  // the row's place
+    const int rr = min(rg * R + col % R, tokens * a.group - 1);  // a column that is no row's has the last row's
+    const int p = len - tokens + rr / a.group;               // the row's place
     const int first_low = max(p - a.window + 1, 0);          // its first token behind the window's edge
     // the row's digits: column col holds digit col / R (+ 2 in a second instruction)
     int qd[M][S][4];
     float weight[M];
     float q_scale;
     {
-        // a column that is no row's has the first row's
-        const int64_t at = (int64_t)(row0 + (real ? rr / a.group : 0)) * a.q_stride + (head * a.group + (real ? rr % a.group : 0)) * D;
+        const int64_t at = (int64_t)(row0 + rr / a.group) * a.q_stride + (head * a.group + rr % a.group) * D;
         float x[S][16], most = 0.0f, finite = 0.0f;
 #pragma unroll
         for (int s = 0; s < S; s++) {

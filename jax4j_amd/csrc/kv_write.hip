@@ -9,6 +9,7 @@
 // it is max(amax / 127, 2^-64); else the scale that is there, times the least power of two under which
 // every code fits 8 bits: the codes that are there are then divided by that power, which rounds them once more per
 // doubling, so that the error of a code stays below one step of the final scale (a half, and a quarter, an eighth.. before).
+// A block of zeros (its scale the least one) gets amax / 127 as one without tokens does.
 // A value that is not finite makes the whole block of its head NaN: the cache has no code for it, and NaN is not lost.
 #include "kv.h"
 
@@ -193,12 +194,16 @@ __device__ __forceinline__ float block_max(float v, float *red) {
     return fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
 }
 
-// The block's scale after values of magnitude up to amax, and 2^-k for the codes that are there.
+// The block's scale after values of magnitude up to amax, and what the codes that are there are multiplied by.
 __device__ __forceinline__ float next_scale(float amax, bool begun, float old, float *shrink) {
     *shrink = 1.0f;
     if (!(amax <= FLT_MAX)) return __builtin_nanf("");
     if (begun && old != old) return old;
-    if (!begun || old <= kKvMinScale) return fmaxf(amax / 127.0f, kKvMinScale);
+    if (!begun || old <= kKvMinScale) {
+        const float s = fmaxf(amax / 127.0f, kKvMinScale);
+        if (begun) *shrink = old / s;
+        return s;
+    }
     const float r = 1.0f / old;
     float a = amax;
     while (a * r >= 127.5f) {

@@ -65,7 +65,9 @@ class Held:
                     self.codes[lo:hi, h] = 0
                     continue
                 if lo == b * BLOCK or s <= TINY:
-                    s = max(top / np.float32(127), TINY)
+                    was, s = s, max(top / np.float32(127), TINY)
+                    if lo > b * BLOCK:
+                        self.codes[b * BLOCK:lo, h] = np.rint(self.codes[b * BLOCK:lo, h] * np.float32(was / s))
                 else:
                     k = 0
                     while np.float32(top * np.float32(0.5) ** k) * (np.float32(1) / s) >= np.float32(127.5):

@@ -178,6 +178,20 @@ def test_append_and_read(model, dim, page, kind, interleaved, rot):
             np.testing.assert_array_equal(x[i], m.of(1, s)[which].values(f, 33))
 
 
+@pytest.mark.parametrize("tiny", [1e-18, 6e-18, 1e-19])
+@pytest.mark.parametrize("size", [0.0, 1e-19, 7e-18, 2e-17, 1.0])
+def test_block_of_tiny_values(model, tiny, size):
+    """Codes of a block at the least scale stay what they stand for when another token sets the scale."""
+    m = model(kv_heads=1, head_dim=64, pages=4, page_tokens=16, sequences=2, sequence_pages=2)
+    rng = np.random.default_rng(5)
+    for n, scale in ((5, tiny), (1, size), (2, tiny), (1, 4 * size)):
+        k, v = scale * rng.uniform(-1, 1, (n, 1, 64)), scale * rng.uniform(-1, 1, (n, 1, 64))
+        m.kv.extend([0], [n])
+        m.write(0, [0], [n], k, v)
+        m.check([0])
+    assert np.abs(m.read(0, [0], [0], 5)[0]).max() < tiny + 2.0 ** -64 + 4 * size / 127  # one step of the scale in all
+
+
 def test_append_of_rows_apart_and_of_uneven_steps(model):
     """k and v inside wider rows; one sequence of many tokens beside many of one."""
     m = model(kv_heads=2, head_dim=64, pages=200, page_tokens=16, sequences=40, sequence_pages=100)
@@ -352,6 +366,24 @@ def test_attend_many_rows_extremes(model, okind):
     m.kv.attend(0, dq.data_ptr(), out.data_ptr(), 4, out_type=KIND[okind])
     got = np.isnan(host(out, okind)).reshape(390, 4, 128)
     assert got[5, 1].all() and got[100, 2].all() and got.sum() == 2 * 128
+
+
+@pytest.mark.parametrize("heads,tokens", [(4, 1), (6, 1), (10, 1), (6, 2), (6, 50)])
+def test_attend_in_place(model, heads, tokens):
+    """Out over q gives the bits that out apart from it gives, ranges of tokens and rows that do not fill a workgroup among them."""
+    m = model(kv_heads=2, head_dim=128, pages=400, page_tokens=16, sequences=3, sequence_pages=200)
+    rng = np.random.default_rng(heads)
+    lens = [3000, 70, tokens]
+    m.kv.extend([0, 1, 2], lens)
+    m.write(0, [0, 1, 2], lens, rng.standard_normal((sum(lens), 2, 128)), rng.standard_normal((sum(lens), 2, 128)))
+    m.kv.begin([0, 1, 2], [tokens] * 3)
+    q = dev(rng.standard_normal((3 * tokens, heads * 128)).astype(np.float32))
+    out = torch.zeros_like(q)
+    torch.cuda.synchronize()
+    m.kv.attend(0, q.data_ptr(), out.data_ptr(), heads)
+    m.kv.attend(0, q.data_ptr(), q.data_ptr(), heads)
+    torch.cuda.synchronize()
+    assert torch.equal(q, out) and bool(torch.isfinite(out).all())
 
 
 def test_attend_extremes(model):

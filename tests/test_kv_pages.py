@@ -259,6 +259,35 @@ def test_a_fork_of_what_the_call_itself_makes_is_refused(shim):
     """)
 
 
+def test_outputs_over_inputs(shim):
+    """In place or apart, columns of the same rows being apart; what lies across is refused."""
+    run(shim, """
+        kv = cache()
+        kv.extend([0, 1], [3, 20])  # 23 rows; heads of 64 floats: k, v 128 a row, q of 4 heads 256
+        a = address(1 << 20)
+        bad = "IllegalArgumentException"
+        row = 4 * (256 + 128 + 128)  # q, k, v of a fused product
+        append = lambda q_out, q=0: kv.append(0, a + 4 * 256, a + 4 * 384, q_ptr=a + q, q_out_ptr=a + q_out, heads=4, stride=512, q_stride=512)
+        append(0)
+        append(23 * row)
+        for q_out in (16, 4 * 256, 4 * 255 * 4, row, 3 * row + 1024, 22 * row):
+            assert refused(lambda: append(q_out), "overlaps") == bad, q_out
+        attend = lambda out, **k: kv.attend(0, a, a + out, 4, q_stride=512, **k)
+        attend(0, out_stride=512)
+        attend(4 * 256, out_stride=512)
+        attend(5 * row + 4 * 256, out_stride=512)
+        attend(23 * row)
+        for out, k in ((0, {}), (0, dict(out_stride=512, out_type=DType.BF16)), (16, dict(out_stride=512)), (4 * 256, {}), (row, dict(out_stride=512))):
+            assert refused(lambda: attend(out, **k), "overlaps") == bad, (out, k)
+        rope = Rope(a, a, 10, 64, positions=a)
+        turn = lambda out: be.rope_into(a, a + out, 23, 4, 64, rope, x_stride=512, out_stride=512)
+        turn(0)
+        turn(1024)
+        for out in (16, 1028, row, row - 16):
+            assert refused(lambda: turn(out), "overlaps") == bad, out
+    """)
+
+
 def test_no_host_memory(shim, monkeypatch):
     """Every call that finds too little host memory for its lists says so, and leaves the cache as it was."""
     monkeypatch.setenv("MALLOC_ARENA_MAX", "1")  # long lists neither from another thread's heap nor from what was freed
