@@ -95,9 +95,9 @@ __device__ __forceinline__ void store(void *p, int64_t i, bool bf16, const float
 // of heads (looked up by every item they were three times as many loads as the values), while the items' values are on
 // their way. In place is fine: a thread reads what it writes.
 constexpr int kRopePairs = 1024;  // of a workgroup's rows together
-// Items of a thread: a head in single pairs is one workgroup's; with pieces of 8 two items leave registers for 7 workgroups a CU.
-constexpr int rope_items(int v) { return v == 8 ? 2 : 4; }
-static_assert(256 * rope_items(1) >= kRopeMaxDim / 2 && 256 * rope_items(4) >= kRopeMaxDim / 8 && 256 * rope_items(8) >= kRopeMaxDim / 16, "");
+// Items of a thread: a head in single pairs is one workgroup's; else two, which leave registers for 6 workgroups a CU and more.
+constexpr int rope_items(int v) { return v == 1 ? 4 : 2; }
+static_assert(256 * rope_items(1) >= kRopeMaxDim / 2 && 256 * rope_items(4) >= 512 && 256 * rope_items(8) >= 512, "");  // see rope_grid
 struct RopeRows {
     const void *x;
     void *out;
@@ -134,7 +134,7 @@ __device__ __forceinline__ void rope_rows(const RopeRows &g, const KvRope &r, in
             const int k = t / r.pairs;
             int place = 0;
             if (step && !r.positions) {
-                const int i = sequence_of(step->row0, step->n, (int)row0 + k);
+                const int at = (int)row0 + k, i = step->rows == step->n ? at : sequence_of(step->row0, step->n, at);  // a token each: no search
                 place = step->len[i] - step->row0[i + 1] + (int)row0 + k;
             }
             angles[t] = turn_of(r, t - k * r.pairs, row0 + k, place);
@@ -216,11 +216,15 @@ __device__ __forceinline__ float next_scale(float amax, bool begun, float old, f
 __device__ __forceinline__ uint32_t code_of(float x, float r) { return (uint32_t)(int)rintf(x * r) & 0xffu; }
 __device__ __forceinline__ uint32_t shrink_of(uint32_t code, float f) { return (uint32_t)(int)rintf((float)(int8_t)code * f) & 0xffu; }
 
-// One block of 16 tokens of a kv head per workgroup, 256 threads; the workgroups behind them turn the queries.
+// One block of 16 tokens of a kv head per workgroup, 256 threads; the workgroups behind them, whose work is shorter, turn the
+// queries. A step of one token is bound by its chain of loads, so what does not need another load's answer goes with it:
+// values and the page, then scales, codes that are there and angles (64 sequences of a token, 8 kv heads of 128 and 32 query
+// heads: 6.5 us, and 5.9 so). A prompt is bound by memory: 16384 blocks 66 us, 5.0 TB/s (one load after the other 98); 2043
+// tokens with their queries 22.2 us, 4.0 TB/s.
 template <int D>
 __global__ void __launch_bounds__(256) append_kernel(KvAppend a) {
     constexpr int P = D + 4;
-    __shared__ float xs[2][kKvBlock][P];
+    __shared__ __align__(16) float xs[2][kKvBlock][P];
     __shared__ float red[2][4];
     const int tid = threadIdx.x;
     const int items = a.items * a.l.kv_heads;
@@ -247,26 +251,51 @@ __global__ void __launch_bounds__(256) append_kernel(KvAppend a) {
     const int b = start / kKvBlock + blk, lo = max(start, b * kKvBlock), hi = min(len, (b + 1) * kKvBlock);
     if (lo >= hi) return;
     const int page = a.step.table[(int64_t)a.step.seq[i] * a.step.sequence_pages + (b >> a.l.block_shift)];
-    if (page < 0) return;
     const int n = hi - lo, place = lo - b * kKvBlock;
+    constexpr int X = (kKvBlock * D / 4 + 255) / 256, A = (kKvBlock * D / 2 + 255) / 256;  // pieces of a thread: values, angles
+    float x[2][X][4];
+    float2 cs[A];
+    // t / pairs: half a step from a whole number is 2^-8 at least, and t is below 2^11
+    const float per_pair = __builtin_amdgcn_rcpf((float)a.rope.pairs);
+    auto row_of = [&](int t) { return (int)(((float)t + 0.5f) * per_pair); };
+#pragma unroll
+    for (int j = 0; j < X; j++) {
+        const int t = tid + 256 * j, r = t / (D / 4), d = (t - r * (D / 4)) * 4;
+        if (r >= n) break;
+        const int64_t at = (int64_t)(row0 + lo - start + r) * a.kv_stride + head * D + d;
+        load<4>(a.k, at, a.bf16 != 0, x[0][j]);
+        load<4>(a.v, at, a.bf16 != 0, x[1][j]);
+    }
+    if (page < 0) return;
     const int in_page = (head << a.l.block_shift) + (b & ((1 << a.l.block_shift) - 1));
     uint8_t *pg = a.l.base + (int64_t)page * a.l.page_bytes;
     uint8_t *kc = pg + in_page * (2 * kKvBlock * D), *vc = kc + kKvBlock * D;
     float *sc = (float *)(pg + a.l.scales) + 2 * in_page;
     const float old_k = place ? sc[0] : 0.0f, old_v = place ? sc[1] : 0.0f;
-    for (int t = tid; t < n * (D / 4); t += 256) {
-        const int r = t / (D / 4), d = (t - r * (D / 4)) * 4;
-        const int64_t at = (int64_t)(row0 + lo - start + r) * a.kv_stride + head * D + d;
-        load<4>(a.k, at, a.bf16 != 0, &xs[0][r][d]);
-        load<4>(a.v, at, a.bf16 != 0, &xs[1][r][d]);
+    uint4 was_v = make_uint4(0, 0, 0, 0);
+    if (tid < D && n < kKvBlock) was_v = *(const uint4 *)(vc + tid * kKvBlock);
+    if (a.rope.pairs)
+#pragma unroll
+        for (int j = 0; j < A; j++) {
+            const int t = tid + 256 * j, r = row_of(t);
+            if (r >= n) break;
+            cs[j] = turn_of(a.rope, t - r * a.rope.pairs, row0 + lo - start + r, lo + r);
+        }
+#pragma unroll
+    for (int j = 0; j < X; j++) {
+        const int t = tid + 256 * j, r = t / (D / 4), d = (t - r * (D / 4)) * 4;
+        if (r >= n) break;
+        *(float4 *)&xs[0][r][d] = make_float4(x[0][j][0], x[0][j][1], x[0][j][2], x[0][j][3]);
+        *(float4 *)&xs[1][r][d] = make_float4(x[1][j][0], x[1][j][1], x[1][j][2], x[1][j][3]);
     }
     __syncthreads();
     if (a.rope.pairs) {
-        for (int t = tid; t < n * a.rope.pairs; t += 256) {
-            const int r = t / a.rope.pairs, p = t - r * a.rope.pairs;
-            const float2 cs = turn_of(a.rope, p, row0 + lo - start + r, lo + r);
+#pragma unroll
+        for (int j = 0; j < A; j++) {
+            const int t = tid + 256 * j, r = row_of(t), p = t - r * a.rope.pairs;
+            if (r >= n) break;
             float *u = a.rope.interleaved ? &xs[0][r][2 * p] : &xs[0][r][p], *w = a.rope.interleaved ? u + 1 : u + a.rope.pairs;
-            turn(cs.x, cs.y, *u, *w);
+            turn(cs[j].x, cs[j].y, *u, *w);
         }
         __syncthreads();
     }
@@ -299,11 +328,9 @@ __global__ void __launch_bounds__(256) append_kernel(KvAppend a) {
             for (int j = 0; j < 4; j++) o |= shrink_of(*p >> (8 * j) & 0xff, fk) << (8 * j);
             *p = o;
         }
-    for (int d = tid; d < D; d += 256) {
+    if (const int d = tid; d < D) {
         uint4 *p = (uint4 *)(vc + d * kKvBlock);
-        uint4 o = make_uint4(0, 0, 0, 0);
-        if (n < kKvBlock) o = *p;
-        uint32_t w[4] = {o.x, o.y, o.z, o.w};
+        uint32_t w[4] = {was_v.x, was_v.y, was_v.z, was_v.w};
         for (int j = 0; j < kKvBlock; j++) {
             const int r = j - place;
             const uint32_t was = w[j / 4] >> (j % 4 * 8) & 0xff;
