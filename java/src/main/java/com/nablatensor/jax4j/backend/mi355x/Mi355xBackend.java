@@ -73,6 +73,7 @@ public final class Mi355xBackend implements ComputeBackend, QuantizedOps {
   /** Plans first, so that matrices they pinned can then be released. */
   private static void drainPending() {
     Mi355xDecodePlan.drainPending();
+    Mi355xKvCache.drainPending();
     Mi355xBuffer.drainPending();
   }
 
@@ -252,6 +253,26 @@ public final class Mi355xBackend implements ComputeBackend, QuantizedOps {
       long h = out.get(JAVA_LONG, 0);
       long[] d = dims(h);
       return new Mi355xBuffer(h, Shape.of(Math.toIntExact(d[0]), Math.toIntExact(d[1])), DType.F32, device, type);
+    }
+  }
+
+  /**
+   * A paged 8-bit key/value cache of `sequences` sequences in `layers` layers (see {@link Mi355xKvCache}): pages of 16, 32
+   * or 64 tokens, heads of 64, 96, 128, 192 or 256 channels, at most sequencePages pages of a sequence.
+   */
+  public Mi355xKvCache kvCache(int layers, int kvHeads, int headDim, int pageTokens, long pages, int sequences, int sequencePages) {
+    try (Arena a = Arena.ofConfined()) {
+      long h = newHandle("kvCache", Mi355xNative.KV_CREATE, Mi355xKvCache.config(a, layers, kvHeads, headDim, pageTokens, pages, sequences, sequencePages));
+      return new Mi355xKvCache(h, sequencePages);
+    }
+  }
+
+  /** Turns F32 heads x [rows, heads, headDim], dense, by rotary positions into out (x itself, or apart); device addresses. */
+  public void rope(long x, long out, long rows, int heads, int headDim, Mi355xKvCache.Rope rope) {
+    ensureInitialized();
+    try (Arena a = Arena.ofConfined()) {
+      Mi355xNative.call("rope", Mi355xNative.ROPE_INTO, MemorySegment.ofAddress(x), MemorySegment.ofAddress(out), Mi355xNative.KIND_F32, rows, heads,
+          headDim, 0L, 0L, rope.segment(a), MemorySegment.NULL);
     }
   }
 

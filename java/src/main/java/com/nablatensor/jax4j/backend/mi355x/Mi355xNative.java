@@ -27,6 +27,8 @@ final class Mi355xNative {
   static final int GEMM_INT8 = 0, GEMM_BF16 = 1;
   /** Batched GEMV arithmetic (enum j4q_gemv_policy). */
   static final int GEMV_MATRIX_CORES = 0, GEMV_FP32 = 1;
+  /** Kinds of values in caller memory (enum j4q_kind). */
+  static final int KIND_F32 = 2, KIND_BF16 = 3;
   /** j4q_buffer_desc: 48 bytes; dims at 16 and 24, device_ptr at 40. */
   static final long BUFFER_DESC_BYTES = 48, DESC_DIM0 = 16, DESC_DIM1 = 24, DESC_DEVICE_PTR = 40;
 
@@ -86,6 +88,32 @@ final class Mi355xNative {
       FunctionDescriptor.of(JAVA_INT, ADDRESS, JAVA_INT, JAVA_LONG, JAVA_LONG, ADDRESS, ADDRESS));
   static final MethodHandle PLAN_RUN = fn("j4q_decode_plan_run", FunctionDescriptor.of(JAVA_INT, JAVA_LONG, ADDRESS));
   static final MethodHandle PLAN_DESTROY = fn("j4q_decode_plan_destroy", FunctionDescriptor.of(JAVA_INT, JAVA_LONG));
+
+  // The 8-bit key/value cache (j4q_kv_*): sequences, counts and argument structs in host memory, the stream last.
+  static final MethodHandle KV_CREATE = fn("j4q_kv_create", FunctionDescriptor.of(JAVA_INT, ADDRESS, ADDRESS));
+  static final MethodHandle KV_DESTROY = fn("j4q_kv_destroy", FunctionDescriptor.of(JAVA_INT, JAVA_LONG));
+  static final MethodHandle KV_INFO = fn("j4q_kv_info", FunctionDescriptor.of(JAVA_INT, JAVA_LONG, ADDRESS));
+  static final MethodHandle KV_TABLES = fn("j4q_kv_tables",
+      FunctionDescriptor.of(JAVA_INT, JAVA_LONG, ADDRESS, JAVA_INT, ADDRESS, ADDRESS, JAVA_INT));
+  static final MethodHandle KV_EXTEND = fn("j4q_kv_extend",
+      FunctionDescriptor.of(JAVA_INT, JAVA_LONG, ADDRESS, ADDRESS, JAVA_INT, ADDRESS));
+  static final MethodHandle KV_BEGIN = fn("j4q_kv_begin",
+      FunctionDescriptor.of(JAVA_INT, JAVA_LONG, ADDRESS, ADDRESS, JAVA_INT, ADDRESS));
+  static final MethodHandle KV_FORK = fn("j4q_kv_fork",
+      FunctionDescriptor.of(JAVA_INT, JAVA_LONG, ADDRESS, ADDRESS, JAVA_INT, JAVA_INT, ADDRESS));
+  static final MethodHandle KV_TRUNCATE = fn("j4q_kv_truncate",
+      FunctionDescriptor.of(JAVA_INT, JAVA_LONG, ADDRESS, ADDRESS, JAVA_INT));
+  static final MethodHandle KV_EVICT = fn("j4q_kv_evict",
+      FunctionDescriptor.of(JAVA_INT, JAVA_LONG, ADDRESS, JAVA_INT, JAVA_INT, JAVA_INT, ADDRESS));
+  static final MethodHandle KV_COMPACT = fn("j4q_kv_compact", FunctionDescriptor.of(JAVA_INT, JAVA_LONG, ADDRESS, ADDRESS));
+  static final MethodHandle KV_APPEND = fn("j4q_kv_append",
+      FunctionDescriptor.of(JAVA_INT, JAVA_LONG, JAVA_INT, ADDRESS, ADDRESS));
+  static final MethodHandle KV_ATTEND = fn("j4q_kv_attend",
+      FunctionDescriptor.of(JAVA_INT, JAVA_LONG, JAVA_INT, ADDRESS, ADDRESS));
+  static final MethodHandle KV_READ = fn("j4q_kv_read",
+      FunctionDescriptor.of(JAVA_INT, JAVA_LONG, JAVA_INT, ADDRESS, ADDRESS, JAVA_LONG, JAVA_INT, ADDRESS, ADDRESS, ADDRESS));
+  static final MethodHandle ROPE_INTO = fn("j4q_rope_into",
+      FunctionDescriptor.of(JAVA_INT, ADDRESS, ADDRESS, JAVA_INT, JAVA_LONG, JAVA_INT, JAVA_INT, JAVA_LONG, JAVA_LONG, ADDRESS, ADDRESS));
 
   /** Status to the reference's exception types (HipRuntime.java:129-141; CpuBackend.java:698-714). */
   static void check(int status, String op) {
