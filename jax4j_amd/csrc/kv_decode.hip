@@ -20,6 +20,11 @@
 // The 32-bit sums of an output stay in the matrix instruction's accumulators over tiles for as long as no t passes m + 4 (m then
 // moves up, the sums go to fp32 and start again), so a tile costs no vector instruction per output. 2^26 x 127 x digits: 65536
 // tokens stay below 2^31 in every digit.
+//
+// A wave walks tiles of its own, loaded a tile ahead into registers, so that nothing but the last sum goes through LDS and no wave
+// waits for another. 8 kv heads of 128, 32 query heads, fp32: 64 sequences of up to 8191 tokens (681 MB) 115 us, 5.9 TB/s, where
+// a plain read reaches 6.0; 131071 tokens of one (269 MB), 32 ranges, 51 us and 5 to join them; 293 tokens 8, the latency of
+// one tile. 32 sequences in a window of 1024, heads of 64 (34 MB): 10 us.
 #include "kv.h"
 
 namespace j4q {

@@ -11,6 +11,12 @@
 // q (scaled by a power of two per row) and w in fp16 round by 2^-11, which a bf16 result hides; for an fp32 result both are a sum
 // of two fp16 (22 bits), twice the matrix instructions.
 // m moves only when a t passes it by 7 octaves (w < 2^15 then), so the outputs are rescaled rarely.
+//
+// 8 kv heads of 128, 32 query heads, a prompt of 8192 into bf16: 553 to 600 us (from one card to another), 917 to 994 TFLOP/s, 67
+// to 72 % of a plain matrix product's rate. Matrix instructions take 48 % of the SIMDs' cycles and vector ones 52 %: of
+// two waves on a SIMD they add, whether or not they are brought side by side (half a round apart, with a barrier more:
+// 2 % slower). Per tile and wave 32 of the first, 210 of the others: 32 exponentials, as many scalings, maxima (16, of three),
+// sums, 16 roundings, 40 for the wave's share of the conversion. Without the fences 2.3 % slower.
 #include <type_traits>
 
 #include "kv.h"
