@@ -1,6 +1,6 @@
 // The 8-bit key/value cache: its layout in memory and what its kernels are given. The host side (pages, tables, checks,
 // entry points) is kv.hip; kernels are in kv_write.hip (rotary positions, append, read, copies of pages), kv_decode.hip
-// (attention of few query rows) and kv_prefill.hip (of many).
+// (attention of few query rows) and kv_prefill.hip (of some, and of many).
 //
 // A pool holds [layer][page]; a page holds page_tokens (16, 32 or 64) consecutive tokens of one sequence in one layer:
 //   [kv head][block of 16 tokens] { K: int8 [16][D] | V: int8 [D][16] }   then   [kv head][block] { float K scale, V scale }
@@ -96,6 +96,7 @@ __host__ __device__ inline int kv_ranges(int tiles, const KvAttend &a) {
 
 constexpr int kKvSplits = 256;  // most ranges of a row's tokens
 hipError_t launch_kv_decode(const KvAttend &a, hipStream_t s, hipEvent_t done);
+hipError_t launch_kv_rows(const KvAttend &a, hipStream_t s, hipEvent_t done);
 hipError_t launch_kv_prefill(const KvAttend &a, hipStream_t s, hipEvent_t done);
 // The parts of every row in one: out = sum of part * 2^(max - largest) / the same of the sums.
 hipError_t launch_kv_join(const KvAttend &a, hipStream_t s, hipEvent_t done);

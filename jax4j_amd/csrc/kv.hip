@@ -23,8 +23,12 @@ namespace {
 
 // Rows of partial results that a cache has room for: (D + 2) floats each.
 constexpr int64_t kPartRows = 65536;
-// Query rows (tokens x group) of a sequence and kv head up to which the kernel for few rows runs.
-constexpr int kFewRows = 16;
+// Query rows (tokens x group) of a sequence and kv head up to which the kernel for few rows runs, which reads the cache once for
+// 8 rows, and that for some rows (32; heads up to 128, whose rows fit the registers). 8 kv heads of 128, fp32, the one and the
+// other: 16 rows of 500 tokens 9.8 and 12.1 us, of 8000 in 64 sequences 234 and 198; 20 rows 9.9 and 12.7, 313 and 200. Up to 16 the
+// short ones decide, and that a bf16 result comes of fp32 weights. Some rows and many: 32 rows of 8000 tokens in 64 sequences 203
+// us and 372, into bf16 186 and 220; of 500 in one 13.6 and 12.5, 12.5 and 11.5.
+constexpr int kFewRows = 16, kSomeRows = 32;
 
 struct Seq {
     int64_t len = 0;
@@ -347,6 +351,16 @@ void split_few(const Kv &k, bool captured, KvAttend *a) {
     set_splits(k, captured, w.most, std::max(w.most <= kAlone ? kAlone : kLeast, (w.tiles * k.c.kv_heads + kFilled - 1) / kFilled), a);
 }
 
+// Some rows: a workgroup is a CU's as well, whose 8 waves take a tile each in a round; ranges of 4 tiles beside each other where
+// there are workgroups to spare (one request, 24 rows of 8 kv heads of 128: 16 tiles 13.5 us in four ranges, 14.1 in one; 63
+// tiles 14.8 in ranges of 4, 15.6 of 8 and 17.7 of 16).
+void split_some(const Kv &k, bool captured, KvAttend *a) {
+    constexpr int64_t kFilled = 256, kAlone = 8, kLeast = 4;
+    a->row_tile = 32;
+    const Walks w = walks_of(k, *a);
+    set_splits(k, captured, w.most, std::max(w.most <= kAlone ? kAlone : kLeast, (w.tiles * k.c.kv_heads + kFilled - 1) / kFilled), a);
+}
+
 // Many rows: workgroups of 256, whose conversion of a tile serves the most rows, or of 128, two to a CU, which fill the chip sooner:
 // 8 kv heads of 128 with 4 query heads each, a chunk of 512 tokens behind 3584 (64 workgroups of 256) 54 us and with 128 58, the
 // last 64 tokens of 4096 (8) 32 and 27; a prompt of 2048, whose workgroups walk 1 to 32 tiles (256) 68 and 62, one of 8192
@@ -363,9 +377,11 @@ void split_many(const Kv &k, bool captured, KvAttend *a) {
     }
     a->splits = 1;
     a->split_tiles = INT_MAX / 2;
-    if (k.c.head_dim <= 128 && groups * k.c.kv_heads >= 448) return;
+    // rows that one workgroup of 128 holds (64 rows of 8000 tokens in 64 sequences: 277 us, of 256 with empty waves 519)
+    const bool wide = k.c.head_dim <= 128 && a->max_rows > 128;
+    if (wide && groups * k.c.kv_heads >= 448) return;
     Walks w = walks_of(k, *a);
-    if (k.c.head_dim > 128 || groups * k.c.kv_heads < 64 || 4 * w.tiles < 3 * w.most * w.groups) {
+    if (!wide || groups * k.c.kv_heads < 64 || 4 * w.tiles < 3 * w.most * w.groups) {
         a->row_tile = 128;
         if (groups * k.c.kv_heads >= 448) return;
         w = walks_of(k, *a);
@@ -817,9 +833,18 @@ int j4q_kv_append(j4q_kv kv, int32_t layer, const j4q_kv_append_args *args, void
     a.q_out = g.q_out;
     a.bf16 = g.type == J4Q_KIND_BF16;
     // workgroups by sequence, unless the steps are so uneven that most of them would have nothing to do
-    const int64_t even = (int64_t)k->step_most_blocks * (int64_t)k->step_seq.size();
-    a.max_blocks = even <= 4ll * k->step_blocks ? k->step_most_blocks : 0;
-    const int64_t items = a.max_blocks ? even : k->step_blocks;
+    int64_t most = k->step_most_blocks, blocks = k->step_blocks;
+    if (capturing(stream ? (hipStream_t)stream : abi::stream())) {  // a replay's tokens may lie across one block more
+        most = blocks = 0;
+        for (int32_t t : k->step_tokens) {
+            const int64_t b = (t - 1 + kKvBlock - 1) / kKvBlock + 1;
+            most = std::max(most, b);
+            blocks += b;
+        }
+    }
+    const int64_t even = most * (int64_t)k->step_seq.size();
+    a.max_blocks = even <= 4 * blocks ? (int32_t)most : 0;
+    const int64_t items = a.max_blocks ? even : blocks;
     if (items * k->c.kv_heads + (int64_t)k->step_rows * a.heads > INT_MAX)
         return report_error(J4Q_EUNSUPPORTED, "kv append: %d tokens of %d heads in a call", k->step_rows, std::max(a.heads, k->c.kv_heads));
     a.items = (int32_t)items;
@@ -862,17 +887,18 @@ int j4q_kv_attend(j4q_kv kv, int32_t layer, const j4q_kv_attend_args *args, void
     a.sinks = g.sinks;
     a.group = g.heads / k->c.kv_heads;
     const int n = (int)k->step_seq.size();
-    int64_t few = 0, many = 0;  // most rows of a sequence and kv head that either kernel has
+    const int some_rows = k->c.head_dim <= 128 ? kSomeRows : kFewRows;
+    int64_t few = 0, some = 0, many = 0;  // most rows of a sequence and kv head that each kernel has
     for (int i = 0; i < n; i++) {
         const Seq &q = k->seqs[(size_t)k->step_seq[(size_t)i]];
         const int64_t first = q.len - k->step_tokens[(size_t)i], rows = (int64_t)k->step_tokens[(size_t)i] * a.group;
         if (q.gone1 > q.gone0 && (q.gone1 - 1 > first - a.window || q.gone0 < a.sinks))
             return report_error(J4Q_EINVAL, "kv attend: tokens [%lld, %lld) of sequence %d are evicted, and the mask shows some of them",
                                 (long long)q.gone0, (long long)q.gone1, k->step_seq[(size_t)i]);
-        int64_t &most = rows > kFewRows ? many : few;
+        int64_t &most = rows > some_rows ? many : rows > kFewRows ? some : few;
         most = std::max(most, rows);
     }
-    if (many > 1 << 22 || n > 65535 || (few && (int64_t)k->c.kv_heads * ((few + 3) / 4) > 65535))
+    if (many > 1 << 22 || n > 65535)
         return report_error(J4Q_EUNSUPPORTED, "kv attend: %lld query rows of %d kv heads in %d sequences", (long long)std::max(few, many), k->c.kv_heads, n);
     a.l = k->layer(layer);
     a.step = k->step();
@@ -885,14 +911,19 @@ int j4q_kv_attend(j4q_kv kv, int32_t layer, const j4q_kv_attend_args *args, void
     a.part_ml = k->part + kPartRows * k->c.head_dim;
     if ((rc = abi::ready_locked())) return rc;
     Call c(*k, stream);
-    // sequences of few rows and of many, in a launch each
+    // sequences of few rows, of some and of many, in a launch each
     if (few && c.e == hipSuccess) {
         a.rows_from = 1, a.rows_to = kFewRows, a.max_rows = (int32_t)few;
         split_few(*k, c.captured, &a);
-        c.e = launch_kv_decode(a, c.s, c.event(!many));
+        c.e = launch_kv_decode(a, c.s, c.event(!some && !many));
+    }
+    if (some && c.e == hipSuccess) {
+        a.rows_from = kFewRows + 1, a.rows_to = some_rows, a.max_rows = (int32_t)some;
+        split_some(*k, c.captured, &a);
+        c.e = launch_kv_rows(a, c.s, c.event(!many));
     }
     if (many && c.e == hipSuccess) {
-        a.rows_from = kFewRows + 1, a.rows_to = INT_MAX, a.max_rows = (int32_t)many;
+        a.rows_from = some_rows + 1, a.rows_to = INT_MAX, a.max_rows = (int32_t)many;
         split_many(*k, c.captured, &a);
         c.e = launch_kv_prefill(a, c.s, c.event(true));
     }

@@ -31,6 +31,8 @@ typedef _Float16 v8h __attribute__((ext_vector_type(8)));
 typedef _Float16 v2h __attribute__((ext_vector_type(2)));
 typedef __bf16 v4b __attribute__((ext_vector_type(4)));
 typedef float v16f __attribute__((ext_vector_type(16)));
+typedef int v4i __attribute__((ext_vector_type(4)));
+typedef int v16i __attribute__((ext_vector_type(16)));
 
 constexpr float kUnit = 8.0f;  // the weight of t = m: 2^8
 constexpr float kHead = 7.0f;
@@ -56,6 +58,13 @@ __device__ __forceinline__ void codes_to_half(uint32_t c, uint32_t *out) {
     const v2h bias = {(_Float16)1152.0f, (_Float16)1152.0f};
     out[0] = __builtin_bit_cast(uint32_t, __builtin_bit_cast(v2h, __builtin_amdgcn_perm(0x64646464u, u, 0x04010400u)) - bias);
     out[1] = __builtin_bit_cast(uint32_t, __builtin_bit_cast(v2h, __builtin_amdgcn_perm(0x64646464u, u, 0x04030402u)) - bias);
+}
+
+// The same, 128 + code in units of 2^-24.
+__device__ __forceinline__ void biased_value(uint32_t c, uint32_t *out) {
+    const uint32_t u = c ^ 0x80808080u;
+    out[0] = __builtin_amdgcn_perm(u, u, 0x0c010c00u);
+    out[1] = __builtin_amdgcn_perm(u, u, 0x0c030c02u);
 }
 
 // 8 values from i on, 16-byte aligned.
@@ -327,7 +336,17 @@ __global__ void __launch_bounds__(64 * W, D <= 128 ? 2 : 1) prefill_kernel(KvAtt
         const int j0 = vis.tile(u) * kKvTile, j1 = j0 + kKvTile - 1;
         return j1 <= p_first && (j0 > p_last - a.window || j1 < a.sinks);
     };
-    for (int u = t0; u < t1;) {
+    // a wave without rows stages its share of the tiles and no more (32 rows of 128: 510 us, 220 so)
+    if (w0 > r1)
+        for (int u = t0; u < t1; u++) {
+            const int buf = (u - t0) & 1;
+#pragma unroll
+            for (int unit = 0; unit < 4 * N; unit++) stage_unit(buf ^ 1, unit);
+            fetch(tile_at(u + 2));
+            look_up(tile_at(u + 3));
+            __syncthreads();
+        }
+    for (int u = w0 > r1 ? t1 : t0; u < t1;) {
         for (; u < t1 && whole(u); u++) round(u, std::false_type());
         for (; u < t1 && !whole(u); u++) round(u, std::true_type());
     }
@@ -362,6 +381,274 @@ __global__ void __launch_bounds__(64 * W, D <= 128 ? 2 : 1) prefill_kernel(KvAtt
     }
 }
 
+// The same for up to 32 rows, where memory is the bound: a wave walks tiles of its own, as in kv_decode.hip, loaded a tile ahead, and
+// nothing goes through LDS but the last sum. What it loads is the operands as they are: 16 channels of a key, for the int8
+// instruction 32x32x32, and 16 tokens of a value channel, converted to fp16 for two steps of 32x32x16. Row m of a score product
+// is token 16 (m / 4 % 2) + 4 (m / 8) + m % 4, so that a lane's 16 scores are those of block l / 32 in order.
+// q enters as whole numbers over its row's largest magnitude, in digits to the base 256: two (16 bits) for a bf16 result, three
+// (24) for an fp32 one. For a bf16 result values enter as (128 + code) 2^-24, a code's byte as an fp16 number below the
+// normal ones, and 128 times the sum of the weights is subtracted in the end: a conversion of three instructions for four
+// codes instead of five. (An error of a weight then counts 128 times where it counted `code` times, at most as much as before for
+// the largest code.)
+// 8 kv heads of 128, 64 sequences of 8000 tokens (1.05 GB), 20 rows: 178 us into bf16, 5.9 TB/s, and 200 fp32; the kernel above
+// took 510 and 787. Pages looked up behind the loads of a tile, or a branch around these, let the compiler wait for them (117
+// us instead of 104, heads of 64); the conversion of keys to fp16 made it 272 fp32.
+template <int D, int P>
+__global__ void __launch_bounds__(512, 2) rows_kernel(KvAttend a) {
+    constexpr int W = 8, S = D / 32;         // waves; pieces of 16 channels that a lane has of a key, and blocks of 32 value channels
+    constexpr int kPitch = D + 4;
+    __shared__ __align__(16) float part[W][32][kPitch];
+    __shared__ float part_ml[W][32][2];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), col = lane & 31, half = lane >> 5;
+    const int i = blockIdx.z, head = blockIdx.y % a.l.kv_heads, rg = blockIdx.y / a.l.kv_heads;
+    const int row0 = a.step.row0[i], tokens = a.step.row0[i + 1] - row0, len = a.step.len[i], rows = tokens * a.group;
+    const int r0 = rg * 32, r1 = min(rows, r0 + 32) - 1;
+    if (r0 >= rows || rows < a.rows_from || rows > a.rows_to) return;
+    const int before = len - tokens;
+    const KvTiles vis = kv_tiles(before + r0 / a.group, before + r1 / a.group, a.window, a.sinks);
+    int t0 = 0, t1 = vis.count();
+    if (a.splits > 1) {
+        const int ranges = kv_ranges(vis.count(), a);
+        if ((int)blockIdx.x >= ranges) return;
+        t0 = blockIdx.x * a.split_tiles;
+        if ((int)blockIdx.x + 1 < ranges) t1 = t0 + a.split_tiles;
+    }
+    const int p_first = before + r0 / a.group, p_last = before + r1 / a.group;
+    const int row = min(r0 + col, r1), place = before + row / a.group;
+
+    const int32_t *table = a.step.table + (int64_t)a.step.seq[i] * a.step.sequence_pages;
+    const int last_block = (len - 1) / kKvBlock, in_mask = (1 << a.l.block_shift) - 1;
+    const int k_block = col >> 2 & 1, k_token = 4 * (col >> 3) + (col & 3);
+    v4i kraw[2][S];
+    uint4 vraw[2][S];
+    float2 sraw[2];
+    // Pages are looked up before the loads of the tile in front of theirs: a wait for them is none for those.
+    struct Pages {
+        int k[2], v[2];
+    } pages;
+    auto look_up = [&](int tile) {
+        Pages p;
+#pragma unroll
+        for (int sub = 0; sub < 2; sub++) {
+            p.k[sub] = table[min(tile * 4 + 2 * sub + k_block, last_block) >> a.l.block_shift];
+            p.v[sub] = table[min(tile * 4 + 2 * sub + half, last_block) >> a.l.block_shift];
+        }
+        return p;
+    };
+    // A page that is not there gives bytes that weigh nothing.
+    auto block_at = [&](int block, int page, int *in) {
+        *in = (head << a.l.block_shift) + (min(block, last_block) & in_mask);
+        return a.l.base + (int64_t)max(page, 0) * a.l.page_bytes;
+    };
+    auto fetch_k = [&](int tile, int sub, const Pages &p) {
+        int in;
+        const uint8_t *pg = block_at(tile * 4 + 2 * sub + k_block, p.k[sub], &in), *k = pg + in * (2 * kKvBlock * D) + k_token * D + half * 16;
+#pragma unroll
+        for (int s = 0; s < S; s++) kraw[sub][s] = *(const v4i *)(k + 32 * s);
+    };
+    auto fetch_v = [&](int tile, int sub, const Pages &p) {
+        int in;
+        const uint8_t *pg = block_at(tile * 4 + 2 * sub + half, p.v[sub], &in), *v = pg + in * (2 * kKvBlock * D) + kKvBlock * D + col * 16;
+        sraw[sub] = *(const float2 *)(pg + a.l.scales + 8 * in);
+#pragma unroll
+        for (int d = 0; d < S; d++) vraw[sub][d] = *(const uint4 *)(v + 512 * d);
+    };
+    if (t0 + wave < t1) {
+        const int tile = vis.tile(t0 + wave);
+        const Pages first = look_up(tile);
+        pages = look_up(vis.tile(min(t0 + wave + W, t1 - 1)));
+#pragma unroll
+        for (int sub = 0; sub < 2; sub++) {
+            fetch_k(tile, sub, first);
+            fetch_v(tile, sub, first);
+        }
+    }
+
+    constexpr int kDigits = P + 1;
+    constexpr float kMost = P == 1 ? 32600.0f : 8355000.0f;  // what the digits hold, and room for rounding
+    v4i q[kDigits][S];                                       // the lowest first
+    float qk;
+    {
+        const int64_t at = (int64_t)(row0 + row / a.group) * a.q_stride + (head * a.group + row % a.group) * D + 16 * half;
+        float x[S][16], most = 0.0f, finite = 0.0f;
+#pragma unroll
+        for (int s = 0; s < S; s++) {
+            load8(a.q, at + 32 * s, a.q_bf16, x[s]);
+            load8(a.q, at + 32 * s + 8, a.q_bf16, x[s] + 8);
+#pragma unroll
+            for (int j = 0; j < 16; j++) {
+                most = fmaxf(most, fabsf(x[s][j]));
+                finite = __builtin_fmaf(x[s][j], 0.0f, finite);  // else NaN
+            }
+        }
+        const Two both = swap32(finite);
+        // at least 2^-90, so that its reciprocal is finite
+        const float unit = fmaxf(max32(most), 0x1p-90f) / kMost, inv = 1.0f / unit;
+        qk = unit * a.scale + (both.a + both.b);
+#pragma unroll
+        for (int s = 0; s < S; s++)
+#pragma unroll
+            for (int n = 0; n < 4; n++) {
+                uint32_t v[4];
+#pragma unroll
+                for (int j = 0; j < 4; j++) v[j] = ((uint32_t)(int)rintf(x[s][4 * n + j] * inv) + 0x808080u) ^ 0x808080u;
+#pragma unroll
+                for (int g = 0; g < kDigits; g++) {
+                    uint32_t w = 0;
+#pragma unroll
+                    for (int j = 0; j < 4; j++) w |= (v[j] >> (8 * g) & 0xffu) << (8 * j);
+                    q[g][s][n] = (int)w;
+                }
+            }
+    }
+
+    v16f o[S];
+#pragma unroll
+    for (int d = 0; d < S; d++)
+#pragma unroll
+        for (int r = 0; r < 16; r++) o[d][r] = 0.0f;
+    float m_at = -__builtin_inff(), base = 0.0f, lim = -__builtin_inff(), l_sum = 0.0f, w_sum = 0.0f;
+    auto halves = [&](uint32_t c0, uint32_t c1) {
+        uint32_t h[4];
+        if constexpr (P == 1) biased_value(c0, h), biased_value(c1, h + 2);
+        else codes_to_half(c0, h), codes_to_half(c1, h + 2);
+        return __builtin_bit_cast(v8h, make_uint4(h[0], h[1], h[2], h[3]));
+    };
+    // One tile. The last one's round is another, since with a branch round the loads of the next the compiler waits for all of them.
+    auto round = [&](int u, auto more) {
+        constexpr bool kMore = decltype(more)::value;
+        const int tile = vis.tile(u), next = vis.tile(min(u + W, t1 - 1)), j0 = tile * kKvTile, j1 = j0 + kKvTile - 1;
+        const Pages at_next = pages;
+        if constexpr (kMore) pages = look_up(vis.tile(min(u + 2 * W, t1 - 1)));
+        const bool masked = !(j1 <= p_first && (j0 > p_last - a.window || j1 < a.sinks));
+#pragma unroll
+        for (int sub = 0; sub < 2; sub++) {
+            v16i high, low;
+            v16f t;
+#pragma unroll
+            for (int r = 0; r < 16; r++) high[r] = low[r] = 0;
+#pragma unroll
+            for (int s = 0; s < S; s++) high = __builtin_amdgcn_mfma_i32_32x32x32_i8(kraw[sub][s], q[kDigits - 1][s], high, 0, 0, 0);
+            if constexpr (P == 2) {
+#pragma unroll
+                for (int s = 0; s < S; s++) low = __builtin_amdgcn_mfma_i32_32x32x32_i8(kraw[sub][s], q[0][s], low, 0, 0, 0);
+            }
+#pragma unroll
+            for (int r = 0; r < 16; r++) high[r] *= 256;
+#pragma unroll
+            for (int s = 0; s < S; s++) high = __builtin_amdgcn_mfma_i32_32x32x32_i8(kraw[sub][s], q[kDigits - 2][s], high, 0, 0, 0);
+            if constexpr (kMore) fetch_k(next, sub, at_next);
+            const bool nan = sraw[sub].y != sraw[sub].y;
+            const float sv = nan ? 1.0f : fmaxf(sraw[sub].y, kKvMinScale), rsv = __builtin_amdgcn_rcpf(sv);
+            const float f = qk * sraw[sub].x, c = (nan ? sraw[sub].y : __builtin_amdgcn_logf(sv)) + base;
+            float most = -__builtin_inff();
+#pragma unroll
+            for (int r = 0; r < 16; r++) t[r] = __builtin_fmaf(P == 2 ? __builtin_fmaf((float)high[r], 256.0f, (float)low[r]) : (float)high[r], f, c);
+            if (masked) {
+                int at0 = j0 + 32 * sub + 16 * half;
+                asm volatile("" : "+v"(at0));  // else the comparisons are made in front of the branch, for every tile
+#pragma unroll
+                for (int r = 0; r < 16; r++) {
+                    const int at = at0 + r;
+                    const bool seen = (at <= place) & ((at > place - a.window) | (at < a.sinks));
+                    t[r] = seen ? t[r] : -__builtin_inff();
+                }
+            }
+#pragma unroll
+            for (int r = 0; r < 16; r++) most = fmaxf(most, t[r]);
+            if (__any(most > lim)) {
+                most = max32(most);
+                if (most > lim) {  // m moves up to the largest t
+                    const bool first = !(m_at > -__builtin_inff());
+                    const float up = first ? most : most - kUnit, shrink = first ? 0.0f : __builtin_amdgcn_exp2f(-up);
+                    m_at = first ? up : m_at + up;
+                    const float shift = kUnit - m_at - base;
+                    base = kUnit - m_at;
+                    lim = kUnit + kHead;
+                    l_sum *= shrink;
+                    w_sum *= shrink;
+#pragma unroll
+                    for (int r = 0; r < 16; r++) t[r] += shift;
+#pragma unroll
+                    for (int d = 0; d < S; d++)
+#pragma unroll
+                        for (int r = 0; r < 16; r++) o[d][r] *= shrink;
+                }
+            }
+            float sum = 0.0f;
+            v8h w[P][2];
+#pragma unroll
+            for (int r = 0; r < 16; r++) {
+                const float e = __builtin_amdgcn_exp2f(t[r]);
+                const _Float16 h = (_Float16)e;
+                w[0][r / 8][r % 8] = h;
+                if constexpr (P == 2) w[1][r / 8][r % 8] = (_Float16)(e - (float)h);
+                sum += e;
+            }
+            l_sum = __builtin_fmaf(sum, rsv, l_sum);
+            w_sum += sum;
+#pragma unroll
+            for (int d = 0; d < S; d++) {
+                const v8h v0 = halves(vraw[sub][d].x, vraw[sub][d].y), v1 = halves(vraw[sub][d].z, vraw[sub][d].w);
+#pragma unroll
+                for (int p = 0; p < P; p++) o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v0, w[p][0], o[d], 0, 0, 0);
+#pragma unroll
+                for (int p = 0; p < P; p++) o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v1, w[p][1], o[d], 0, 0, 0);
+            }
+            if constexpr (kMore) fetch_v(next, sub, at_next);
+        }
+    };
+    int u = t0 + wave;
+    for (; u + W < t1; u += W) round(u, std::true_type());
+    if (u < t1) round(u, std::false_type());
+
+    if constexpr (P == 1) {
+        const Two all = swap32(w_sum);
+#pragma unroll
+        for (int d = 0; d < S; d++)
+#pragma unroll
+            for (int r = 0; r < 16; r++) o[d][r] = __builtin_fmaf(o[d][r], 0x1p24f, -128.0f * (all.a + all.b));
+    }
+    const Two both = swap32(l_sum);
+#pragma unroll
+    for (int d = 0; d < S; d++)
+#pragma unroll
+        for (int g = 0; g < 4; g++)
+            *(float4 *)&part[wave][col][32 * d + 8 * g + 4 * half] = make_float4(o[d][4 * g], o[d][4 * g + 1], o[d][4 * g + 2], o[d][4 * g + 3]);
+    if (half == 0) {
+        part_ml[wave][col][0] = m_at;
+        part_ml[wave][col][1] = both.a + both.b;
+    }
+    __syncthreads();
+    for (int at = threadIdx.x; at < 32 * (D / 4); at += 512) {
+        const int in = at / (D / 4), d = (at - in * (D / 4)) * 4, r = r0 + in;
+        if (r > r1) break;
+        float most = -__builtin_inff(), total = 0.0f;
+        for (int w = 0; w < W; w++) most = fmaxf(most, part_ml[w][in][0]);
+        float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        for (int w = 0; w < W; w++) {
+            const float f = most > -__builtin_inff() ? __builtin_amdgcn_exp2f(part_ml[w][in][0] - most) : 1.0f;
+            const float4 x = *(const float4 *)&part[w][in][d];
+            sum.x = __builtin_fmaf(x.x, f, sum.x), sum.y = __builtin_fmaf(x.y, f, sum.y);
+            sum.z = __builtin_fmaf(x.z, f, sum.z), sum.w = __builtin_fmaf(x.w, f, sum.w);
+            total = __builtin_fmaf(part_ml[w][in][1], f, total);
+        }
+        if (a.splits > 1) {
+            const int64_t slot = (((int64_t)i * a.l.kv_heads + head) * a.max_rows + r) * a.splits + blockIdx.x;
+            *(float4 *)(a.part + slot * D + d) = sum;
+            if (d == 0) {
+                a.part_ml[2 * slot] = most;
+                a.part_ml[2 * slot + 1] = total;
+            }
+        } else {
+            const float f = total == 0.0f ? 0.0f : 1.0f / total;
+            const int64_t to = (int64_t)(row0 + r / a.group) * a.out_stride + (head * a.group + r % a.group) * D + d;
+            if constexpr (P == 1) *(v4b *)((uint16_t *)a.out + to) = v4b{(__bf16)(sum.x * f), (__bf16)(sum.y * f), (__bf16)(sum.z * f), (__bf16)(sum.w * f)};
+            else *(float4 *)((float *)a.out + to) = make_float4(sum.x * f, sum.y * f, sum.z * f, sum.w * f);
+        }
+    }
+}
+
 template <int W, int P>
 hipError_t prefill(const KvAttend &a, hipStream_t s, hipEvent_t done) {
     const dim3 grid((unsigned)(a.l.kv_heads * a.splits), (unsigned)((a.max_rows + 32 * W - 1) / (32 * W)), (unsigned)a.step.n);
@@ -375,7 +662,24 @@ hipError_t prefill(const KvAttend &a, hipStream_t s, hipEvent_t done) {
     return hipErrorInvalidValue;
 }
 
+template <int D, int P>
+hipError_t rows(const KvAttend &a, hipStream_t s, hipEvent_t done) {
+    const dim3 grid((unsigned)a.splits, (unsigned)(a.l.kv_heads * ((a.max_rows + 31) / 32)), (unsigned)a.step.n);
+    return launch_with_event(rows_kernel<D, P>, grid, dim3(512), s, done, a);
+}
+
 }  // namespace
+
+hipError_t launch_kv_rows(const KvAttend &a, hipStream_t s, hipEvent_t done) {
+    hipEvent_t last = a.splits > 1 ? nullptr : done;
+    hipError_t e = hipErrorInvalidValue;
+    switch (a.l.dim) {
+    case 64: e = a.out_bf16 ? rows<64, 1>(a, s, last) : rows<64, 2>(a, s, last); break;
+    case 96: e = a.out_bf16 ? rows<96, 1>(a, s, last) : rows<96, 2>(a, s, last); break;
+    case 128: e = a.out_bf16 ? rows<128, 1>(a, s, last) : rows<128, 2>(a, s, last); break;
+    }
+    return e == hipSuccess && a.splits > 1 ? launch_kv_join(a, s, done) : e;
+}
 
 hipError_t launch_kv_prefill(const KvAttend &a, hipStream_t s, hipEvent_t done) {
     hipEvent_t last = a.splits > 1 ? nullptr : done;

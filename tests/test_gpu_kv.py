@@ -321,6 +321,96 @@ def test_attend_many_rows(model, dim, group, page, okind):
 
 
 @pytest.mark.parametrize("okind", ["bf16", "f32"])
+@pytest.mark.parametrize("dim,group,tokens,page", [(64, 8, 3, 16), (64, 32, 1, 64), (96, 4, 5, 32), (128, 4, 8, 64), (128, 7, 4, 32), (128, 1, 17, 16),
+                                                   (128, 1, 32, 16), (128, 2, 9, 64), (192, 4, 6, 32), (256, 8, 4, 16)])
+def test_attend_some_rows(model, dim, group, tokens, page, okind):
+    """17 to 32 rows of a sequence (drafts that are verified): from the step alone to thousands of tokens in several ranges."""
+    m = model(kv_heads=2, head_dim=dim, pages=600, page_tokens=page, sequences=5, sequence_pages=300)
+    rng = np.random.default_rng(dim + group + tokens)
+    seqs, lens = [4, 0, 2, 1, 3], [tokens, tokens + 1, 128, 700, 3500]
+    m.grow(rng, seqs, lens, 2.0)
+    for window, sinks, more in ((0, 0, {}), (50, 3, dict(qkind="bf16", pad=8, scale=0.3)), (1, 0, {}), (130, 66, {}), (1700, 4, {})):
+        check_attend(m, rng, seqs, [tokens] * 5, 2 * group, window=window, sinks=sinks, okind=okind, begin=True, size=2.0, **more)
+
+
+@pytest.mark.parametrize("okind", ["bf16", "f32"])
+def test_attend_steps_of_every_kind(model, okind):
+    """Few, some and many rows in one call, each long and short."""
+    m = model(kv_heads=2, head_dim=128, pages=900, page_tokens=16, sequences=6, sequence_pages=400)
+    rng = np.random.default_rng(37)
+    seqs, tokens = [3, 0, 5, 1, 2, 4], [6, 1, 40, 4, 8, 100]
+    m.grow(rng, seqs, [3000, 2500, 20, 700, 1, 1500])
+    m.grow(rng, seqs, tokens)
+    for window, sinks in ((0, 0), (500, 4)):
+        check_attend(m, rng, seqs, tokens, 8, window=window, sinks=sinks, okind=okind)
+
+
+@pytest.mark.parametrize("okind", ["bf16", "f32"])
+def test_attend_some_rows_extremes(model, okind):
+    """Tokens far ahead, blocks of zeros and of values far below others', keys and queries of all magnitudes, rows that are not finite."""
+    m = model(kv_heads=1, head_dim=128, pages=160, page_tokens=16, sequences=3, sequence_pages=150)
+    rng = np.random.default_rng(41)
+    m.kv.extend([0, 1, 2], [400, 60, 1500])
+    k, v = rng.standard_normal((1960, 1, 128)), rng.standard_normal((1960, 1, 128))
+    k[100:104] *= 20
+    v[:16] *= 1e-3
+    v[200:240], k[300:320] = 0, 0
+    v[400:460] *= 1e-12
+    k[400:460] *= 1e12
+    k[460:480] += 3  # first tokens that draw the weight and give little
+    v[460:480] *= 1e-4
+    m.write(0, [0, 1, 2], [400, 60, 1500], k, v)
+    for size in (1e-20, 1.0, 3.0):
+        check_attend(m, rng, [0, 2], [8, 8], 4, size=size, begin=True, okind=okind)
+    check_attend(m, rng, [1], [7], 4, size=1e-12, begin=True, okind=okind)
+    q = rng.standard_normal((8, 4 * 128))
+    q[5, 130], q[2, 300] = np.nan, -np.inf
+    dq = dev(q.astype(np.float32))
+    out = dev_as(np.zeros((8, 512)), okind)[0]
+    m.kv.begin([0], [8])
+    torch.cuda.synchronize()
+    m.kv.attend(0, dq.data_ptr(), out.data_ptr(), 4, out_type=KIND[okind])
+    got = np.isnan(host(out, okind)).reshape(8, 4, 128)
+    assert got[5, 1].all() and got[2, 2].all() and got.sum() == 2 * 128
+
+
+@pytest.mark.parametrize("tokens", [6, 20])
+def test_captured_steps_of_several_tokens(model, tokens):
+    """The same of 24 and of 80 rows, while the sequence grows from one range of tokens to several."""
+    m = model(kv_heads=2, head_dim=128, pages=400, page_tokens=16, sequences=2, sequence_pages=300)
+    rng = np.random.default_rng(43)
+    m.grow(rng, [0, 1], [300, 5])
+    q, k, v = (torch.randn((2 * tokens, h, 128), device="cuda") for h in (8, 2, 2))
+    out = torch.zeros_like(q)
+    s = torch.cuda.Stream()
+    m.kv.extend([0, 1], [tokens] * 2)
+    g = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(g, stream=s):
+        m.kv.append(0, k.data_ptr(), v.data_ptr(), stream=s.cuda_stream)
+        m.kv.attend(0, q.data_ptr(), out.data_ptr(), 8, stream=s.cuda_stream)
+    for i in range(6):
+        if i:
+            m.kv.extend([0], [700])
+            more = [torch.randn((700, 2, 128), device="cuda") for _ in range(2)]
+            torch.cuda.synchronize()
+            m.kv.append(0, more[0].data_ptr(), more[1].data_ptr())
+            m.kv.extend([0, 1], [tokens] * 2)
+        torch.cuda.synchronize()
+        for x in (q, k, v):
+            x.copy_(torch.randn_like(x))
+        torch.cuda.synchronize()
+        g.replay()
+        torch.cuda.synchronize()
+        got = out.clone()
+        m.kv.append(0, k.data_ptr(), v.data_ptr())
+        m.kv.attend(0, q.data_ptr(), out.data_ptr(), 8)
+        torch.cuda.synchronize()
+        # other ranges of the tokens, so other roundings
+        assert torch.allclose(got, out, rtol=0, atol=1e-5 * float(v.abs().max() + 4)), i
+
+
+@pytest.mark.parametrize("okind", ["bf16", "f32"])
 def test_attend_uneven_steps(model, okind):
     """A chunk of a prompt beside sequences of one token and of a few, short and long."""
     m = model(kv_heads=2, head_dim=128, pages=900, page_tokens=16, sequences=6, sequence_pages=400)

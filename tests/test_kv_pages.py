@@ -234,6 +234,28 @@ def test_what_a_step_launches(shim):
     assert counts[:2] == [1, 1] and counts[2] <= 2 and counts[3:] == [2, 0]
 
 
+def test_captured_append_reaches_every_block_of_a_replay(shim):
+    """16 tokens at the beginning of a block are one block's, in a replay two blocks'; 400 uneven ones are up to 26 and 1."""
+    run(shim, """
+        kv = cache(pages=200, sequences=10, sequence_pages=100)
+        a = address(1 << 22)
+        def groups(stream):
+            log()
+            kv.append(0, a, a, stream=stream)
+            return int(launches()[0][3])
+        kv.extend([0, 1], [16, 16])
+        assert groups(0) == 2 * 2
+        fake.fake_capture(0x70, 1)
+        assert groups(0x70) == 2 * 2 * 2
+        fake.fake_capture(0x70, 0)
+        kv.extend(range(10), [400] + [1] * 9)
+        assert groups(0) == 2 * (25 + 9)
+        fake.fake_capture(0x70, 1)
+        assert groups(0x70) == 2 * (26 + 9)
+        fake.fake_capture(0x70, 0)
+    """)
+
+
 def test_memory_of_a_cache_is_given_back(shim):
     run(shim, """
         before = fake.fake_used()
