@@ -306,8 +306,9 @@ int j4q_decode_plan_destroy(j4q_plan plan);
  * that order; then per layer j4q_kv_append and j4q_kv_attend. Pages and lengths are host state: a call that cannot be
  * served changes nothing. Calls on one cache run in order, on whichever streams they are issued; under stream capture
  * only append and attend may be called, the caller orders the graph's launches, and a launch serves the step
- * that j4q_kv_extend or j4q_kv_begin have set up by then (of the sequences and tokens a sequence that it was captured
- * with). */
+ * that j4q_kv_extend or j4q_kv_begin have set up by then (as many sequences, in their order as many tokens each, as when it
+ * was captured). What append and attend refuse is then the caller's to avoid: a sequence forked behind its extend,
+ * masks that show evicted tokens. */
 typedef uint64_t j4q_kv; /* 0 is never a valid handle */
 
 typedef struct j4q_kv_config {

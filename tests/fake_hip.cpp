@@ -22,7 +22,7 @@ std::map<const void *, size_t> vars;
 std::set<void *> captured;   // streams under capture
 std::set<void *> exclusive;  // ... of which these forbid hipMalloc and hipFree meanwhile (the global mode)
 uint64_t capacity = 288ull << 30, used = 0;
-bool events_done = true, launches_fail = false;
+bool events_done = true;
 uintptr_t next_handle = 0x1000;
 hipError_t last = hipSuccess;
 std::string text, out;
@@ -65,7 +65,6 @@ void dealloc(void *p) {
 #define LOCK std::lock_guard<std::recursive_mutex> lk(mu)
 
 // ---- the test's side
-F void fake_fail_launches(int on) { launches_fail = on != 0; }
 F void fake_capacity(uint64_t n) { capacity = n; }
 F uint64_t fake_used() { return used; }
 // on: 0 ends the capture, 1 begins one in the relaxed mode, 2 in the global mode
@@ -172,13 +171,11 @@ F hipError_t hipOccupancyMaxActiveBlocksPerMultiprocessor(int *n, const void *f,
 }
 F hipError_t hipLaunchKernel(const void *f, dim3 g, dim3 b, void **, size_t, hipStream_t s) {
     LOCK;
-    if (launches_fail) return ret(hipErrorLaunchFailure);
     log("launch %s grid %u %u block %u on %p", kernels[f].c_str(), g.x, g.y, b.x, (void *)s);
     return hipSuccess;
 }
 F hipError_t hipExtLaunchKernel(const void *f, dim3 g, dim3 b, void **, size_t, hipStream_t s, hipEvent_t, hipEvent_t stop, int) {
     LOCK;
-    if (launches_fail) return ret(hipErrorLaunchFailure);
     log("launch %s grid %u %u block %u on %p done %p", kernels[f].c_str(), g.x, g.y, b.x, (void *)s, (void *)stop);
     return hipSuccess;
 }

@@ -3,6 +3,7 @@ what calls refuse, and what they launch."""
 from __future__ import annotations
 
 import ctypes as C
+import subprocess
 
 import pytest
 
@@ -346,9 +347,27 @@ def test_no_host_memory(shim, monkeypatch):
     """)
 
 
-def test_a_change_that_the_device_did_not_get(shim):
+@pytest.fixture(scope="module")
+def failing_shim(tmp_path_factory):
+    """The same runtime, whose launches fail while fake_fail_launches(1) holds."""
+    folder = tmp_path_factory.mktemp("failing_hip")
+    text = (fakehip.TESTS / "fake_hip.cpp").read_text()
+    for name in ("hipLaunchKernel", "hipExtLaunchKernel"):
+        head = f"F hipError_t {name}("
+        at = text.index("LOCK;", text.index(head)) + len("LOCK;")
+        text = text[:at] + " if (launches_fail) return ret(hipErrorLaunchFailure);" + text[at:]
+    at = text.index("F hipError_t hipLaunchKernel(")
+    text = text[:at] + "static bool launches_fail = false;\nF void fake_fail_launches(int on) { launches_fail = on != 0; }\n" + text[at:]
+    (folder / "fake_hip.cpp").write_text(text)
+    lib = folder / "fake_hip.so"
+    subprocess.run(["g++", "-std=c++17", "-O1", "-shared", "-fPIC", "-D__HIP_PLATFORM_AMD__", f"-I{fakehip.ROCM / 'include'}",
+                    "-o", str(lib), str(folder / "fake_hip.cpp")], check=True)
+    return lib
+
+
+def test_a_change_that_the_device_did_not_get(failing_shim):
     """Its tables are then not the host's: the cache is refused, and can be looked at and destroyed."""
-    run(shim, """
+    run(failing_shim, """
         a = address(1 << 20)
         for change in (lambda kv: kv.extend([1], [16]), lambda kv: kv.begin([0], [1]), lambda kv: kv.fork([0], [2]), lambda kv: kv.evict([0], 1),
                        lambda kv: (kv.truncate([3], [0]), kv.compact())):
