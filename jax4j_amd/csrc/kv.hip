@@ -342,10 +342,11 @@ void set_splits(const Kv &k, bool captured, int64_t most, int64_t split_tiles, K
 }
 
 // Few rows: one workgroup of a CU's registers each, so ranges where the rows alone leave CUs idle. Joining them costs 4 to 5 us, a
-// round of the 8 waves over a tile each 2.4 (one request, 8 kv heads of 128: 16 tiles 11.3 us in one range, 13.2 in two; 32
-// tiles 16.2 and, in four, 13.7; 128 tiles 46 and, in sixteen, 14.1).
+// round of the 8 waves over a tile each 2.4, and less where only four of them have one, alone on their SIMDs (one request, 8 kv
+// heads of 128: 11 tiles 10.0 us in one range, 10.7 in three; 16 tiles 11.3, and 13.2 in two; heads of 64 7.7, 9.2 in four; 32
+// tiles 16.2, 12.7 in four, 11.2 in eight; 128 tiles 46, 14.0 in sixteen, 12.9 in thirty-two).
 void split_few(const Kv &k, bool captured, KvAttend *a) {
-    constexpr int64_t kFilled = 256, kAlone = 16, kLeast = 8;
+    constexpr int64_t kFilled = 256, kAlone = 16, kLeast = 4;
     a->row_tile = a->max_rows <= 4 ? 4 : 8;
     const Walks w = walks_of(k, *a);
     set_splits(k, captured, w.most, std::max(w.most <= kAlone ? kAlone : kLeast, (w.tiles * k.c.kv_heads + kFilled - 1) / kFilled), a);
