@@ -341,25 +341,30 @@ void set_splits(const Kv &k, bool captured, int64_t most, int64_t split_tiles, K
     a->split_tiles = (int32_t)std::max(split_tiles, (most + a->splits - 1) / a->splits);
 }
 
+// One range up to `alone` tiles; else ranges of four or more that fill the CUs once.
+void split_filled(const Kv &k, bool captured, int64_t alone, KvAttend *a) {
+    constexpr int64_t kFilled = 256, kLeast = 4;
+    const Walks w = walks_of(k, *a);
+    if (w.groups * k.c.kv_heads >= kFilled / 2) alone = 32;
+    set_splits(k, captured, w.most, std::max(w.most <= alone ? alone : kLeast, (w.tiles * k.c.kv_heads + kFilled - 1) / kFilled), a);
+}
+
 // Few rows: one workgroup of a CU's registers each, so ranges where the rows alone leave CUs idle. Joining them costs 4 to 5 us, a
 // round of the 8 waves over a tile each 2.4, and less where only four of them have one, alone on their SIMDs (one request, 8 kv
 // heads of 128: 11 tiles 10.0 us in one range, 10.7 in three; 16 tiles 11.3, and 13.2 in two; heads of 64 7.7, 9.2 in four; 32
-// tiles 16.2, 12.7 in four, 11.2 in eight; 128 tiles 46, 14.0 in sixteen, 12.9 in thirty-two).
+// tiles 16.2, 12.7 in four, 11.2 in eight; 128 tiles 46, 14.0 in sixteen, 12.9 in thirty-two). Half of the CUs are better left idle
+// for up to 32 tiles (16 requests: 32 tiles 18.3 us in one range, 20.2 in two; 64 tiles 35.3 and 34.7).
 void split_few(const Kv &k, bool captured, KvAttend *a) {
-    constexpr int64_t kFilled = 256, kAlone = 16, kLeast = 4;
     a->row_tile = a->max_rows <= 4 ? 4 : 8;
-    const Walks w = walks_of(k, *a);
-    set_splits(k, captured, w.most, std::max(w.most <= kAlone ? kAlone : kLeast, (w.tiles * k.c.kv_heads + kFilled - 1) / kFilled), a);
+    split_filled(k, captured, 16, a);
 }
 
 // Some rows: a workgroup is a CU's as well, whose 8 waves take a tile each in a round; ranges of 4 tiles beside each other where
 // there are workgroups to spare (one request, 24 rows of 8 kv heads of 128: 16 tiles 13.5 us in four ranges, 14.1 in one; 63
 // tiles 14.8 in ranges of 4, 15.6 of 8 and 17.7 of 16).
 void split_some(const Kv &k, bool captured, KvAttend *a) {
-    constexpr int64_t kFilled = 256, kAlone = 8, kLeast = 4;
     a->row_tile = 32;
-    const Walks w = walks_of(k, *a);
-    set_splits(k, captured, w.most, std::max(w.most <= kAlone ? kAlone : kLeast, (w.tiles * k.c.kv_heads + kFilled - 1) / kFilled), a);
+    split_filled(k, captured, 8, a);
 }
 
 // Many rows: workgroups of 256, whose conversion of a tile serves the most rows, or of 128, two to a CU, which fill the chip sooner:
