@@ -60,13 +60,6 @@ __device__ __forceinline__ void codes_to_half(uint32_t c, uint32_t *out) {
     out[1] = __builtin_bit_cast(uint32_t, __builtin_bit_cast(v2h, __builtin_amdgcn_perm(0x64646464u, u, 0x04030402u)) - bias);
 }
 
-// The same, 128 + code in units of 2^-24.
-__device__ __forceinline__ void biased_value(uint32_t c, uint32_t *out) {
-    const uint32_t u = c ^ 0x80808080u;
-    out[0] = __builtin_amdgcn_perm(u, u, 0x0c010c00u);
-    out[1] = __builtin_amdgcn_perm(u, u, 0x0c030c02u);
-}
-
 // 8 values from i on, 16-byte aligned.
 __device__ __forceinline__ void load8(const void *p, int64_t i, int bf16, float *x) {
     if (bf16) {
@@ -386,10 +379,8 @@ __global__ void __launch_bounds__(64 * W, D <= 128 ? 2 : 1) prefill_kernel(KvAtt
 // instruction 32x32x32, and 16 tokens of a value channel, converted to fp16 for two steps of 32x32x16. Row m of a score product
 // is token 16 (m / 4 % 2) + 4 (m / 8) + m % 4, so that a lane's 16 scores are those of block l / 32 in order.
 // q enters as whole numbers over its row's largest magnitude, in digits to the base 256: two (16 bits) for a bf16 result, three
-// (24) for an fp32 one. For a bf16 result values enter as (128 + code) 2^-24, a code's byte as an fp16 number below the
-// normal ones, and 128 times the sum of the weights is subtracted in the end: a conversion of three instructions for four
-// codes instead of five. (An error of a weight then counts 128 times where it counted `code` times, at most as much as before for
-// the largest code.)
+// (24) for an fp32 one. Values enter as the codes that they are: with a bias that is taken off in the end (three instructions for
+// four codes instead of five) every weight's rounding counts 128 times in every channel, however small its codes.
 // 8 kv heads of 128, 64 sequences of 8000 tokens (1.05 GB), 20 rows: 178 us into bf16, 5.9 TB/s, and 200 fp32; the kernel above
 // took 510 and 787. Pages looked up behind the loads of a tile, or a branch around these, let the compiler wait for them (117
 // us instead of 104, heads of 64); the conversion of keys to fp16 made it 272 fp32.
@@ -507,11 +498,10 @@ __global__ void __launch_bounds__(512, 2) rows_kernel(KvAttend a) {
     for (int d = 0; d < S; d++)
 #pragma unroll
         for (int r = 0; r < 16; r++) o[d][r] = 0.0f;
-    float m_at = -__builtin_inff(), base = 0.0f, lim = -__builtin_inff(), l_sum = 0.0f, w_sum = 0.0f;
+    float m_at = -__builtin_inff(), base = 0.0f, lim = -__builtin_inff(), l_sum = 0.0f;
     auto halves = [&](uint32_t c0, uint32_t c1) {
         uint32_t h[4];
-        if constexpr (P == 1) biased_value(c0, h), biased_value(c1, h + 2);
-        else codes_to_half(c0, h), codes_to_half(c1, h + 2);
+        codes_to_half(c0, h), codes_to_half(c1, h + 2);
         return __builtin_bit_cast(v8h, make_uint4(h[0], h[1], h[2], h[3]));
     };
     // One tile. The last one's round is another, since with a branch round the loads of the next the compiler waits for all of them.
@@ -566,7 +556,6 @@ __global__ void __launch_bounds__(512, 2) rows_kernel(KvAttend a) {
                     base = kUnit - m_at;
                     lim = kUnit + kHead;
                     l_sum *= shrink;
-                    w_sum *= shrink;
 #pragma unroll
                     for (int r = 0; r < 16; r++) t[r] += shift;
 #pragma unroll
@@ -586,7 +575,6 @@ __global__ void __launch_bounds__(512, 2) rows_kernel(KvAttend a) {
                 sum += e;
             }
             l_sum = __builtin_fmaf(sum, rsv, l_sum);
-            w_sum += sum;
 #pragma unroll
             for (int d = 0; d < S; d++) {
                 const v8h v0 = halves(vraw[sub][d].x, vraw[sub][d].y), v1 = halves(vraw[sub][d].z, vraw[sub][d].w);
@@ -602,13 +590,6 @@ __global__ void __launch_bounds__(512, 2) rows_kernel(KvAttend a) {
     for (; u + W < t1; u += W) round(u, std::true_type());
     if (u < t1) round(u, std::false_type());
 
-    if constexpr (P == 1) {
-        const Two all = swap32(w_sum);
-#pragma unroll
-        for (int d = 0; d < S; d++)
-#pragma unroll
-            for (int r = 0; r < 16; r++) o[d][r] = __builtin_fmaf(o[d][r], 0x1p24f, -128.0f * (all.a + all.b));
-    }
     const Two both = swap32(l_sum);
 #pragma unroll
     for (int d = 0; d < S; d++)

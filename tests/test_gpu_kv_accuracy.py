@@ -1,0 +1,110 @@
+"""How near attention over the 8-bit cache comes to the formula in 64 bits, row by row, relative to the row's own size.
+
+The bars of test_gpu_kv.py bound the worst case by the largest value of a sequence; a mean of thousands of values is far smaller
+than that. Here an error is the 2-norm over a row's channels (or over some of them, with codes small beside the others')
+of the difference, over that of the row.
+
+A bf16 result is off by 2^-8 of each channel at most. Fp16 weights are off by 2^-11 of themselves at most, in any direction, so the
+row by no more than that share of it (errors of one sign are a factor, others average as the values do). Queries are in bf16
+here, which fp16 holds as they are; as whole numbers of 16 bits over the row's largest magnitude they are off by max|q| / 65200 in any
+direction, at most, by 1/sqrt(3) of it in the mean square, so a score by d = scale |k| max|q| / 65200 / sqrt(3), and a row by as
+much of its size; five times that covers the rows of a call.
+"""
+from __future__ import annotations
+
+import numpy as np
+import pytest
+import torch
+
+import kv_ref as R
+from test_gpu_kv import KIND, dev_as, host, model  # noqa: F401
+
+gpu = pytest.mark.gpu
+
+
+def exact(q, k, v, first, window=0, sinks=0):
+    """Rows q [rows, heads, dim] at places first.. to k, v [tokens, kv heads, dim], all finite, in 64 bits."""
+    q, k, v = (x.astype(np.float64) for x in (q, k, v))
+    rows, heads, dim = q.shape
+    g, out = heads // k.shape[1], np.empty(q.shape)
+    p, j = first + np.arange(rows)[:, None], np.arange(k.shape[0])[None]
+    seen = j <= p
+    if window:
+        seen &= (j > p - window) | (j < sinks)
+    for h in range(heads):
+        s = np.where(seen, q[:, h] @ k[:, h // g].T * dim ** -0.5, -np.inf)
+        w = np.exp(s - s.max(1, keepdims=True))
+        out[:, h] = w @ v[:, h // g] / w.sum(1, keepdims=True)
+    return out
+
+
+def off(got, want, groups=None):
+    """The largest error of a row and head, over each group of channels."""
+    groups = [slice(None)] if groups is None else groups
+    return max(float((np.linalg.norm((got - want)[..., g], axis=-1) / np.linalg.norm(want[..., g], axis=-1)).max()) for g in groups)
+
+
+def bar(q, k):
+    most = np.abs(q).max() / 65200 / 3 ** 0.5
+    return 2.0 ** -8 + 2.0 ** -11 + 5 * most * np.linalg.norm(k, axis=-1).max() * q.shape[-1] ** -0.5
+
+
+def attend(m, q, window=0, sinks=0):
+    """The step's queries, into bf16."""
+    rows, heads, dim = q.shape
+    dq, _ = dev_as(q, "bf16")
+    out = dev_as(np.zeros((rows, heads, dim)), "bf16")[0]
+    torch.cuda.synchronize()
+    m.kv.attend(0, dq.data_ptr(), out.data_ptr(), heads, q_type=KIND["bf16"], out_type=KIND["bf16"], window=window, sinks=sinks)
+    return host(out, "bf16")
+
+
+def bf16(x):
+    return R.from_bf16(R.to_bf16(x))
+
+
+# rows of a kv head of the kernels for some rows and for many (workgroups of 128 rows and of 256)
+@gpu
+@pytest.mark.parametrize("dim,heads,tokens", [(64, 4, 6), (96, 8, 4), (128, 4, 8), (128, 4, 20), (128, 4, 600), (256, 4, 20)])
+@pytest.mark.parametrize("length,size", [(40, 4.0), (700, 1.0), (3500, 1.0)])
+def test_channels_of_small_codes(model, dim, heads, tokens, length, size):  # noqa: F811
+    """Channels whose values are a tenth and a thirtieth of the others': codes up to 13 and 4 beside 127. From weights on a few
+    tokens to means of all."""
+    m = model(kv_heads=1, head_dim=dim, pages=300, page_tokens=16, sequences=1, sequence_pages=300)
+    rng = np.random.default_rng(dim + tokens + length)
+    k, v = (rng.standard_normal((length + tokens, 1, dim)) for _ in range(2))
+    part = np.arange(dim) % 3
+    v *= np.array([1, 0.1, 1 / 30])[part]
+    m.kv.extend([0], [length + tokens])
+    m.write(0, [0], [length + tokens], k, v)
+    m.kv.begin([0], [tokens])
+    q = bf16(size * rng.standard_normal((tokens, heads, dim)))
+    k, v = (h.values() for h in m.of(0, 0))
+    want = exact(q, k, v, length)
+    e = off(attend(m, q), want, [part == i for i in range(3)])
+    assert e <= bar(q, k), f"off by {e:.3g} of a row, bar {bar(q, k):.3g}"
+
+
+@gpu
+@pytest.mark.parametrize("dim,heads,tokens", [(64, 4, 6), (96, 8, 4), (128, 4, 8), (128, 4, 20), (128, 4, 600), (256, 4, 20)])
+@pytest.mark.parametrize("ahead", [0.2, 1.3, 4.5])
+def test_equal_weights_behind_leading_tokens(model, dim, heads, tokens, ahead):  # noqa: F811
+    """A token of every 64 ahead, the others of the same key, blocks of one scale: weights whose roundings are all the same, under
+    values whose mean is small."""
+    length = 6000
+    m = model(kv_heads=1, head_dim=dim, pages=450, page_tokens=16, sequences=1, sequence_pages=450)
+    rng = np.random.default_rng(dim + tokens)
+    one = rng.standard_normal(dim)
+    k = np.repeat(one[None, None], length + tokens, 0)
+    q = bf16(one + 0.02 * rng.standard_normal((tokens, heads, dim)))
+    k[::64, 0] += ahead * one / (one @ one) * dim ** 0.5
+    v = rng.standard_normal((length + tokens, 1, dim))
+    v[:, 0, 0] = 5 * rng.choice([-1, 1], length + tokens)  # the largest of every block
+    v[::64] = 0
+    m.kv.extend([0], [length + tokens])
+    m.write(0, [0], [length + tokens], k, v)
+    m.kv.begin([0], [tokens])
+    k, v = (h.values() for h in m.of(0, 0))
+    want = exact(q, k, v, length)
+    e = off(attend(m, q), want)
+    assert e <= bar(q, k), f"off by {e:.3g} of a row, bar {bar(q, k):.3g}"
