@@ -41,6 +41,13 @@ struct RelaxedCapture {
     ~RelaxedCapture() { (void)hipThreadExchangeStreamCaptureMode(&mode); }
 };
 
+inline bool completed(hipEvent_t e) {
+    const RelaxedCapture relaxed;
+    const bool is = hipEventQuery(e) == hipSuccess;
+    (void)hipGetLastError();
+    return is;
+}
+
 class BlockCache {
 public:
     static constexpr uint64_t kMaxBlock = 4ull << 20, kMaxBytes = 64ull << 20;
@@ -151,11 +158,6 @@ private:
         if (t.ptr) (void)hipFree(t.ptr);
         if (t.done) (void)hipEventDestroy(t.done);
     }
-    static bool idle(const Slot &t) {
-        const bool is = hipEventQuery(t.done) == hipSuccess;
-        (void)hipGetLastError();
-        return is;
-    }
     static hipEvent_t new_event() {
         hipEvent_t e = nullptr;
         if (hipEventCreateWithFlags(&e, hipEventDisableTiming | hipEventDisableSystemFence) != hipSuccess) {
@@ -171,7 +173,7 @@ private:
         while (want < bytes) want *= 2;
         if (bytes_ + want > kMaxAll)  // what no call uses any more (hipFree waits for the device)
             for (size_t i = shared_.size(); i-- > 0;)
-                if (idle(shared_[i])) {
+                if (completed(shared_[i].done)) {
                     drop(shared_[i]);
                     bytes_ -= shared_[i].bytes;
                     shared_.erase(shared_.begin() + (long)i);
@@ -215,11 +217,9 @@ private:
         Slot *best = nullptr;
         for (Slot &t : shared_)
             if (t.bytes >= bytes && t.last == s) best = &t;
-        if (!best) {
-            const RelaxedCapture relaxed;
+        if (!best)
             for (Slot &t : shared_)
-                if (!best && t.bytes >= bytes && idle(t)) best = &t;
-        }
+                if (!best && t.bytes >= bytes && completed(t.done)) best = &t;
         if (!best) {
             Slot t;
             t.done = new_event();

@@ -1,0 +1,90 @@
+"""Calls on one key/value cache over streams whose handles do not tell them apart: every result is that of the calls in order."""
+from __future__ import annotations
+
+import threading
+
+import numpy as np
+import pytest
+import torch
+
+from jax4j_amd import _native as N
+from test_gpu_kept_memory import Hip
+from test_gpu_kv import dev, model  # noqa: F401
+
+pytestmark = pytest.mark.gpu
+
+
+class Steps:
+    """Tokens of one sequence, appended and attended to."""
+
+    def __init__(self, model):  # noqa: F811
+        self.kv = model(kv_heads=2, head_dim=128, pages=100, page_tokens=16, sequences=1, sequence_pages=100).kv
+        rng = np.random.default_rng(7)
+        self.k, self.v, self.q = (dev(rng.standard_normal((12, 100, h, 128)).astype(np.float32)) for h in (2, 2, 8))
+        self.out = torch.zeros_like(self.q)
+        torch.cuda.synchronize()
+
+    def append(self, i, stream):
+        self.kv.extend([0], [100], stream=stream)
+        self.kv.append(0, self.k[i].data_ptr(), self.v[i].data_ptr(), stream=stream)
+
+    def attend(self, i, stream):
+        self.kv.attend(0, self.q[i].data_ptr(), self.out[i].data_ptr(), 8, stream=stream)
+
+    def check(self, n):
+        torch.cuda.synchronize()
+        got = self.out.clone()
+        self.kv.truncate([0], [0])
+        for i in range(n):
+            self.append(i, 0)
+            self.attend(i, 0)
+        torch.cuda.synchronize()
+        assert torch.equal(got[:n], self.out[:n]) and bool(self.out[:n].abs().amax((1, 2, 3)).min() > 0)
+
+
+def test_one_handle_in_two_threads(model):  # noqa: F811
+    """hipStreamPerThread: appended behind a long kernel in one thread, attended to in another, and back."""
+    steps, lib = Steps(model), N.load()
+    turn, failed = [threading.Event() for _ in range(14)], []
+
+    def work(me):
+        try:
+            for i in range(12):
+                if i % 2 == me:
+                    assert turn[i].wait(60)
+                    if i:
+                        steps.attend(i - 1, 2)
+                    assert lib.j4q_spin(500, 2) == 0
+                    steps.append(i, 2)
+                    turn[i + 1].set()
+            assert turn[13].wait(60)  # its stream lives until all is done
+        except BaseException as e:
+            failed.append(e)
+        finally:
+            for t in turn:
+                t.set()
+
+    threads = [threading.Thread(target=work, args=(me,)) for me in (0, 1)]
+    for t in threads:
+        t.start()
+    turn[0].set()
+    assert turn[12].wait(60)
+    steps.attend(11, 0)
+    torch.cuda.synchronize()
+    turn[13].set()
+    for t in threads:
+        t.join(60)
+    assert not failed, failed
+    steps.check(12)
+
+
+def test_a_stream_created_where_one_was_destroyed(model):  # noqa: F811
+    steps, lib, hip = Steps(model), N.load(), Hip()
+    for i in range(12):
+        assert lib.j4q_spin(500, hip.stream) == 0
+        steps.append(i, hip.stream.value)
+        hip.ok("hipStreamDestroy", hip.stream)  # its calls are still queued
+        hip = Hip()
+        steps.attend(i, hip.stream.value)
+    hip.close()
+    steps.check(12)

@@ -1,0 +1,33 @@
+"""The order of calls on one key/value cache over the streams that they come on, without a GPU (fakehip.py)."""
+from __future__ import annotations
+
+import pytest
+
+from test_kv_pages import run, shim  # noqa: F401
+
+
+@pytest.mark.parametrize("handle", [1, 2, 0x70], ids=["hipStreamLegacy", "hipStreamPerThread", "a stream's"])
+def test_an_equal_handle_may_be_another_stream(shim, handle):  # noqa: F811
+    """A thread's own stream has the same handle in every thread, a new stream may have that of one destroyed: a call waits for the
+    call before it, unless that one is done."""
+    run(shim, f"""
+        kv = cache(pages=60, sequences=4, sequence_pages=60)
+        a = address(1 << 20)
+        kv.extend([0], [20], stream={handle})
+        def waits(call):
+            lines = log()
+            call()
+            return [l.split()[0] for l in log() if l.split()[0] in ("wait", "record", "launch")]
+        calls = (lambda s: kv.append(0, a, a, stream=s), lambda s: kv.attend(0, a, a + 65536, 2, stream=s), lambda s: kv.read(0, [0], [0], 4, a, a, stream=s),
+                 lambda s: kv.begin([0], [1], stream=s), lambda s: kv.fork([0], [1], stream=s), lambda s: kv.extend([0], [1], stream=s))
+        for call in calls:
+            for done in (0, 1):
+                kv.truncate([1], [0])
+                fake.fake_events_done(done)
+                got = waits(lambda: call({handle}))
+                assert got[:2] == (["launch"] if done else ["wait", "launch"])[:len(got)] and "record" not in got, got
+        fake.fake_events_done(0)
+        # the engine's own is one stream: nothing there, and what leaves it or comes to it waits
+        got = [waits(lambda: kv.attend(0, a, a + 65536, 2, stream=s)) for s in (0, 0, {handle}, 0)]
+        assert got == [["wait", "launch"], ["launch"], ["record", "wait", "launch"], ["wait", "launch"]], got
+    """)
