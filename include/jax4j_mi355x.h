@@ -304,7 +304,8 @@ int j4q_decode_plan_destroy(j4q_plan plan);
  *
  * A step: j4q_kv_extend names the sequences and how many tokens each gets; rows of q, k, v and out are these tokens in
  * that order; then per layer j4q_kv_append and j4q_kv_attend. Pages and lengths are host state: a call that cannot be
- * served changes nothing. Calls on one cache run in order, on whichever streams they are issued; under stream capture
+ * served changes nothing. Calls on one cache run in order, on whichever streams they are issued (but from the engine
+ * stream to another one only while the engine stream is not under capture); under stream capture
  * only append and attend may be called, the caller orders the graph's launches, and a launch serves the step
  * that j4q_kv_extend or j4q_kv_begin have set up by then (as many sequences, in their order as many tokens each, as when it
  * was captured). What append and attend refuse is then the caller's to avoid: a sequence forked behind its extend,

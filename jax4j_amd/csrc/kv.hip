@@ -139,15 +139,20 @@ struct Call {
     bool captured;
     hipError_t e = hipSuccess;
 
-    Call(Kv &kv, void *stream) : k(kv), s(stream ? (hipStream_t)stream : abi::stream()) {
-        captured = capturing(s);
+    Call(Kv &kv, void *stream) : k(kv), s(stream ? (hipStream_t)stream : abi::stream()), captured(capturing(s)) {}
+    bool from_engine() const { return k.used && k.last == abi::stream() && s != k.last; }
+    // Before anything changes: whether the call can go out on its stream. capture: why a captured graph cannot hold it, or nullptr.
+    int check(const char *op, const char *capture) const {
+        if (captured) return capture ? report_error(J4Q_EINVAL, "%s: %s", op, capture) : J4Q_OK;
+        if (from_engine() && capturing(abi::stream()))  // an event recorded there now would draw this call into the graph
+            return report_error(J4Q_EINVAL, "%s: another stream cannot wait for the cache's last call while the engine stream, where that is, is captured", op);
+        return J4Q_OK;
+    }
+    // Before the first launch.
+    void order() {
         if (captured || !k.used) return;
-        if (k.last == abi::stream()) {
-            if (s == k.last) return;
-            e = hipEventRecord(k.done, k.last);
-        } else if (s == k.last && completed(k.done)) {
-            return;
-        }
+        if (from_engine()) e = hipEventRecord(k.done, k.last);
+        else if (s == k.last && (s == abi::stream() || completed(k.done))) return;
         if (e == hipSuccess) e = hipStreamWaitEvent(s, k.done, 0);
     }
     bool recorded() const { return !captured && s != abi::stream(); }
@@ -223,11 +228,7 @@ int check_seqs(const Kv &k, const char *op, const int32_t *seqs, int32_t n, bool
 }
 
 // What a replayed graph cannot do: it would repeat changes that the host has made once.
-int refuse_capture(const char *op, void *stream) {
-    if (capturing(stream ? (hipStream_t)stream : abi::stream()))
-        return report_error(J4Q_EINVAL, "%s: changes the cache's pages, which a captured graph cannot repeat", op);
-    return J4Q_OK;
-}
+constexpr char kChanges[] = "changes the cache's pages, which a captured graph cannot repeat";
 
 void end_step(Kv &k) {
     k.step_seq.clear();
@@ -437,7 +438,7 @@ int j4q_kv_create(const j4q_kv_config *config, j4q_kv *out) try {
     std::lock_guard<std::mutex> lk(abi::lock());
     int rc = abi::ready_locked();
     if (rc) return rc;
-    if ((rc = refuse_capture("kv cache", nullptr))) return rc;
+    if (capturing(abi::stream())) return report_error(J4Q_EINVAL, "kv cache: %s", kChanges);
     std::unique_ptr<Kv> k(new Kv);
     g_kvs.reserve(g_kvs.size() + 1);
     k->seqs.resize((size_t)c.sequences);
@@ -578,7 +579,9 @@ int j4q_kv_extend(j4q_kv kv, const int32_t *seqs, const int32_t *tokens, int32_t
     }
     if (need > k->free_pages)
         return report_error(J4Q_ENOMEM, "kv extend failed: %lld pages needed, %lld free", (long long)need, (long long)k->free_pages);
-    if ((rc = abi::ready_locked()) || (rc = refuse_capture("kv extend", stream))) return rc;
+    if ((rc = abi::ready_locked())) return rc;
+    Call c(*k, stream);
+    if ((rc = c.check("kv extend", kChanges))) return rc;
     Changes ch;
     Pairs pairs;
     ch.runs.reserve((size_t)need + step_changes(n));
@@ -605,7 +608,7 @@ int j4q_kv_extend(j4q_kv kv, const int32_t *seqs, const int32_t *tokens, int32_t
         }
     }
     set_step(*k, seqs, tokens, n, &ch);
-    Call c(*k, stream);
+    c.order();
     copy_pages(c, pairs, false);
     ch.launch(c, true);
     return c.end_change("kv extend");
@@ -623,11 +626,13 @@ int j4q_kv_begin(j4q_kv kv, const int32_t *seqs, const int32_t *tokens, int32_t 
     for (int32_t i = 0; i < n; i++)
         if (tokens[i] > k->seqs[(size_t)seqs[i]].len)
             return report_error(J4Q_EINVAL, "kv begin: sequence %d has %lld tokens, not %d", seqs[i], (long long)k->seqs[(size_t)seqs[i]].len, tokens[i]);
-    if ((rc = abi::ready_locked()) || (rc = refuse_capture("kv begin", stream))) return rc;
+    if ((rc = abi::ready_locked())) return rc;
+    Call c(*k, stream);
+    if ((rc = c.check("kv begin", kChanges))) return rc;
     Changes ch;
     ch.runs.reserve(step_changes(n));
     set_step(*k, seqs, tokens, n, &ch);
-    Call c(*k, stream);
+    c.order();
     ch.launch(c, true);
     return c.end_change("kv begin");
 } catch (const std::exception &) {
@@ -655,7 +660,9 @@ int j4q_kv_fork(j4q_kv kv, const int32_t *src, const int32_t *dst, int32_t n, in
         if (made[(size_t)src[i]]) return report_error(J4Q_EINVAL, "kv fork: sequence %d is made by this call and copied by it", src[i]);
     if (need > k->free_pages)
         return report_error(J4Q_ENOMEM, "kv fork failed: %lld pages needed, %lld free", (long long)need, (long long)k->free_pages);
-    if ((rc = abi::ready_locked()) || (rc = refuse_capture("kv fork", stream))) return rc;
+    if ((rc = abi::ready_locked())) return rc;
+    Call c(*k, stream);
+    if ((rc = c.check("kv fork", kChanges))) return rc;
     Changes ch;
     Pairs pairs;
     ch.runs.reserve(entries);
@@ -674,7 +681,7 @@ int j4q_kv_fork(j4q_kv kv, const int32_t *src, const int32_t *dst, int32_t n, in
         }
     }
     k->step_checked = false;
-    Call c(*k, stream);
+    c.order();
     copy_pages(c, pairs, false);
     ch.launch(c, true);
     return c.end_change("kv fork");
@@ -721,7 +728,9 @@ int j4q_kv_evict(j4q_kv kv, const int32_t *seqs, int32_t n, int32_t window, int3
     if (rc) return rc;
     if (window < 1 || sinks < 0) return report_error(J4Q_EINVAL, "kv evict: a window of %d tokens, %d first ones (at least 1, 0)", window, sinks);
     if ((rc = check_seqs(*k, "kv evict", seqs, n, true))) return rc;
-    if ((rc = abi::ready_locked()) || (rc = refuse_capture("kv evict", stream))) return rc;
+    if ((rc = abi::ready_locked())) return rc;
+    Call c(*k, stream);
+    if ((rc = c.check("kv evict", kChanges))) return rc;
     const int64_t per = k->c.page_tokens, first = (sinks + per - 1) / per;
     // the next token, at place len, sees j > len - window and j < sinks; an earlier one sees more
     auto last = [&](const Seq &q) { return std::max<int64_t>(0, (q.len - window + 1) / per); };
@@ -743,7 +752,7 @@ int j4q_kv_evict(j4q_kv kv, const int32_t *seqs, int32_t n, int32_t window, int3
         q.gone1 = std::max(q.gone1, end * per);
     }
     k->step_checked = false;
-    Call c(*k, stream);
+    c.order();
     ch.launch(c, true);
     return c.end_change("kv evict");
 } catch (const std::exception &) {
@@ -755,7 +764,9 @@ int j4q_kv_compact(j4q_kv kv, int64_t *moved, void *stream) try {
     Kv *k;
     int rc = get(kv, "kv compact", &k);
     if (rc) return rc;
-    if ((rc = abi::ready_locked()) || (rc = refuse_capture("kv compact", stream))) return rc;
+    if ((rc = abi::ready_locked())) return rc;
+    Call c(*k, stream);
+    if ((rc = c.check("kv compact", kChanges))) return rc;
     const int64_t live = k->c.pages - k->free_pages;
     Pairs pairs;
     std::vector<int32_t> to((size_t)k->c.pages, -1);
@@ -788,7 +799,7 @@ int j4q_kv_compact(j4q_kv kv, int64_t *moved, void *stream) try {
     while (k->hint + 1 < (int64_t)k->free_bits.size() && !k->free_bits[(size_t)k->hint]) k->hint++;
     if (moved) *moved = (int64_t)pairs.size();
     if (pairs.empty()) return J4Q_OK;
-    Call c(*k, stream);
+    c.order();
     copy_pages(c, pairs, false);
     ch.launch(c, true);
     return c.end_change("kv compact");
@@ -845,9 +856,12 @@ int j4q_kv_append(j4q_kv kv, int32_t layer, const j4q_kv_append_args *args, void
     a.q = g.q;
     a.q_out = g.q_out;
     a.bf16 = g.type == J4Q_KIND_BF16;
+    if ((rc = abi::ready_locked())) return rc;
+    Call c(*k, stream);
+    if ((rc = c.check("kv append", nullptr))) return rc;
     // workgroups by sequence, unless the steps are so uneven that most of them would have nothing to do
     int64_t most = k->step_most_blocks, blocks = k->step_blocks;
-    if (capturing(stream ? (hipStream_t)stream : abi::stream())) {  // a replay's tokens may lie across one block more
+    if (c.captured) {  // a replay's tokens may lie across one block more
         most = blocks = 0;
         for (int32_t t : k->step_tokens) {
             const int64_t b = (t - 1 + kKvBlock - 1) / kKvBlock + 1;
@@ -861,8 +875,7 @@ int j4q_kv_append(j4q_kv kv, int32_t layer, const j4q_kv_append_args *args, void
     if (items * k->c.kv_heads + (int64_t)k->step_rows * a.heads > INT_MAX)
         return report_error(J4Q_EUNSUPPORTED, "kv append: %d tokens of %d heads in a call", k->step_rows, std::max(a.heads, k->c.kv_heads));
     a.items = (int32_t)items;
-    if ((rc = abi::ready_locked())) return rc;
-    Call c(*k, stream);
+    c.order();
     if (c.e == hipSuccess) c.e = launch_kv_append(a, c.s, c.event(true));
     return c.end("kv append");
 } catch (const std::exception &) {
@@ -924,6 +937,8 @@ int j4q_kv_attend(j4q_kv kv, int32_t layer, const j4q_kv_attend_args *args, void
     a.part_ml = k->part + kPartRows * k->c.head_dim;
     if ((rc = abi::ready_locked())) return rc;
     Call c(*k, stream);
+    if ((rc = c.check("kv attend", nullptr))) return rc;
+    c.order();
     // sequences of few rows, of some and of many, in a launch each
     if (few && c.e == hipSuccess) {
         a.rows_from = 1, a.rows_to = kFewRows, a.max_rows = (int32_t)few;
@@ -959,9 +974,9 @@ int j4q_kv_read(j4q_kv kv, int32_t layer, const int32_t *seqs, const int64_t *fi
     for (int32_t i = 0; i < n; i++)
         if (first[i] < 0 || first[i] > 1 << 30) return report_error(J4Q_EINVAL, "kv read: first token %lld", (long long)first[i]);
     if ((rc = abi::ready_locked())) return rc;
-    if (capturing(stream ? (hipStream_t)stream : abi::stream()))
-        return report_error(J4Q_EINVAL, "kv read: lengths of now, which a captured graph would repeat");
     Call c(*k, stream);
+    if ((rc = c.check("kv read", "lengths of now, which a captured graph would repeat"))) return rc;
+    c.order();
     for (int32_t at = 0; at < n && c.e == hipSuccess; at += kKvReadSeqs) {
         KvRead r;
         r.l = k->layer(layer);

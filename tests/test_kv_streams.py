@@ -31,3 +31,34 @@ def test_an_equal_handle_may_be_another_stream(shim, handle):  # noqa: F811
         got = [waits(lambda: kv.attend(0, a, a + 65536, 2, stream=s)) for s in (0, 0, {handle}, 0)]
         assert got == [["wait", "launch"], ["launch"], ["record", "wait", "launch"], ["wait", "launch"]], got
     """)
+
+
+def test_no_event_goes_into_a_graph_of_the_engine_stream(shim):  # noqa: F811
+    """The last call is on the engine stream, which is captured now: a call on another stream could only wait for an event of the
+    graph, and would become part of it. It is refused before it changes anything, and goes through after the capture."""
+    run(shim, """
+        kv = cache(pages=60, sequences=4, sequence_pages=60)
+        a = address(1 << 20)
+        kv.extend([0, 3], [20, 40])
+        kv.append(0, a, a)
+        kv.truncate([3], [0])
+        kv.extend([0], [30])
+        engine = be.stream()
+        calls = [lambda: kv.append(0, a, a, stream=0x70), lambda: kv.attend(0, a, a + 65536, 2, stream=0x70),
+                 lambda: kv.read(0, [0], [0], 4, a, a, stream=0x70), lambda: kv.begin([0], [1], stream=0x70), lambda: kv.fork([0], [1], stream=0x70),
+                 lambda: kv.extend([0], [1], stream=0x70), lambda: kv.evict([0], 4, stream=0x70), lambda: kv.compact(stream=0x70)]
+        state = lambda: (kv.info(), kv.tables(range(4)).tolist(), kv.lengths(range(4)).tolist())
+        for call in calls:
+            kv.attend(0, a, a + 65536, 2)
+            was = state()
+            log()
+            fake.fake_capture(C.c_void_p(engine), 1)
+            assert refused(call, "engine stream", "captured") == "IllegalArgumentException"
+            assert state() == was and not log("record", "wait", "launch")
+            kv.attend(0, a, a + 65536, 2)  # into the graph
+            assert launches()
+            fake.fake_capture(C.c_void_p(engine), 0)
+            call()
+            lines = [l.split()[0] for l in log("record", "wait", "launch")]
+            assert lines[:3] == ["record", "wait", "launch"] or not lines, lines
+    """)
