@@ -46,7 +46,7 @@ def test_no_event_goes_into_a_graph_of_the_engine_stream(shim):  # noqa: F811
         engine = be.stream()
         calls = [lambda: kv.append(0, a, a, stream=0x70), lambda: kv.attend(0, a, a + 65536, 2, stream=0x70),
                  lambda: kv.read(0, [0], [0], 4, a, a, stream=0x70), lambda: kv.begin([0], [1], stream=0x70), lambda: kv.fork([0], [1], stream=0x70),
-                 lambda: kv.extend([0], [1], stream=0x70), lambda: kv.evict([0], 4, stream=0x70), lambda: kv.compact(stream=0x70)]
+                 lambda: kv.extend([0], [1], stream=0x70), lambda: kv.compact(stream=0x70), lambda: kv.evict([0], 4, stream=0x70)]
         state = lambda: (kv.info(), kv.tables(range(4)).tolist(), kv.lengths(range(4)).tolist())
         for call in calls:
             kv.attend(0, a, a + 65536, 2)
