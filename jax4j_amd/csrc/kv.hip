@@ -137,12 +137,20 @@ struct Call {
     Kv &k;
     hipStream_t s;
     bool captured;
-    hipError_t e = hipSuccess;
+    hipError_t e;
 
-    Call(Kv &kv, void *stream) : k(kv), s(stream ? (hipStream_t)stream : abi::stream()), captured(capturing(s)) {}
+    Call(Kv &kv, void *stream) : k(kv), s(stream ? (hipStream_t)stream : abi::stream()) {
+        hipStreamCaptureStatus st = hipStreamCaptureStatusNone;
+        e = hipStreamIsCapturing(s, &st);
+        captured = st != hipStreamCaptureStatusNone;
+    }
     bool from_engine() const { return k.used && k.last == abi::stream() && s != k.last; }
     // Before anything changes: whether the call can go out on its stream. capture: why a captured graph cannot hold it, or nullptr.
     int check(const char *op, const char *capture) const {
+        if (e != hipSuccess) {  // neither kind of call: the one would wait for nothing, the other be a graph's
+            (void)hipGetLastError();
+            return report_hip(op, e);
+        }
         if (captured) return capture ? report_error(J4Q_EINVAL, "%s: %s", op, capture) : J4Q_OK;
         if (from_engine() && capturing(abi::stream()))  // an event recorded there now would draw this call into the graph
             return report_error(J4Q_EINVAL, "%s: another stream cannot wait for the cache's last call while the engine stream, where that is, is captured", op);

@@ -42,8 +42,9 @@ class Steps:
         assert torch.equal(got[:n], self.out[:n]) and bool(self.out[:n].abs().amax((1, 2, 3)).min() > 0)
 
 
-def test_one_handle_in_two_threads(model):  # noqa: F811
-    """hipStreamPerThread: appended behind a long kernel in one thread, attended to in another, and back."""
+@pytest.mark.parametrize("handle", [1, 2], ids=["hipStreamLegacy", "hipStreamPerThread"])
+def test_one_handle_in_two_threads(model, handle):  # noqa: F811
+    """A stream of each thread's own, or one for both: appended behind a long kernel in one thread, attended to in another, and back."""
     steps, lib = Steps(model), N.load()
     turn, failed = [threading.Event() for _ in range(14)], []
 
@@ -53,9 +54,9 @@ def test_one_handle_in_two_threads(model):  # noqa: F811
                 if i % 2 == me:
                     assert turn[i].wait(60)
                     if i:
-                        steps.attend(i - 1, 2)
-                    assert lib.j4q_spin(500, 2) == 0
-                    steps.append(i, 2)
+                        steps.attend(i - 1, handle)
+                    assert lib.j4q_spin(500, handle) == 0
+                    steps.append(i, handle)
                     turn[i + 1].set()
             assert turn[13].wait(60)  # its stream lives until all is done
         except BaseException as e:

@@ -1,8 +1,11 @@
 """The order of calls on one key/value cache over the streams that they come on, without a GPU (fakehip.py)."""
 from __future__ import annotations
 
+import subprocess
+
 import pytest
 
+import fakehip
 from test_kv_pages import run, shim  # noqa: F401
 
 
@@ -61,4 +64,41 @@ def test_no_event_goes_into_a_graph_of_the_engine_stream(shim):  # noqa: F811
             call()
             lines = [l.split()[0] for l in log("record", "wait", "launch")]
             assert lines[:3] == ["record", "wait", "launch"] or not lines, lines
+    """)
+
+
+@pytest.fixture(scope="module")
+def unsure_shim(tmp_path_factory):
+    """The same runtime, which does not tell whether stream 0x70 is captured (as of hipStreamLegacy beside another's capture)."""
+    folder = tmp_path_factory.mktemp("unsure_hip")
+    text = (fakehip.TESTS / "fake_hip.cpp").read_text()
+    head = "F hipError_t hipStreamIsCapturing("
+    at = text.index("LOCK;", text.index(head)) + len("LOCK;")
+    text = text[:at] + " if (s == (hipStream_t)0x70 && unsure) return ret(hipErrorStreamCaptureImplicit);" + text[at:]
+    at = text.index(head)
+    text = text[:at] + "static bool unsure = false;\nF void fake_unsure(int on) { unsure = on != 0; }\n" + text[at:]
+    (folder / "fake_hip.cpp").write_text(text)
+    lib = folder / "fake_hip.so"
+    subprocess.run(["g++", "-std=c++17", "-O1", "-shared", "-fPIC", "-D__HIP_PLATFORM_AMD__", f"-I{fakehip.ROCM / 'include'}",
+                    "-o", str(lib), str(folder / "fake_hip.cpp")], check=True)
+    return lib
+
+
+def test_a_stream_that_may_be_captured_or_not(unsure_shim):
+    """Neither kind of call would be right there: one without a wait would race, one with an event be part of a graph."""
+    run(unsure_shim, """
+        kv = cache(pages=60, sequences=4, sequence_pages=60)
+        a = address(1 << 20)
+        kv.extend([0], [20], stream=0x60)
+        state = lambda: (kv.info(), kv.tables(range(4)).tolist(), kv.lengths(range(4)).tolist())
+        for call in (lambda: kv.append(0, a, a, stream=0x70), lambda: kv.attend(0, a, a + 65536, 2, stream=0x70),
+                     lambda: kv.read(0, [0], [0], 4, a, a, stream=0x70), lambda: kv.begin([0], [1], stream=0x70), lambda: kv.fork([0], [1], stream=0x70),
+                     lambda: kv.extend([0], [1], stream=0x70), lambda: kv.compact(stream=0x70), lambda: kv.evict([0], 4, stream=0x70)):
+            was = state()
+            log()
+            fake.fake_unsure(1)
+            assert refused(call, "failed") == "RuntimeError"
+            assert state() == was and not log("record", "wait", "launch")
+            fake.fake_unsure(0)
+            call()
     """)
