@@ -136,7 +136,7 @@ bool aligned(const void *p, uintptr_t a) { return ((uintptr_t)p & (a - 1)) == 0;
 struct Call {
     Kv &k;
     hipStream_t s;
-    bool captured;
+    bool captured, behind = true;
     hipError_t e;
 
     Call(Kv &kv, void *stream) : k(kv), s(stream ? (hipStream_t)stream : abi::stream()) {
@@ -162,6 +162,7 @@ struct Call {
         if (from_engine()) e = hipEventRecord(k.done, k.last);
         else if (s == k.last && (s == abi::stream() || completed(k.done))) return;
         if (e == hipSuccess) e = hipStreamWaitEvent(s, k.done, 0);
+        behind = e == hipSuccess;
     }
     bool recorded() const { return !captured && s != abi::stream(); }
     hipEvent_t event(bool last) const { return last && recorded() ? k.done : nullptr; }
@@ -170,6 +171,10 @@ struct Call {
         return end(op);
     }
     int end(const char *op) {
+        if (!behind) {  // nothing went out, and the call before is still what the next one waits for
+            (void)hipGetLastError();  // a launch checks for errors by the last one
+            return report_hip(op, e);
+        }
         if (e != hipSuccess && recorded()) (void)hipEventRecord(k.done, s);
         if (!captured) {
             k.last = s;

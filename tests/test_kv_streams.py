@@ -67,21 +67,26 @@ def test_no_event_goes_into_a_graph_of_the_engine_stream(shim):  # noqa: F811
     """)
 
 
-@pytest.fixture(scope="module")
-def unsure_shim(tmp_path_factory):
-    """The same runtime, which does not tell whether stream 0x70 is captured (as of hipStreamLegacy beside another's capture)."""
-    folder = tmp_path_factory.mktemp("unsure_hip")
+def changed_shim(folder, function, line, switch):
+    """The same runtime, in one of whose functions this line comes first while fake_<switch>(1) holds."""
     text = (fakehip.TESTS / "fake_hip.cpp").read_text()
-    head = "F hipError_t hipStreamIsCapturing("
+    head = f"F hipError_t {function}("
     at = text.index("LOCK;", text.index(head)) + len("LOCK;")
-    text = text[:at] + " if (s == (hipStream_t)0x70 && unsure) return ret(hipErrorStreamCaptureImplicit);" + text[at:]
+    text = text[:at] + f" if ({switch}) {{ {line} }}" + text[at:]
     at = text.index(head)
-    text = text[:at] + "static bool unsure = false;\nF void fake_unsure(int on) { unsure = on != 0; }\n" + text[at:]
+    text = text[:at] + f"static bool {switch} = false;\nF void fake_{switch}(int on) {{ {switch} = on != 0; }}\n" + text[at:]
     (folder / "fake_hip.cpp").write_text(text)
     lib = folder / "fake_hip.so"
     subprocess.run(["g++", "-std=c++17", "-O1", "-shared", "-fPIC", "-D__HIP_PLATFORM_AMD__", f"-I{fakehip.ROCM / 'include'}",
                     "-o", str(lib), str(folder / "fake_hip.cpp")], check=True)
     return lib
+
+
+@pytest.fixture(scope="module")
+def unsure_shim(tmp_path_factory):
+    """It does not tell whether stream 0x70 is captured (as of hipStreamLegacy beside another's capture)."""
+    return changed_shim(tmp_path_factory.mktemp("unsure_hip"), "hipStreamIsCapturing",
+                        "if (s == (hipStream_t)0x70) return ret(hipErrorStreamCaptureImplicit);", "unsure")
 
 
 def test_a_stream_that_may_be_captured_or_not(unsure_shim):
@@ -101,4 +106,38 @@ def test_a_stream_that_may_be_captured_or_not(unsure_shim):
             assert state() == was and not log("record", "wait", "launch")
             fake.fake_unsure(0)
             call()
+    """)
+
+
+@pytest.fixture(scope="module")
+def no_wait_shim(tmp_path_factory):
+    return changed_shim(tmp_path_factory.mktemp("no_wait_hip"), "hipStreamWaitEvent", "return ret(hipErrorInvalidHandle);", "no_wait")
+
+
+def test_a_call_that_could_not_wait_is_not_waited_for(no_wait_shim):
+    """Its stream is not behind the call before it: that one stays what the next call waits for."""
+    run(no_wait_shim, """
+        kv = cache(pages=60, sequences=4, sequence_pages=60)
+        a = address(1 << 20)
+        fake.fake_events_done(0)
+        for first in (0x60, 0):
+            for failing in (0x70, 0):
+                if failing == first:
+                    continue
+                kv.extend([0], [5], stream=first)
+                log()
+                fake.fake_no_wait(1)
+                assert refused(lambda: kv.attend(0, a, a + 65536, 2, stream=failing), "failed") == "RuntimeError"
+                fake.fake_no_wait(0)
+                assert [l.split()[-1] for l in log("record", "launch")] == ([hex(be.stream())] if first == 0 else [])
+                kv.attend(0, a, a + 65536, 2, stream=first)
+                assert bool(log("wait")) == (first != 0)
+                fake.fake_no_wait(1)
+                assert refused(lambda: kv.attend(0, a, a + 65536, 2, stream=failing), "failed") == "RuntimeError"
+                fake.fake_no_wait(0)
+                log()
+                kv.attend(0, a, a + 65536, 2, stream=0x80)
+                lines = [l.split() for l in log("record", "wait", "launch")]
+                assert [l[0] for l in lines][:3] == ["record"] * (first == 0) + ["wait", "launch"] + ["launch"] * (first != 0 and len(lines) > 2), lines
+                assert first or lines[0][-1] == hex(be.stream())
     """)
