@@ -396,9 +396,10 @@ typedef struct j4q_kv_attend_args {
     float scale;             /* 0: 1 / sqrt(head_dim) */
 } j4q_kv_attend_args;
 /* out = softmax(scale q k) v of every row of the step over the tokens j <= p of its sequence, p its own place, with
- * j > p - window or j < sinks. Up to 16 rows (tokens x heads / kv_heads of a sequence) nothing of q or the weights is
- * rounded that fp32 holds beside the row's largest; more rows take them in 22 bits or more where out is fp32, and where it is
- * bf16, q in 16 bits or fp16 and the weights in fp16. Bit for bit the same on every call with equal lengths. */
+ * j > p - window or j < sinks. Up to 16 rows (tokens x heads / kv_heads of a sequence) nothing of q is rounded that fp32
+ * holds beside the row's largest, and a weight is off by 2^-27 of the row's largest at most. More rows take both in 22 bits or
+ * more where out is fp32, and where it is bf16, q in 16 bits or fp16 and the weights in fp16 (a weight far below the row's
+ * largest is off by 2^-33 of that at most). Bit for bit the same on every call with equal lengths. */
 int j4q_kv_attend(j4q_kv kv, int32_t layer, const j4q_kv_attend_args *args, void *stream);
 /* Tokens [first[i], first[i] + count) of seqs[i] in `layer` as the cache holds them: fp32 [n][count][kv_heads][head_dim],
  * 16-byte aligned (either may be NULL); zeros where there is no token. */

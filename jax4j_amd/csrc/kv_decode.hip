@@ -8,9 +8,11 @@
 // divides it out again. A visible token of a block of NaN has t = NaN, and so has its row.
 //
 // Both products run on the int8 matrix instruction 16x16x64 over the codes as they lie in memory, with exact 32-bit sums.
-// The other operand is fp32 (q, w); it enters as four digits to the base 256 from -128 to 127 of a whole number of 31 bits (q over
-// its row's largest magnitude / 2^30; w below 2^30), so nothing that fp32 holds beside the row's largest value is lost. The digits
-// fill the 16 columns of the second operand: 4 rows x 4 digits in one instruction, or 8 rows x 2 digits in two. Operands:
+// The other operand is fp32 (q, w); it enters as four digits to the base 256 from -128 to 127 of a whole number of 31 bits: q over
+// its row's largest magnitude / 2^30, so nothing that fp32 holds beside that is lost; w below 2^30, rounded to the nearest, so a
+// weight is off by 2^-27 of the largest that its wave has seen at most, either way (cut off, thousands of tokens far below a
+// dominant one lost half a unit each: 0.6 to 1.4 % of their sum). The digits fill the 16 columns of the second operand: 4 rows x
+// 4 digits in one instruction, or 8 rows x 2 digits in two. Operands:
 //   scores   A = 16 tokens x 64 channels of K, B = 64 channels x 16 (digit, row):  C[token][digit, row]
 //   output   A = 16 channels x 64 tokens of V, B = 64 tokens x 16 (digit, row) of w: C[channel][digit, row]
 // Lane l holds rows 4 (l / 16) + i of C in column l % 16, bytes 16 (l / 16).. of k in A's row and B's column l % 16. The 16
@@ -294,7 +296,7 @@ __global__ void __launch_bounds__(64 * waves_of(D), waves_of(D) / 4) decode_kern
         for (int j = 0; j < 16; j++) {
             const float e = __builtin_amdgcn_exp2f(t[j] + base);
             l_sum = __builtin_fmaf(e, rsv, l_sum);
-            w[j] = digits_of((int)e);
+            w[j] = digits_of((int)__builtin_rintf(e));
         }
 #pragma unroll
         for (int m = 0; m < M; m++) {

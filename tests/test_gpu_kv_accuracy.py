@@ -108,3 +108,37 @@ def test_equal_weights_behind_leading_tokens(model, dim, heads, tokens, ahead): 
     want = exact(q, k, v, length)
     e = off(attend(m, q), want)
     assert e <= bar(q, k), f"off by {e:.3g} of a row, bar {bar(q, k):.3g}"
+
+
+@gpu
+@pytest.mark.parametrize("group", [1, 3, 4, 8, 16])
+@pytest.mark.parametrize("dim", [64, 128, 256])
+def test_weights_far_below_a_dominant_one(model, dim, group):  # noqa: F811
+    """Up to 16 rows: a first token of nearly all the weight and no value, and thousands of a value of 1 at 2^-26 to 2^-20 of it.
+
+    Weights are whole numbers of 2^-26 of the largest that their wave has seen. Rounded to the nearest, those of the wave with the
+    first token (an eighth of them at least, a quarter at most) are each off by half a unit at most, evenly spread: sqrt(n / 12)
+    units together, of which six times are allowed. Cut off they would be off by n / 2 units."""
+    length, seqs = 8192, 32
+    m = model(kv_heads=8, head_dim=dim, pages=128, page_tokens=64, sequences=seqs, sequence_pages=128)
+    rng = np.random.default_rng(dim + group)
+    u = rng.choice([-1.0, 1.0], dim) * dim ** -0.5
+    x = rng.uniform(0, 6 * np.log(2), (length, 8, 1))
+    x[0] = 26 * np.log(2)
+    v = np.ones((length, 8, dim))
+    v[0] = 0
+    m.kv.extend([0], [length])
+    m.write(0, [0], [length], x * u, v)
+    m.kv.fork([0] * (seqs - 1), range(1, seqs))  # a workgroup each for all of a sequence and kv head
+    m.kv.begin(range(seqs), [1] * seqs)
+    q = (dim ** 0.5 * u * rng.uniform(0.98, 1.02, (seqs, 8 * group, 1))).astype(np.float32)
+    dq, out = torch.from_numpy(q).cuda(), torch.zeros(q.shape, device="cuda")
+    torch.cuda.synchronize()
+    m.kv.attend(0, dq.data_ptr(), out.data_ptr(), 8 * group)
+    k, v = (h.values() for h in m.of(0, 0))
+    want = exact(q, k, v, length)  # the mean of the values is the share of the weight that the first token leaves
+    units = want / (1 - want) * 2.0 ** 26
+    logs = np.log2(127)
+    e = np.abs(host(out) / want - 1)
+    allowed = 6 * (length / 4 / 12) ** 0.5 / units + 2 * 2.0 ** -22 * (27 + logs + 8)
+    assert (e <= allowed).all(), f"off by {e.max():.3g} of a row, bar {allowed.min():.3g}"
