@@ -135,10 +135,10 @@ __global__ void __launch_bounds__(64 * waves_of(D), waves_of(D) / 4) decode_kern
     const KvTiles vis = kv_tiles(q_first, q_last, a.window, a.sinks);
     int t0 = 0, t1 = vis.count();
     if (a.splits > 1) {
-        const int ranges = kv_ranges(vis.count(), a);
-        if ((int)blockIdx.x >= ranges) return;
-        t0 = blockIdx.x * a.split_tiles;
-        if ((int)blockIdx.x + 1 < ranges) t1 = t0 + a.split_tiles;
+        const int each = kv_range_tiles(t1, a);
+        t0 = blockIdx.x * each;
+        if (t0 >= t1) return;
+        t1 = min(t1, t0 + each);
     }
 
     const int32_t *table = a.step.table + (int64_t)a.step.seq[i] * a.step.sequence_pages;

@@ -96,10 +96,10 @@ __global__ void __launch_bounds__(64 * W, D <= 128 ? 2 : 1) prefill_kernel(KvAtt
     const KvTiles vis = kv_tiles(before + r0 / a.group, before + r1 / a.group, a.window, a.sinks);
     int t0 = 0, t1 = vis.count();
     if (a.splits > 1) {
-        const int ranges = kv_ranges(t1, a);
-        if (split >= ranges) return;
-        t0 = split * a.split_tiles;
-        if (split + 1 < ranges) t1 = t0 + a.split_tiles;
+        const int each = kv_range_tiles(t1, a);
+        t0 = split * each;
+        if (t0 >= t1) return;
+        t1 = min(t1, t0 + each);
     }
     // the wave's rows, and its places; the lane's row
     const int w0 = r0 + wave * 32, w1 = min(r1, w0 + 31);
@@ -399,10 +399,10 @@ __global__ void __launch_bounds__(512, 2) rows_kernel(KvAttend a) {
     const KvTiles vis = kv_tiles(before + r0 / a.group, before + r1 / a.group, a.window, a.sinks);
     int t0 = 0, t1 = vis.count();
     if (a.splits > 1) {
-        const int ranges = kv_ranges(vis.count(), a);
-        if ((int)blockIdx.x >= ranges) return;
-        t0 = blockIdx.x * a.split_tiles;
-        if ((int)blockIdx.x + 1 < ranges) t1 = t0 + a.split_tiles;
+        const int each = kv_range_tiles(t1, a);
+        t0 = blockIdx.x * each;
+        if (t0 >= t1) return;
+        t1 = min(t1, t0 + each);
     }
     const int p_first = before + r0 / a.group, p_last = before + r1 / a.group;
     const int row = min(r0 + col, r1), place = before + row / a.group;
