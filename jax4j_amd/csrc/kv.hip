@@ -362,11 +362,12 @@ void set_splits(const Kv &k, bool captured, int64_t most, int64_t split_tiles, K
     a->split_tiles = (int32_t)std::max(split_tiles, (most + a->splits - 1) / a->splits);
 }
 
-// One range up to `alone` tiles; else ranges of four or more that fill the CUs once.
-void split_filled(const Kv &k, bool captured, int64_t alone, KvAttend *a) {
+// One range up to `alone` tiles, or up to `half` where half of the CUs have a workgroup; else ranges of four or more that fill the CUs
+// once.
+void split_filled(const Kv &k, bool captured, int64_t alone, int64_t half, KvAttend *a) {
     constexpr int64_t kFilled = 256, kLeast = 4;
     const Walks w = walks_of(k, *a);
-    if (w.groups * k.c.kv_heads >= kFilled / 2) alone = 32;
+    if (w.groups * k.c.kv_heads >= kFilled / 2) alone = half;
     set_splits(k, captured, w.most, std::max(w.most <= alone ? alone : kLeast, (w.tiles * k.c.kv_heads + kFilled - 1) / kFilled), a);
 }
 
@@ -374,18 +375,23 @@ void split_filled(const Kv &k, bool captured, int64_t alone, KvAttend *a) {
 // round of the 8 waves over a tile each 2.4, and less where only four of them have one, alone on their SIMDs (one request, 8 kv
 // heads of 128: 11 tiles 10.0 us in one range, 10.7 in three; 16 tiles 11.3, and 13.2 in two; heads of 64 7.7, 9.2 in four; 32
 // tiles 16.2, 12.7 in four, 11.2 in eight; 128 tiles 46, 14.0 in sixteen, 12.9 in thirty-two). Half of the CUs are better left idle
-// for up to 32 tiles (16 requests: 32 tiles 18.3 us in one range, 20.2 in two; 64 tiles 35.3 and 34.7).
+// for up to 32 tiles (16 requests, 32 tiles in one range and in two: heads of 64 11.8 us and 13.6, of 96 13.9 and 15.6, of 128 19.1
+// and 21.9, of 192 22.4 and 26.1; heads of 128, 64 tiles 35.3 and 34.7). Heads of 256, whose four waves have twice the bytes a
+// tile, are cut sooner (one request, in one range and in ranges of four: 8 tiles 13.5 and 14.5, 12 tiles 16.0 and 14.7, 16 tiles
+// 18.4 and 14.8; 16 requests, in one and in two: 24 tiles 27.3 and 28.4, 32 tiles 33.8 to 35.0 and 33.6 to 33.8).
 void split_few(const Kv &k, bool captured, KvAttend *a) {
     a->row_tile = a->max_rows <= 4 ? 4 : 8;
-    split_filled(k, captured, 16, a);
+    if (k.c.head_dim > 192) split_filled(k, captured, 8, 24, a);
+    else split_filled(k, captured, 16, 32, a);
 }
 
 // Some rows: a workgroup is a CU's as well, whose 8 waves take a tile each in a round; ranges of 4 tiles beside each other where
 // there are workgroups to spare (one request, 24 rows of 8 kv heads of 128: 16 tiles 13.5 us in four ranges, 14.1 in one; 63
-// tiles 14.8 in ranges of 4, 15.6 of 8 and 17.7 of 16).
+// tiles 14.8 in ranges of 4, 15.6 of 8 and 17.7 of 16; 16 requests, 32 tiles in one range and in two: heads of 64 14.2 and 15.7, of
+// 96 16.4 and 18.5, of 128 20.7 and 23.2).
 void split_some(const Kv &k, bool captured, KvAttend *a) {
     a->row_tile = 32;
-    split_filled(k, captured, 8, a);
+    split_filled(k, captured, 8, 32, a);
 }
 
 // Many rows: workgroups of 256, whose conversion of a tile serves the most rows, or of 128, two to a CU, which fill the chip sooner:

@@ -6,6 +6,7 @@ import subprocess
 
 import pytest
 
+import fakehip
 from jax4j_amd import build
 
 SOURCE = r"""
@@ -48,3 +49,22 @@ def program(tmp_path_factory):
 def test_ranges_of_a_rows_tiles(program):
     p = subprocess.run([str(program)], capture_output=True, text=True)
     assert p.stdout == "even\n", p.stdout + p.stderr
+
+
+def test_ranges_by_head_size_and_requests(tmp_path):
+    """Ranges of a call (without a GPU): one up to as many tiles as were measured to be better off so, for each head size."""
+    fakehip.run(fakehip.build_shim(tmp_path), """
+        from jax4j_amd import KvCache
+        a = address(1 << 20)
+        for dim in (64, 96, 128, 192, 256):
+            kv = KvCache(be, layers=1, kv_heads=8, head_dim=dim, pages=16 * 64, page_tokens=64, sequences=16, sequence_pages=64)
+            one, half = (8, 24) if dim == 256 else (16, 32)
+            for requests, tiles, ranges in ((1, one, 1), (1, one + 1, (one + 4) // 4), (16, half, 1), (16, half + 1, 2)):
+                kv.truncate(range(16), [0] * 16)
+                kv.extend(range(requests), [64 * tiles] * requests)
+                kv.begin(range(requests), [1] * requests)
+                log()
+                kv.attend(0, a, a, 32)
+                assert int(launches()[0][3]) == ranges, (dim, requests, tiles)
+            kv.destroy()
+    """)
