@@ -54,6 +54,21 @@ def _addresses(*ps) -> list:
     return [p if p is None else index(p) for p in ps]
 
 
+def _int32(v) -> int:
+    """A number as the library takes it: ctypes would hand over its low bits, whatever the others are."""
+    v = index(v)
+    if not -0x80000000 <= v < 0x80000000:
+        raise IllegalArgumentException("a number does not fit 32 bits")
+    return v
+
+
+def _int64(v) -> int:
+    v = index(v)
+    if not -(1 << 63) <= v < 1 << 63:
+        raise IllegalArgumentException("a number does not fit 64 bits")
+    return v
+
+
 def _as_u8(blocks) -> np.ndarray:
     if isinstance(blocks, np.ndarray):
         return np.ascontiguousarray(blocks).reshape(-1).view(np.uint8)
@@ -292,6 +307,8 @@ class Mi355xBackend:
         kind = N.KIND_F32 if dtype is DType.F32 else N.KIND_BF16 if dtype is DType.BF16 else 0
         if not type(x_ptr) is type(out_ptr) is type(stream) is int:
             x_ptr, out_ptr, stream = _addresses(x_ptr, out_ptr, stream)
+        if (heads | head_dim) >> 31 or (rows | x_stride | out_stride) >> 63:  # _int32, _int64 of each take 0.5 us
+            raise IllegalArgumentException(f"rope_into: {rows} rows of {heads} heads of {head_dim}, strides of {x_stride}, {out_stride} values")
         check(self._lib().j4q_rope_into(x_ptr, out_ptr, kind, rows, heads, head_dim, x_stride, out_stride, rope.ref, stream), "rope_into")
 
     def decode_plan(self, layers, head, batch: int, io: dict) -> "DecodePlan":

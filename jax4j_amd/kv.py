@@ -22,7 +22,7 @@ from operator import index
 import numpy as np
 
 from . import _native as N
-from .backend import Mi355xBackend, _addresses, check
+from .backend import Mi355xBackend, _addresses, _int32, _int64, check
 from .tensor import DType, IllegalArgumentException
 
 def _kind(dtype: DType) -> int:
@@ -39,13 +39,6 @@ def _ints(values, code="i") -> array:
         return array(code, values if type(values) is list else list(values))
     except OverflowError:
         raise IllegalArgumentException(f"a number does not fit {8 * array(code).itemsize} bits") from None
-
-
-def _int32(v) -> int:
-    v = index(v)
-    if not -0x80000000 <= v < 0x80000000:
-        raise IllegalArgumentException("a number does not fit 32 bits")
-    return v
 
 
 def _at(a: array) -> int:
@@ -80,7 +73,7 @@ class Rope:
             axes = (C.c_uint8 * len(axes))(*axes)
         self._axes = axes
         cos, sin, at = _addresses(cos_ptr, sin_ptr, positions)
-        self.args = N.RopeArgs(cos, sin, rows, dims, int(interleaved), at or None, C.cast(axes, C.c_void_p) if axes else None)
+        self.args = N.RopeArgs(cos, sin, _int64(rows), _int32(dims), int(interleaved), at or None, C.cast(axes, C.c_void_p) if axes else None)
         self.ref = C.pointer(self.args)
 
 
@@ -92,7 +85,7 @@ class KvCache:
         self._be = backend
         self.handle = 0
         sequence_pages = pages if sequence_pages is None else sequence_pages
-        self._config = N.KvConfig(*map(_int32, (layers, kv_heads, head_dim, page_tokens)), index(pages), *map(_int32, (sequences, sequence_pages)))
+        self._config = N.KvConfig(*map(_int32, (layers, kv_heads, head_dim, page_tokens)), _int64(pages), *map(_int32, (sequences, sequence_pages)))
         out = C.c_uint64()
         check(backend._lib().j4q_kv_create(C.byref(self._config), C.byref(out)), "kv cache")
         self.handle = out.value
@@ -168,6 +161,8 @@ class KvCache:
         queries [rows, heads, head_dim] too are turned, into ``q_out_ptr`` (0: in place). Strides are in values, 0: dense."""
         if not type(k_ptr) is type(v_ptr) is type(q_ptr) is type(q_out_ptr) is type(stream) is int:
             k_ptr, v_ptr, q_ptr, q_out_ptr, stream = _addresses(k_ptr, v_ptr, q_ptr, q_out_ptr, stream)
+        if stride >> 63 or q_stride >> 63:
+            raise IllegalArgumentException(f"strides of {stride}, {q_stride} values")
         a = N.KvAppendArgs(k_ptr, v_ptr, stride, _kind(dtype), _int32(heads), q_ptr, q_out_ptr or q_ptr, q_stride, rope.ref if rope else None)
         check(self._be._lib().j4q_kv_append(self.handle, _int32(layer), C.byref(a), stream), "kv append")
 
@@ -177,6 +172,8 @@ class KvCache:
         with j > p - window (0: no window) or j < sinks. ``scale`` 0: 1 / sqrt(head_dim)."""
         if not type(q_ptr) is type(out_ptr) is type(stream) is int:
             q_ptr, out_ptr, stream = _addresses(q_ptr, out_ptr, stream)
+        if q_stride >> 63 or out_stride >> 63:
+            raise IllegalArgumentException(f"strides of {q_stride}, {out_stride} values")
         a = N.KvAttendArgs(q_ptr, out_ptr, q_stride, out_stride, _kind(q_type), _kind(out_type), _int32(heads), _int32(window), _int32(sinks), scale)
         check(self._be._lib().j4q_kv_attend(self.handle, _int32(layer), C.byref(a), stream), "kv attend")
 
@@ -185,4 +182,4 @@ class KvCache:
         s, f = _ints(seqs), _ints(first, "q")
         _equal(s, f, "first tokens")
         k, v, st = _addresses(k_ptr, v_ptr, stream)
-        check(self._be._lib().j4q_kv_read(self.handle, _int32(layer), _at(s), _at(f), index(count), len(s), k, v, st), "kv read")
+        check(self._be._lib().j4q_kv_read(self.handle, _int32(layer), _at(s), _at(f), _int64(count), len(s), k, v, st), "kv read")
