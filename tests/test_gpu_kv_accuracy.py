@@ -142,3 +142,78 @@ def test_weights_far_below_a_dominant_one(model, dim, group):  # noqa: F811
     e = np.abs(host(out) / want - 1)
     allowed = 6 * (length / 4 / 12) ** 0.5 / units + 2 * 2.0 ** -22 * (27 + logs + 8)
     assert (e <= allowed).all(), f"off by {e.max():.3g} of a row, bar {allowed.min():.3g}"
+
+
+@gpu
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+@pytest.mark.parametrize("dim,heads,tokens", [(64, 4, 6), (128, 4, 8), (128, 4, 20), (128, 4, 600), (256, 4, 20)])
+def test_weights_of_more_rows_far_below_a_dominant_one(model, dim, heads, tokens, kind):  # noqa: F811
+    """The same of 17 rows on: weights in fp16 (for fp32 a sum of two), whole numbers of 2^-32 of the largest down there."""
+    length = 8192
+    m = model(kv_heads=1, head_dim=dim, pages=150, page_tokens=64, sequences=1, sequence_pages=150)
+    rng = np.random.default_rng(dim + tokens)
+    u = rng.choice([-1.0, 1.0], dim) * dim ** -0.5
+    x = rng.uniform(0, 6 * np.log(2), (length + tokens, 1, 1))
+    x[0] = 26 * np.log(2)
+    v = np.ones((length + tokens, 1, dim))
+    v[0] = 0
+    m.kv.extend([0], [length + tokens])
+    m.write(0, [0], [length + tokens], x * u, v)
+    m.kv.begin([0], [tokens])
+    q = bf16(dim ** 0.5 * u * rng.uniform(0.98, 1.02, (tokens, heads, 1)))
+    dq, _ = dev_as(q, kind)
+    out = dev_as(np.zeros(q.shape), kind)[0]
+    torch.cuda.synchronize()
+    m.kv.attend(0, dq.data_ptr(), out.data_ptr(), heads, q_type=KIND[kind], out_type=KIND[kind])
+    k, v = (h.values() for h in m.of(0, 0))
+    want = exact(q, k, v, length)
+    units = want / (1 - want) * 2.0 ** 32
+    allowed = 6 * (length / 12) ** 0.5 / units + (bar(q, k) if kind == "bf16" else 4 * 2.0 ** -22 * (27 + np.log2(127) + 8))
+    e = np.abs(host(out, kind) / want - 1)
+    assert (e <= allowed).all(), f"off by {e.max():.3g} of a row, bar {allowed.min():.3g}"
+
+
+# rows for some and for many, ranges of tokens in several workgroups, windows with first tokens
+MASKED = [(128, 4, 8, 3500, 0, 0), (64, 4, 6, 6000, 1700, 4), (96, 8, 4, 3500, 130, 66), (128, 4, 40, 6000, 0, 0), (128, 4, 40, 6000, 1700, 4),
+          (128, 4, 40, 6000, 3000, 500), (256, 4, 20, 3500, 50, 3), (128, 4, 600, 1500, 700, 5)]
+
+
+def masked_inputs(dim, heads, tokens, length, window, sinks):
+    rng = np.random.default_rng(dim + tokens + window)
+    k, v = (rng.standard_normal((length + tokens, 1, dim)) for _ in range(2))
+    return bf16(rng.standard_normal((tokens, heads, dim))), k, v
+
+
+@gpu
+@pytest.mark.parametrize("case", MASKED, ids=str)
+def test_masks_of_long_contexts(model, case):  # noqa: F811
+    dim, _, tokens, length, window, sinks = case
+    m = model(kv_heads=1, head_dim=dim, pages=450, page_tokens=16, sequences=1, sequence_pages=450)
+    q, k, v = masked_inputs(*case)
+    m.kv.extend([0], [length + tokens])
+    m.write(0, [0], [length + tokens], k, v)
+    m.kv.begin([0], [tokens])
+    k, v = (h.values() for h in m.of(0, 0))
+    e = off(attend(m, q, window, sinks), exact(q, k, v, length, window, sinks))
+    assert e <= bar(q, k), f"off by {e:.3g} of a row, bar {bar(q, k):.3g}"
+
+
+@pytest.mark.parametrize("case", MASKED, ids=str)
+def test_masks_off_by_one_token_fail(case):
+    """What the bar above sees: the formula itself with a token too many or too few at either end (no GPU)."""
+    _, _, tokens, length, window, sinks = case
+    q, k, v = masked_inputs(*case)
+    held = []
+    for x in (k, v):
+        held.append(R.Held(*x.shape[1:]))
+        held[-1].append(x)
+    k, v = (h.values() for h in held)
+    want = exact(q, k, v, length, window, sinks)
+    wrong = {"one back": (length - 1, window and window - 1, sinks), "one ahead": (length + 1, window and window + 1, sinks)}
+    if window:
+        wrong |= {"window less": (length, window - 1, sinks), "window more": (length, window + 1, sinks), "a first one more": (length, window, sinks + 1),
+                  "a first one less": (length, window, sinks - 1)}
+    for name, mask in wrong.items():
+        rows = slice(None, -1) if name == "one ahead" else slice(None)  # behind the last token is none
+        e = off(exact(q, k, v, *mask)[rows], want[rows])
+        assert e > 2 * bar(q, k), f"{name}: {e:.3g}, bar {bar(q, k):.3g}"
