@@ -109,7 +109,8 @@ def generate(m, a):
     logits = m.step([0, 1], prompts)
     # the first prompt's likeliest tokens as beams beside it
     beams = list(range(2, 2 + a.beams - 1))
-    m.cache.fork([0] * len(beams), beams, stream=m.stream.cuda_stream)
+    if beams:
+        m.cache.fork([0] * len(beams), beams, stream=m.stream.cuda_stream)
     top = torch.topk(logits[0], a.beams).indices.tolist()
     seqs, tokens = [0, *beams, 1], [*top, int(logits[1].argmax())]
     start, end = (torch.cuda.Event(enable_timing=True) for _ in range(2))
