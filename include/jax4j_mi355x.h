@@ -399,7 +399,9 @@ typedef struct j4q_kv_attend_args {
  * j > p - window or j < sinks. Up to 16 rows (tokens x heads / kv_heads of a sequence) nothing of q is rounded that fp32
  * holds beside the row's largest, and a weight is off by 2^-27 of the row's largest at most. More rows take both in 22 bits or
  * more where out is fp32, and where it is bf16, q in 16 bits or fp16 and the weights in fp16 (a weight far below the row's
- * largest is off by 2^-33 of that at most). Bit for bit the same on every call with equal lengths. */
+ * largest is off by 2^-33 of that at most). A token whose weight times its block's value scale is below 2^-134 of the
+ * row's largest such product counts as none: the values that a row sees, blocks of zeros (as 2^-57) among them, have to lie within
+ * 2^100 of one another. Bit for bit the same on every call with equal lengths. */
 int j4q_kv_attend(j4q_kv kv, int32_t layer, const j4q_kv_attend_args *args, void *stream);
 /* Tokens [first[i], first[i] + count) of seqs[i] in `layer` as the cache holds them: fp32 [n][count][kv_heads][head_dim],
  * 16-byte aligned (either may be NULL); zeros where there is no token. */

@@ -395,9 +395,9 @@ void split_some(const Kv &k, bool captured, KvAttend *a) {
 }
 
 // Many rows: workgroups of 256, whose conversion of a tile serves the most rows, or of 128, two to a CU, which fill the chip sooner:
-// 8 kv heads of 128 with 4 query heads each, a chunk of 512 tokens behind 3584 (64 workgroups of 256) 54 us and with 128 58, the
-// last 64 tokens of 4096 (8) 32 and 27; a prompt of 2048, whose workgroups walk 1 to 32 tiles (256) 68 and 62, one of 8192
-// (1024) 632 and 670.
+// 8 kv heads of 128 with 4 query heads each, into bf16, a chunk of 512 tokens behind 3584 (64 workgroups of 256) 55 us and with 128
+// 67, the last 64 tokens of 4096 (8) 30 and 26; a prompt of 2048, whose workgroups walk 1 to 32 tiles (256) 70 and 65, one of
+// 8192 (1024) 561 and 602.
 // Ranges by what they are estimated to cost: a tile takes a workgroup 1.3 us (of 128 rows), the chip's throughput has a floor,
 // and parts are written and read back, behind a launch. (The last 64 tokens of 4096, one kv head: 33.4 us in 4 ranges, 17.8 in 16.)
 void split_many(const Kv &k, bool captured, KvAttend *a) {
