@@ -1,12 +1,14 @@
 """Calls on one key/value cache over streams whose handles do not tell them apart: every result is that of the calls in order."""
 from __future__ import annotations
 
+import ctypes as C
 import threading
 
 import numpy as np
 import pytest
 import torch
 
+from jax4j_amd import IllegalArgumentException
 from jax4j_amd import _native as N
 from test_gpu_kept_memory import Hip
 from test_gpu_kv import dev, model  # noqa: F401
@@ -89,3 +91,36 @@ def test_a_stream_created_where_one_was_destroyed(model):  # noqa: F811
         steps.attend(i, hip.stream.value)
     hip.close()
     steps.check(12)
+
+
+def test_the_engine_stream_captured(model, backend):  # noqa: F811
+    """Attention captured on the engine stream: a call on another stream is refused meanwhile and goes through afterwards, and every
+    replay gives what the same call gives."""
+    steps, hip = Steps(model), Hip()
+    st, graph, run = C.c_void_p(backend.stream()), C.c_void_p(), C.c_void_p()
+    steps.append(0, 0)
+    steps.append(1, 0)
+    steps.kv.begin([0], [100])
+    steps.attend(1, 0)
+    torch.cuda.synchronize()
+    hip.ok("hipStreamBeginCapture", st, 2)  # relaxed
+    steps.attend(0, 0)
+    with pytest.raises(IllegalArgumentException, match="engine stream"):
+        steps.append(2, hip.stream.value)
+    with pytest.raises(IllegalArgumentException, match="engine stream"):
+        steps.attend(2, hip.stream.value)
+    hip.ok("hipStreamEndCapture", st, C.byref(graph))
+    hip.ok("hipGraphInstantiate", C.byref(run), graph, None, None, C.c_size_t(0))
+    assert steps.kv.lengths([0]).tolist() == [200]
+    for _ in range(4):
+        steps.out[0].zero_()
+        torch.cuda.synchronize()
+        hip.ok("hipGraphLaunch", run, st)
+        hip.wait()
+        got = steps.out[0].clone()
+        steps.attend(0, hip.stream.value)
+        torch.cuda.synchronize()
+        assert torch.allclose(got, steps.out[0], rtol=0, atol=4e-5) and bool(got.abs().max() > 0)  # perhaps in other ranges of the tokens
+    hip.ok("hipGraphExecDestroy", run)
+    hip.ok("hipGraphDestroy", graph)
+    hip.close()
