@@ -300,7 +300,8 @@ int j4q_decode_plan_destroy(j4q_plan plan);
  * every block of 16 tokens and kv head, in pages of page_tokens tokens that all layers have in common. Where new tokens
  * begin a block its scale is max(amax / 127, 2^-64); a later token that does not fit doubles it until it does, and the
  * block's codes are divided by as much (rounded to even, as every code is: an error below one step of the final
- * scale). A block with a value that is not finite is NaN as a whole, and so is a row that sees it.
+ * scale). A block with a value that is not finite is NaN as a whole, also when that token is cut off, and so is a row that sees
+ * any token of it.
  *
  * A step: j4q_kv_extend names the sequences and how many tokens each gets; rows of q, k, v and out are these tokens in
  * that order; then per layer j4q_kv_append and j4q_kv_attend. Pages and lengths are host state: a call that cannot be

@@ -11,7 +11,7 @@
 // The other operand is fp32 (q, w); it enters as four digits to the base 256 from -128 to 127 of a whole number of 31 bits: q over
 // its row's largest magnitude / 2^30, so nothing that fp32 holds beside that is lost; w below 2^30, rounded to the nearest, so a
 // weight is off by 2^-27 of the largest that its wave has seen at most, either way (cut off, thousands of tokens far below a
-// dominant one lost half a unit each: 0.6 to 1.4 % of their sum). The digits fill the 16 columns of the second operand: 4 rows x
+// dominant one lost half a unit each: 0.6 to 1.2 % of their sum). The digits fill the 16 columns of the second operand: 4 rows x
 // 4 digits in one instruction, or 8 rows x 2 digits in two. Operands:
 //   scores   A = 16 tokens x 64 channels of K, B = 64 channels x 16 (digit, row):  C[token][digit, row]
 //   output   A = 16 channels x 64 tokens of V, B = 64 tokens x 16 (digit, row) of w: C[channel][digit, row]
