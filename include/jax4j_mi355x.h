@@ -408,6 +408,101 @@ int j4q_kv_attend(j4q_kv kv, int32_t layer, const j4q_kv_attend_args *args, void
  * 16-byte aligned (either may be NULL); zeros where there is no token. */
 int j4q_kv_read(j4q_kv kv, int32_t layer, const int32_t *seqs, const int64_t *first, int64_t count, int32_t n, float *k, float *v, void *stream);
 
+/* ---- a block of experts: norms, routing, the experts' products (engine-local; the reference has none of them) ---- */
+
+/* A norm over the values of a row: kind J4Q_NORM_RMS x / sqrt(mean(x^2) + eps) * (weight + weight_add) + bias, or
+ * J4Q_NORM_LAYER with (x - mean(x)) and the variance. weight (NULL: 1) and bias (NULL: 0): device memory, fp32 [dim]. */
+enum j4q_norm_kind { J4Q_NORM_RMS = 1, J4Q_NORM_LAYER = 2 };
+typedef struct j4q_norm {
+    int32_t kind;
+    float eps;
+    const float *weight, *bias;
+    float weight_add;        /* e.g. 1 where a file holds weights less 1 */
+} j4q_norm;
+
+typedef struct j4q_norm_args {
+    const void *residual;    /* [rows][dim], NULL: zeros */
+    const void *block;       /* a block's output [rows][dim]; NULL: none */
+    const void *gate;        /* NULL: 1; [dim], or [ceil(rows / gate_every)][dim]: row r takes gate row r / gate_every */
+    void *residual_out;      /* h in the residual's type; NULL: not stored; may be the residual itself */
+    void *out;               /* [rows][dim], NULL where `before` is */
+    int64_t rows, gate_every; /* gate_every 0: one gate for all rows */
+    int64_t residual_stride, block_stride, gate_stride, residual_out_stride, out_stride; /* values from a row to the next; 0: dim */
+    int32_t dim;             /* up to 32768 */
+    int32_t residual_type, block_type, gate_type, out_type; /* J4Q_KIND_F32 or J4Q_KIND_BF16 */
+    float scale;
+    const j4q_norm *after;   /* the norm behind the block; NULL: none */
+    const j4q_norm *before;  /* the next block's; NULL: none (residual_out alone) */
+} j4q_norm_args;
+/* h = residual + scale * gate * after(block); residual_out = h; out = before(h), of h before it is rounded. All in 32 bits, sums in
+ * 64. An output may be an input of the same type and stride, else they lie apart. */
+int j4q_norm_into(const j4q_norm_args *args, void *stream);
+
+enum j4q_route_score { J4Q_ROUTE_SOFTMAX = 0, J4Q_ROUTE_SIGMOID = 1 };
+typedef struct j4q_route_args {
+    const void *logits;      /* [rows][experts], J4Q_KIND_F32 or J4Q_KIND_BF16 */
+    const float *bias;       /* NULL, or [experts]: added to the scores for the choice alone */
+    int32_t *ids;            /* [rows][top_k] */
+    float *weights;          /* [rows][top_k] */
+    int64_t rows, stride;    /* values from a row of logits to the next; 0: experts */
+    int32_t type, experts;   /* up to 1024 */
+    int32_t top_k;           /* up to 64 */
+    int32_t score;           /* j4q_route_score */
+    int32_t groups;          /* equal parts of the experts (up to 64); 0 or 1: none */
+    int32_t top_groups;      /* how many of them are open */
+    int32_t group_best;      /* 1 or 2: a group's rank is the sum of so many of its best */
+    int32_t renormalize;     /* the weights of a row are divided by their sum */
+    float scale;
+} j4q_route_args;
+/* The top_k experts of every row, the best first, and their weights. The choice goes by the logits, or with a bias by score + bias in 64
+ * bits; of equals the expert (or group) with the lowest index is first. A logit (or sum with the bias) that is NaN or -inf is never
+ * chosen; a slot that finds no expert gets id -1 and weight 0. Weights are scores (softmax over all experts, or sigmoid), without the
+ * bias, times `scale`. */
+int j4q_route_into(const j4q_route_args *args, void *stream);
+
+/* The matrices of a layer of experts: gate and up [experts * ffn, dim] of one type, down [experts * dim, ffn], expert after expert, as
+ * j4q_gguf_upload gives GGUF's three-dimensional tensors. Types Q8_0 (columns a multiple of 64), Q4_0 (of 128), Q4_K and Q6_K. The
+ * handle keeps the buffers from being released, and holds a power of two for each row and a bound for each expert, which
+ * j4q_experts_create computes once. */
+typedef uint64_t j4q_experts; /* 0 is never a valid handle */
+enum j4q_activation { J4Q_ACT_SILU = 0, J4Q_ACT_GELU = 1 /* the tanh form */, J4Q_ACT_RELU = 2 };
+typedef struct j4q_experts_config {
+    j4q_buffer gate, up, down;
+    int32_t experts;         /* up to 1024 */
+    int32_t activation;      /* j4q_activation */
+} j4q_experts_config;
+typedef struct j4q_experts_desc {
+    j4q_experts_config config;
+    int64_t dim, ffn;
+    uint64_t weight_bytes;   /* GGUF bytes of the three matrices */
+    uint64_t bytes;          /* device memory of the handle itself */
+} j4q_experts_desc;
+typedef struct j4q_experts_args {
+    const void *x;           /* [rows][dim], 16-byte aligned */
+    const int32_t *ids;      /* [rows][top_k]; an id outside [0, experts) is no expert */
+    const float *weights;    /* [rows][top_k] */
+    void *out;               /* [rows][dim], 16-byte aligned, apart from the others */
+    int64_t rows;            /* rows * top_k up to 2^22 */
+    int64_t x_stride, out_stride; /* values from a row to the next, 0: dim; a multiple of 16 bytes */
+    int32_t top_k;           /* up to 64 */
+    int32_t type;            /* of x and out: J4Q_KIND_F32 or J4Q_KIND_BF16 */
+    void *workspace;         /* NULL: the engine's; else 256-byte aligned device memory that no other call uses meanwhile */
+    uint64_t workspace_bytes; /* at least what j4q_experts_workspace says */
+} j4q_experts_args;
+/* Waits for the device. */
+int j4q_experts_create(const j4q_experts_config *config, j4q_experts *out);
+/* Waits for the device. 0 is a no-op. */
+int j4q_experts_destroy(j4q_experts experts);
+int j4q_experts_info(j4q_experts experts, j4q_experts_desc *out);
+/* out[r] = sum over the slots s of a row of weights[r][s] * down_e (act(gate_e x_r) * (up_e x_r)), e = ids[r][s]; a row without experts is
+ * zeros, the same expert twice counts twice. fp32: as j4q_quant_matvec_into's batches, x and the inner activations in 22 bits, weights as
+ * they are or in 22 bits, sums in 32. bf16: the inner activations in 11 bits, and in a prompt the weights too. A row of x with a value
+ * that is not finite gives a row of NaN where it has an expert. Bit for bit the same on every call with the same arguments. The engine's
+ * workspace is as j4q_quant_matvec_into's: under stream capture two memory nodes, which a caller's own workspace saves. */
+int j4q_experts_apply(j4q_experts experts, const j4q_experts_args *args, void *stream);
+/* Bytes of workspace that a call of so many rows takes. */
+int j4q_experts_workspace(j4q_experts experts, int64_t rows, int32_t top_k, int type, uint64_t *bytes);
+
 /* ---- GGUF files (the step before uploadQuantized; engine-local) ---------------------- */
 /* The reference receives quantized blobs from an external caller (spi/QuantizedOps.java:24)
  * and knows the GGUF type ids (core/tensor/QuantType.java:3-13); this reader supplies them

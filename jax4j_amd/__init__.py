@@ -4,6 +4,7 @@ The engine is the C-ABI library ``lib/libjax4j_mi355x.so`` (HIP kernels in ``csr
 this package is its host-side mirror of the reference's QuantizedOps SPI.
 """
 from .backend import Mi355xBackend, check, default_backend
+from .experts import Experts, Norm
 from .kv import KvCache, Rope
 from .tensor import (
     Device,
@@ -20,6 +21,8 @@ __all__ = [
     "Mi355xBackend",
     "default_backend",
     "check",
+    "Experts",
+    "Norm",
     "KvCache",
     "Rope",
     "Device",

@@ -30,6 +30,14 @@ GEMM_BF16 = 1
 # j4q_gemv_policy
 GEMV_MATRIX_CORES = 0
 GEMV_FP32 = 1
+# j4q_norm_kind, j4q_route_score, j4q_activation
+NORM_RMS = 1
+NORM_LAYER = 2
+ROUTE_SOFTMAX = 0
+ROUTE_SIGMOID = 1
+ACT_SILU = 0
+ACT_GELU = 1
+ACT_RELU = 2
 
 
 class DeviceProps(C.Structure):
@@ -167,6 +175,97 @@ class KvAttendArgs(C.Structure):
     ]
 
 
+class NormKind(C.Structure):
+    _fields_ = [
+        ("kind", C.c_int32),
+        ("eps", C.c_float),
+        ("weight", C.c_void_p),
+        ("bias", C.c_void_p),
+        ("weight_add", C.c_float),
+    ]
+
+
+class NormArgs(C.Structure):
+    _fields_ = [
+        ("residual", C.c_void_p),
+        ("block", C.c_void_p),
+        ("gate", C.c_void_p),
+        ("residual_out", C.c_void_p),
+        ("out", C.c_void_p),
+        ("rows", C.c_int64),
+        ("gate_every", C.c_int64),
+        ("residual_stride", C.c_int64),
+        ("block_stride", C.c_int64),
+        ("gate_stride", C.c_int64),
+        ("residual_out_stride", C.c_int64),
+        ("out_stride", C.c_int64),
+        ("dim", C.c_int32),
+        ("residual_type", C.c_int32),
+        ("block_type", C.c_int32),
+        ("gate_type", C.c_int32),
+        ("out_type", C.c_int32),
+        ("scale", C.c_float),
+        ("after", C.POINTER(NormKind)),
+        ("before", C.POINTER(NormKind)),
+    ]
+
+
+class RouteArgs(C.Structure):
+    _fields_ = [
+        ("logits", C.c_void_p),
+        ("bias", C.c_void_p),
+        ("ids", C.c_void_p),
+        ("weights", C.c_void_p),
+        ("rows", C.c_int64),
+        ("stride", C.c_int64),
+        ("type", C.c_int32),
+        ("experts", C.c_int32),
+        ("top_k", C.c_int32),
+        ("score", C.c_int32),
+        ("groups", C.c_int32),
+        ("top_groups", C.c_int32),
+        ("group_best", C.c_int32),
+        ("renormalize", C.c_int32),
+        ("scale", C.c_float),
+    ]
+
+
+class ExpertsConfig(C.Structure):
+    _fields_ = [
+        ("gate", C.c_uint64),
+        ("up", C.c_uint64),
+        ("down", C.c_uint64),
+        ("experts", C.c_int32),
+        ("activation", C.c_int32),
+    ]
+
+
+class ExpertsDesc(C.Structure):
+    _fields_ = [
+        ("config", ExpertsConfig),
+        ("dim", C.c_int64),
+        ("ffn", C.c_int64),
+        ("weight_bytes", C.c_uint64),
+        ("bytes", C.c_uint64),
+    ]
+
+
+class ExpertsArgs(C.Structure):
+    _fields_ = [
+        ("x", C.c_void_p),
+        ("ids", C.c_void_p),
+        ("weights", C.c_void_p),
+        ("out", C.c_void_p),
+        ("rows", C.c_int64),
+        ("x_stride", C.c_int64),
+        ("out_stride", C.c_int64),
+        ("top_k", C.c_int32),
+        ("type", C.c_int32),
+        ("workspace", C.c_void_p),
+        ("workspace_bytes", C.c_uint64),
+    ]
+
+
 _i32, _i64, _u64, _vp = C.c_int32, C.c_int64, C.c_uint64, C.c_void_p
 _buf = C.c_uint64
 _pbuf = C.POINTER(C.c_uint64)
@@ -229,6 +328,13 @@ SIGNATURES = {
     "j4q_kv_append": [_u64, _i32, C.POINTER(KvAppendArgs), _vp],
     "j4q_kv_attend": [_u64, _i32, C.POINTER(KvAttendArgs), _vp],
     "j4q_kv_read": [_u64, _i32, _vp, _vp, _i64, _i32, _vp, _vp, _vp],
+    "j4q_norm_into": [C.POINTER(NormArgs), _vp],
+    "j4q_route_into": [C.POINTER(RouteArgs), _vp],
+    "j4q_experts_create": [C.POINTER(ExpertsConfig), C.POINTER(_u64)],
+    "j4q_experts_destroy": [_u64],
+    "j4q_experts_info": [_u64, C.POINTER(ExpertsDesc)],
+    "j4q_experts_workspace": [_u64, _i64, _i32, C.c_int, C.POINTER(_u64)],
+    "j4q_experts_apply": [_u64, C.POINTER(ExpertsArgs), _vp],
     "j4q_gguf_open": [C.c_char_p, C.POINTER(_u64)],
     "j4q_gguf_close": [_u64],
     "j4q_gguf_file_info": [_u64, C.POINTER(GgufInfo)],

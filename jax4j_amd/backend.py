@@ -69,6 +69,14 @@ def _int64(v) -> int:
     return v
 
 
+def _kind(dtype: DType) -> int:
+    if dtype is DType.F32:
+        return N.KIND_F32
+    if dtype is DType.BF16:
+        return N.KIND_BF16
+    raise IllegalArgumentException(f"values are F32 or BF16, not {dtype}")
+
+
 def _as_u8(blocks) -> np.ndarray:
     if isinstance(blocks, np.ndarray):
         return np.ascontiguousarray(blocks).reshape(-1).view(np.uint8)
@@ -310,6 +318,39 @@ class Mi355xBackend:
         if (heads | head_dim) >> 31 or (rows | x_stride | out_stride) >> 63:  # _int32, _int64 of each take 0.5 us
             raise IllegalArgumentException(f"rope_into: {rows} rows of {heads} heads of {head_dim}, strides of {x_stride}, {out_stride} values")
         check(self._lib().j4q_rope_into(x_ptr, out_ptr, kind, rows, heads, head_dim, x_stride, out_stride, rope.ref, stream), "rope_into")
+
+    def norm_into(self, residual_ptr: int, out_ptr: int, rows: int, dim: int, before: "Norm | None" = None, *, residual_type: DType = DType.F32,
+                  out_type: DType = DType.F32, block_ptr: int = 0, block_type: DType = DType.F32, after: "Norm | None" = None, gate_ptr: int = 0,
+                  gate_type: DType = DType.F32, gate_every: int = 0, scale: float = 1.0, residual_out_ptr: int = 0, residual_stride: int = 0,
+                  block_stride: int = 0, gate_stride: int = 0, residual_out_stride: int = 0, out_stride: int = 0, stream: int = 0) -> None:
+        """h = residual + scale * gate * after(block), stored at ``residual_out_ptr`` (0: nowhere) in the residual's type; before(h) at
+        ``out_ptr``. Every part but one input and one output may be absent (0, None). ``gate``: [dim], or with ``gate_every`` a row
+        for so many rows. Strides in values, 0: dim."""
+        if not type(residual_ptr) is type(out_ptr) is type(block_ptr) is type(gate_ptr) is type(residual_out_ptr) is type(stream) is int:
+            residual_ptr, out_ptr, block_ptr, gate_ptr, residual_out_ptr, stream = _addresses(residual_ptr, out_ptr, block_ptr, gate_ptr, residual_out_ptr, stream)
+        if dim >> 31 or (rows | gate_every | residual_stride | block_stride | gate_stride | residual_out_stride | out_stride) >> 63:
+            raise IllegalArgumentException(f"norm_into: {rows} rows of {dim} values, or a stride, are negative or do not fit")
+        a = N.NormArgs(residual_ptr, block_ptr, gate_ptr, residual_out_ptr, out_ptr, rows, gate_every, residual_stride, block_stride, gate_stride,
+                       residual_out_stride, out_stride, dim, _kind(residual_type), _kind(block_type), _kind(gate_type), _kind(out_type), scale,
+                       after.ref if after else None, before.ref if before else None)
+        check(self._lib().j4q_norm_into(C.byref(a), stream), "norm_into")
+
+    def route_into(self, logits_ptr: int, ids_ptr: int, weights_ptr: int, rows: int, experts: int, top_k: int, *, dtype: DType = DType.F32,
+                   stride: int = 0, score: str = "softmax", bias_ptr: int = 0, groups: int = 1, top_groups: int = 1, group_best: int = 1,
+                   renormalize: bool = False, scale: float = 1.0, stream: int = 0) -> None:
+        """The ``top_k`` experts of every row of logits [rows, experts]: int32 ids and fp32 weights [rows, top_k], the best first; id -1
+        and weight 0 where none is left. ``score``: "softmax" or "sigmoid"; ``bias``: fp32 [experts], for the choice alone; ``groups``:
+        only experts of the ``top_groups`` groups with the largest sum of their ``group_best`` best."""
+        s = {"softmax": N.ROUTE_SOFTMAX, "sigmoid": N.ROUTE_SIGMOID}.get(score)
+        if s is None:
+            raise IllegalArgumentException(f"unknown score {score!r} (softmax or sigmoid)")
+        if not type(logits_ptr) is type(ids_ptr) is type(weights_ptr) is type(bias_ptr) is type(stream) is int:
+            logits_ptr, ids_ptr, weights_ptr, bias_ptr, stream = _addresses(logits_ptr, ids_ptr, weights_ptr, bias_ptr, stream)
+        if (experts | top_k | groups | top_groups | group_best) >> 31 or (rows | stride) >> 63:
+            raise IllegalArgumentException(f"route_into: {rows} rows, {top_k} of {experts} experts in {groups} groups")
+        a = N.RouteArgs(logits_ptr, bias_ptr, ids_ptr, weights_ptr, rows, stride, _kind(dtype), experts, top_k, s, groups, top_groups, group_best,
+                        int(bool(renormalize)), scale)
+        check(self._lib().j4q_route_into(C.byref(a), stream), "route_into")
 
     def decode_plan(self, layers, head, batch: int, io: dict) -> "DecodePlan":
         """The quantized matmuls of a decode step as one replayable plan (engine-local).

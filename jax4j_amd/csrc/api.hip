@@ -433,6 +433,8 @@ std::mutex &lock() { return g_mu; }
 int ready_locked() { return ensure_ready(); }
 hipStream_t stream() { return g_stream; }
 hipError_t malloc_locked(void **p, uint64_t bytes) { return dev_malloc(p, bytes); }
+hipError_t workspace_begin_locked(hipStream_t s, uint64_t bytes, Workspace *ws) { return g_workspaces.begin(s, g_stream, bytes, ws); }
+void workspace_end_locked(hipStream_t s, const Workspace &ws, bool launched) { g_workspaces.end(s, ws, launched); }
 
 int quant_locked(j4q_buffer h, const char *op, QuantRef *out) {
     Buf *b;
@@ -729,7 +731,7 @@ int j4q_release(j4q_buffer h) {
     if ((rc = get_buf(h, 0, "release", &b))) return rc;
     if (b->pins > 0)
         return fail(J4Q_EINVAL,
-                    "release: buffer 0x%llx is read by %d live decode plan(s), e.g. 0x%llx; destroy the plan first",
+                    "release: buffer 0x%llx is read by %d live decode plan(s) or experts, e.g. 0x%llx; destroy those first",
                     (unsigned long long)h, (int)b->pins, (unsigned long long)b->last_plan);
     if (b->dev) {
         if ((rc = ensure_ready())) return rc;

@@ -27,6 +27,10 @@ hipStream_t stream();
 // given back where it was short.
 hipError_t malloc_locked(void **p, uint64_t bytes);
 
+// With the lock held: a workspace as j4q_quant_matvec_into takes it (kept_memory.h). launched: whether every launch went out.
+hipError_t workspace_begin_locked(hipStream_t s, uint64_t bytes, Workspace *ws);
+void workspace_end_locked(hipStream_t s, const Workspace &ws, bool launched);
+
 // A resident quantized matrix, as the kernels see it.
 struct QuantRef {
     int qtype;

@@ -1,0 +1,109 @@
+// The experts' products of a layer (j4q_experts_apply): out_r = sum_s w_rs down_e (act(gate_e x_r) * (up_e x_r)), e = ids_rs.
+// Engine-local; the reference has no experts. What the kernels share; launches and checks: experts.hip.
+//
+// Pairs (row, slot) are put in the order of their experts, each expert's in the order of the rows, and cut into tiles of pairs that
+// share an expert; all of it on the GPU, so that a call waits for nothing and may be captured. A launch per step:
+//  1. experts_plan: order and tiles; x as fp16.   2. gate|up of every tile, the activation in its epilogue.
+//  3. down of every tile, a weighted partial result for each pair.   4. experts_combine: the sums of a row's pairs, slot by slot.
+//
+// Activations enter the matrix cores as fp16: x' = x 2^e, e a power for each row that brings its largest magnitude into
+// [2^14, 2^15), as one value (bf16 x: exact down to 2^-28 of the largest) or as hi + lo (fp32 x: 22 bits down to 2^-18). The inner
+// activations are stored the same way, at a power that is known before they are: |g u| <= |x|^2 G U, with G and U
+// the largest norms of the expert's gate and up rows, so h' = h 2^(14 - ceil(log2 of that)) cannot overflow. Where the vectors are no
+// worse than random the bound is about `dim` times what is typical: 2^12 of fp16's 2^29 normal binades at dim 4096.
+//
+// Layout of x' and h' (block layout): of every 32 values, 16-byte chunk g = 0..3 holds elements 4 g + {0, 2, 1, 3} and then
+// 16 + 4 g + {0, 2, 1, 3}: what masking dword g of a block of codes yields, for every type alike, so that a lane of the matrix core reads
+// its 8 values with one load and codes are never reordered.
+#pragma once
+
+#include "gemv_lanes.h"
+#include "j4q_common.h"
+
+namespace j4q {
+namespace ex {
+
+using gmf::h2;
+using gmf::h4;
+using gmf::h8;
+using gemv::f32x4;
+using gemv::kOob;
+using gemv::make_rsrc;
+using gemv::u32x2;
+using gemv::u32x4;
+
+constexpr int kBound = 14;       // |h'| <= 2^kBound
+constexpr int kNothing = -4096;  // exponent of a norm of 0
+
+// A tile: pairs [first, first + count) of the order, all of one expert.
+struct Tile {
+    int32_t expert, first, count, pad;
+};
+
+struct Weights {
+    QMat gate, up, down;
+    int up_type, down_type;
+    int experts, dim, ffn, act;
+    const int32_t *bound;                       // ceil(log2(G U)) of each expert
+    const int32_t *gate_pow, *up_pow, *down_pow;  // of each row: max |w| 2^pow in [2^13, 2^14)
+};
+
+struct Call {
+    const void *x;
+    int64_t x_stride;  // values
+    const int32_t *ids;
+    const float *weights;
+    void *out;
+    int64_t out_stride;
+    int rows, top, pairs;
+    bool half;      // bf16 x and out; x' and h' have no lo part
+    int tile_rows;  // pairs of a tile
+    int tiles;      // of the grid: no call has more
+    // workspace
+    int32_t *order, *tile_count;
+    Tile *tile;
+    _Float16 *xa, *ha;         // hi; lo behind all of hi
+    int32_t *x_pow, *x_norm;   // of each row: e, and an exponent with |x| <= 2^it
+    float *part;               // [pairs][dim]
+};
+
+__device__ __forceinline__ int h_pow(const Weights &w, int expert, int x_norm) { return kBound - (2 * x_norm + w.bound[expert]); }
+
+// Where element c of a row lies in the block layout.
+__device__ __forceinline__ int slot_of(int c) {
+    const int r = c & 15, i = r & 3;
+    return (c & ~31) + 8 * (r >> 2) + 4 * (c >> 4 & 1) + ((i & 1) << 1 | i >> 1);
+}
+
+__device__ __forceinline__ float activate(float g, int act) {
+    if (act == 2) return g < 0.f ? 0.f : g;  // NaN stays NaN
+    if (act == 1) {
+        const float t = 0.7978845608028654f * (g + 0.044715f * g * g * g);
+        return g / (1.f + expf(-2.f * t));  // (1 + tanh t) / 2 = 1 / (1 + e^-2t)
+    }
+    return g / (1.f + expf(-g));
+}
+
+// View of one expert's rows.
+__device__ __forceinline__ QMat expert_of(const QMat &m, int fmt, int e, int64_t rows) {
+    QMat o = m;
+    const int64_t first = (int64_t)e * rows, k = m.cols;
+    o.rows = rows;
+    switch (fmt) {
+    case Q8_0: o.qs += first * k; o.sc += first * (k / 16); break;
+    case Q4_0:
+    case Q4_K: o.qs += first * (k / 2); o.sc += first * (k / 16); break;
+    default:
+        o.qs += first * (k / 2);
+        o.qh += first * (k / 4);
+        o.sc += first * (k / 16);
+        o.d += first * (k / 128);
+        break;
+    }
+    return o;
+}
+
+hipError_t launch_few(const Weights &w, const Call &c, bool down, hipStream_t s);
+
+}  // namespace ex
+}  // namespace j4q

@@ -1,0 +1,538 @@
+// The experts' products of a layer, host side, and what surrounds the products: the pairs in the order of their experts, x as fp16, the
+// weighted sums (experts.h).
+#include <limits.h>
+
+#include <exception>
+#include <memory>
+#include <vector>
+
+#include "arguments.h"
+#include "engine.h"
+#include "experts.h"
+#include "kept_memory.h"
+
+namespace j4q {
+namespace ex {
+namespace {
+
+constexpr int kMaxExperts = 1024, kMaxTop = 64, kPlanThreads = 512;
+
+// ---- the order of the pairs, and x' -------------------------------------------------------
+
+__device__ __forceinline__ int wave_total(int v) {
+#pragma unroll
+    for (int o = 32; o > 0; o /= 2) v += __shfl_xor(v, o);
+    return v;
+}
+
+// Workgroup e < experts: the pairs of expert e in rising order, behind those of the experts before it, and their tiles. Every
+// workgroup counts all ids itself, so that none waits for another; each of its waves then places the matches of a contiguous part.
+__device__ void order_pairs(const Weights &w, const Call &c, int e) {
+    __shared__ int hist[kMaxExperts];
+    __shared__ int wave_count[kPlanThreads / 64], sums[2][kPlanThreads / 64];
+    const int t = (int)threadIdx.x, lane = t & 63, wave = t >> 6;
+    for (int i = t; i < w.experts; i += kPlanThreads) hist[i] = 0;
+    __syncthreads();
+    const int part = (c.pairs + kPlanThreads - 1) / kPlanThreads * 64, from = wave * part, to = from + part < c.pairs ? from + part : c.pairs;
+    int mine = 0;
+    for (int i = from + lane; i < to; i += 64) {
+        const int id = c.ids[i];
+        if (id >= 0 && id < w.experts) atomicAdd(&hist[id], 1);
+        mine += id == e;
+    }
+    mine = wave_total(mine);
+    if (lane == 0) wave_count[wave] = mine;
+    __syncthreads();
+    int before = 0, tiles = 0;  // of the experts before this one
+    for (int i = t; i < e; i += kPlanThreads) {
+        before += hist[i];
+        tiles += (hist[i] + c.tile_rows - 1) / c.tile_rows;
+    }
+    before = wave_total(before);
+    tiles = wave_total(tiles);
+    if (lane == 0) sums[0][wave] = before, sums[1][wave] = tiles;
+    __syncthreads();
+    before = tiles = 0;
+#pragma unroll
+    for (int v = 0; v < kPlanThreads / 64; v++) before += sums[0][v], tiles += sums[1][v];
+    const int count = hist[e], own = (count + c.tile_rows - 1) / c.tile_rows;
+    for (int i = t; i < own; i += kPlanThreads) {
+        const int left = count - i * c.tile_rows;
+        c.tile[tiles + i] = Tile{e, before + i * c.tile_rows, left < c.tile_rows ? left : c.tile_rows, 0};
+    }
+    if (e == w.experts - 1 && t == 0) c.tile_count[0] = tiles + own;
+    if (!count) return;
+    int at = before;
+    for (int v = 0; v < wave; v++) at += wave_count[v];
+    for (int i0 = from; i0 < to; i0 += 64) {
+        const int i = i0 + lane;
+        const bool is = i < to && c.ids[i] == e;
+        const uint64_t all = __ballot(is);
+        if (is) c.order[at + __popcll(all & ((1ull << lane) - 1))] = i;
+        at += __popcll(all);
+    }
+}
+
+// Row r of x as x' in the block layout, its power and its norm's exponent.
+__device__ void convert_row(const Weights &w, const Call &c, int r) {
+    __shared__ float most[kPlanThreads / 64], squares[kPlanThreads / 64];
+    const int t = (int)threadIdx.x, K = w.dim;
+    const uint8_t *const x = (const uint8_t *)c.x + (int64_t)r * c.x_stride * (c.half ? 2 : 4);
+    // thread t and pass p: the 8 elements of chunk g = i % 4 of block i / 4, i = t + threads * p
+    auto load = [&](int i, float (&v)[8]) __attribute__((always_inline)) {
+        const int at = (i >> 2) * 32 + 4 * (i & 3);
+        if (c.half) {
+            const u32x2 a = *reinterpret_cast<const u32x2 *>(x + 2 * at), b = *reinterpret_cast<const u32x2 *>(x + 2 * at + 32);
+#pragma unroll
+            for (int j = 0; j < 2; j++) {
+                v[2 * j] = __builtin_bit_cast(float, a[j] << 16);
+                v[2 * j + 1] = __builtin_bit_cast(float, a[j] & 0xFFFF0000u);
+                v[4 + 2 * j] = __builtin_bit_cast(float, b[j] << 16);
+                v[5 + 2 * j] = __builtin_bit_cast(float, b[j] & 0xFFFF0000u);
+            }
+        } else {
+            const f32x4 a = *reinterpret_cast<const f32x4 *>(x + 4 * at), b = *reinterpret_cast<const f32x4 *>(x + 4 * at + 64);
+#pragma unroll
+            for (int j = 0; j < 4; j++) v[j] = a[j], v[4 + j] = b[j];
+        }
+    };
+    float top = 0.f;
+    bool finite = true;
+    for (int i = t; i < K / 8; i += kPlanThreads) {
+        float v[8];
+        load(i, v);
+#pragma unroll
+        for (int j = 0; j < 8; j++) {
+            top = fmaxf(top, fabsf(v[j]));
+            finite &= fabsf(v[j]) <= 3.402823466e38f;
+        }
+    }
+    top = finite ? top : __builtin_inff();
+#pragma unroll
+    for (int o = 32; o > 0; o /= 2) top = fmaxf(top, __shfl_xor(top, o));
+    if ((t & 63) == 0) most[t >> 6] = top;
+    __syncthreads();
+#pragma unroll
+    for (int v = 0; v < kPlanThreads / 64; v++) top = fmaxf(top, most[v]);
+    finite = top <= 3.402823466e38f;
+    int e = 0;
+    if (finite && top > 0.f) {
+        (void)frexpf(top, &e);
+        e = 15 - e;
+    }
+    float sum = 0.f;
+    const int64_t lo = (int64_t)c.rows * K;
+    _Float16 *const out = c.xa + (int64_t)r * K;
+    for (int i = t; i < K / 8; i += kPlanThreads) {
+        float v[8];
+        load(i, v);
+        h8 h, l;
+#pragma unroll
+        for (int j = 0; j < 8; j++) {
+            const int from = (j & 4) | (j & 1) << 1 | (j >> 1 & 1);  // 0, 2, 1, 3
+            const float s = finite ? __builtin_ldexpf(v[from], e) : __builtin_nanf("");
+            sum = __builtin_fmaf(s, s, sum);
+            h[j] = (_Float16)s;
+            l[j] = (_Float16)(s - (float)h[j]);
+        }
+        *reinterpret_cast<h8 *>(out + 8 * i) = h;
+        if (!c.half) *reinterpret_cast<h8 *>(out + lo + 8 * i) = l;
+    }
+#pragma unroll
+    for (int o = 32; o > 0; o /= 2) sum += __shfl_xor(sum, o);
+    if ((t & 63) == 0) squares[t >> 6] = sum;
+    __syncthreads();
+    if (t) return;
+    sum = 0.f;
+    for (int v = 0; v < kPlanThreads / 64; v++) sum += squares[v];
+    int norm = kNothing;
+    if (finite && sum > 0.f) {
+        (void)frexpf(sum * 1.0001f, &norm);  // above what the sum was rounded by
+        norm = ((norm + 1) >> 1) - e;
+    }
+    c.x_pow[r] = e;
+    c.x_norm[r] = finite ? norm : 0;
+}
+
+// grid: experts workgroups, and one for each row.
+__global__ void __launch_bounds__(kPlanThreads)
+experts_plan(Weights w, Call c) {
+    if ((int)blockIdx.x < w.experts) order_pairs(w, c, (int)blockIdx.x);
+    else convert_row(w, c, (int)blockIdx.x - w.experts);
+}
+
+// ---- the sums -------------------------------------------------------------------------------
+
+// out[r] = sum over its slots, one after another, of the weighted partial results. A thread per 4 columns.
+__global__ void __launch_bounds__(256)
+experts_combine(Weights w, Call c) {
+    const int r = (int)(blockIdx.z * gridDim.y + blockIdx.y), col = 4 * (int)(blockIdx.x * 256 + threadIdx.x);
+    if (r >= c.rows || col >= w.dim) return;
+    f32x4 s = {};
+    for (int k = 0; k < c.top; k++) {
+        const int64_t pair = (int64_t)r * c.top + k;
+        const int id = c.ids[pair];
+        if (id < 0 || id >= w.experts) continue;
+        s += *reinterpret_cast<const f32x4 *>(c.part + pair * w.dim + col);
+    }
+    if (c.half) {
+        typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
+        *reinterpret_cast<bf16x4 *>((uint16_t *)c.out + (int64_t)r * c.out_stride + col) = __builtin_convertvector(s, bf16x4);
+    } else {
+        *reinterpret_cast<f32x4 *>((float *)c.out + (int64_t)r * c.out_stride + col) = s;
+    }
+}
+
+// ---- what is known of the weights -----------------------------------------------------------
+
+// Of rows [row0, row0 + gridDim.x) of a matrix, dequantized at v: max |w| 2^pow in [2^13, 2^14) and the exponent of the norm.
+__global__ void __launch_bounds__(256)
+row_stats(const float *__restrict__ v, int cols, int64_t row0, int32_t *__restrict__ pow, int32_t *__restrict__ norm) {
+    __shared__ float most[4];
+    __shared__ double squares[4];
+    const int t = (int)threadIdx.x;
+    const float *const row = v + (int64_t)blockIdx.x * cols;
+    float top = 0.f;
+    double sum = 0.;
+    for (int i = t; i < cols; i += 256) {
+        top = fmaxf(top, fabsf(row[i]));
+        sum += (double)row[i] * (double)row[i];
+    }
+#pragma unroll
+    for (int o = 32; o > 0; o /= 2) {
+        top = fmaxf(top, __shfl_xor(top, o));
+        sum += __shfl_xor(sum, o);
+    }
+    if ((t & 63) == 0) most[t >> 6] = top, squares[t >> 6] = sum;
+    __syncthreads();
+    if (t) return;
+    int p = 0, q = kNothing;
+    top = fmaxf(fmaxf(most[0], most[1]), fmaxf(most[2], most[3]));
+    sum = (squares[0] + squares[1]) + (squares[2] + squares[3]);
+    if (top > 0.f && top <= 3.402823466e38f) {
+        (void)frexpf(top, &p);
+        p = 14 - p;
+    }
+    if (sum > 0.) {
+        if (sum < 1e300) {
+            (void)frexp(sum * 1.0001, &q);
+            q = (q + 1) >> 1;
+        } else {  // weights that are not finite: what they reach is not either
+            q = 0;
+        }
+    }
+    pow[row0 + blockIdx.x] = p;
+    if (norm) norm[row0 + blockIdx.x] = q;
+}
+
+// bound[e] = the largest of gate's exponents of expert e + the largest of up's.
+__global__ void __launch_bounds__(256)
+expert_bound(const int32_t *__restrict__ gate, const int32_t *__restrict__ up, int ffn, int32_t *__restrict__ bound) {
+    __shared__ int most[2][4];
+    const int t = (int)threadIdx.x;
+    const int64_t first = (int64_t)blockIdx.x * ffn;
+    int a = 2 * kNothing, b = 2 * kNothing;
+    for (int i = t; i < ffn; i += 256) {
+        a = a > gate[first + i] ? a : gate[first + i];
+        b = b > up[first + i] ? b : up[first + i];
+    }
+#pragma unroll
+    for (int o = 32; o > 0; o /= 2) {
+        const int x = __shfl_xor(a, o), y = __shfl_xor(b, o);
+        a = a > x ? a : x;
+        b = b > y ? b : y;
+    }
+    if ((t & 63) == 0) most[0][t >> 6] = a, most[1][t >> 6] = b;
+    __syncthreads();
+    if (t) return;
+    for (int v = 1; v < 4; v++) {
+        a = a > most[0][v] ? a : most[0][v];
+        b = b > most[1][v] ? b : most[1][v];
+    }
+    bound[blockIdx.x] = a + b;
+}
+
+// ---- handles --------------------------------------------------------------------------------
+
+struct Experts {
+    j4q_experts_config c{};
+    uint32_t gen = 0;
+    bool live = false;
+    Weights w{};
+    uint64_t weight_bytes = 0, bytes = 0;
+    void *dev = nullptr;
+};
+
+std::vector<std::unique_ptr<Experts>> g_experts;
+
+Experts *lookup(j4q_experts h) {
+    const uint64_t lo = h & 0xffffffffu;
+    if (lo == 0 || lo > g_experts.size()) return nullptr;
+    Experts *k = g_experts[lo - 1].get();
+    return k->live && k->gen == (uint32_t)(h >> 32) ? k : nullptr;
+}
+
+int get(j4q_experts h, const char *op, Experts **out) {
+    *out = lookup(h);
+    return *out ? J4Q_OK : report_error(J4Q_EHANDLE, "%s: unknown or destroyed experts 0x%llx", op, (unsigned long long)h);
+}
+
+int no_memory(const char *op) { return report_error(J4Q_ENOMEM, "%s failed: out of host memory", op); }
+
+bool type_ok(int type, int64_t cols) {
+    switch (type) {
+    case Q8_0: return cols % 64 == 0;
+    case Q4_0: return cols % 128 == 0;
+    case Q4_K:
+    case Q6_K: return cols % 256 == 0;
+    default: return false;
+    }
+}
+
+// The powers of a matrix's rows, and with norm the exponents of their norms. scratch: room for `chunk` dequantized rows.
+hipError_t stats(int type, const QMat &m, float *scratch, int64_t chunk, int32_t *pow, int32_t *norm, hipStream_t s) {
+    hipError_t e = hipSuccess;
+    for (int64_t r = 0; r < m.rows && e == hipSuccess; r += chunk) {
+        const int64_t n = m.rows - r < chunk ? m.rows - r : chunk;
+        e = launch_dequant_rows(type, m, r, n, scratch, s);
+        if (e == hipSuccess) {
+            row_stats<<<(unsigned)n, 256, 0, s>>>(scratch, (int)m.cols, r, pow, norm);
+            e = hipGetLastError();
+        }
+    }
+    return e;
+}
+
+int create(const j4q_experts_config &c, j4q_experts *out) {
+    abi::QuantRef gate, up, down;
+    int rc;
+    if ((rc = abi::quant_locked(c.gate, "experts", &gate)) || (rc = abi::quant_locked(c.up, "experts", &up)) || (rc = abi::quant_locked(c.down, "experts", &down)))
+        return rc;
+    const int64_t E = c.experts, dim = gate.cols, ffn = down.cols;
+    if (gate.qtype != up.qtype || gate.rows != up.rows || gate.cols != up.cols)
+        return report_error(J4Q_EINVAL, "experts: gate is type %d [%lld, %lld], up type %d [%lld, %lld]", gate.qtype, (long long)gate.rows, (long long)gate.cols,
+                            up.qtype, (long long)up.rows, (long long)up.cols);
+    if (gate.rows != E * ffn || down.rows != E * dim)
+        return report_error(J4Q_EINVAL, "experts: %lld experts with gate and up [%lld, %lld], down [%lld, %lld]", (long long)E, (long long)gate.rows,
+                            (long long)gate.cols, (long long)down.rows, (long long)down.cols);
+    if (!type_ok(gate.qtype, dim) || !type_ok(down.qtype, ffn) || dim > 65536 || ffn > 65536)
+        return report_error(J4Q_EUNSUPPORTED, "experts: type %d of %lld columns, type %d of %lld (Q8_0, a multiple of 64 columns, Q4_0, of 128, Q4_K, Q6_K; at most 65536)",
+                            gate.qtype, (long long)dim, down.qtype, (long long)ffn);
+    if ((rc = abi::ready_locked())) return rc;
+    if (capturing(abi::stream())) return report_error(J4Q_EINVAL, "experts: the engine stream is captured");
+    size_t slot = 0;
+    while (slot < g_experts.size() && g_experts[slot]->live) slot++;
+    if (slot == g_experts.size()) g_experts.emplace_back(new Experts);
+    Experts &k = *g_experts[slot];
+    const uint64_t words = (uint64_t)(4 * E * ffn + E * dim + E);  // powers of gate, up, down; norms of gate, up; bounds
+    const int64_t wide = dim > ffn ? dim : ffn, chunk = (16 << 20) / wide;
+    void *dev = nullptr;
+    hipError_t e = abi::malloc_locked(&dev, words * 4);
+    if (e != hipSuccess) return report_hip("experts", e);
+    Workspace ws;
+    const hipStream_t s = abi::stream();
+    e = abi::workspace_begin_locked(s, (uint64_t)(chunk * wide) * 4, &ws);
+    if (e == hipSuccess) {
+        int32_t *const at = (int32_t *)dev;
+        k.w = Weights{};
+        k.w.gate = gate.m;
+        k.w.up = up.m;
+        k.w.down = down.m;
+        k.w.up_type = gate.qtype;
+        k.w.down_type = down.qtype;
+        k.w.experts = (int)E;
+        k.w.dim = (int)dim;
+        k.w.ffn = (int)ffn;
+        k.w.act = c.activation;
+        int32_t *const gate_pow = at + E, *const up_pow = gate_pow + E * ffn, *const gate_norm = up_pow + E * ffn, *const up_norm = gate_norm + E * ffn,
+                      *const down_pow = up_norm + E * ffn;
+        k.w.bound = at;
+        k.w.gate_pow = gate_pow;
+        k.w.up_pow = up_pow;
+        k.w.down_pow = down_pow;
+        e = stats(gate.qtype, gate.m, ws.ptr, chunk, gate_pow, gate_norm, s);
+        if (e == hipSuccess) e = stats(up.qtype, up.m, ws.ptr, chunk, up_pow, up_norm, s);
+        if (e == hipSuccess) e = stats(down.qtype, down.m, ws.ptr, chunk, down_pow, nullptr, s);
+        if (e == hipSuccess) {
+            expert_bound<<<(unsigned)E, 256, 0, s>>>(gate_norm, up_norm, (int)ffn, at);
+            e = hipGetLastError();
+        }
+        abi::workspace_end_locked(s, ws, e == hipSuccess);
+        if (e == hipSuccess) e = hipStreamSynchronize(s);
+    }
+    if (e != hipSuccess) {
+        (void)hipFree(dev);
+        return report_hip("experts", e);
+    }
+    k.c = c;
+    k.dev = dev;
+    k.bytes = words * 4;
+    k.weight_bytes = gate.gguf_bytes + up.gguf_bytes + down.gguf_bytes;
+    k.gen++;
+    k.live = true;
+    const j4q_experts h = (uint64_t)k.gen << 32 | (uint64_t)(slot + 1);
+    for (j4q_buffer b : {c.gate, c.up, c.down}) (void)abi::pin_locked(b, h);
+    *out = h;
+    return J4Q_OK;
+}
+
+// The parts of a call's workspace; bytes in all.
+uint64_t lay_out(const Weights &w, Call *c, uint8_t *base) {
+    uint64_t at = 0;
+    auto take = [&](uint64_t n) {
+        uint8_t *const p = base + at;
+        at += align256(n);
+        return p;
+    };
+    const uint64_t planes = c->half ? 1 : 2, P = (uint64_t)c->pairs, T = (uint64_t)c->rows;
+    c->tile_count = (int32_t *)take(4);
+    c->order = (int32_t *)take(4 * P);
+    c->tile = (Tile *)take(sizeof(Tile) * (uint64_t)c->tiles);
+    c->x_pow = (int32_t *)take(4 * T);
+    c->x_norm = (int32_t *)take(4 * T);
+    c->xa = (_Float16 *)take(2 * planes * T * (uint64_t)w.dim);
+    c->ha = (_Float16 *)take(2 * planes * P * (uint64_t)w.ffn);
+    c->part = (float *)take(4 * P * (uint64_t)w.dim);
+    return at;
+}
+
+// Rows of a tile, and how many tiles a call has at most.
+void shape(const Weights &w, Call *c) {
+    c->tile_rows = 16;
+    const int some = w.experts < c->pairs ? w.experts : c->pairs;
+    c->tiles = some + (c->pairs - some) / c->tile_rows;
+}
+
+int check_size(const Weights &, const char *op, int64_t rows, int32_t top, int type) {
+    if (!dense_type(type)) return report_error(J4Q_EUNSUPPORTED, "%s: type %d (J4Q_KIND_F32 or J4Q_KIND_BF16)", op, type);
+    if (rows < 1 || top < 1 || top > kMaxTop) return report_error(J4Q_EINVAL, "%s: %lld rows of %d experts (1 to %d)", op, (long long)rows, top, kMaxTop);
+    if (rows > (1 << 22) / top) return report_error(J4Q_EUNSUPPORTED, "%s: %lld rows of %d experts (at most %d pairs)", op, (long long)rows, top, 1 << 22);
+    return J4Q_OK;
+}
+
+hipError_t launch(const Weights &w, const Call &c, hipEvent_t done, hipStream_t s) {
+    experts_plan<<<(unsigned)(w.experts + c.rows), kPlanThreads, 0, s>>>(w, c);
+    hipError_t e = hipGetLastError();
+    if (e == hipSuccess) e = launch_few(w, c, false, s);
+    if (e == hipSuccess) e = launch_few(w, c, true, s);
+    if (e != hipSuccess) return e;
+    const int y = c.rows < 32768 ? c.rows : 32768;
+    return launch_with_event(experts_combine, dim3((unsigned)((w.dim + 1023) / 1024), (unsigned)y, (unsigned)((c.rows + y - 1) / y)), dim3(256), s, done, w, c);
+}
+
+int apply(const Experts &k, const j4q_experts_args &a, hipStream_t s) {
+    Call c{};
+    c.x = a.x;
+    c.x_stride = a.x_stride ? a.x_stride : k.w.dim;
+    c.ids = a.ids;
+    c.weights = a.weights;
+    c.out = a.out;
+    c.out_stride = a.out_stride ? a.out_stride : k.w.dim;
+    c.rows = (int)a.rows;
+    c.top = a.top_k;
+    c.pairs = c.rows * c.top;
+    c.half = a.type == J4Q_KIND_BF16;
+    const int64_t e = dense_size(a.type), dim = k.w.dim;
+    for (int64_t st : {c.x_stride, c.out_stride})
+        if (st < dim || st > 1ll << 40 || st * e % 16) return report_error(J4Q_EINVAL, "experts apply: rows of %lld values %lld apart, a multiple of 16 bytes", (long long)dim, (long long)st);
+    if (!aligned(a.x, 16) || !aligned(a.out, 16) || !aligned(a.ids, 4) || !aligned(a.weights, 4))
+        return report_error(J4Q_EINVAL, "experts apply: x and out must be 16-byte aligned, ids and weights 4-byte aligned");
+    const uint64_t out_bytes = (uint64_t)(((c.rows - 1) * c.out_stride + dim) * e), x_bytes = (uint64_t)(((c.rows - 1) * c.x_stride + dim) * e);
+    if (overlap(c.x, c.x_stride * e, dim * e, c.out, c.out_stride * e, dim * e, c.rows) || overlap(c.ids, (uint64_t)c.pairs * 4, c.out, out_bytes) ||
+        overlap(c.weights, (uint64_t)c.pairs * 4, c.out, out_bytes))
+        return report_error(J4Q_EUNSUPPORTED, "experts apply: out must lie apart from x, ids and weights");
+    shape(k.w, &c);
+    const uint64_t bytes = lay_out(k.w, &c, nullptr);
+    Workspace ws;
+    if (a.workspace) {
+        if (!aligned(a.workspace, 256) || a.workspace_bytes < bytes)
+            return report_error(J4Q_EINVAL, "experts apply: a workspace of %llu bytes, 256-byte aligned, is needed", (unsigned long long)bytes);
+        if (overlap(a.workspace, bytes, c.x, x_bytes) || overlap(a.workspace, bytes, c.out, out_bytes) || overlap(a.workspace, bytes, c.ids, (uint64_t)c.pairs * 4) ||
+            overlap(a.workspace, bytes, c.weights, (uint64_t)c.pairs * 4))
+            return report_error(J4Q_EUNSUPPORTED, "experts apply: the workspace must lie apart from the other arguments");
+    }
+    int rc;
+    if ((rc = abi::ready_locked())) return rc;
+    if (!s) s = abi::stream();
+    if (a.workspace) {
+        lay_out(k.w, &c, (uint8_t *)a.workspace);
+        const hipError_t err = launch(k.w, c, nullptr, s);
+        return err == hipSuccess ? J4Q_OK : report_hip("experts apply", err);
+    }
+    hipError_t err = abi::workspace_begin_locked(s, bytes, &ws);
+    if (err != hipSuccess) return report_hip("experts apply", err);
+    lay_out(k.w, &c, (uint8_t *)ws.ptr);
+    err = launch(k.w, c, ws.done, s);
+    abi::workspace_end_locked(s, ws, err == hipSuccess);
+    return err == hipSuccess ? J4Q_OK : report_hip("experts apply", err);
+}
+
+}  // namespace
+}  // namespace ex
+}  // namespace j4q
+
+using namespace j4q;
+
+extern "C" {
+
+int j4q_experts_create(const j4q_experts_config *config, j4q_experts *out) try {
+    if (!config || !out) return report_error(J4Q_EINVAL, "experts: NULL argument");
+    if (config->experts < 1 || config->experts > ex::kMaxExperts) return report_error(J4Q_EINVAL, "experts: %d of them (1 to %d)", config->experts, ex::kMaxExperts);
+    if (config->activation < J4Q_ACT_SILU || config->activation > J4Q_ACT_RELU) return report_error(J4Q_EUNSUPPORTED, "experts: unknown activation %d", config->activation);
+    std::lock_guard<std::mutex> lk(abi::lock());
+    return ex::create(*config, out);
+} catch (const std::exception &) {
+    return ex::no_memory("experts");
+}
+
+int j4q_experts_destroy(j4q_experts h) {
+    if (h == 0) return J4Q_OK;
+    std::lock_guard<std::mutex> lk(abi::lock());
+    ex::Experts *k;
+    int rc;
+    if ((rc = ex::get(h, "experts destroy", &k)) || (rc = abi::ready_locked())) return rc;
+    const hipError_t e = hipDeviceSynchronize();
+    if (e != hipSuccess) return report_hip("experts destroy", e);
+    (void)hipFree(k->dev);
+    for (j4q_buffer b : {k->c.gate, k->c.up, k->c.down}) abi::unpin_locked(b);
+    k->dev = nullptr;
+    k->live = false;
+    return J4Q_OK;
+}
+
+int j4q_experts_info(j4q_experts h, j4q_experts_desc *out) {
+    if (!out) return report_error(J4Q_EINVAL, "experts info: NULL argument");
+    std::lock_guard<std::mutex> lk(abi::lock());
+    ex::Experts *k;
+    const int rc = ex::get(h, "experts info", &k);
+    if (rc) return rc;
+    *out = j4q_experts_desc{k->c, k->w.dim, k->w.ffn, k->weight_bytes, k->bytes};
+    return J4Q_OK;
+}
+
+int j4q_experts_workspace(j4q_experts h, int64_t rows, int32_t top_k, int type, uint64_t *bytes) {
+    if (!bytes) return report_error(J4Q_EINVAL, "experts workspace: NULL argument");
+    std::lock_guard<std::mutex> lk(abi::lock());
+    ex::Experts *k;
+    int rc;
+    if ((rc = ex::get(h, "experts workspace", &k)) || (rc = ex::check_size(k->w, "experts workspace", rows, top_k, type))) return rc;
+    ex::Call c{};
+    c.rows = (int)rows;
+    c.top = top_k;
+    c.pairs = c.rows * c.top;
+    c.half = type == J4Q_KIND_BF16;
+    ex::shape(k->w, &c);
+    *bytes = ex::lay_out(k->w, &c, nullptr);
+    return J4Q_OK;
+}
+
+int j4q_experts_apply(j4q_experts h, const j4q_experts_args *args, void *stream) {
+    if (!args || !args->x || !args->ids || !args->weights || !args->out) return report_error(J4Q_EINVAL, "experts apply: NULL argument");
+    std::lock_guard<std::mutex> lk(abi::lock());
+    ex::Experts *k;
+    int rc;
+    if ((rc = ex::get(h, "experts apply", &k)) || (rc = ex::check_size(k->w, "experts apply", args->rows, args->top_k, args->type))) return rc;
+    return ex::apply(*k, *args, (hipStream_t)stream);
+}
+
+}  // extern "C"

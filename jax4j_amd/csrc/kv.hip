@@ -14,6 +14,7 @@
 #include <memory>
 #include <vector>
 
+#include "arguments.h"
 #include "engine.h"
 #include "kept_memory.h"
 #include "kv.h"
@@ -125,8 +126,6 @@ int get(j4q_kv h, const char *op, Kv **out, bool lost_too = false) {
 
 // What an entry point answers where host memory ran out in it.
 int no_memory(const char *op) { return report_error(J4Q_ENOMEM, "%s failed: out of host memory", op); }
-
-bool aligned(const void *p, uintptr_t a) { return ((uintptr_t)p & (a - 1)) == 0; }
 
 // One call's launches on its stream, behind the cache's last call. That one's last launch has completed k.done, but on the engine
 // stream, which outlives the cache: there calls follow one another, and the event is recorded only when a call leaves it (a launch
@@ -312,8 +311,6 @@ int fill_rope(const char *op, const j4q_rope *r, int32_t head_dim, int64_t rows,
     return J4Q_OK;
 }
 
-bool dense_type(int t) { return t == J4Q_KIND_F32 || t == J4Q_KIND_BF16; }
-
 // Row strides in elements (0: rows lie one behind the other), rows of 16-byte pieces.
 int check_stride(const char *op, const char *what, const void *p, int type, int64_t width, int64_t *stride) {
     const int64_t e = type == J4Q_KIND_BF16 ? 2 : 4;
@@ -321,15 +318,6 @@ int check_stride(const char *op, const char *what, const void *p, int type, int6
     if (!aligned(p, 16) || *stride < width || *stride * e % 16 != 0 || *stride > (1ll << 40))
         return report_error(J4Q_EINVAL, "%s: %s must be 16-byte aligned, its rows %lld values or more apart, a multiple of 16 bytes", op, what, (long long)width);
     return J4Q_OK;
-}
-
-// Whether two tensors of rows `width` bytes wide share a byte.
-bool overlap(const void *a, int64_t a_stride, int64_t a_width, const void *b, int64_t b_stride, int64_t b_width, int64_t rows) {
-    const uintptr_t a0 = (uintptr_t)a, b0 = (uintptr_t)b;
-    if (a0 >= b0 + (rows - 1) * b_stride + b_width || b0 >= a0 + (rows - 1) * a_stride + a_width) return false;
-    if (a_stride != b_stride) return true;
-    const int64_t between = (int64_t)(b0 - a0) % a_stride, at = between < 0 ? between + a_stride : between;  // windows of the same rows
-    return at < a_width || at + b_width > a_stride;
 }
 
 // Tiles of 64 tokens that the workgroups of a call's sequences walk for one kv head: all of them, the longest walk's, and how many

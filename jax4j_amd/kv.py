@@ -22,15 +22,8 @@ from operator import index
 import numpy as np
 
 from . import _native as N
-from .backend import Mi355xBackend, _addresses, _int32, _int64, check
+from .backend import Mi355xBackend, _addresses, _int32, _int64, _kind, check
 from .tensor import DType, IllegalArgumentException
-
-def _kind(dtype: DType) -> int:
-    if dtype is DType.F32:
-        return N.KIND_F32
-    if dtype is DType.BF16:
-        return N.KIND_BF16
-    raise IllegalArgumentException(f"values are F32 or BF16, not {dtype}")
 
 
 def _ints(values, code="i") -> array:
