@@ -103,7 +103,9 @@ __device__ __forceinline__ QMat expert_of(const QMat &m, int fmt, int e, int64_t
     return o;
 }
 
+// The products of every tile: of up to 16 pairs, or of 32, 64 (and 128, bf16).
 hipError_t launch_few(const Weights &w, const Call &c, bool down, hipStream_t s);
+hipError_t launch_many(const Weights &w, const Call &c, bool down, hipStream_t s);
 
 }  // namespace ex
 }  // namespace j4q

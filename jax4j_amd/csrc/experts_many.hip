@@ -1,0 +1,393 @@
+// Products of tiles of up to 32 TM pairs with an expert's rows, weights as fp16 (experts.h).
+//
+// A workgroup of 4 waves has one tile of pairs; wave v has two groups of 32 rows of W, the same rows of gate and up or 64 rows of down,
+// for all pairs: 2 TM v_mfma_f32_32x32x16_f16 accumulators. Each x' operand read from LDS feeds two MFMAs, and the activation needs no
+// exchange. W is the first operand, so a lane holds 4 consecutive columns of the result for one pair. Two workgroups share a CU.
+//
+// K advances in stages of two 32-blocks. Lane (r, h) = (lane % 32, lane / 32) has block h of the stage: of row r of W, which it
+// dequantizes, and of pair r's x'. MFMA p = 0..3 takes dword p of the codes and chunk p of the block layout. x' goes from
+// global memory into one of two stage buffers (rows of 128 bytes, 16-byte chunk c of row r at slot c ^ ((r / 2) % 8)), W into units of
+// two stages as in gemm_tile.h, whose WUnit and order of waits this is: X of stage i + 1 is issued behind the barrier of stage i,
+// the unit after the next one at odd stages, and operands of MFMA p + 1 are dequantized under those of p.
+//
+// A weight is fp16(fma(code, s 2^pow, o 2^pow)), rounded once, with the row's power 2^pow that brings its largest magnitude into
+// [2^13, 2^14) and leaves again in the epilogue: 11 bits down to 2^-27 of that. The code is an fp16 subnormal (a field masked out), so
+// one v_fma_mix per weight does it. HL (fp32 x): hi + lo of both operands and three products, 22 bits.
+#include <type_traits>
+
+#include "experts.h"
+#include "gemm_tile.h"
+
+namespace j4q {
+namespace ex {
+namespace {
+
+using gw::dma16;
+using gw::lds_barrier;
+using gw::load_order;
+using gw::wait_vm_lgkm0;
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef int32_t i32x4 __attribute__((ext_vector_type(4)));
+
+template <int FMT>
+using Unit = gt::WUnit<FMT, 8>;  // 4 waves of two groups of rows
+
+// fp16(fma(c, s, o)) of two codes, and with HL what that leaves.
+template <bool HL>
+__device__ __forceinline__ void dequantize(uint32_t c, float s, float o, uint32_t &hi, uint32_t &lo) {
+    const h2 v = __builtin_bit_cast(h2, c);
+    const float a = __builtin_fmaf((float)v.x, s, o), b = __builtin_fmaf((float)v.y, s, o);
+    const h2 h = {(_Float16)a, (_Float16)b};
+    hi = __builtin_bit_cast(uint32_t, h);
+    if constexpr (HL) {
+        const h2 l = {(_Float16)(a - (float)h.x), (_Float16)(b - (float)h.y)};
+        lo = __builtin_bit_cast(uint32_t, l);
+    }
+}
+
+template <bool HL>
+struct Operand {
+    h8 hi, lo;
+};
+template <>
+struct Operand<false> {
+    h8 hi;
+};
+
+// One block of a row of W as it lies in LDS; scales s and offsets o of its elements 0..15 and 16..31.
+template <int FMT>
+struct Block {
+    u32x4 q[FMT == Q8_0 ? 2 : 1];
+    u32x2 hi;
+    u32x4 s;
+};
+struct Scale {
+    float s[2], o[2];
+};
+
+// LDS of a workgroup with TM groups of 32 pairs.
+template <int FMT, bool HL, int TM>
+struct Lds {
+    static constexpr int kPlane = 32 * TM * 128, kX = (HL ? 2 : 1) * kPlane;
+};
+
+// The tile's rows of x' as byte offsets from `base`, and where its results go.
+template <int FMT, bool HL, int TM, bool DOWN>
+__device__ __forceinline__ void run(const Weights &w, const Call &c, const Tile &tile, int chunk, uint8_t *xs0, uint8_t *xs1, uint8_t *ws0, uint8_t *ws1) {
+    using U = Unit<FMT>;
+    using L = Lds<FMT, HL, TM>;
+    constexpr int WL = 2 * U::kLoads, XL = (HL ? 2 : 1) * TM, QR = U::QR;
+    const int expert = tile.expert, count = tile.count, first = tile.first;
+    const int lane = (int)threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+    const int r32 = lane & 31, h = lane >> 5;
+    const int K = DOWN ? w.ffn : w.dim, N = DOWN ? w.dim : w.ffn, ns = K / 64, nsb = K / 256;
+    // first row of W of each group
+    const int n0 = DOWN ? 256 * chunk + 64 * wave : 128 * chunk + 32 * wave, n1 = DOWN ? n0 + 32 : n0;
+    U unit[2];
+    if constexpr (DOWN) {
+        const QMat m = expert_of(w.down, FMT, expert, N);
+        unit[0].init(m, n0, 2 * wave, lane);
+        unit[1].init(m, n1, 2 * wave + 1, lane);
+    } else {
+        unit[0].init(expert_of(w.gate, FMT, expert, N), n0, 2 * wave, lane);
+        unit[1].init(expert_of(w.up, FMT, expert, N), n1, 2 * wave + 1, lane);
+    }
+    const int32_t *const pow0 = (DOWN ? w.down_pow : w.gate_pow) + (int64_t)expert * N, *const pow1 = (DOWN ? w.down_pow : w.up_pow) + (int64_t)expert * N;
+    float power[2];
+    power[0] = n0 + r32 < N ? __builtin_ldexpf(1.f, pow0[n0 + r32]) : 1.f;
+    power[1] = n1 + r32 < N ? __builtin_ldexpf(1.f, pow1[n1 + r32]) : 1.f;
+
+    // X load j of this wave fills rows 8 (4 j + wave) .. + 7; lane L slot L % 8 of row 8 (4 j + wave) + L / 8.
+    const _Float16 *const base = DOWN ? c.ha + (int64_t)first * K : c.xa;
+    const uint64_t plane = DOWN ? (uint64_t)c.pairs * (uint64_t)K * 2u : (uint64_t)c.rows * (uint64_t)K * 2u;
+    const uint64_t held = DOWN ? (uint64_t)count * (uint64_t)K * 2u : plane;
+    const __amdgpu_buffer_rsrc_t xr = make_rsrc(base, held), xl = make_rsrc(HL ? (const uint8_t *)base + plane : (const uint8_t *)base, HL ? held : 0);
+    uint32_t xoff[TM];
+#pragma unroll
+    for (int j = 0; j < TM; j++) {
+        const int row = 8 * (4 * j + wave) + (lane >> 3), chunk16 = (lane & 7) ^ ((row >> 1) & 7);
+        uint32_t at = kOob;
+        if (row < count) at = (uint32_t)(DOWN ? row : c.order[first + row] / c.top) * (uint32_t)K * 2u + (uint32_t)chunk16 * 16u;
+        xoff[j] = at;
+    }
+    auto load_x = [&](int i, uint8_t *xb) __attribute__((always_inline)) {
+        const uint32_t so = i < ns ? (uint32_t)i * 128u : 0u;
+#pragma unroll
+        for (int j = 0; j < TM; j++) {
+            dma16(xr, xb + (4 * j + wave) * 1024, i < ns ? xoff[j] : kOob, so);
+            if constexpr (HL) dma16(xl, xb + L::kPlane + (4 * j + wave) * 1024, i < ns ? xoff[j] : kOob, so);
+        }
+    };
+    auto load_w = [&](int u, uint8_t *wb) __attribute__((always_inline)) {
+        unit[0].load(u, 2 * u < ns, wb);
+        unit[1].load(u, 2 * u < ns, wb);
+    };
+
+    auto read_block = [&](int j, int group, const uint8_t *wb, Block<FMT> &o) __attribute__((always_inline)) {
+        const int swz = U::swz(r32), blk = 2 * (j & 1) + h, unit_row = 32 * (2 * wave + group) + r32;
+        const uint8_t *const row = wb + unit_row * QR, *const slot = wb + U::kS + (2 * wave + group) * U::kSlot;
+#pragma unroll
+        for (int k = 0; k < U::QL / 2; k++) o.q[k] = *reinterpret_cast<const u32x4 *>(row + (((U::QL / 2 * blk + k) ^ swz) << 4));
+        if constexpr (FMT == Q4_K) o.s = *reinterpret_cast<const u32x4 *>(slot + r32 * 16);
+        else o.s[0] = *reinterpret_cast<const uint16_t *>(slot + r32 * 8 + blk * 2);
+        if constexpr (FMT == Q6_K) {
+            o.hi = *reinterpret_cast<const u32x2 *>(wb + U::kH + unit_row * 32 + blk * 8);
+            o.s[1] = *reinterpret_cast<const uint32_t *>(slot + 256 + r32 * 4);
+        }
+    };
+    auto decode_scale = [&](int j, int group, const Block<FMT> &b) __attribute__((always_inline)) -> Scale {
+        constexpr float k24 = gt::kTwo24, k20 = gt::kTwo20;
+        const float pw = power[group];
+        Scale c;
+        if constexpr (FMT == Q8_0) {
+            const float d = half_bits_to_float(b.s[0]) * pw;
+            c.s[0] = c.s[1] = d * k24;
+            c.o[0] = c.o[1] = -128.f * d;
+        } else if constexpr (FMT == Q4_0) {
+            const float d = half_bits_to_float(b.s[0]) * pw;
+            c.s[0] = d * k24;
+            c.s[1] = d * k20;
+            c.o[0] = c.o[1] = -8.f * d;
+        } else if constexpr (FMT == Q4_K) {
+            const int jsb = 2 * (j & 3) + h;
+            const uint32_t sc = __builtin_amdgcn_ubfe(b.s[1], 4 * jsb, 4) | (__builtin_amdgcn_ubfe(b.s[3], 2 * jsb, 2) << 4);
+            const uint32_t mn = __builtin_amdgcn_ubfe(b.s[2], 4 * jsb, 4) | (__builtin_amdgcn_ubfe(b.s[3], 16 + 2 * jsb, 2) << 4);
+            const float d = half_bits_to_float(b.s[0] & 0xFFFFu) * pw * (float)sc;
+            c.s[0] = d * k24;
+            c.s[1] = d * k20;
+            c.o[0] = c.o[1] = -(half_bits_to_float(b.s[0] >> 16) * pw * (float)mn);
+        } else {
+            const int n = (group ? n1 : n0) + r32;
+            const uint32_t odd = ((uint32_t)n * (uint32_t)nsb + (uint32_t)(j >> 2)) & 1u;  // an expert's rows are a multiple of 64
+            const float d = half_bits_to_float(odd ? b.s[1] >> 16 : b.s[1] & 0xFFFFu) * pw;
+            const float da = d * (float)(int8_t)(b.s[0] & 0xFFu), db = d * (float)(int8_t)(b.s[0] >> 8);
+            c.s[0] = da * k24;
+            c.o[0] = -32.f * da;
+            c.s[1] = db * k20;
+            c.o[1] = -32.f * db;
+        }
+        return c;
+    };
+    // Operand p of a block.
+    auto operand = [&](const Block<FMT> &b, const Scale &c, int p, Operand<HL> &out) __attribute__((always_inline)) {
+        uint32_t part[4];
+        if constexpr (FMT == Q8_0) {
+            const uint32_t u = b.q[0][p] ^ 0x80808080u, v = b.q[1][p] ^ 0x80808080u;
+            part[0] = u & 0x00FF00FFu;
+            part[1] = u >> 8 & 0x00FF00FFu;
+            part[2] = v & 0x00FF00FFu;
+            part[3] = v >> 8 & 0x00FF00FFu;
+        } else {
+            const uint32_t v = b.q[0][p], t = v >> 8;
+            part[0] = v & 0x000F000Fu;
+            part[1] = t & 0x000F000Fu;
+            part[2] = v & 0x00F000F0u;
+            part[3] = t & 0x00F000F0u;
+            if constexpr (FMT == Q6_K) {
+                const uint32_t raw = b.hi[p >> 1], hw = p & 1 ? __builtin_amdgcn_alignbit(raw, raw, 8) : raw, u = hw >> 2;
+                part[0] |= hw & 0x00300030u;
+                part[1] |= u & 0x00300030u;
+                part[2] |= hw & 0x03000300u;
+                part[3] |= u & 0x03000300u;
+            }
+        }
+        u32x4 hi, lo;
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+            uint32_t x = 0, y = 0;
+            dequantize<HL>(part[k], c.s[k >> 1], c.o[k >> 1], x, y);
+            hi[k] = x;
+            lo[k] = y;
+        }
+        out.hi = __builtin_bit_cast(h8, hi);
+        if constexpr (HL) out.lo = __builtin_bit_cast(h8, lo);
+    };
+
+    f32x16 acc[2][TM];
+#pragma unroll
+    for (int t = 0; t < TM; t++) acc[0][t] = acc[1][t] = f32x16{};
+    const int xrow = r32 * 128, xsw = (r32 >> 1) & 7;
+    auto read_x = [&](const uint8_t *xb, int p, Operand<HL> (&a)[TM]) __attribute__((always_inline)) {
+#pragma unroll
+        for (int t = 0; t < TM; t++) {
+            const uint8_t *const at = xb + t * 32 * 128 + xrow + (((4 * h + p) ^ xsw) << 4);
+            a[t].hi = *reinterpret_cast<const h8 *>(at);
+            if constexpr (HL) a[t].lo = *reinterpret_cast<const h8 *>(at + L::kPlane);
+        }
+    };
+    Block<FMT> blk[2][2];  // [stage parity][group]
+    Scale sc[2][2];
+    Operand<HL> b[2][2];   // of MFMA p and p + 1
+    auto stage = [&](auto S_, int i) __attribute__((always_inline)) {
+        constexpr int S = decltype(S_)::value, cur = S & 1;
+        uint8_t *const xb = cur ? xs1 : xs0, *const xn = cur ? xs0 : xs1;
+        constexpr int ur = (S + 1) / 2 % 2, un = (S + 3) / 2 % 2;
+        uint8_t *const wc = ur ? ws1 : ws0, *const wn = un ? ws1 : ws0;
+        wait_vm_lgkm0<S % 2 == 0 ? WL : 0>();
+        lds_barrier();
+        Operand<HL> a[2][TM];
+        read_x(xb, 0, a[0]);
+        read_block(i + 1, 0, wc, blk[cur ^ 1][0]);
+        read_block(i + 1, 1, wc, blk[cur ^ 1][1]);
+        load_x(i + 1, xn);
+        load_order();  // X first: the wait at an even stage leaves the newest unit of W outstanding
+        if constexpr (S % 2 == 1) load_w((i + 3) / 2, wn);
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int p = 0; p < 4; p++) {
+            if (p < 3) read_x(xb, p + 1, a[(p + 1) & 1]);
+            if (p == 1) {
+                sc[cur ^ 1][0] = decode_scale(i + 1, 0, blk[cur ^ 1][0]);
+                sc[cur ^ 1][1] = decode_scale(i + 1, 1, blk[cur ^ 1][1]);
+            }
+#pragma unroll
+            for (int g = 0; g < 2; g++) {
+#pragma unroll
+                for (int t = 0; t < TM; t++) {
+                    if constexpr (HL) {
+                        acc[g][t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(b[p & 1][g].lo, a[p & 1][t].hi, acc[g][t], 0, 0, 0);
+                        acc[g][t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(b[p & 1][g].hi, a[p & 1][t].lo, acc[g][t], 0, 0, 0);
+                    }
+                    acc[g][t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(b[p & 1][g].hi, a[p & 1][t].hi, acc[g][t], 0, 0, 0);
+                }
+                if (p < 3) operand(blk[cur][g], sc[cur][g], p + 1, b[(p + 1) & 1][g]);
+                else operand(blk[cur ^ 1][g], sc[cur ^ 1][g], 0, b[0][g]);
+            }
+        }
+        // computed here, between the MFMAs, although the last stage does not use it
+        asm volatile("" : "+v"(b[0][0].hi), "+v"(b[0][1].hi));
+    };
+
+    load_w(0, ws0);
+    load_order();
+    load_x(0, xs0);
+    load_order();
+    load_w(1, ws1);
+    wait_vm_lgkm0<XL + WL>();
+    asm volatile("" ::: "memory");
+#pragma unroll
+    for (int g = 0; g < 2; g++) {
+        read_block(0, g, ws0, blk[0][g]);
+        sc[0][g] = decode_scale(0, g, blk[0][g]);
+        operand(blk[0][g], sc[0][g], 0, b[0][g]);
+    }
+#define J4Q_STAGE(S) stage(std::integral_constant<int, S>{}, i + S);
+    int i = 0;
+    for (; i + 4 <= ns; i += 4) {
+        J4Q_STAGE(0) J4Q_STAGE(1) J4Q_STAGE(2) J4Q_STAGE(3)
+    }
+    if constexpr (FMT == Q8_0 || FMT == Q4_0) {
+        if (i < ns) {
+            J4Q_STAGE(0)
+            if (i + 1 < ns) {
+                J4Q_STAGE(1)
+                if (i + 2 < ns) J4Q_STAGE(2)
+            }
+        }
+    }
+#undef J4Q_STAGE
+    __builtin_amdgcn_s_waitcnt(0);  // no LDS load outlives the workgroup
+
+    // Element v of acc[g][t]: row n + 8 (v / 4) + 4 h + v % 4 of the group, pair 32 t + r32.
+    i32x4 p0[4], p1[4];
+#pragma unroll
+    for (int q = 0; q < 4; q++) {
+        const int a = n0 + 8 * q + 4 * h, e = n1 + 8 * q + 4 * h;
+        p0[q] = a < N ? *reinterpret_cast<const i32x4 *>(pow0 + a) : i32x4{};
+        p1[q] = e < N ? *reinterpret_cast<const i32x4 *>(pow1 + e) : i32x4{};
+    }
+#pragma unroll
+    for (int t = 0; t < TM; t++) {
+        const int m = 32 * t + r32;
+        if (m >= count) continue;
+        const int pair = c.order[first + m], token = pair / c.top, hp = h_pow(w, expert, c.x_norm[token]);
+        if constexpr (DOWN) {
+            const float weight = c.weights[pair];
+            float *const out = c.part + (int64_t)pair * N;
+#pragma unroll
+            for (int g = 0; g < 2; g++)
+#pragma unroll
+                for (int q = 0; q < 4; q++) {
+                    const int n = (g ? n1 : n0) + 8 * q + 4 * h;
+                    f32x4 v;
+#pragma unroll
+                    for (int j = 0; j < 4; j++) v[j] = __builtin_ldexpf(acc[g][t][4 * q + j] * weight, -hp - (g ? p1[q][j] : p0[q][j]));
+                    if (n < N) *reinterpret_cast<f32x4 *>(out + n) = v;
+                }
+        } else {
+            const int e = -c.x_pow[token];
+            if (n0 >= N) continue;
+            _Float16 *const out = c.ha + (int64_t)(first + m) * N + n0;
+            const int64_t lo = (int64_t)c.pairs * N;
+#pragma unroll
+            for (int k = 0; k < 2; k++) {  // chunk 2 k + h of the block: elements of q = k, then of q = 2 + k
+                h8 hi, rest;
+#pragma unroll
+                for (int s = 0; s < 8; s++) {
+                    const int q = k + 2 * (s >> 2), j = (s & 1) << 1 | (s >> 1 & 1);
+                    const float gv = __builtin_ldexpf(acc[0][t][4 * q + j], e - p0[q][j]), uv = __builtin_ldexpf(acc[1][t][4 * q + j], e - p1[q][j]);
+                    const float v = __builtin_ldexpf(activate(gv, w.act) * uv, hp);
+                    hi[s] = (_Float16)v;
+                    rest[s] = (_Float16)(v - (float)hi[s]);
+                }
+                *reinterpret_cast<h8 *>(out + 8 * (2 * k + h)) = hi;
+                if constexpr (HL) *reinterpret_cast<h8 *>(out + lo + 8 * (2 * k + h)) = rest;
+            }
+        }
+    }
+}
+
+// grid: tiles * chunks, rounded up to whole eighths; a chunk is 128 columns of the result (down: 256).
+template <int FMT, bool HL, int TM, bool DOWN>
+__global__ void __launch_bounds__(256, 2)
+experts_many(Weights w, Call c) {
+    constexpr int kX = Lds<FMT, HL, TM>::kX, kW = Unit<FMT>::kBytes;
+    static_assert(2 * (kX + kW) <= 163840, "LDS");
+    __shared__ __attribute__((aligned(1024))) uint8_t xs0[kX], xs1[kX];
+    __shared__ __attribute__((aligned(1024))) uint8_t ws0[kW], ws1[kW];
+    const int N = DOWN ? w.dim : w.ffn, chunks = DOWN ? (N + 255) / 256 : (N + 127) / 128, tiles = c.tile_count[0];
+    // Workgroup b runs on XCD b % 8, and each XCD takes a contiguous range, down groups of 4 tiles of pairs: most often of one
+    // expert, whose rows of W they share in the XCD's L2.
+    const int total = tiles * chunks, per = (total + 7) / 8, at = (int)(blockIdx.x % 8) * per + (int)(blockIdx.x / 8);
+    if ((int)(blockIdx.x / 8) >= per || at >= total) return;
+    const int mg = at / (4 * chunks), gm = tiles - 4 * mg < 4 ? tiles - 4 * mg : 4, rem = at - 4 * mg * chunks;
+    Tile tile = c.tile[4 * mg + rem % gm];
+    tile.expert = __builtin_amdgcn_readfirstlane(tile.expert);
+    tile.first = __builtin_amdgcn_readfirstlane(tile.first);
+    tile.count = __builtin_amdgcn_readfirstlane(tile.count);
+    run<FMT, HL, TM, DOWN>(w, c, tile, rem / gm, xs0, xs1, ws0, ws1);
+}
+
+template <int FMT, bool DOWN>
+hipError_t launch_type(const Weights &w, const Call &c, hipStream_t s) {
+    const int N = DOWN ? w.dim : w.ffn, chunks = DOWN ? (N + 255) / 256 : (N + 127) / 128;
+    const int64_t total = ((int64_t)c.tiles * chunks + 7) / 8 * 8;
+    if (total > 0xffffff) return hipErrorInvalidValue;
+    const dim3 grid((unsigned)total);
+    if (c.half) {
+        if (c.tile_rows == 128) experts_many<FMT, false, 4, DOWN><<<grid, 256, 0, s>>>(w, c);
+        else if (c.tile_rows == 64) experts_many<FMT, false, 2, DOWN><<<grid, 256, 0, s>>>(w, c);
+        else if (c.tile_rows == 32) experts_many<FMT, false, 1, DOWN><<<grid, 256, 0, s>>>(w, c);
+        else return hipErrorInvalidValue;
+    } else {
+        if (c.tile_rows == 64) experts_many<FMT, true, 2, DOWN><<<grid, 256, 0, s>>>(w, c);
+        else if (c.tile_rows == 32) experts_many<FMT, true, 1, DOWN><<<grid, 256, 0, s>>>(w, c);
+        else return hipErrorInvalidValue;
+    }
+    return hipGetLastError();
+}
+
+}  // namespace
+
+hipError_t launch_many(const Weights &w, const Call &c, bool down, hipStream_t s) {
+    switch (down ? w.down_type : w.up_type) {
+    case Q8_0: return down ? launch_type<Q8_0, true>(w, c, s) : launch_type<Q8_0, false>(w, c, s);
+    case Q4_0: return down ? launch_type<Q4_0, true>(w, c, s) : launch_type<Q4_0, false>(w, c, s);
+    case Q4_K: return down ? launch_type<Q4_K, true>(w, c, s) : launch_type<Q4_K, false>(w, c, s);
+    case Q6_K: return down ? launch_type<Q6_K, true>(w, c, s) : launch_type<Q6_K, false>(w, c, s);
+    default: return hipErrorInvalidValue;
+    }
+}
+
+}  // namespace ex
+}  // namespace j4q
