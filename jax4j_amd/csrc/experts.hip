@@ -399,7 +399,7 @@ uint64_t lay_out(const Weights &w, Call *c, uint8_t *base) {
 // Rows of a tile, and how many tiles a call has at most.
 void shape(const Weights &w, Call *c) {
     const int each = c->pairs / w.experts;
-    c->tile_rows = each < 24 ? 16 : each < 40 ? 32 : each < 96 || !c->half ? 64 : 128;
+    c->tile_rows = each < 24 ? (c->half ? 16 : 8) : each < 40 ? 32 : each < 96 || !c->half ? 64 : 128;
     const int some = w.experts < c->pairs ? w.experts : c->pairs;
     c->tiles = some + (c->pairs - some) / c->tile_rows;
 }
@@ -414,7 +414,7 @@ int check_size(const Weights &, const char *op, int64_t rows, int32_t top, int t
 hipError_t launch(const Weights &w, const Call &c, hipEvent_t done, hipStream_t s) {
     experts_plan<<<(unsigned)(w.experts + c.rows), kPlanThreads, 0, s>>>(w, c);
     hipError_t e = hipGetLastError();
-    const auto products = c.tile_rows == 16 ? launch_few : launch_many;
+    const auto products = c.tile_rows <= 16 ? launch_few : launch_many;
     if (e == hipSuccess) e = products(w, c, false, s);
     if (e == hipSuccess) e = products(w, c, true, s);
     if (e != hipSuccess) return e;
