@@ -24,9 +24,14 @@ struct Raw {
 };
 
 // The 8 codes of a dword (and Q6_K's high bits, or Q8_0's dword of the block's second half) as fp16 whole numbers.
+// `one`: 1024 and 1024, below which the bits are whole numbers, in a register (or_one()): a mask and that are one v_and_or then.
+__device__ __forceinline__ uint32_t or_one() {
+    uint32_t one = 0x64006400u;
+    asm("" : "+v"(one));
+    return one;
+}
 template <int FMT>
-__device__ __forceinline__ h8 codes(uint32_t v, uint32_t more) {
-    constexpr uint32_t one = 0x64006400u;  // 1024: the bits below are whole numbers
+__device__ __forceinline__ h8 codes(uint32_t v, uint32_t more, uint32_t one) {
     u32x4 r;
     if constexpr (FMT == Q8_0) {
         const uint32_t a = v ^ 0x80808080u, b = more ^ 0x80808080u;
@@ -41,10 +46,11 @@ __device__ __forceinline__ h8 codes(uint32_t v, uint32_t more) {
         uint32_t e0 = (v & 0x000F000Fu) | one, e1 = (t & 0x000F000Fu) | one, f0 = (v & 0x00F000F0u) | one, f1 = (t & 0x00F000F0u) | one;
         if constexpr (FMT == Q6_K) {
             const uint32_t u = more >> 2;
-            e0 |= more & 0x00300030u;
-            e1 |= u & 0x00300030u;
-            f0 |= more & 0x03000300u;
-            f1 |= u & 0x03000300u;
+            asm("" : "+v"(e0), "+v"(e1), "+v"(f0), "+v"(f1));  // a second v_and_or each, not two masks and an or of three
+            e0 = (more & 0x00300030u) | e0;
+            e1 = (u & 0x00300030u) | e1;
+            f0 = (more & 0x03000300u) | f0;
+            f1 = (u & 0x03000300u) | f1;
         }
         const h2 low = both(-1024.f - o), sixteenth = both(0.0625f), high = both(-64.f - o);
         r[0] = bits(as_h2(e0) + low);
@@ -73,13 +79,13 @@ __device__ __forceinline__ float block_sum(const Operands<Q4_K> &a, int g) {
     return g < 2 ? (g ? s[1] : s[0]) : (g == 2 ? s[2] : s[3]);
 }
 
-// acc += x' . W tile over half i of a slice; lane (n, g): rows 4 g + j of the operand, row n of W.
+// acc - low += x' . W tile over half i of a slice (low: Q4_K's minima); lane (n, g): rows 4 g + j of the operand, row n of W.
 template <int FMT>
-__device__ __forceinline__ void multiply(const Raw<FMT> &r, const Operands<FMT> &a, int i, int g, f32x4 &acc) {
+__device__ __forceinline__ void multiply(const Raw<FMT> &r, const Operands<FMT> &a, int i, int g, uint32_t one, f32x4 &acc, f32x4 &low) {
     if constexpr (FMT == Q8_0) {
 #pragma unroll
         for (int t = 0; t < 2; t++) {
-            const f32x4 c = __builtin_amdgcn_mfma_f32_16x16x32_f16(a.x[t], codes<FMT>(r.v[2 * t], r.v[2 * t + 1]), f32x4{}, 0, 0, 0);
+            const f32x4 c = __builtin_amdgcn_mfma_f32_16x16x32_f16(a.x[t], codes<FMT>(r.v[2 * t], r.v[2 * t + 1], one), f32x4{}, 0, 0, 0);
             const float d = (float)as_h2(r.s[i])[t];
 #pragma unroll
             for (int j = 0; j < 4; j++) acc[j] = __builtin_fmaf(d, c[j], acc[j]);
@@ -87,7 +93,7 @@ __device__ __forceinline__ void multiply(const Raw<FMT> &r, const Operands<FMT> 
         return;
     }
     float scale[4];
-    f32x4 low = {};
+    f32x4 part;  // Q6_K: before the superblock's scale
     if constexpr (FMT == Q4_K) {
         // lane group g decodes block 4 i + g
         const int sj = 4 * i + g;
@@ -99,26 +105,37 @@ __device__ __forceinline__ void multiply(const Raw<FMT> &r, const Operands<FMT> 
 #pragma unroll
         for (int t = 0; t < 4; t++) scale[t] = (float)as_h2(r.s[2 * i + t / 2])[t & 1];
     }
+    // the products first: a fold waits for its own
+    f32x4 c[4], c1[4];
 #pragma unroll
     for (int t = 0; t < 4; t++) {
         if constexpr (FMT == Q6_K) {
-            const h8 w = codes<FMT>(r.v[t], r.h[t]);
-            const f32x4 c0 = __builtin_amdgcn_mfma_f32_16x16x16f16(__builtin_shufflevector(a.x[t], a.x[t], 0, 1, 2, 3),
-                                                                   __builtin_shufflevector(w, w, 0, 1, 2, 3), f32x4{}, 0, 0, 0);
-            const f32x4 c1 = __builtin_amdgcn_mfma_f32_16x16x16f16(__builtin_shufflevector(a.x[t], a.x[t], 4, 5, 6, 7),
-                                                                   __builtin_shufflevector(w, w, 4, 5, 6, 7), f32x4{}, 0, 0, 0);
-            const float d = half_bits_to_float(r.d);
-            const uint32_t sw = r.s[2 * i + t / 2] >> (16 * (t & 1));
-            const float s0 = d * (float)(int8_t)(sw & 0xFFu), s1 = d * (float)(int8_t)(sw >> 8 & 0xFFu);
-#pragma unroll
-            for (int j = 0; j < 4; j++) acc[j] = __builtin_fmaf(s1, c1[j], __builtin_fmaf(s0, c0[j], acc[j]));
+            const h8 w = codes<FMT>(r.v[t], r.h[t], one);
+            c[t] = __builtin_amdgcn_mfma_f32_16x16x16f16(__builtin_shufflevector(a.x[t], a.x[t], 0, 1, 2, 3), __builtin_shufflevector(w, w, 0, 1, 2, 3),
+                                                         f32x4{}, 0, 0, 0);
+            c1[t] = __builtin_amdgcn_mfma_f32_16x16x16f16(__builtin_shufflevector(a.x[t], a.x[t], 4, 5, 6, 7), __builtin_shufflevector(w, w, 4, 5, 6, 7),
+                                                          f32x4{}, 0, 0, 0);
         } else {
-            const f32x4 c = __builtin_amdgcn_mfma_f32_16x16x32_f16(a.x[t], codes<FMT>(r.v[t], 0u), f32x4{}, 0, 0, 0);
-#pragma unroll
-            for (int j = 0; j < 4; j++) acc[j] = __builtin_fmaf(scale[t], c[j], acc[j]);
+            c[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a.x[t], codes<FMT>(r.v[t], 0u, one), f32x4{}, 0, 0, 0);
         }
     }
-    if constexpr (FMT == Q4_K) acc -= low;
+#pragma unroll
+    for (int t = 0; t < 4; t++) {
+        if constexpr (FMT == Q6_K) {
+            const uint32_t sw = r.s[2 * i + t / 2] >> (16 * (t & 1));
+            const float s0 = (float)(int8_t)(sw & 0xFFu), s1 = (float)(int8_t)(sw >> 8 & 0xFFu);
+#pragma unroll
+            for (int j = 0; j < 4; j++) part[j] = __builtin_fmaf(s1, c1[t][j], t ? __builtin_fmaf(s0, c[t][j], part[j]) : s0 * c[t][j]);
+        } else {
+#pragma unroll
+            for (int j = 0; j < 4; j++) acc[j] = __builtin_fmaf(scale[t], c[t][j], acc[j]);
+        }
+    }
+    if constexpr (FMT == Q6_K) {
+        const float d = half_bits_to_float(r.d);
+#pragma unroll
+        for (int j = 0; j < 4; j++) acc[j] = __builtin_fmaf(d, part[j], acc[j]);
+    }
 }
 
 }  // namespace ex

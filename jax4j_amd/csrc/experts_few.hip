@@ -116,7 +116,8 @@ experts_few(Weights w, Call c) {
         dma16(xr, buf + R::kX + 1024 * wave, live && (int)(u * (R::kCols / 8) + xchunk) < K / 8 ? xoff : kOob, u * (R::kCols * 2u));
     };
 
-    f32x4 acc = {};
+    f32x4 acc = {}, low = {};
+    const uint32_t one = or_one();
     auto stage = [&](int i, const uint8_t *buf, uint8_t *next) __attribute__((always_inline)) {
         wait_vm_lgkm0<(D - 2) * R::kLoads>();
         lds_barrier();
@@ -146,7 +147,7 @@ experts_few(Weights w, Call c) {
                     r.h[b] = __builtin_amdgcn_alignbit(v, v, (uint32_t)(g & 1) * 8u);
                 }
             }
-            multiply<FMT>(r, a, half, g, acc);
+            multiply<FMT>(r, a, half, g, one, acc, low);
         }
     };
     load(0, b0);
@@ -167,7 +168,7 @@ experts_few(Weights w, Call c) {
     float *const red = reinterpret_cast<float *>(b0);
     static_assert(R::kBytes >= kWaves * 1024, "results in a buffer");
 #pragma unroll
-    for (int j = 0; j < 4; j++) red[wave * 256 + (4 * g + j) * 16 + n] = acc[j];
+    for (int j = 0; j < 4; j++) red[wave * 256 + (4 * g + j) * 16 + n] = acc[j] - low[j];
     __syncthreads();
     auto value = [&](int tile16, int o) __attribute__((always_inline)) -> float {
         const float *const v = red + tile16 * 256 + o;
