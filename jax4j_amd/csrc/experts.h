@@ -59,12 +59,13 @@ struct Call {
     bool half;      // bf16 x and out; x' and h' have no lo part
     int tile_rows;  // pairs of a tile
     int tiles;      // of the grid: no call has more
+    int splits;     // of down's K, whose partial results are added too
     // workspace
     int32_t *order, *tile_count;
     Tile *tile;
     _Float16 *xa, *ha;         // hi; lo behind all of hi
     int32_t *x_pow, *x_norm;   // of each row: e, and an exponent with |x| <= 2^it
-    float *part;               // [pairs][dim]
+    float *part;               // [splits][pairs][dim]
 };
 
 __device__ __forceinline__ int h_pow(const Weights &w, int expert, int x_norm) { return kBound - (2 * x_norm + w.bound[expert]); }
@@ -103,7 +104,8 @@ __device__ __forceinline__ QMat expert_of(const QMat &m, int fmt, int e, int64_t
     return o;
 }
 
-// The products of every tile: of up to 16 pairs, or of 32, 64 (and 128, bf16).
+// The products of every tile: of up to 16 pairs (fp32: 8), or of 32, 64 (and 128, bf16).
+int splits_few(const Weights &w, int tiles);
 hipError_t launch_few(const Weights &w, const Call &c, bool down, hipStream_t s);
 hipError_t launch_many(const Weights &w, const Call &c, bool down, hipStream_t s);
 

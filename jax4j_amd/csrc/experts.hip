@@ -163,7 +163,7 @@ experts_plan(Weights w, Call c) {
 
 // ---- the sums -------------------------------------------------------------------------------
 
-// out[r] = sum over its slots, one after another, of the weighted partial results. A thread per 4 columns.
+// out[r] = sum over its slots, and each one's splits, one after another, of the weighted partial results. A thread per 4 columns.
 __global__ void __launch_bounds__(256)
 experts_combine(Weights w, Call c) {
     const int r = (int)(blockIdx.z * gridDim.y + blockIdx.y), col = 4 * (int)(blockIdx.x * 256 + threadIdx.x);
@@ -173,7 +173,7 @@ experts_combine(Weights w, Call c) {
         const int64_t pair = (int64_t)r * c.top + k;
         const int id = c.ids[pair];
         if (id < 0 || id >= w.experts) continue;
-        s += *reinterpret_cast<const f32x4 *>(c.part + pair * w.dim + col);
+        for (int v = 0; v < c.splits; v++) s += *reinterpret_cast<const f32x4 *>(c.part + ((int64_t)v * c.pairs + pair) * w.dim + col);
     }
     if (c.half) {
         typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
@@ -392,7 +392,7 @@ uint64_t lay_out(const Weights &w, Call *c, uint8_t *base) {
     c->x_norm = (int32_t *)take(4 * T);
     c->xa = (_Float16 *)take(2 * planes * T * (uint64_t)w.dim);
     c->ha = (_Float16 *)take(2 * planes * P * (uint64_t)w.ffn);
-    c->part = (float *)take(4 * P * (uint64_t)w.dim);
+    c->part = (float *)take(4 * (uint64_t)c->splits * P * (uint64_t)w.dim);
     return at;
 }
 
@@ -402,6 +402,7 @@ void shape(const Weights &w, Call *c) {
     c->tile_rows = each < 24 ? (c->half ? 16 : 8) : each < 40 ? 32 : each < 96 || !c->half ? 64 : 128;
     const int some = w.experts < c->pairs ? w.experts : c->pairs;
     c->tiles = some + (c->pairs - some) / c->tile_rows;
+    c->splits = c->tile_rows <= 16 ? splits_few(w, c->tiles) : 1;
 }
 
 int check_size(const Weights &, const char *op, int64_t rows, int32_t top, int type) {

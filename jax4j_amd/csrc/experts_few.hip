@@ -8,8 +8,9 @@
 // A workgroup of 8 waves has one tile of pairs; wave v has 16 rows of W over all of K: of gate (v < 4) or up, of the same 64 columns
 // of the result, or of down's 128. K advances in stages of 256 columns (Q8_0: 128) through a ring of D buffers: at stage i a wave
 // waits for its own loads of stage i, meets the others, issues stage i + D - 1 into the buffer of stage i - 1, and multiplies.
-// Two workgroups share a CU. 16-byte chunks lie swizzled: chunk c of row r of W at c ^ ((r / 2) % 8), of x' at c ^ r, so that the 16 rows
-// of an operand read fall on distinct banks.
+// Two workgroups share a CU. 16-byte chunks lie swizzled: chunk c of row r of W at c ^ ((r / 2) % 4), of x' at c ^ r, so that the rows
+// of an operand read fall on distinct banks (of W, two on each: with three bits of the row the places of 8 blocks in 3 buffers would not
+// fit the registers).
 #include <type_traits>
 
 #include "experts_codes.h"
@@ -19,6 +20,7 @@ namespace j4q {
 namespace ex {
 namespace {
 
+using gmf::lane_off;  // (a select, no branch)
 using gw::dma16;
 using gw::dma4s;
 using gw::lds_barrier;
@@ -51,7 +53,7 @@ struct Stream {
         sr = make_rsrc(m.sc, rows * (k / 16));
 #pragma unroll
         for (int j = 0; j < 2; j++) {
-            const int r = 8 * j + (lane >> 3), c = (lane & 7) ^ ((r >> 1) & 7);
+            const int r = 8 * j + (lane >> 3), c = (lane & 7) ^ ((r >> 1) & 3);
             qoff[j] = ok ? (uint32_t)(row0 + r) * qrow + (uint32_t)c * 16u : kOob;
         }
         const uint32_t r = (uint32_t)(row0 + (lane >> 2)), part = (uint32_t)lane & 3u;
@@ -59,23 +61,24 @@ struct Stream {
         if constexpr (FMT == Q6_K) {
             hr = make_rsrc(m.qh, rows * (k / 4));
             dr = make_rsrc(m.d, rows * (k / 128));
-            hoff = ok ? r * (uint32_t)(K / 4) + ((part ^ (r >> 1 & 3u)) * 16u) : kOob;
+            hoff = ok ? r * (uint32_t)(K / 4) + ((part ^ (r >> 1 & 1u)) * 16u) : kOob;
             doff = ok && lane < 16 ? (uint32_t)(row0 + lane) * (uint32_t)(K / 128) : kOob;
         }
     }
-    __device__ __forceinline__ void load(int i, bool live, uint8_t *at, int lane) const {
+    // In two parts, each with the other half of the stage before it.
+    __device__ __forceinline__ void load(int part, int i, bool live, uint8_t *at, int lane) const {
         const uint32_t u = live ? (uint32_t)i : 0u;
-#pragma unroll
-        for (int j = 0; j < 2; j++) dma16(qr, at + 1024 * j, live ? qoff[j] : kOob, u * 128u);
-        if constexpr (FMT == Q6_K) dma16(hr, at + R::kHigh, live ? hoff : kOob, u * 64u);
+        dma16(qr, at + 1024 * part, lane_off(qoff[part], live), u * 128u);
+        if (part == 0) return;
+        if constexpr (FMT == Q6_K) dma16(hr, at + R::kHigh, lane_off(hoff, live), u * 64u);
         // a dword of two blocks' scales (Q8_0, Q4_0) behind the row's last block: nothing
-        const bool in = FMT == Q4_K || FMT == Q6_K || (int)(u * R::kBlocks) + 2 * (lane & 3) < K / 32;
-        dma4s(sr, at + R::kScale, live && in ? soff : kOob, u * (R::kBlocks * 2u));
-        if constexpr (FMT == Q6_K) dma4s(dr, at + R::kD, live && doff != kOob ? (doff + 2u * u) & ~3u : kOob, 0u);
+        const bool in = (FMT == Q4_K) | (FMT == Q6_K) | ((int)(u * R::kBlocks) + 2 * (lane & 3) < K / 32);
+        dma4s(sr, at + R::kScale, lane_off(soff, live & in), u * (R::kBlocks * 2u));
+        if constexpr (FMT == Q6_K) dma4s(dr, at + R::kD, lane_off((doff + 2u * u) & ~3u, live & (doff != kOob)), 0u);
     }
 };
 
-// grid: (ceil(N / 64) or down ceil(N / 128), tiles over y and z).
+// grid: (ceil(N / 64) or down ceil(N / 128) * splits, tiles over y and z).
 template <int FMT, bool HL, bool DOWN>
 __global__ void __launch_bounds__(kWaves * 64, 4)
 experts_few(Weights w, Call c) {
@@ -91,8 +94,11 @@ experts_few(Weights w, Call c) {
               first = __builtin_amdgcn_readfirstlane(tile.first);
     const int lane = (int)threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
     const int n = lane & 15, g = lane >> 4;
-    const int K = DOWN ? w.ffn : w.dim, N = DOWN ? w.dim : w.ffn, ns = (K + R::kCols - 1) / R::kCols;
-    const int row0 = DOWN ? 128 * (int)blockIdx.x + 16 * wave : 64 * (int)blockIdx.x + 16 * (wave & 3);
+    const int K = DOWN ? w.ffn : w.dim, N = DOWN ? w.dim : w.ffn, all = (K + R::kCols - 1) / R::kCols;
+    // down: K in c.splits ranges of whole stages
+    const int chunks = DOWN ? (N + 127) / 128 : (int)gridDim.x, split = DOWN ? (int)blockIdx.x / chunks : 0, chunk = (int)blockIdx.x - split * chunks;
+    const int each = DOWN ? (all + c.splits - 1) / c.splits : all, from = split * each, ns = all < from + each ? all : from + each;
+    const int row0 = DOWN ? 128 * chunk + 16 * wave : 64 * chunk + 16 * (wave & 3);
     Stream<FMT> s;
     s.init(expert_of(DOWN ? w.down : wave < 4 ? w.gate : w.up, FMT, expert, N), row0, lane, row0 < N);
 
@@ -109,51 +115,66 @@ experts_few(Weights w, Call c) {
             xoff = (uint32_t)at_row * 2u + xchunk * 16u;
         }
     }
-    auto load = [&](int i, uint8_t *buf) __attribute__((always_inline)) {
+    auto load = [&](int part, int i, uint8_t *buf) __attribute__((always_inline)) {
         const bool live = i < ns;
         const uint32_t u = live ? (uint32_t)i : 0u;
-        s.load(i, live, buf + wave * R::kWave, lane);
-        dma16(xr, buf + R::kX + 1024 * wave, live && (int)(u * (R::kCols / 8) + xchunk) < K / 8 ? xoff : kOob, u * (R::kCols * 2u));
+        s.load(part, i, live, buf + wave * R::kWave, lane);
+        if (part == 0) dma16(xr, buf + R::kX + 1024 * wave, lane_off(xoff, live & ((int)(u * (R::kCols / 8) + xchunk) < K / 8)), u * (R::kCols * 2u));
     };
 
     f32x4 acc = {}, low = {};
     const uint32_t one = or_one();
+    // Places in a buffer of what this lane reads of four blocks; the next four lie 64 (W) and 256 bytes (x') behind.
+    uint32_t xat[4], wat[4];
+#pragma unroll
+    for (int k = 0; k < 4; k++) {
+        xat[k] = (uint32_t)(R::kX + n * (R::kCols * 2) + (((4 * k + g) ^ n) << 4));
+        wat[k] = (uint32_t)(wave * R::kWave + n * 128 + ((k ^ (n >> 1 & 3)) << 4) + 4 * g);
+    }
+    uint32_t hat[2];
+#pragma unroll
+    for (int k = 0; k < 2; k++) hat[k] = (uint32_t)(wave * R::kWave + R::kHigh + n * 64 + ((k ^ (n >> 1 & 1)) << 4) + 4 * (g >> 1));
+    const uint32_t sat = (uint32_t)(wave * R::kWave + R::kScale + n * 16);
     auto stage = [&](int i, const uint8_t *buf, uint8_t *next) __attribute__((always_inline)) {
         wait_vm_lgkm0<(D - 2) * R::kLoads>();
         lds_barrier();
-        load(i + D - 1, next);
-        __builtin_amdgcn_sched_barrier(0);
-        const uint8_t *const wb = buf + wave * R::kWave, *const xb = buf + R::kX + n * (R::kCols * 2);
-        const int wsw = (n >> 1) & 7;
         Raw<FMT> r;
-        r.s = *reinterpret_cast<const u32x4 *>(wb + R::kScale + n * 16);
+        r.s = *reinterpret_cast<const u32x4 *>(buf + sat);
         if constexpr (FMT == Q6_K) {
-            const uint32_t d = *reinterpret_cast<const uint32_t *>(wb + R::kD + n * 4);
+            const uint32_t d = *reinterpret_cast<const uint32_t *>(buf + wave * R::kWave + R::kD + n * 4);
             r.d = ((row0 + n) * (K / 256) + i) & 1 ? d >> 16 : d & 0xFFFFu;
         }
-#pragma unroll
-        for (int half = 0; half < 2; half++) {
-            constexpr int B = R::kBlocks / 2;
+        auto part = [&](auto half_) __attribute__((always_inline)) {
+            constexpr int half = decltype(half_)::value, B = R::kBlocks / 2;
             Operands<FMT> a;
 #pragma unroll
-            for (int b = 0; b < B; b++) a.x[b] = *reinterpret_cast<const h8 *>(xb + (((4 * (B * half + b) + g) ^ n) << 4));
+            for (int k = 0; k < B; k++) a.x[k] = *reinterpret_cast<const h8 *>(buf + xat[(B * half + k) & 3] + 256 * ((B * half + k) >> 2));
 #pragma unroll
-            for (int b = 0; b < 4; b++) r.v[b] = *reinterpret_cast<const uint32_t *>(wb + n * 128 + (((4 * half + b) ^ wsw) << 4) + 4 * g);
+            for (int k = 0; k < 4; k++) r.v[k] = *reinterpret_cast<const uint32_t *>(buf + wat[k] + 64 * half);
             if constexpr (FMT == Q6_K) {
 #pragma unroll
-                for (int b = 0; b < 4; b++) {
-                    const int at16 = (2 * half + (b >> 1)) ^ (n >> 1 & 3);
-                    const uint32_t v = *reinterpret_cast<const uint32_t *>(wb + R::kHigh + n * 64 + (at16 << 4) + 8 * (b & 1) + 4 * (g >> 1));
-                    r.h[b] = __builtin_amdgcn_alignbit(v, v, (uint32_t)(g & 1) * 8u);
+                for (int k = 0; k < 4; k += 2) {
+                    const uint8_t *const at = buf + hat[k / 2] + 32 * half;
+                    const uint32_t u = *reinterpret_cast<const uint32_t *>(at), v = *reinterpret_cast<const uint32_t *>(at + 8);
+                    r.h[k] = __builtin_amdgcn_alignbit(u, u, (uint32_t)(g & 1) * 8u);
+                    r.h[k + 1] = __builtin_amdgcn_alignbit(v, v, (uint32_t)(g & 1) * 8u);
                 }
             }
+            __builtin_amdgcn_sched_barrier(0);
+            load(half, i + D - 1, next);
+            __builtin_amdgcn_sched_barrier(0);
             multiply<FMT>(r, a, half, g, one, acc, low);
-        }
+            __builtin_amdgcn_sched_barrier(0);
+        };
+        part(std::integral_constant<int, 0>{});
+        part(std::integral_constant<int, 1>{});
     };
-    load(0, b0);
-    __builtin_amdgcn_sched_barrier(0);
-    if constexpr (D == 3) load(1, b1);
-    for (int i = 0; i < ns; i += D) {
+#pragma unroll
+    for (int k = 0; k < 2 * (D - 1); k++) {
+        load(k & 1, from + (k >> 1), k < 2 ? b0 : b1);
+        __builtin_amdgcn_sched_barrier(0);
+    }
+    for (int i = from; i < ns; i += D) {
         if constexpr (D == 3) {
             stage(i, b0, b2);
             stage(i + 1, b1, b0);  // behind the last stage: zeros
@@ -176,11 +197,11 @@ experts_few(Weights w, Call c) {
     };
     constexpr int kOut = HL ? 128 : 256, COLS = DOWN ? kWaves : kWaves / 2;
     for (int o = (int)threadIdx.x; o < COLS * kOut; o += kWaves * 64) {
-        const int ct = o / kOut, i = o % kOut, q = i >> 4, col = 16 * (COLS * (int)blockIdx.x + ct) + (i & 15);
+        const int ct = o / kOut, i = o % kOut, q = i >> 4, col = 16 * (COLS * chunk + ct) + (i & 15);
         if (q >= count || col >= N) continue;
         const int pair = c.order[first + q], token = pair / c.top, pow = h_pow(w, expert, c.x_norm[token]);
         if constexpr (DOWN) {
-            c.part[(int64_t)pair * N + col] = __builtin_ldexpf(value(ct, i) * c.weights[pair], -pow);  // the weight first: the product alone may not fit
+            c.part[((int64_t)split * c.pairs + pair) * N + col] = __builtin_ldexpf(value(ct, i) * c.weights[pair], -pow);  // the weight first: the product alone may not fit
         } else {
             const int e = -c.x_pow[token];
             const float h = __builtin_ldexpf(activate(__builtin_ldexpf(value(ct, i), e), w.act) * __builtin_ldexpf(value(4 + ct, i), e), pow);
@@ -196,7 +217,7 @@ template <int FMT, bool HL, bool DOWN>
 hipError_t launch(const Weights &w, const Call &c, hipStream_t s) {
     const int N = DOWN ? w.dim : w.ffn, cols = DOWN ? 128 : 64;
     const int y = c.tiles < 32768 ? c.tiles : 32768;
-    const dim3 grid((unsigned)((N + cols - 1) / cols), (unsigned)y, (unsigned)((c.tiles + y - 1) / y));
+    const dim3 grid((unsigned)((N + cols - 1) / cols * (DOWN ? c.splits : 1)), (unsigned)y, (unsigned)((c.tiles + y - 1) / y));
     experts_few<FMT, HL, DOWN><<<grid, kWaves * 64, 0, s>>>(w, c);
     return hipGetLastError();
 }
@@ -208,6 +229,13 @@ hipError_t launch_type(const Weights &w, const Call &c, bool down, hipStream_t s
 }
 
 }  // namespace
+
+// Three workgroups for each CU of an MI355X (a constant, so that results do not depend on the device), of at least 1024 columns (5
+// tokens through 2 of 8 experts, Q6_K 4096 x 14336: 104 us without).
+int splits_few(const Weights &w, int tiles) {
+    const int64_t groups = (int64_t)tiles * ((w.dim + 127) / 128), want = (768 + groups - 1) / groups, most = w.ffn / 1024;
+    return (int)(want < most ? want : most > 1 ? most : 1);
+}
 
 hipError_t launch_few(const Weights &w, const Call &c, bool down, hipStream_t s) {
     switch (down ? w.down_type : w.up_type) {
