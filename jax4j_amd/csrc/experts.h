@@ -57,6 +57,7 @@ struct Call {
     int64_t out_stride;
     int rows, top, pairs;
     bool half;      // bf16 x and out; x' and h' have no lo part
+    bool one;       // a single row on its own kernels
     int tile_rows;  // pairs of a tile
     int tiles;      // of the grid: no call has more
     int splits;     // of down's K, whose partial results are added too
@@ -108,6 +109,9 @@ __device__ __forceinline__ QMat expert_of(const QMat &m, int fmt, int e, int64_t
 int splits_few(const Weights &w, int tiles);
 hipError_t launch_few(const Weights &w, const Call &c, bool down, hipStream_t s);
 hipError_t launch_many(const Weights &w, const Call &c, bool down, hipStream_t s);
+// All of a call of one row, whose c.part is [top][ffn]; `done` as launch_with_event takes it.
+bool one_fits(const Weights &w, int top);
+hipError_t launch_one(const Weights &w, const Call &c, hipEvent_t done, hipStream_t s);
 
 }  // namespace ex
 }  // namespace j4q

@@ -384,6 +384,10 @@ uint64_t lay_out(const Weights &w, Call *c, uint8_t *base) {
         at += align256(n);
         return p;
     };
+    if (c->one) {
+        c->part = (float *)take(4 * (uint64_t)c->pairs * (uint64_t)w.ffn);
+        return at;
+    }
     const uint64_t planes = c->half ? 1 : 2, P = (uint64_t)c->pairs, T = (uint64_t)c->rows;
     c->tile_count = (int32_t *)take(4);
     c->order = (int32_t *)take(4 * P);
@@ -398,6 +402,7 @@ uint64_t lay_out(const Weights &w, Call *c, uint8_t *base) {
 
 // Rows of a tile, and how many tiles a call has at most.
 void shape(const Weights &w, Call *c) {
+    c->one = c->rows == 1 && one_fits(w, c->top);
     const int each = c->pairs / w.experts;
     c->tile_rows = each < 24 ? (c->half ? 16 : 8) : each < 40 ? 32 : each < 96 || !c->half ? 64 : 128;
     const int some = w.experts < c->pairs ? w.experts : c->pairs;
@@ -413,6 +418,7 @@ int check_size(const Weights &, const char *op, int64_t rows, int32_t top, int t
 }
 
 hipError_t launch(const Weights &w, const Call &c, hipEvent_t done, hipStream_t s) {
+    if (c.one) return launch_one(w, c, done, s);
     experts_plan<<<(unsigned)(w.experts + c.rows), kPlanThreads, 0, s>>>(w, c);
     hipError_t e = hipGetLastError();
     const auto products = c.tile_rows <= 16 ? launch_few : launch_many;
