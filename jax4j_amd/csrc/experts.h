@@ -40,6 +40,14 @@ struct Tile {
     int32_t expert, first, count, pad;
 };
 
+// The tiles of gate|up's launch, or of down's.
+struct Tiles {
+    int rows;  // pairs of a tile
+    int most;  // of the grid: no call has more
+    int32_t *count;
+    Tile *tile;
+};
+
 struct Weights {
     QMat gate, up, down;
     int up_type, down_type;
@@ -58,12 +66,11 @@ struct Call {
     int rows, top, pairs;
     bool half;      // bf16 x and out; x' and h' have no lo part
     bool one;       // a single row on its own kernels
-    int tile_rows;  // pairs of a tile
-    int tiles;      // of the grid: no call has more
+    bool few;       // tiles of up to 16 pairs
     int splits;     // of down's K, whose partial results are added too
+    Tiles up, down;
     // workspace
-    int32_t *order, *tile_count;
-    Tile *tile;
+    int32_t *order;
     _Float16 *xa, *ha;         // hi; lo behind all of hi
     int32_t *x_pow, *x_norm;   // of each row: e, and an exponent with |x| <= 2^it
     float *part;               // [splits][pairs][dim]
@@ -105,7 +112,8 @@ __device__ __forceinline__ QMat expert_of(const QMat &m, int fmt, int e, int64_t
     return o;
 }
 
-// The products of every tile: of up to 16 pairs (fp32: 8), or of 32, 64 (and 128, bf16).
+// The products of every tile: of up to 16 pairs (fp32: 8), or of rows_many(), by the type of the matrix.
+int rows_many(int type, bool half, int each);
 int splits_few(const Weights &w, int tiles);
 hipError_t launch_few(const Weights &w, const Call &c, bool down, hipStream_t s);
 hipError_t launch_many(const Weights &w, const Call &c, bool down, hipStream_t s);

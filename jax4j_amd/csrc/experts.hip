@@ -27,49 +27,98 @@ __device__ __forceinline__ int wave_total(int v) {
 
 // Workgroup e < experts: the pairs of expert e in rising order, behind those of the experts before it, and their tiles. Every
 // workgroup counts all ids itself, so that none waits for another; each of its waves then places the matches of a contiguous part.
+// Bound by the latency of its loads: four ids a lane and load, four loads on their way (32744 pairs of 64 experts one by one 38 us).
 __device__ void order_pairs(const Weights &w, const Call &c, int e) {
+    constexpr int kWaves = kPlanThreads / 64, kStep = 1024;  // ids of a wave and step
     __shared__ int hist[kMaxExperts];
-    __shared__ int wave_count[kPlanThreads / 64], sums[2][kPlanThreads / 64];
+    __shared__ int wave_count[kWaves], sums[3][kWaves];
     const int t = (int)threadIdx.x, lane = t & 63, wave = t >> 6;
     for (int i = t; i < w.experts; i += kPlanThreads) hist[i] = 0;
     __syncthreads();
-    const int part = (c.pairs + kPlanThreads - 1) / kPlanThreads * 64, from = wave * part, to = from + part < c.pairs ? from + part : c.pairs;
+    const int part = (c.pairs + kWaves * kStep - 1) / (kWaves * kStep) * kStep, from = wave * part, to = from + part < c.pairs ? from + part : c.pairs;
+    typedef int32_t i32x4 __attribute__((ext_vector_type(4), aligned(4)));
+    // ids i + 256 u + 4 lane .. + 3, u = 0 .. 3; those behind the part's end are no expert's
+    auto load = [&](int i, int (&id)[4][4]) __attribute__((always_inline)) {
+#pragma unroll
+        for (int u = 0; u < 4; u++) {
+            const int at = i + 256 * u + 4 * lane;
+            if (at + 3 < to) {
+                const i32x4 v = *reinterpret_cast<const i32x4 *>(c.ids + at);
+#pragma unroll
+                for (int j = 0; j < 4; j++) id[u][j] = v[j];
+            } else {
+#pragma unroll
+                for (int j = 0; j < 4; j++) id[u][j] = at + j < to ? c.ids[at + j] : -1;
+            }
+        }
+    };
     int mine = 0;
-    for (int i = from + lane; i < to; i += 64) {
-        const int id = c.ids[i];
-        if (id >= 0 && id < w.experts) atomicAdd(&hist[id], 1);
-        mine += id == e;
+    for (int i = from; i < to; i += kStep) {
+        int id[4][4];
+        load(i, id);
+#pragma unroll
+        for (int u = 0; u < 4; u++)
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                const int v = id[u][j];
+                if (v >= 0 && v < w.experts) atomicAdd(&hist[v], 1);
+                mine += v == e;
+            }
     }
     mine = wave_total(mine);
     if (lane == 0) wave_count[wave] = mine;
     __syncthreads();
-    int before = 0, tiles = 0;  // of the experts before this one
+    int before = 0, up = 0, down = 0;  // pairs and tiles of the experts before this one
     for (int i = t; i < e; i += kPlanThreads) {
         before += hist[i];
-        tiles += (hist[i] + c.tile_rows - 1) / c.tile_rows;
+        up += (hist[i] + c.up.rows - 1) / c.up.rows;
+        down += (hist[i] + c.down.rows - 1) / c.down.rows;
     }
     before = wave_total(before);
-    tiles = wave_total(tiles);
-    if (lane == 0) sums[0][wave] = before, sums[1][wave] = tiles;
+    up = wave_total(up);
+    down = wave_total(down);
+    if (lane == 0) sums[0][wave] = before, sums[1][wave] = up, sums[2][wave] = down;
     __syncthreads();
-    before = tiles = 0;
+    before = up = down = 0;
 #pragma unroll
-    for (int v = 0; v < kPlanThreads / 64; v++) before += sums[0][v], tiles += sums[1][v];
-    const int count = hist[e], own = (count + c.tile_rows - 1) / c.tile_rows;
-    for (int i = t; i < own; i += kPlanThreads) {
-        const int left = count - i * c.tile_rows;
-        c.tile[tiles + i] = Tile{e, before + i * c.tile_rows, left < c.tile_rows ? left : c.tile_rows, 0};
-    }
-    if (e == w.experts - 1 && t == 0) c.tile_count[0] = tiles + own;
+    for (int v = 0; v < kWaves; v++) before += sums[0][v], up += sums[1][v], down += sums[2][v];
+    const int count = hist[e];
+    auto tiles = [&](const Tiles &all, int first) {
+        const int own = (count + all.rows - 1) / all.rows;
+        for (int i = t; i < own; i += kPlanThreads) {
+            const int left = count - i * all.rows;
+            all.tile[first + i] = Tile{e, before + i * all.rows, left < all.rows ? left : all.rows, 0};
+        }
+        if (e == w.experts - 1 && t == 0) all.count[0] = first + own;
+    };
+    tiles(c.up, up);
+    tiles(c.down, down);
     if (!count) return;
     int at = before;
     for (int v = 0; v < wave; v++) at += wave_count[v];
-    for (int i0 = from; i0 < to; i0 += 64) {
-        const int i = i0 + lane;
-        const bool is = i < to && c.ids[i] == e;
-        const uint64_t all = __ballot(is);
-        if (is) c.order[at + __popcll(all & ((1ull << lane) - 1))] = i;
-        at += __popcll(all);
+    if (!wave_count[wave]) return;
+    for (int i = from; i < to; i += kStep) {
+        int id[4][4];
+        load(i, id);
+#pragma unroll
+        for (int u = 0; u < 4; u++) {
+            // matches of the lanes before this one, and of this one's before each of its own
+            int own = 0;
+#pragma unroll
+            for (int j = 0; j < 4; j++) own += id[u][j] == e;
+            int ahead = 0, total = 0;
+#pragma unroll
+            for (int b = 0; b < 3; b++) {  // own is 0 .. 4
+                const uint64_t set = __ballot(own >> b & 1);
+                ahead += __popcll(set & ((1ull << lane) - 1)) << b;
+                total += __popcll(set) << b;
+            }
+            int place = at + ahead;
+#pragma unroll
+            for (int j = 0; j < 4; j++)
+                if (id[u][j] == e) c.order[place++] = i + 256 * u + 4 * lane + j;
+            at += total;
+        }
     }
 }
 
@@ -389,9 +438,11 @@ uint64_t lay_out(const Weights &w, Call *c, uint8_t *base) {
         return at;
     }
     const uint64_t planes = c->half ? 1 : 2, P = (uint64_t)c->pairs, T = (uint64_t)c->rows;
-    c->tile_count = (int32_t *)take(4);
+    c->up.count = (int32_t *)take(8);
+    c->down.count = c->up.count + 1;
     c->order = (int32_t *)take(4 * P);
-    c->tile = (Tile *)take(sizeof(Tile) * (uint64_t)c->tiles);
+    c->up.tile = (Tile *)take(sizeof(Tile) * (uint64_t)c->up.most);
+    c->down.tile = (Tile *)take(sizeof(Tile) * (uint64_t)c->down.most);
     c->x_pow = (int32_t *)take(4 * T);
     c->x_norm = (int32_t *)take(4 * T);
     c->xa = (_Float16 *)take(2 * planes * T * (uint64_t)w.dim);
@@ -403,11 +454,12 @@ uint64_t lay_out(const Weights &w, Call *c, uint8_t *base) {
 // Rows of a tile, and how many tiles a call has at most.
 void shape(const Weights &w, Call *c) {
     c->one = c->rows == 1 && one_fits(w, c->top);
-    const int each = c->pairs / w.experts;
-    c->tile_rows = each < 24 ? (c->half ? 16 : 8) : each < 40 ? 32 : each < 96 || !c->half ? 64 : 128;
-    const int some = w.experts < c->pairs ? w.experts : c->pairs;
-    c->tiles = some + (c->pairs - some) / c->tile_rows;
-    c->splits = c->tile_rows <= 16 ? splits_few(w, c->tiles) : 1;
+    const int each = c->pairs / w.experts, some = w.experts < c->pairs ? w.experts : c->pairs, few = c->half ? 16 : 8;
+    c->few = each < 24;
+    c->up.rows = c->few ? few : rows_many(w.up_type, c->half, each);
+    c->down.rows = c->few ? few : rows_many(w.down_type, c->half, each);
+    for (Tiles *t : {&c->up, &c->down}) t->most = some + (c->pairs - some) / t->rows;
+    c->splits = c->few ? splits_few(w, c->down.most) : 1;
 }
 
 int check_size(const Weights &, const char *op, int64_t rows, int32_t top, int type) {
@@ -421,7 +473,7 @@ hipError_t launch(const Weights &w, const Call &c, hipEvent_t done, hipStream_t 
     if (c.one) return launch_one(w, c, done, s);
     experts_plan<<<(unsigned)(w.experts + c.rows), kPlanThreads, 0, s>>>(w, c);
     hipError_t e = hipGetLastError();
-    const auto products = c.tile_rows <= 16 ? launch_few : launch_many;
+    const auto products = c.few ? launch_few : launch_many;
     if (e == hipSuccess) e = products(w, c, false, s);
     if (e == hipSuccess) e = products(w, c, true, s);
     if (e != hipSuccess) return e;

@@ -87,9 +87,10 @@ experts_few(Weights w, Call c) {
     static_assert(2 * D * R::kBytes <= 163840, "two workgroups' LDS");
     __shared__ __attribute__((aligned(1024))) uint8_t b0[R::kBytes], b1[R::kBytes], b2[D == 3 ? R::kBytes : 16];
     const int at = (int)(blockIdx.z * gridDim.y + blockIdx.y);
-    if (at >= c.tiles) return;
-    const Tile tile = c.tile[at];  // (with the count, not behind it)
-    if (at >= c.tile_count[0]) return;
+    const Tiles &tiles = DOWN ? c.down : c.up;
+    if (at >= tiles.most) return;
+    const Tile tile = tiles.tile[at];  // (with the count, not behind it)
+    if (at >= tiles.count[0]) return;
     const int expert = __builtin_amdgcn_readfirstlane(tile.expert), count = __builtin_amdgcn_readfirstlane(tile.count),
               first = __builtin_amdgcn_readfirstlane(tile.first);
     const int lane = (int)threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
@@ -216,8 +217,8 @@ experts_few(Weights w, Call c) {
 template <int FMT, bool HL, bool DOWN>
 hipError_t launch(const Weights &w, const Call &c, hipStream_t s) {
     const int N = DOWN ? w.dim : w.ffn, cols = DOWN ? 128 : 64;
-    const int y = c.tiles < 32768 ? c.tiles : 32768;
-    const dim3 grid((unsigned)((N + cols - 1) / cols * (DOWN ? c.splits : 1)), (unsigned)y, (unsigned)((c.tiles + y - 1) / y));
+    const int tiles = (DOWN ? c.down : c.up).most, y = tiles < 32768 ? tiles : 32768;
+    const dim3 grid((unsigned)((N + cols - 1) / cols * (DOWN ? c.splits : 1)), (unsigned)y, (unsigned)((tiles + y - 1) / y));
     experts_few<FMT, HL, DOWN><<<grid, kWaves * 64, 0, s>>>(w, c);
     return hipGetLastError();
 }

@@ -8,7 +8,8 @@
 // dequantizes, and of pair r's x'. MFMA p = 0..3 takes dword p of the codes and chunk p of the block layout. x' goes from
 // global memory into one of two stage buffers (rows of 128 bytes, 16-byte chunk c of row r at slot c ^ ((r / 2) % 8)), W into units of
 // two stages as in gemm_tile.h, whose WUnit and order of waits this is: X of stage i + 1 is issued behind the barrier of stage i,
-// the unit after the next one at odd stages, and operands of MFMA p + 1 are dequantized under those of p.
+// the unit after the next one at odd stages (Q8_0: units of one stage, at every one), and operands of MFMA p + 1 are dequantized under
+// those of p.
 //
 // A weight is fp16(fma(code, s 2^pow, o 2^pow)), rounded once, with the row's power 2^pow that brings its largest magnitude into
 // [2^13, 2^14) and leaves again in the epilogue: 11 bits down to 2^-27 of that. The code is an fp16 subnormal (a field masked out), so
@@ -29,8 +30,39 @@ using gw::wait_vm_lgkm0;
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef int32_t i32x4 __attribute__((ext_vector_type(4)));
 
+// W of 4 waves of two groups of 32 rows in LDS, a unit at a time: two stages.
 template <int FMT>
-using Unit = gt::WUnit<FMT, 8>;  // 4 waves of two groups of rows
+struct Unit : gt::WUnit<FMT, 8> {
+    static constexpr int kStages = 2;
+};
+// Q8_0: one stage, 64 bytes of codes a row (chunk c of row r at slot c ^ ((r / 4) % 4)) and a dword of scales; units of two stages
+// would leave room for one workgroup a CU.
+template <>
+struct Unit<Q8_0> {
+    static constexpr int kStages = 1, QR = 64, QL = 2, kLoads = 3, kS = 8 * 32 * QR, kSlot = 256, kBytes = kS + 8 * kSlot;
+    __amdgpu_buffer_rsrc_t qr, sr;
+    uint32_t qoff[QL], soff;
+    int wave;
+    static __device__ __forceinline__ int swz(int row) { return (row >> 2) & 3; }
+    __device__ __forceinline__ void init(const QMat &w, int nw, int wave_, int lane) {
+        const int N = (int)w.rows, K = (int)w.cols;
+        wave = wave_;
+        qr = make_rsrc(w.qs, (uint64_t)N * (uint64_t)K);
+        sr = make_rsrc(w.sc, (uint64_t)N * (uint64_t)(K / 16));
+#pragma unroll
+        for (int j = 0; j < QL; j++) {
+            const int row = 16 * j + (lane >> 2), c = (lane & 3) ^ swz(row), n = nw + row;
+            qoff[j] = n < N ? (uint32_t)n * (uint32_t)K + (uint32_t)c * 16u : kOob;
+        }
+        soff = lane < 32 && nw + lane < N ? (uint32_t)(nw + lane) * (uint32_t)(K / 16) : kOob;
+    }
+    __device__ __forceinline__ void load(int u, bool live, uint8_t *wb) const {
+        const uint32_t uu = live ? (uint32_t)u : 0u;
+#pragma unroll
+        for (int j = 0; j < QL; j++) dma16(qr, wb + (wave * QL + j) * 1024, live ? qoff[j] : kOob, uu * 64u);
+        gw::dma4s(sr, wb + kS + wave * kSlot, live ? soff : kOob, uu * 4u);
+    }
+};
 
 // fp16(fma(c, s, o)) of two codes, and with HL what that leaves.
 template <bool HL>
@@ -119,17 +151,17 @@ __device__ __forceinline__ void run(const Weights &w, const Call &c, const Tile 
         }
     };
     auto load_w = [&](int u, uint8_t *wb) __attribute__((always_inline)) {
-        unit[0].load(u, 2 * u < ns, wb);
-        unit[1].load(u, 2 * u < ns, wb);
+        unit[0].load(u, U::kStages * u < ns, wb);
+        unit[1].load(u, U::kStages * u < ns, wb);
     };
 
     auto read_block = [&](int j, int group, const uint8_t *wb, Block<FMT> &o) __attribute__((always_inline)) {
-        const int swz = U::swz(r32), blk = 2 * (j & 1) + h, unit_row = 32 * (2 * wave + group) + r32;
+        const int swz = U::swz(r32), blk = U::kStages == 2 ? 2 * (j & 1) + h : h, unit_row = 32 * (2 * wave + group) + r32;
         const uint8_t *const row = wb + unit_row * QR, *const slot = wb + U::kS + (2 * wave + group) * U::kSlot;
 #pragma unroll
-        for (int k = 0; k < U::QL / 2; k++) o.q[k] = *reinterpret_cast<const u32x4 *>(row + (((U::QL / 2 * blk + k) ^ swz) << 4));
+        for (int k = 0; k < (FMT == Q8_0 ? 2 : 1); k++) o.q[k] = *reinterpret_cast<const u32x4 *>(row + ((((FMT == Q8_0 ? 2 : 1) * blk + k) ^ swz) << 4));
         if constexpr (FMT == Q4_K) o.s = *reinterpret_cast<const u32x4 *>(slot + r32 * 16);
-        else o.s[0] = *reinterpret_cast<const uint16_t *>(slot + r32 * 8 + blk * 2);
+        else o.s[0] = *reinterpret_cast<const uint16_t *>(slot + r32 * (4 * U::kStages) + blk * 2);
         if constexpr (FMT == Q6_K) {
             o.hi = *reinterpret_cast<const u32x2 *>(wb + U::kH + unit_row * 32 + blk * 8);
             o.s[1] = *reinterpret_cast<const uint32_t *>(slot + 256 + r32 * 4);
@@ -221,9 +253,10 @@ __device__ __forceinline__ void run(const Weights &w, const Call &c, const Tile 
     auto stage = [&](auto S_, int i) __attribute__((always_inline)) {
         constexpr int S = decltype(S_)::value, cur = S & 1;
         uint8_t *const xb = cur ? xs1 : xs0, *const xn = cur ? xs0 : xs1;
-        constexpr int ur = (S + 1) / 2 % 2, un = (S + 3) / 2 % 2;
+        constexpr bool pairs = U::kStages == 2;
+        constexpr int ur = pairs ? (S + 1) / 2 % 2 : (S + 1) % 2, un = pairs ? (S + 3) / 2 % 2 : S % 2;
         uint8_t *const wc = ur ? ws1 : ws0, *const wn = un ? ws1 : ws0;
-        wait_vm_lgkm0<S % 2 == 0 ? WL : 0>();
+        wait_vm_lgkm0<pairs && S % 2 == 0 ? WL : 0>();
         lds_barrier();
         Operand<HL> a[2][TM];
         read_x(xb, 0, a[0]);
@@ -231,7 +264,8 @@ __device__ __forceinline__ void run(const Weights &w, const Call &c, const Tile 
         read_block(i + 1, 1, wc, blk[cur ^ 1][1]);
         load_x(i + 1, xn);
         load_order();  // X first: the wait at an even stage leaves the newest unit of W outstanding
-        if constexpr (S % 2 == 1) load_w((i + 3) / 2, wn);
+        if constexpr (!pairs) load_w(i + 2, wn);
+        else if constexpr (S % 2 == 1) load_w((i + 3) / 2, wn);
         __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int p = 0; p < 4; p++) {
@@ -342,16 +376,16 @@ template <int FMT, bool HL, int TM, bool DOWN>
 __global__ void __launch_bounds__(256, 2)
 experts_many(Weights w, Call c) {
     constexpr int kX = Lds<FMT, HL, TM>::kX, kW = Unit<FMT>::kBytes;
-    static_assert(2 * (kX + kW) <= 163840, "LDS");
+    static_assert(4 * (kX + kW) <= 163840, "two workgroups' LDS");
     __shared__ __attribute__((aligned(1024))) uint8_t xs0[kX], xs1[kX];
     __shared__ __attribute__((aligned(1024))) uint8_t ws0[kW], ws1[kW];
-    const int N = DOWN ? w.dim : w.ffn, chunks = DOWN ? (N + 255) / 256 : (N + 127) / 128, tiles = c.tile_count[0];
+    const int N = DOWN ? w.dim : w.ffn, chunks = DOWN ? (N + 255) / 256 : (N + 127) / 128, tiles = (DOWN ? c.down : c.up).count[0];
     // Workgroup b runs on XCD b % 8, and each XCD takes a contiguous range, down groups of 4 tiles of pairs: most often of one
     // expert, whose rows of W they share in the XCD's L2.
     const int total = tiles * chunks, per = (total + 7) / 8, at = (int)(blockIdx.x % 8) * per + (int)(blockIdx.x / 8);
     if ((int)(blockIdx.x / 8) >= per || at >= total) return;
     const int mg = at / (4 * chunks), gm = tiles - 4 * mg < 4 ? tiles - 4 * mg : 4, rem = at - 4 * mg * chunks;
-    Tile tile = c.tile[4 * mg + rem % gm];
+    Tile tile = (DOWN ? c.down : c.up).tile[4 * mg + rem % gm];
     tile.expert = __builtin_amdgcn_readfirstlane(tile.expert);
     tile.first = __builtin_amdgcn_readfirstlane(tile.first);
     tile.count = __builtin_amdgcn_readfirstlane(tile.count);
@@ -361,23 +395,40 @@ experts_many(Weights w, Call c) {
 template <int FMT, bool DOWN>
 hipError_t launch_type(const Weights &w, const Call &c, hipStream_t s) {
     const int N = DOWN ? w.dim : w.ffn, chunks = DOWN ? (N + 255) / 256 : (N + 127) / 128;
-    const int64_t total = ((int64_t)c.tiles * chunks + 7) / 8 * 8;
+    const Tiles &tiles = DOWN ? c.down : c.up;
+    const int64_t total = ((int64_t)tiles.most * chunks + 7) / 8 * 8;
     if (total > 0xffffff) return hipErrorInvalidValue;
     const dim3 grid((unsigned)total);
-    if (c.half) {
-        if (c.tile_rows == 128) experts_many<FMT, false, 4, DOWN><<<grid, 256, 0, s>>>(w, c);
-        else if (c.tile_rows == 64) experts_many<FMT, false, 2, DOWN><<<grid, 256, 0, s>>>(w, c);
-        else if (c.tile_rows == 32) experts_many<FMT, false, 1, DOWN><<<grid, 256, 0, s>>>(w, c);
-        else return hipErrorInvalidValue;
-    } else {
-        if (c.tile_rows == 64) experts_many<FMT, true, 2, DOWN><<<grid, 256, 0, s>>>(w, c);
-        else if (c.tile_rows == 32) experts_many<FMT, true, 1, DOWN><<<grid, 256, 0, s>>>(w, c);
-        else return hipErrorInvalidValue;
+    bool launched = false;
+#define J4Q_MANY(HL, TM)                                                \
+    if (c.half == !HL && tiles.rows == 32 * TM) {                       \
+        experts_many<FMT, HL, TM, DOWN><<<grid, 256, 0, s>>>(w, c);     \
+        launched = true;                                                \
     }
+    J4Q_MANY(false, 1)
+    J4Q_MANY(false, 2)
+    if constexpr (FMT == Q6_K) {
+        J4Q_MANY(false, 3)
+    } else {
+        J4Q_MANY(false, 4)
+    }
+    J4Q_MANY(true, 1)
+    if constexpr (FMT != Q6_K) {
+        J4Q_MANY(true, 2)
+    }
+#undef J4Q_MANY
+    if (!launched) return hipErrorInvalidValue;
     return hipGetLastError();
 }
 
 }  // namespace
+
+// `each`: pairs per expert on average. The most pairs a tile with which two workgroups' LDS fit a CU.
+int rows_many(int type, bool half, int each) {
+    if (each < 40 || (!half && type == Q6_K)) return 32;
+    if (each < 96 || !half) return 64;
+    return type == Q6_K ? 96 : 128;
+}
 
 hipError_t launch_many(const Weights &w, const Call &c, bool down, hipStream_t s) {
     switch (down ? w.down_type : w.up_type) {
