@@ -389,7 +389,12 @@ experts_many(Weights w, Call c) {
     tile.expert = __builtin_amdgcn_readfirstlane(tile.expert);
     tile.first = __builtin_amdgcn_readfirstlane(tile.first);
     tile.count = __builtin_amdgcn_readfirstlane(tile.count);
-    run<FMT, HL, TM, DOWN>(w, c, tile, rem / gm, xs0, xs1, ws0, ws1);
+    // a tile of fewer pairs (every expert's last one) with as many groups of 32 as it has
+    const int groups = (tile.count + 31) / 32, chunk = rem / gm;
+    if (groups >= TM) run<FMT, HL, TM, DOWN>(w, c, tile, chunk, xs0, xs1, ws0, ws1);
+    else if (TM > 3 && groups == 3) run<FMT, HL, TM < 3 ? TM : 3, DOWN>(w, c, tile, chunk, xs0, xs1, ws0, ws1);
+    else if (TM > 2 && groups == 2) run<FMT, HL, TM < 2 ? TM : 2, DOWN>(w, c, tile, chunk, xs0, xs1, ws0, ws1);
+    else run<FMT, HL, 1, DOWN>(w, c, tile, chunk, xs0, xs1, ws0, ws1);
 }
 
 template <int FMT, bool DOWN>
