@@ -2,6 +2,7 @@
 // weighted sums (experts.h).
 #include <limits.h>
 
+#include <algorithm>
 #include <exception>
 #include <memory>
 #include <vector>
@@ -212,23 +213,60 @@ experts_plan(Weights w, Call c) {
 
 // ---- the sums -------------------------------------------------------------------------------
 
-// out[r] = sum over its slots, and each one's splits, one after another, of the weighted partial results. A thread per 4 columns.
+// out[r] = sum over its slots, and each one's splits, one after another, of the weighted partial results. A thread per 4 columns, or 8
+// where the partial results are fp16; the loads of 4 slots are on their way together.
+template <bool SMALL>
 __global__ void __launch_bounds__(256)
 experts_combine(Weights w, Call c) {
-    const int r = (int)(blockIdx.z * gridDim.y + blockIdx.y), col = 4 * (int)(blockIdx.x * 256 + threadIdx.x);
+    constexpr int V = SMALL ? 8 : 4;
+    const int r = (int)(blockIdx.z * gridDim.y + blockIdx.y), col = V * (int)(blockIdx.x * 256 + threadIdx.x);
     if (r >= c.rows || col >= w.dim) return;
-    f32x4 s = {};
-    for (int k = 0; k < c.top; k++) {
-        const int64_t pair = (int64_t)r * c.top + k;
-        const int id = c.ids[pair];
-        if (id < 0 || id >= w.experts) continue;
-        for (int v = 0; v < c.splits; v++) s += *reinterpret_cast<const f32x4 *>(c.part + ((int64_t)v * c.pairs + pair) * w.dim + col);
+    float s[V] = {};
+    const int64_t first = (int64_t)r * c.top;
+    if constexpr (SMALL) {
+        const int norm = c.x_norm[r];
+        for (int k0 = 0; k0 < c.top; k0 += 4) {
+            h8 v[4];
+            float weight[4];
+            int pow[4];
+            bool is[4];
+#pragma unroll
+            for (int u = 0; u < 4; u++) {
+                const int k = k0 + u < c.top ? k0 + u : k0, id = c.ids[first + k];
+                is[u] = k0 + u < c.top && id >= 0 && id < w.experts;
+                weight[u] = c.weights[first + k];
+                pow[u] = is[u] ? -part_pow(w, id, norm) : 0;
+                v[u] = h8{};
+                if (is[u]) v[u] = *reinterpret_cast<const h8 *>((const _Float16 *)c.part + (first + k) * w.dim + col);
+            }
+#pragma unroll
+            for (int u = 0; u < 4; u++)
+                if (is[u]) {
+#pragma unroll
+                    for (int j = 0; j < V; j++) s[j] += __builtin_ldexpf((float)v[u][j] * weight[u], pow[u]);
+                }
+        }
+    } else {
+        for (int k = 0; k < c.top; k++) {
+            const int64_t pair = first + k;
+            const int id = c.ids[pair];
+            if (id < 0 || id >= w.experts) continue;
+            for (int v = 0; v < c.splits; v++) {
+                const f32x4 p = *reinterpret_cast<const f32x4 *>(c.part + ((int64_t)v * c.pairs + pair) * w.dim + col);
+#pragma unroll
+                for (int j = 0; j < V; j++) s[j] += p[j];
+            }
+        }
     }
     if (c.half) {
-        typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
-        *reinterpret_cast<bf16x4 *>((uint16_t *)c.out + (int64_t)r * c.out_stride + col) = __builtin_convertvector(s, bf16x4);
+        typedef __bf16 bf16xv __attribute__((ext_vector_type(V)));
+        typedef float f32xv __attribute__((ext_vector_type(V)));
+        f32xv t;
+#pragma unroll
+        for (int j = 0; j < V; j++) t[j] = s[j];
+        *reinterpret_cast<bf16xv *>((uint16_t *)c.out + (int64_t)r * c.out_stride + col) = __builtin_convertvector(t, bf16xv);
     } else {
-        *reinterpret_cast<f32x4 *>((float *)c.out + (int64_t)r * c.out_stride + col) = s;
+        *reinterpret_cast<f32x4 *>((float *)c.out + (int64_t)r * c.out_stride + col) = f32x4{s[0], s[1], s[2], s[3]};
     }
 }
 
@@ -271,19 +309,19 @@ row_stats(const float *__restrict__ v, int cols, int64_t row0, int32_t *__restri
         }
     }
     pow[row0 + blockIdx.x] = p;
-    if (norm) norm[row0 + blockIdx.x] = q;
+    norm[row0 + blockIdx.x] = q;
 }
 
-// bound[e] = the largest of gate's exponents of expert e + the largest of up's.
+// bound[e] = the largest of gate's exponents of expert e (of `rows` rows) + the largest of up's, or + add where there are none.
 __global__ void __launch_bounds__(256)
-expert_bound(const int32_t *__restrict__ gate, const int32_t *__restrict__ up, int ffn, int32_t *__restrict__ bound) {
+expert_bound(const int32_t *__restrict__ gate, const int32_t *__restrict__ up, int add, int rows, int32_t *__restrict__ bound) {
     __shared__ int most[2][4];
     const int t = (int)threadIdx.x;
-    const int64_t first = (int64_t)blockIdx.x * ffn;
-    int a = 2 * kNothing, b = 2 * kNothing;
-    for (int i = t; i < ffn; i += 256) {
+    const int64_t first = (int64_t)blockIdx.x * rows;
+    int a = 2 * kNothing, b = up ? 2 * kNothing : add;
+    for (int i = t; i < rows; i += 256) {
         a = a > gate[first + i] ? a : gate[first + i];
-        b = b > up[first + i] ? b : up[first + i];
+        if (up) b = b > up[first + i] ? b : up[first + i];
     }
 #pragma unroll
     for (int o = 32; o > 0; o /= 2) {
@@ -338,7 +376,7 @@ bool type_ok(int type, int64_t cols) {
     }
 }
 
-// The powers of a matrix's rows, and with norm the exponents of their norms. scratch: room for `chunk` dequantized rows.
+// The powers of a matrix's rows and the exponents of their norms. scratch: room for `chunk` dequantized rows.
 hipError_t stats(int type, const QMat &m, float *scratch, int64_t chunk, int32_t *pow, int32_t *norm, hipStream_t s) {
     hipError_t e = hipSuccess;
     for (int64_t r = 0; r < m.rows && e == hipSuccess; r += chunk) {
@@ -367,13 +405,14 @@ int create(const j4q_experts_config &c, j4q_experts *out) {
     if (!type_ok(gate.qtype, dim) || !type_ok(down.qtype, ffn) || dim > 65536 || ffn > 65536)
         return report_error(J4Q_EUNSUPPORTED, "experts: type %d of %lld columns, type %d of %lld (Q8_0, a multiple of 64 columns, Q4_0, of 128, Q4_K, Q6_K; at most 65536)",
                             gate.qtype, (long long)dim, down.qtype, (long long)ffn);
+    if (dim * ffn >= 1ll << 31) return report_error(J4Q_EUNSUPPORTED, "experts: matrices of %lld x %lld values (fewer than 2^31)", (long long)dim, (long long)ffn);
     if ((rc = abi::ready_locked())) return rc;
     if (capturing(abi::stream())) return report_error(J4Q_EINVAL, "experts: the engine stream is captured");
     size_t slot = 0;
     while (slot < g_experts.size() && g_experts[slot]->live) slot++;
     if (slot == g_experts.size()) g_experts.emplace_back(new Experts);
     Experts &k = *g_experts[slot];
-    const uint64_t words = (uint64_t)(4 * E * ffn + E * dim + E);  // powers of gate, up, down; norms of gate, up; bounds
+    const uint64_t words = (uint64_t)(4 * E * ffn + 2 * E * dim + 2 * E);  // bounds; powers and norms of gate, up, down
     const int64_t wide = dim > ffn ? dim : ffn, chunk = (16 << 20) / wide;
     void *dev = nullptr;
     hipError_t e = abi::malloc_locked(&dev, words * 4);
@@ -393,17 +432,21 @@ int create(const j4q_experts_config &c, j4q_experts *out) {
         k.w.dim = (int)dim;
         k.w.ffn = (int)ffn;
         k.w.act = c.activation;
-        int32_t *const gate_pow = at + E, *const up_pow = gate_pow + E * ffn, *const gate_norm = up_pow + E * ffn, *const up_norm = gate_norm + E * ffn,
-                      *const down_pow = up_norm + E * ffn;
+        int32_t *const gate_pow = at + 2 * E, *const up_pow = gate_pow + E * ffn, *const gate_norm = up_pow + E * ffn, *const up_norm = gate_norm + E * ffn,
+                      *const down_pow = up_norm + E * ffn, *const down_norm = down_pow + E * dim;
+        int root = 0;  // 4^root >= ffn
+        while (1ll << (2 * root) < ffn) root++;
         k.w.bound = at;
+        k.w.bound_down = at + E;
         k.w.gate_pow = gate_pow;
         k.w.up_pow = up_pow;
         k.w.down_pow = down_pow;
         e = stats(gate.qtype, gate.m, ws.ptr, chunk, gate_pow, gate_norm, s);
         if (e == hipSuccess) e = stats(up.qtype, up.m, ws.ptr, chunk, up_pow, up_norm, s);
-        if (e == hipSuccess) e = stats(down.qtype, down.m, ws.ptr, chunk, down_pow, nullptr, s);
+        if (e == hipSuccess) e = stats(down.qtype, down.m, ws.ptr, chunk, down_pow, down_norm, s);
         if (e == hipSuccess) {
-            expert_bound<<<(unsigned)E, 256, 0, s>>>(gate_norm, up_norm, (int)ffn, at);
+            expert_bound<<<(unsigned)E, 256, 0, s>>>(gate_norm, up_norm, 0, (int)ffn, at);
+            expert_bound<<<(unsigned)E, 256, 0, s>>>(down_norm, nullptr, root, (int)dim, at + E);
             e = hipGetLastError();
         }
         abi::workspace_end_locked(s, ws, e == hipSuccess);
@@ -447,7 +490,7 @@ uint64_t lay_out(const Weights &w, Call *c, uint8_t *base) {
     c->x_norm = (int32_t *)take(4 * T);
     c->xa = (_Float16 *)take(2 * planes * T * (uint64_t)w.dim);
     c->ha = (_Float16 *)take(2 * planes * P * (uint64_t)w.ffn);
-    c->part = (float *)take(4 * (uint64_t)c->splits * P * (uint64_t)w.dim);
+    c->part = (float *)take((c->small ? 2 : 4 * (uint64_t)c->splits) * P * (uint64_t)w.dim);
     return at;
 }
 
@@ -460,9 +503,10 @@ void shape(const Weights &w, Call *c) {
     c->down.rows = c->few ? few : rows_many(w.down_type, c->half, each);
     for (Tiles *t : {&c->up, &c->down}) t->most = some + (c->pairs - some) / t->rows;
     c->splits = c->few ? splits_few(w, c->down.most) : 1;
+    c->small = c->half && !c->few;
 }
 
-int check_size(const Weights &, const char *op, int64_t rows, int32_t top, int type) {
+int check_size(const char *op, int64_t rows, int32_t top, int type) {
     if (!dense_type(type)) return report_error(J4Q_EUNSUPPORTED, "%s: type %d (J4Q_KIND_F32 or J4Q_KIND_BF16)", op, type);
     if (rows < 1 || top < 1 || top > kMaxTop) return report_error(J4Q_EINVAL, "%s: %lld rows of %d experts (1 to %d)", op, (long long)rows, top, kMaxTop);
     if (rows > (1 << 22) / top) return report_error(J4Q_EUNSUPPORTED, "%s: %lld rows of %d experts (at most %d pairs)", op, (long long)rows, top, 1 << 22);
@@ -478,7 +522,60 @@ hipError_t launch(const Weights &w, const Call &c, hipEvent_t done, hipStream_t 
     if (e == hipSuccess) e = products(w, c, true, s);
     if (e != hipSuccess) return e;
     const int y = c.rows < 32768 ? c.rows : 32768;
-    return launch_with_event(experts_combine, dim3((unsigned)((w.dim + 1023) / 1024), (unsigned)y, (unsigned)((c.rows + y - 1) / y)), dim3(256), s, done, w, c);
+    const int cols = c.small ? 2048 : 1024;
+    const dim3 grid((unsigned)((w.dim + cols - 1) / cols), (unsigned)y, (unsigned)((c.rows + y - 1) / y));
+    return c.small ? launch_with_event(experts_combine<true>, grid, dim3(256), s, done, w, c) : launch_with_event(experts_combine<false>, grid, dim3(256), s, done, w, c);
+}
+
+// A call of many rows runs as ranges of rows, one after another in the same workspace: the products address x' and h' by 32-bit offsets,
+// and what a range of 2^17 pairs needs (2 GiB of results at dim 4096, fp32) is enough for whole tiles of 1024 experts.
+struct Ranges {
+    int count, rows, larger;  // `larger` ranges of rows + 1 and then count - larger of rows
+};
+
+Ranges ranges(const Weights &w, const Call &c) {
+    const int64_t bytes = c.half ? 2 : 4, limit = (1ll << 31) - 1;
+    int64_t most = (1 << 17) / c.top;
+    most = std::min(most, limit / (bytes * w.dim));
+    most = std::min(most, limit / (bytes * w.ffn * c.top));
+    const int n = (int)((c.rows + most - 1) / most);
+    return {n, c.rows / n, c.rows % n};
+}
+
+Call range(const Weights &w, const Call &all, int first, int rows) {
+    Call c = all;
+    const int64_t e = c.half ? 2 : 4;
+    c.x = (const uint8_t *)all.x + first * all.x_stride * e;
+    c.out = (uint8_t *)all.out + first * all.out_stride * e;
+    c.ids = all.ids + (int64_t)first * c.top;
+    c.weights = all.weights + (int64_t)first * c.top;
+    c.rows = rows;
+    c.pairs = rows * c.top;
+    shape(w, &c);
+    return c;
+}
+
+uint64_t workspace(const Weights &w, const Call &all) {
+    const Ranges r = ranges(w, all);
+    uint64_t most = 0;
+    for (int more = 0; more < 2; more++) {
+        if (!(more ? r.larger : r.count - r.larger)) continue;
+        Call c = range(w, all, 0, r.rows + more);
+        most = std::max(most, lay_out(w, &c, nullptr));
+    }
+    return most;
+}
+
+hipError_t launch_all(const Weights &w, const Call &all, void *space, hipEvent_t done, hipStream_t s) {
+    const Ranges r = ranges(w, all);
+    hipError_t e = hipSuccess;
+    for (int i = 0, first = 0; i < r.count && e == hipSuccess; i++) {
+        Call c = range(w, all, first, r.rows + (i < r.larger));
+        lay_out(w, &c, (uint8_t *)space);
+        e = launch(w, c, i + 1 == r.count ? done : nullptr, s);
+        first += c.rows;
+    }
+    return e;
 }
 
 int apply(const Experts &k, const j4q_experts_args &a, hipStream_t s) {
@@ -491,39 +588,36 @@ int apply(const Experts &k, const j4q_experts_args &a, hipStream_t s) {
     c.out_stride = a.out_stride ? a.out_stride : k.w.dim;
     c.rows = (int)a.rows;
     c.top = a.top_k;
-    c.pairs = c.rows * c.top;
     c.half = a.type == J4Q_KIND_BF16;
     const int64_t e = dense_size(a.type), dim = k.w.dim;
     for (int64_t st : {c.x_stride, c.out_stride})
         if (st < dim || st > 1ll << 40 || st * e % 16) return report_error(J4Q_EINVAL, "experts apply: rows of %lld values %lld apart, a multiple of 16 bytes", (long long)dim, (long long)st);
     if (!aligned(a.x, 16) || !aligned(a.out, 16) || !aligned(a.ids, 4) || !aligned(a.weights, 4))
         return report_error(J4Q_EINVAL, "experts apply: x and out must be 16-byte aligned, ids and weights 4-byte aligned");
-    const uint64_t out_bytes = (uint64_t)(((c.rows - 1) * c.out_stride + dim) * e), x_bytes = (uint64_t)(((c.rows - 1) * c.x_stride + dim) * e);
-    if (overlap(c.x, c.x_stride * e, dim * e, c.out, c.out_stride * e, dim * e, c.rows) || overlap(c.ids, (uint64_t)c.pairs * 4, c.out, out_bytes) ||
-        overlap(c.weights, (uint64_t)c.pairs * 4, c.out, out_bytes))
+    const uint64_t out_bytes = (uint64_t)(((c.rows - 1) * c.out_stride + dim) * e), x_bytes = (uint64_t)(((c.rows - 1) * c.x_stride + dim) * e),
+                   pair_bytes = (uint64_t)c.rows * (uint64_t)c.top * 4;
+    if (overlap(c.x, c.x_stride * e, dim * e, c.out, c.out_stride * e, dim * e, c.rows) || overlap(c.ids, pair_bytes, c.out, out_bytes) ||
+        overlap(c.weights, pair_bytes, c.out, out_bytes))
         return report_error(J4Q_EUNSUPPORTED, "experts apply: out must lie apart from x, ids and weights");
-    shape(k.w, &c);
-    const uint64_t bytes = lay_out(k.w, &c, nullptr);
-    Workspace ws;
+    const uint64_t bytes = workspace(k.w, c);
     if (a.workspace) {
         if (!aligned(a.workspace, 256) || a.workspace_bytes < bytes)
             return report_error(J4Q_EINVAL, "experts apply: a workspace of %llu bytes, 256-byte aligned, is needed", (unsigned long long)bytes);
-        if (overlap(a.workspace, bytes, c.x, x_bytes) || overlap(a.workspace, bytes, c.out, out_bytes) || overlap(a.workspace, bytes, c.ids, (uint64_t)c.pairs * 4) ||
-            overlap(a.workspace, bytes, c.weights, (uint64_t)c.pairs * 4))
+        if (overlap(a.workspace, bytes, c.x, x_bytes) || overlap(a.workspace, bytes, c.out, out_bytes) || overlap(a.workspace, bytes, c.ids, pair_bytes) ||
+            overlap(a.workspace, bytes, c.weights, pair_bytes))
             return report_error(J4Q_EUNSUPPORTED, "experts apply: the workspace must lie apart from the other arguments");
     }
     int rc;
     if ((rc = abi::ready_locked())) return rc;
     if (!s) s = abi::stream();
     if (a.workspace) {
-        lay_out(k.w, &c, (uint8_t *)a.workspace);
-        const hipError_t err = launch(k.w, c, nullptr, s);
+        const hipError_t err = launch_all(k.w, c, a.workspace, nullptr, s);
         return err == hipSuccess ? J4Q_OK : report_hip("experts apply", err);
     }
+    Workspace ws;
     hipError_t err = abi::workspace_begin_locked(s, bytes, &ws);
     if (err != hipSuccess) return report_hip("experts apply", err);
-    lay_out(k.w, &c, (uint8_t *)ws.ptr);
-    err = launch(k.w, c, ws.done, s);
+    err = launch_all(k.w, c, ws.ptr, ws.done, s);
     abi::workspace_end_locked(s, ws, err == hipSuccess);
     return err == hipSuccess ? J4Q_OK : report_hip("experts apply", err);
 }
@@ -576,14 +670,12 @@ int j4q_experts_workspace(j4q_experts h, int64_t rows, int32_t top_k, int type, 
     std::lock_guard<std::mutex> lk(abi::lock());
     ex::Experts *k;
     int rc;
-    if ((rc = ex::get(h, "experts workspace", &k)) || (rc = ex::check_size(k->w, "experts workspace", rows, top_k, type))) return rc;
+    if ((rc = ex::get(h, "experts workspace", &k)) || (rc = ex::check_size("experts workspace", rows, top_k, type))) return rc;
     ex::Call c{};
     c.rows = (int)rows;
     c.top = top_k;
-    c.pairs = c.rows * c.top;
     c.half = type == J4Q_KIND_BF16;
-    ex::shape(k->w, &c);
-    *bytes = ex::lay_out(k->w, &c, nullptr);
+    *bytes = ex::workspace(k->w, c);
     return J4Q_OK;
 }
 
@@ -592,7 +684,7 @@ int j4q_experts_apply(j4q_experts h, const j4q_experts_args *args, void *stream)
     std::lock_guard<std::mutex> lk(abi::lock());
     ex::Experts *k;
     int rc;
-    if ((rc = ex::get(h, "experts apply", &k)) || (rc = ex::check_size(k->w, "experts apply", args->rows, args->top_k, args->type))) return rc;
+    if ((rc = ex::get(h, "experts apply", &k)) || (rc = ex::check_size("experts apply", args->rows, args->top_k, args->type))) return rc;
     return ex::apply(*k, *args, (hipStream_t)stream);
 }
 

@@ -330,43 +330,62 @@ __device__ __forceinline__ void run(const Weights &w, const Call &c, const Tile 
         p0[q] = a < N ? *reinterpret_cast<const i32x4 *>(pow0 + a) : i32x4{};
         p1[q] = e < N ? *reinterpret_cast<const i32x4 *>(pow1 + e) : i32x4{};
     }
+    if constexpr (DOWN) {
+        // Through LDS, 32 pairs at a time, so that whole lines are stored: a pair's 64 columns of this wave are 8 chunks of 16 bytes of
+        // fp16, or 16 of fp32; chunk k of pair p at k ^ (p % 8).
+        __syncthreads();  // all waves have read their W
+        uint8_t *const place = (wave < 2 ? ws0 : ws1) + (wave & 1) * 8192;
+        constexpr int C = HL ? 16 : 8;  // chunks of a pair
 #pragma unroll
-    for (int t = 0; t < TM; t++) {
-        const int m = 32 * t + r32;
-        if (m >= count) continue;
-        const int pair = c.order[first + m], token = pair / c.top, hp = h_pow(w, expert, c.x_norm[token]);
-        if constexpr (DOWN) {
-            const float weight = c.weights[pair];
-            float *const out = c.part + (int64_t)pair * N;
+        for (int t = 0; t < TM; t++) {
+            const int m = 32 * t + r32;
+            const int pair = c.order[first + (m < count ? m : 0)], token = pair / c.top, norm = c.x_norm[token];
+            const float weight = HL ? c.weights[pair] : 1.f;
+            const int up = HL ? -h_pow(w, expert, norm) : part_pow(w, expert, norm) - h_pow(w, expert, norm);
 #pragma unroll
             for (int g = 0; g < 2; g++)
 #pragma unroll
                 for (int q = 0; q < 4; q++) {
-                    const int n = (g ? n1 : n0) + 8 * q + 4 * h;
                     f32x4 v;
 #pragma unroll
-                    for (int j = 0; j < 4; j++) v[j] = __builtin_ldexpf(acc[g][t][4 * q + j] * weight, -hp - (g ? p1[q][j] : p0[q][j]));
-                    if (n < N) *reinterpret_cast<f32x4 *>(out + n) = v;
+                    for (int j = 0; j < 4; j++) v[j] = __builtin_ldexpf(HL ? acc[g][t][4 * q + j] * weight : acc[g][t][4 * q + j], up - (g ? p1[q][j] : p0[q][j]));
+                    if constexpr (HL) *reinterpret_cast<f32x4 *>(place + r32 * 256 + (((8 * g + 2 * q + h) ^ (r32 & 7)) << 4)) = v;
+                    else *reinterpret_cast<h4 *>(place + r32 * 128 + (((4 * g + q) ^ (r32 & 7)) << 4) + 8 * h) = __builtin_convertvector(v, h4);
                 }
-        } else {
-            const int e = -c.x_pow[token];
-            if (n0 >= N) continue;
-            _Float16 *const out = c.ha + (int64_t)(first + m) * N + n0;
-            const int64_t lo = (int64_t)c.pairs * N;
+            asm volatile("" ::: "memory");  // a wave's own place, whose operations are in order
 #pragma unroll
-            for (int k = 0; k < 2; k++) {  // chunk 2 k + h of the block: elements of q = k, then of q = 2 + k
-                h8 hi, rest;
-#pragma unroll
-                for (int s = 0; s < 8; s++) {
-                    const int q = k + 2 * (s >> 2), j = (s & 1) << 1 | (s >> 1 & 1);
-                    const float gv = __builtin_ldexpf(acc[0][t][4 * q + j], e - p0[q][j]), uv = __builtin_ldexpf(acc[1][t][4 * q + j], e - p1[q][j]);
-                    const float v = __builtin_ldexpf(activate(gv, w.act) * uv, hp);
-                    hi[s] = (_Float16)v;
-                    rest[s] = (_Float16)(v - (float)hi[s]);
-                }
-                *reinterpret_cast<h8 *>(out + 8 * (2 * k + h)) = hi;
-                if constexpr (HL) *reinterpret_cast<h8 *>(out + lo + 8 * (2 * k + h)) = rest;
+            for (int i = 0; i < C / 2; i++) {
+                const int p = (64 / C) * i + lane / C, k = lane % C, n = n0 + (HL ? 4 : 8) * k;
+                const u32x4 v = *reinterpret_cast<const u32x4 *>(place + p * (16 * C) + ((k ^ (p & 7)) << 4));
+                if (32 * t + p >= count || n >= N) continue;
+                const int64_t at = (int64_t)c.order[first + 32 * t + p] * N + n;
+                if constexpr (HL) *reinterpret_cast<u32x4 *>(c.part + at) = v;
+                else *reinterpret_cast<u32x4 *>((_Float16 *)c.part + at) = v;
             }
+            asm volatile("" ::: "memory");
+        }
+        return;
+    }
+#pragma unroll
+    for (int t = 0; t < TM; t++) {
+        const int m = 32 * t + r32;
+        if (m >= count || n0 >= N) continue;
+        const int pair = c.order[first + m], token = pair / c.top, hp = h_pow(w, expert, c.x_norm[token]), e = -c.x_pow[token];
+        _Float16 *const out = c.ha + (int64_t)(first + m) * N + n0;
+        const int64_t lo = (int64_t)c.pairs * N;
+#pragma unroll
+        for (int k = 0; k < 2; k++) {  // chunk 2 k + h of the block: elements of q = k, then of q = 2 + k
+            h8 hi, rest;
+#pragma unroll
+            for (int s = 0; s < 8; s++) {
+                const int q = k + 2 * (s >> 2), j = (s & 1) << 1 | (s >> 1 & 1);
+                const float gv = __builtin_ldexpf(acc[0][t][4 * q + j], e - p0[q][j]), uv = __builtin_ldexpf(acc[1][t][4 * q + j], e - p1[q][j]);
+                const float v = __builtin_ldexpf(activate(gv, w.act) * uv, hp);
+                hi[s] = (_Float16)v;
+                rest[s] = (_Float16)(v - (float)hi[s]);
+            }
+            *reinterpret_cast<h8 *>(out + 8 * (2 * k + h)) = hi;
+            if constexpr (HL) *reinterpret_cast<h8 *>(out + lo + 8 * (2 * k + h)) = rest;
         }
     }
 }
@@ -377,6 +396,7 @@ __global__ void __launch_bounds__(256, 2)
 experts_many(Weights w, Call c) {
     constexpr int kX = Lds<FMT, HL, TM>::kX, kW = Unit<FMT>::kBytes;
     static_assert(4 * (kX + kW) <= 163840, "two workgroups' LDS");
+    static_assert(kW >= 16384, "two waves' results in a buffer of W");
     __shared__ __attribute__((aligned(1024))) uint8_t xs0[kX], xs1[kX];
     __shared__ __attribute__((aligned(1024))) uint8_t ws0[kW], ws1[kW];
     const int N = DOWN ? w.dim : w.ffn, chunks = DOWN ? (N + 255) / 256 : (N + 127) / 128, tiles = (DOWN ? c.down : c.up).count[0];

@@ -3,7 +3,7 @@
 // A call of a few microseconds: what bounds it is what waits for what, and then the stream of W. As in the batch-1 GEMV (gemv_impl.h,
 // whose loads and dot products these are) a wave has whole rows of W, a lane the 32 columns of a chunk, so that its loads are
 // contiguous kilobytes, and x lies in LDS; the matrix cores, of whose 16 operand rows one row would use one, gain nothing here
-// (with them, 8 of 64 Q4_K / Q6_K experts 2048 x 1024: 8.5 and 12.9 us; this way 6.9 and 7.5). All weights of a wave are on their way before
+// (with them, 8 of 64 Q4_K / Q6_K experts 2048 x 1024: 8.5 and 12.9 us; this way 9.6 and 8.3, 16.9 a call). All weights of a wave are on their way before
 // it waits for x.
 //  - experts_one_up: a workgroup has a slot and 16 rows of gate and of up, a wave two of each.
 //  - experts_one_down: a wave has a row of the result for all slots, its chunks running over slots and ffn; h, times the slot's weight, lies in

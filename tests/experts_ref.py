@@ -130,7 +130,8 @@ def experts(x, ids, weights, gate, up, down, act, kind, exact_weights):
     2^-40 of it; weights are exact, or rounded to 11 bits; a sum of K products in 32 bits, a rounding for each, and for each block's scale, its
     minimum and what a wave or split adds: K + K / 8 + 40 of them at most. The inner activations have 22 or 11 bits, below the normal range
     2^-25 at a power that takes their bound |x|^2 G U to 2^14; the activation and the product with up: the slope of an activation is at
-    most 1.13, expf within 2 steps, and five roundings more."""
+    most 1.13, expf within 2 steps, and five roundings more. For results in bf16 a pair's share is rounded to 11 bits, below the normal range
+    2^-25 at a power that takes its bound |x|^2 G U D sqrt(ffn), rounded up by 2^5 at most, to 2^14."""
     t, top = ids.shape
     half = kind == "bf16"
     y, off = np.zeros(x.shape), np.zeros(x.shape)
@@ -153,6 +154,8 @@ def experts(x, ids, weights, gate, up, down, act, kind, exact_weights):
             eh = ea * (np.abs(u) + eu) + np.abs(a) * eu + 3 * STEP["f32"] * np.abs(h)
             eh = eh + np.maximum((2.0 ** -11 if half else 2.0 ** -22) * np.abs(h), 2.0 ** (-25 - 14 + 3) * bound)
             part, ep = down[0][e] @ h, ad @ (few(h.size) * np.abs(h) + eh)
+            if half:
+                ep = ep + np.maximum(2.0 ** -11 * np.abs(part), 2.0 ** (-25 - 14 + 5) * bound * np.sqrt(h.size * (down[0][e] ** 2).sum(1).max()))
             w = float(weights[r, s])
             y[r] += w * part
             off[r] += abs(w) * (ep + (top + 1) * STEP["f32"] * np.abs(part))

@@ -198,6 +198,61 @@ def test_a_row_does_not_depend_on_the_others(layer):
     assert np.array_equal(a[order], b)
 
 
+@pytest.mark.parametrize("up,down", PAIRS)
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+@pytest.mark.parametrize("rows", [50, 200, 330])
+def test_pairs_enough_for_each_size_of_tile(layer, up, down, kind, rows):
+    """25, 100 and 165 pairs an expert, on average, and one expert with a pair, one with 33, 65 and 97."""
+    l = layer(up, down, 6, 256, 256)
+    x, ids, w = inputs(l, rows, 3, kind, seed=rows)
+    check(l, x, ids, w, kind, apply(l, x, ids, w, kind))
+    if rows < 330:
+        return
+    for few in (1, 33, 65, 97):
+        i = ids.copy()
+        i[i == 2] = -1
+        i[:few, 1] = 2
+        check(l, x, i, w, kind, apply(l, x, i, w, kind))
+
+
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+def test_a_row_of_more_than_the_kernel_of_one_holds(layer, kind):
+    l = layer("Q4_K", "Q6_K", 3, 8448, 256)
+    x, ids, w = inputs(l, 1, 2, kind)
+    check(l, x, ids, w, kind, apply(l, x, ids, w, kind))
+    l = layer("Q8_0", "Q8_0", 6, 64, 8192)
+    x, ids, w = inputs(l, 1, 6, kind)
+    check(l, x, ids, w, kind, apply(l, x, ids, w, kind))
+
+
+def some_rows(l, x, ids, w, kind, got, rows):
+    check(l, x[rows].cpu(), ids[rows], w[rows], kind, got[rows])
+
+
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+@pytest.mark.parametrize("workspace", [True, False])
+def test_more_rows_than_a_range(layer, kind, workspace):
+    """At most 2^17 pairs run together: three ranges, of 32834, 32833 and 32833 rows."""
+    l = layer("Q8_0", "Q8_0", 6, 64, 64)
+    x, ids, w = inputs(l, 98500, 3, kind)
+    got = apply(l, x, ids, w, kind, workspace=workspace)
+    some_rows(l, x, ids, w, kind, got, np.r_[0:9, 32830:32840, 65660:65672, 98490:98500])
+    parts = [apply(l, x[a:b], ids[a:b], w[a:b], kind) for a, b in ((0, 32834), (32834, 65667), (65667, 98500))]
+    assert np.array_equal(got, np.concatenate(parts))
+
+
+@pytest.mark.parametrize("dim,ffn,rows", [(65536, 64, 8200), (64, 65536, 4110)])
+def test_activations_of_more_than_2_31_bytes(layer, dim, ffn, rows):
+    l = layer("Q8_0", "Q8_0", 2, dim, ffn)
+    top = 1 if dim > ffn else 2
+    gen = torch.Generator(device="cuda").manual_seed(5)
+    x = torch.randn(rows, dim, generator=gen, device="cuda")
+    ids = np.arange(rows * top, dtype=np.int32).reshape(rows, top) % 2
+    w = np.random.default_rng(1).random((rows, top)).astype(np.float32)
+    got = apply(l, x, ids, w, "f32")
+    some_rows(l, x, ids, w, "f32", got, np.r_[0:2, rows // 2 - 2:rows // 2 + 2, rows - 2:rows])
+
+
 def test_two_streams_at_once(layer):
     l = layer("Q4_K", "Q6_K", 6, 512, 256)
     jobs = []
