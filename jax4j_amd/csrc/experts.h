@@ -65,6 +65,7 @@ struct Call {
     void *out;
     int64_t out_stride;
     int rows, top, pairs;
+    uint32_t top_inverse;  // ceil(2^32 / top); not used for 1
     bool half;      // bf16 x and out; x' and h' have no lo part
     bool one;       // a single row on its own kernels
     bool few;       // tiles of up to 16 pairs
@@ -85,19 +86,30 @@ __device__ __forceinline__ int h_pow(const Weights &w, int expert, int x_norm) {
 // further root of ffn below h's, 2^6 at 4096. Half of fp32's bytes: 32744 pairs of dim 2048, 643 -> 574 us of the whole.
 __device__ __forceinline__ int part_pow(const Weights &w, int expert, int x_norm) { return h_pow(w, expert, x_norm) - w.bound_down[expert]; }
 
+// pair / top: the inverse is above by less than top / 2^32 of itself, and pair * top < 2^32.
+__device__ __forceinline__ int row_of(const Call &c, int pair) { return c.top == 1 ? pair : (int)__umulhi((uint32_t)pair, c.top_inverse); }
+
 // Where element c of a row lies in the block layout.
 __device__ __forceinline__ int slot_of(int c) {
     const int r = c & 15, i = r & 3;
     return (c & ~31) + 8 * (r >> 2) + 4 * (c >> 4 & 1) + ((i & 1) << 1 | i >> 1);
 }
 
+// e^x, within 3 steps: v_exp_f32 of the product with log2 e, and what the product's rounding left.
+__device__ __forceinline__ float exp_of(float x) {
+    constexpr float kLog2e = 1.44269504f, kLow = 1.92596303e-8f, kLn2 = 0.693147181f;
+    const float t = x * kLog2e, e = __builtin_amdgcn_exp2f(t), rest = __builtin_fmaf(x, kLow, __builtin_fmaf(x, kLog2e, -t));
+    return fabsf(t) < 128.f ? __builtin_fmaf(e, rest * kLn2, e) : e;
+}
+
+// v_rcp_f32 is within a step; where it is 0 (g below -88) so is the result.
 __device__ __forceinline__ float activate(float g, int act) {
     if (act == 2) return g < 0.f ? 0.f : g;  // NaN stays NaN
     if (act == 1) {
         const float t = 0.7978845608028654f * (g + 0.044715f * g * g * g);
-        return g / (1.f + expf(-2.f * t));  // (1 + tanh t) / 2 = 1 / (1 + e^-2t)
+        return g * __builtin_amdgcn_rcpf(1.f + exp_of(-2.f * t));  // (1 + tanh t) / 2 = 1 / (1 + e^-2t)
     }
-    return g / (1.f + expf(-g));
+    return g * __builtin_amdgcn_rcpf(1.f + exp_of(-g));
 }
 
 // View of one expert's rows.

@@ -551,6 +551,7 @@ Call range(const Weights &w, const Call &all, int first, int rows) {
     c.weights = all.weights + (int64_t)first * c.top;
     c.rows = rows;
     c.pairs = rows * c.top;
+    c.top_inverse = (uint32_t)(((1ull << 32) + (uint64_t)c.top - 1) / (uint64_t)c.top);
     shape(w, &c);
     return c;
 }

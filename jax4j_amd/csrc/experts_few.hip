@@ -112,7 +112,7 @@ experts_few(Weights w, Call c) {
         const int r = (64 / XC) * wave + lane / XC, m = HL ? r & 7 : r;
         xchunk = (uint32_t)((lane % XC) ^ (r & 15));
         if (r < 16 && m < count) {
-            const int64_t at_row = (int64_t)(DOWN ? m : c.order[first + m] / c.top) * K + (HL && r >= 8 ? plane : 0);
+            const int64_t at_row = (int64_t)(DOWN ? m : row_of(c, c.order[first + m])) * K + (HL && r >= 8 ? plane : 0);
             xoff = (uint32_t)at_row * 2u + xchunk * 16u;
         }
     }
@@ -200,7 +200,7 @@ experts_few(Weights w, Call c) {
     for (int o = (int)threadIdx.x; o < COLS * kOut; o += kWaves * 64) {
         const int ct = o / kOut, i = o % kOut, q = i >> 4, col = 16 * (COLS * chunk + ct) + (i & 15);
         if (q >= count || col >= N) continue;
-        const int pair = c.order[first + q], token = pair / c.top, pow = h_pow(w, expert, c.x_norm[token]);
+        const int pair = c.order[first + q], token = row_of(c, pair), pow = h_pow(w, expert, c.x_norm[token]);
         if constexpr (DOWN) {
             c.part[((int64_t)split * c.pairs + pair) * N + col] = __builtin_ldexpf(value(ct, i) * c.weights[pair], -pow);  // the weight first: the product alone may not fit
         } else {

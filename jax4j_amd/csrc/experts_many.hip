@@ -64,15 +64,16 @@ struct Unit<Q8_0> {
     }
 };
 
-// fp16(fma(c, s, o)) of two codes, and with HL what that leaves.
+// fp16(fma(c, s, o)) of two codes, and with HL what that leaves; `minus` is -1 in a register, with which the subtraction and its
+// rounding are one v_fma_mix.
 template <bool HL>
-__device__ __forceinline__ void dequantize(uint32_t c, float s, float o, uint32_t &hi, uint32_t &lo) {
+__device__ __forceinline__ void dequantize(uint32_t c, float s, float o, float minus, uint32_t &hi, uint32_t &lo) {
     const h2 v = __builtin_bit_cast(h2, c);
     const float a = __builtin_fmaf((float)v.x, s, o), b = __builtin_fmaf((float)v.y, s, o);
     const h2 h = {(_Float16)a, (_Float16)b};
     hi = __builtin_bit_cast(uint32_t, h);
     if constexpr (HL) {
-        const h2 l = {(_Float16)(a - (float)h.x), (_Float16)(b - (float)h.y)};
+        const h2 l = {(_Float16)__builtin_fmaf((float)h.x, minus, a), (_Float16)__builtin_fmaf((float)h.y, minus, b)};
         lo = __builtin_bit_cast(uint32_t, l);
     }
 }
@@ -139,7 +140,7 @@ __device__ __forceinline__ void run(const Weights &w, const Call &c, const Tile 
     for (int j = 0; j < TM; j++) {
         const int row = 8 * (4 * j + wave) + (lane >> 3), chunk16 = (lane & 7) ^ ((row >> 1) & 7);
         uint32_t at = kOob;
-        if (row < count) at = (uint32_t)(DOWN ? row : c.order[first + row] / c.top) * (uint32_t)K * 2u + (uint32_t)chunk16 * 16u;
+        if (row < count) at = (uint32_t)(DOWN ? row : row_of(c, c.order[first + row])) * (uint32_t)K * 2u + (uint32_t)chunk16 * 16u;
         xoff[j] = at;
     }
     auto load_x = [&](int i, uint8_t *xb) __attribute__((always_inline)) {
@@ -200,6 +201,8 @@ __device__ __forceinline__ void run(const Weights &w, const Call &c, const Tile 
         }
         return c;
     };
+    float minus = -1.f;
+    asm("" : "+v"(minus));
     // Operand p of a block.
     auto operand = [&](const Block<FMT> &b, const Scale &c, int p, Operand<HL> &out) __attribute__((always_inline)) {
         uint32_t part[4];
@@ -227,7 +230,7 @@ __device__ __forceinline__ void run(const Weights &w, const Call &c, const Tile 
 #pragma unroll
         for (int k = 0; k < 4; k++) {
             uint32_t x = 0, y = 0;
-            dequantize<HL>(part[k], c.s[k >> 1], c.o[k >> 1], x, y);
+            dequantize<HL>(part[k], c.s[k >> 1], c.o[k >> 1], minus, x, y);
             hi[k] = x;
             lo[k] = y;
         }
@@ -247,6 +250,7 @@ __device__ __forceinline__ void run(const Weights &w, const Call &c, const Tile 
             if constexpr (HL) a[t].lo = *reinterpret_cast<const h8 *>(at + L::kPlane);
         }
     };
+    constexpr int kShadow = HL ? 6 : TM >= 4 ? 5 : TM == 3 ? 7 : TM == 2 ? 9 : 18;
     Block<FMT> blk[2][2];  // [stage parity][group]
     Scale sc[2][2];
     Operand<HL> b[2][2];   // of MFMA p and p + 1
@@ -287,6 +291,12 @@ __device__ __forceinline__ void run(const Weights &w, const Call &c, const Tile 
                 if (p < 3) operand(blk[cur][g], sc[cur][g], p + 1, b[(p + 1) & 1][g]);
                 else operand(blk[cur ^ 1][g], sc[cur ^ 1][g], 0, b[0][g]);
             }
+        }
+        // vector instructions in the shadow of every MFMA, rather than behind a run of them
+#pragma unroll
+        for (int k = 0; k < 8 * TM * (HL ? 3 : 1); k++) {
+            __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+            __builtin_amdgcn_sched_group_barrier(0x002, kShadow, 0);
         }
         // computed here, between the MFMAs, although the last stage does not use it
         asm volatile("" : "+v"(b[0][0].hi), "+v"(b[0][1].hi));
@@ -339,7 +349,7 @@ __device__ __forceinline__ void run(const Weights &w, const Call &c, const Tile 
 #pragma unroll
         for (int t = 0; t < TM; t++) {
             const int m = 32 * t + r32;
-            const int pair = c.order[first + (m < count ? m : 0)], token = pair / c.top, norm = c.x_norm[token];
+            const int pair = c.order[first + (m < count ? m : 0)], token = row_of(c, pair), norm = c.x_norm[token];
             const float weight = HL ? c.weights[pair] : 1.f;
             const int up = HL ? -h_pow(w, expert, norm) : part_pow(w, expert, norm) - h_pow(w, expert, norm);
 #pragma unroll
@@ -370,7 +380,7 @@ __device__ __forceinline__ void run(const Weights &w, const Call &c, const Tile 
     for (int t = 0; t < TM; t++) {
         const int m = 32 * t + r32;
         if (m >= count || n0 >= N) continue;
-        const int pair = c.order[first + m], token = pair / c.top, hp = h_pow(w, expert, c.x_norm[token]), e = -c.x_pow[token];
+        const int pair = c.order[first + m], token = row_of(c, pair), hp = h_pow(w, expert, c.x_norm[token]), e = -c.x_pow[token];
         _Float16 *const out = c.ha + (int64_t)(first + m) * N + n0;
         const int64_t lo = (int64_t)c.pairs * N;
 #pragma unroll

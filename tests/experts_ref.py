@@ -130,7 +130,7 @@ def experts(x, ids, weights, gate, up, down, act, kind, exact_weights):
     2^-40 of it; weights are exact, or rounded to 11 bits; a sum of K products in 32 bits, a rounding for each, and for each block's scale, its
     minimum and what a wave or split adds: K + K / 8 + 40 of them at most. The inner activations have 22 or 11 bits, below the normal range
     2^-25 at a power that takes their bound |x|^2 G U to 2^14; the activation and the product with up: the slope of an activation is at
-    most 1.13, expf within 2 steps, and five roundings more. For results in bf16 a pair's share is rounded to 11 bits, below the normal range
+    most 1.13, its exponential is within 3 half steps, its reciprocal 2, and three roundings more. For results in bf16 a pair's share is rounded to 11 bits, below the normal range
     2^-25 at a power that takes its bound |x|^2 G U D sqrt(ffn), rounded up by 2^5 at most, to 2^14."""
     t, top = ids.shape
     half = kind == "bf16"
