@@ -86,9 +86,11 @@ __device__ void order_pairs(const Weights &w, const Call &c, int e) {
     const int count = hist[e];
     auto tiles = [&](const Tiles &all, int first) {
         const int own = (count + all.rows - 1) / all.rows;
+        // of whole groups of 32 pairs (up to 16: a tile), as even as they can be
+        const int per = own && all.rows >= 32 ? ((count + own - 1) / own + 31) / 32 * 32 : all.rows;
         for (int i = t; i < own; i += kPlanThreads) {
-            const int left = count - i * all.rows;
-            all.tile[first + i] = Tile{e, before + i * all.rows, left < all.rows ? left : all.rows, 0};
+            const int left = count - i * per;
+            all.tile[first + i] = Tile{e, before + i * per, left < per ? left : per, 0};
         }
         if (e == w.experts - 1 && t == 0) all.count[0] = first + own;
     };

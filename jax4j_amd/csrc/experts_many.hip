@@ -2,7 +2,8 @@
 //
 // A workgroup of 4 waves has one tile of pairs; wave v has two groups of 32 rows of W, the same rows of gate and up or 64 rows of down,
 // for all pairs: 2 TM v_mfma_f32_32x32x16_f16 accumulators. Each x' operand read from LDS feeds two MFMAs, and the activation needs no
-// exchange. W is the first operand, so a lane holds 4 consecutive columns of the result for one pair. Two workgroups share a CU.
+// exchange. W is the first operand, so a lane holds 4 consecutive columns of the result for one pair. Two workgroups share a CU; or (TEAMS =
+// 2) one of two such teams has it alone, which share W, with half of the tile's pairs each.
 //
 // K advances in stages of two 32-blocks. Lane (r, h) = (lane % 32, lane / 32) has block h of the stage: of row r of W, which it
 // dequantizes, and of pair r's x'. MFMA p = 0..3 takes dword p of the codes and chunk p of the block layout. x' goes from
@@ -104,26 +105,33 @@ struct Lds {
     static constexpr int kPlane = 32 * TM * 128, kX = (HL ? 2 : 1) * kPlane;
 };
 
-// The tile's rows of x' as byte offsets from `base`, and where its results go.
-template <int FMT, bool HL, int TM, bool DOWN>
-__device__ __forceinline__ void run(const Weights &w, const Call &c, const Tile &tile, int chunk, uint8_t *xs0, uint8_t *xs1, uint8_t *ws0, uint8_t *ws1) {
+// The products of one team of 4 waves; first and count: its pairs of the tile.
+template <int FMT, bool HL, int TM, bool DOWN, int TEAMS>
+__device__ __forceinline__ void run(const Weights &w, const Call &c, int expert, int first, int count, int chunk, int team, uint8_t *xs0, uint8_t *xs1, uint8_t *ws0,
+                                    uint8_t *ws1, uint8_t *team_place) {
     using U = Unit<FMT>;
     using L = Lds<FMT, HL, TM>;
-    constexpr int WL = 2 * U::kLoads, XL = (HL ? 2 : 1) * TM, QR = U::QR;
-    const int expert = tile.expert, count = tile.count, first = tile.first;
-    const int lane = (int)threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+    constexpr int G = 2 / TEAMS, WL = G * U::kLoads,  // groups of W that a wave loads: its two, or one of the two it shares with the other team's
+                   XL = (HL ? 2 : 1) * TM, QR = U::QR;
+    const int lane = (int)threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6) & 3;
     const int r32 = lane & 31, h = lane >> 5;
     const int K = DOWN ? w.ffn : w.dim, N = DOWN ? w.dim : w.ffn, ns = K / 64, nsb = K / 256;
     // first row of W of each group
     const int n0 = DOWN ? 256 * chunk + 64 * wave : 128 * chunk + 32 * wave, n1 = DOWN ? n0 + 32 : n0;
-    U unit[2];
+    U unit[G];
     if constexpr (DOWN) {
         const QMat m = expert_of(w.down, FMT, expert, N);
-        unit[0].init(m, n0, 2 * wave, lane);
-        unit[1].init(m, n1, 2 * wave + 1, lane);
+#pragma unroll
+        for (int g = 0; g < G; g++) {
+            const int group = TEAMS == 2 ? team : g;
+            unit[g].init(m, group ? n1 : n0, 2 * wave + group, lane);
+        }
     } else {
-        unit[0].init(expert_of(w.gate, FMT, expert, N), n0, 2 * wave, lane);
-        unit[1].init(expert_of(w.up, FMT, expert, N), n1, 2 * wave + 1, lane);
+#pragma unroll
+        for (int g = 0; g < G; g++) {
+            const int group = TEAMS == 2 ? team : g;
+            unit[g].init(expert_of(group ? w.up : w.gate, FMT, expert, N), n0, 2 * wave + group, lane);
+        }
     }
     const int32_t *const pow0 = (DOWN ? w.down_pow : w.gate_pow) + (int64_t)expert * N, *const pow1 = (DOWN ? w.down_pow : w.up_pow) + (int64_t)expert * N;
     float power[2];
@@ -152,8 +160,8 @@ __device__ __forceinline__ void run(const Weights &w, const Call &c, const Tile 
         }
     };
     auto load_w = [&](int u, uint8_t *wb) __attribute__((always_inline)) {
-        unit[0].load(u, U::kStages * u < ns, wb);
-        unit[1].load(u, U::kStages * u < ns, wb);
+#pragma unroll
+        for (int g = 0; g < G; g++) unit[g].load(u, U::kStages * u < ns, wb);
     };
 
     auto read_block = [&](int j, int group, const uint8_t *wb, Block<FMT> &o) __attribute__((always_inline)) {
@@ -308,7 +316,8 @@ __device__ __forceinline__ void run(const Weights &w, const Call &c, const Tile 
     load_order();
     load_w(1, ws1);
     wait_vm_lgkm0<XL + WL>();
-    asm volatile("" ::: "memory");
+    if constexpr (TEAMS == 2) lds_barrier();  // half of its W came by the other team
+    else asm volatile("" ::: "memory");
 #pragma unroll
     for (int g = 0; g < 2; g++) {
         read_block(0, g, ws0, blk[0][g]);
@@ -332,6 +341,10 @@ __device__ __forceinline__ void run(const Weights &w, const Call &c, const Tile 
 #undef J4Q_STAGE
     __builtin_amdgcn_s_waitcnt(0);  // no LDS load outlives the workgroup
 
+    if (TEAMS == 2 && count == 0) {
+        if constexpr (DOWN) __syncthreads();
+        return;
+    }
     // Element v of acc[g][t]: row n + 8 (v / 4) + 4 h + v % 4 of the group, pair 32 t + r32.
     i32x4 p0[4], p1[4];
 #pragma unroll
@@ -343,8 +356,9 @@ __device__ __forceinline__ void run(const Weights &w, const Call &c, const Tile 
     if constexpr (DOWN) {
         // Through LDS, 32 pairs at a time, so that whole lines are stored: a pair's 64 columns of this wave are 8 chunks of 16 bytes of
         // fp16, or 16 of fp32; chunk k of pair p at k ^ (p % 8).
-        __syncthreads();  // all waves have read their W
-        uint8_t *const place = (wave < 2 ? ws0 : ws1) + (wave & 1) * 8192;
+        __syncthreads();  // all waves have read their W and x'
+        // 8 KiB a wave: in the buffers of W, of two teams in those of x'
+        uint8_t *const place = TEAMS == 2 ? team_place : (wave < 2 ? ws0 : ws1) + (wave & 1) * 8192;
         constexpr int C = HL ? 16 : 8;  // chunks of a pair
 #pragma unroll
         for (int t = 0; t < TM; t++) {
@@ -401,30 +415,35 @@ __device__ __forceinline__ void run(const Weights &w, const Call &c, const Tile 
 }
 
 // grid: tiles * chunks, rounded up to whole eighths; a chunk is 128 columns of the result (down: 256).
-template <int FMT, bool HL, int TM, bool DOWN>
-__global__ void __launch_bounds__(256, 2)
+template <int FMT, bool HL, int TM, bool DOWN, int TEAMS>
+__global__ void __launch_bounds__(256 * TEAMS, 2)
 experts_many(Weights w, Call c) {
     constexpr int kX = Lds<FMT, HL, TM>::kX, kW = Unit<FMT>::kBytes;
-    static_assert(4 * (kX + kW) <= 163840, "two workgroups' LDS");
-    static_assert(kW >= 16384, "two waves' results in a buffer of W");
-    __shared__ __attribute__((aligned(1024))) uint8_t xs0[kX], xs1[kX];
+    static_assert(2 * (TEAMS * kX + kW) * (2 / TEAMS) <= 163840, "a CU's LDS");
+    static_assert(TEAMS == 2 ? kX >= 16384 : kW >= 16384, "room for the waves' results");
+    // arrays of their own: what tells the compiler that a read of one need not wait for loads into another
+    __shared__ __attribute__((aligned(1024))) uint8_t xs0[TEAMS * kX], xs1[TEAMS * kX];
     __shared__ __attribute__((aligned(1024))) uint8_t ws0[kW], ws1[kW];
     const int N = DOWN ? w.dim : w.ffn, chunks = DOWN ? (N + 255) / 256 : (N + 127) / 128, tiles = (DOWN ? c.down : c.up).count[0];
     // Workgroup b runs on XCD b % 8, and each XCD takes a contiguous range, down groups of 4 tiles of pairs: most often of one
     // expert, whose rows of W they share in the XCD's L2.
     const int total = tiles * chunks, per = (total + 7) / 8, at = (int)(blockIdx.x % 8) * per + (int)(blockIdx.x / 8);
     if ((int)(blockIdx.x / 8) >= per || at >= total) return;
-    const int mg = at / (4 * chunks), gm = tiles - 4 * mg < 4 ? tiles - 4 * mg : 4, rem = at - 4 * mg * chunks;
-    Tile tile = (DOWN ? c.down : c.up).tile[4 * mg + rem % gm];
-    tile.expert = __builtin_amdgcn_readfirstlane(tile.expert);
-    tile.first = __builtin_amdgcn_readfirstlane(tile.first);
-    tile.count = __builtin_amdgcn_readfirstlane(tile.count);
-    // a tile of fewer pairs (every expert's last one) with as many groups of 32 as it has
-    const int groups = (tile.count + 31) / 32, chunk = rem / gm;
-    if (groups >= TM) run<FMT, HL, TM, DOWN>(w, c, tile, chunk, xs0, xs1, ws0, ws1);
-    else if (TM > 3 && groups == 3) run<FMT, HL, TM < 3 ? TM : 3, DOWN>(w, c, tile, chunk, xs0, xs1, ws0, ws1);
-    else if (TM > 2 && groups == 2) run<FMT, HL, TM < 2 ? TM : 2, DOWN>(w, c, tile, chunk, xs0, xs1, ws0, ws1);
-    else run<FMT, HL, 1, DOWN>(w, c, tile, chunk, xs0, xs1, ws0, ws1);
+    const int mg = at / (4 * chunks), gm = tiles - 4 * mg < 4 ? tiles - 4 * mg : 4, rem = at - 4 * mg * chunks, chunk = rem / gm;
+    const Tile tile = (DOWN ? c.down : c.up).tile[4 * mg + rem % gm];
+    const int expert = __builtin_amdgcn_readfirstlane(tile.expert), all = __builtin_amdgcn_readfirstlane(tile.count);
+    // the groups of 32 pairs, fewer in an expert's last tile, half of them for each team
+    const int team = TEAMS == 2 ? __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 8) : 0, groups = ((all + 31) / 32 + TEAMS - 1) / TEAMS;
+    const int skip = 32 * groups * team, first = __builtin_amdgcn_readfirstlane(tile.first) + skip;
+    const int left = all - skip < 0 ? 0 : all - skip, count = left < 32 * groups ? left : 32 * groups;
+    const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+    uint8_t *const place = (wave < 4 ? xs0 : xs1) + (wave & 3) * 8192;
+#define J4Q_RUN(T) run<FMT, HL, (TM < T ? TM : T), DOWN, TEAMS>(w, c, expert, first, count, chunk, team, xs0 + team * kX, xs1 + team * kX, ws0, ws1, place)
+    if (groups >= TM) J4Q_RUN(TM);
+    else if (TM > 3 && groups == 3) J4Q_RUN(3);
+    else if (TM > 2 && groups == 2) J4Q_RUN(2);
+    else J4Q_RUN(1);
+#undef J4Q_RUN
 }
 
 template <int FMT, bool DOWN>
@@ -435,21 +454,23 @@ hipError_t launch_type(const Weights &w, const Call &c, hipStream_t s) {
     if (total > 0xffffff) return hipErrorInvalidValue;
     const dim3 grid((unsigned)total);
     bool launched = false;
-#define J4Q_MANY(HL, TM)                                                \
-    if (c.half == !HL && tiles.rows == 32 * TM) {                       \
-        experts_many<FMT, HL, TM, DOWN><<<grid, 256, 0, s>>>(w, c);     \
-        launched = true;                                                \
+#define J4Q_MANY(HL, TM, TEAMS)                                                    \
+    if (c.half == !HL && tiles.rows == 32 * TM * TEAMS) {                          \
+        experts_many<FMT, HL, TM, DOWN, TEAMS><<<grid, 256 * TEAMS, 0, s>>>(w, c); \
+        launched = true;                                                           \
     }
-    J4Q_MANY(false, 1)
-    J4Q_MANY(false, 2)
+    J4Q_MANY(false, 1, 1)
+    J4Q_MANY(false, 2, 1)
     if constexpr (FMT == Q6_K) {
-        J4Q_MANY(false, 3)
+        J4Q_MANY(false, 3, 1)
     } else {
-        J4Q_MANY(false, 4)
+        J4Q_MANY(false, 4, 1)
     }
-    J4Q_MANY(true, 1)
-    if constexpr (FMT != Q6_K) {
-        J4Q_MANY(true, 2)
+    J4Q_MANY(true, 1, 1)
+    if constexpr (FMT == Q6_K) {
+        J4Q_MANY(true, 2, 2)
+    } else {
+        J4Q_MANY(true, 2, 1)
     }
 #undef J4Q_MANY
     if (!launched) return hipErrorInvalidValue;
@@ -458,9 +479,13 @@ hipError_t launch_type(const Weights &w, const Call &c, hipStream_t s) {
 
 }  // namespace
 
-// `each`: pairs per expert on average. The most pairs a tile with which two workgroups' LDS fit a CU.
+// `each`: pairs per expert on average. The most pairs a tile with which two workgroups' LDS fit a CU: they run out of phase, one's
+// MFMAs under the other's barriers (two teams in one workgroup of bf16, tiles of 256: 1737 -> 1916 us). With Q6_K and fp32 those are tiles
+// of 32, and two teams with 64 each are faster from some 200 pairs an expert on (8192 pairs of 32 experts, 2048 x 2048: 976 -> 850 us; 1024
+// of 8: 184 -> 195).
 int rows_many(int type, bool half, int each) {
-    if (each < 40 || (!half && type == Q6_K)) return 32;
+    if (!half && type == Q6_K) return each < 192 ? 32 : 128;
+    if (each < 40) return 32;
     if (each < 96 || !half) return 64;
     return type == Q6_K ? 96 : 128;
 }

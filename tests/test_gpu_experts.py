@@ -200,13 +200,13 @@ def test_a_row_does_not_depend_on_the_others(layer):
 
 @pytest.mark.parametrize("up,down", PAIRS)
 @pytest.mark.parametrize("kind", ["f32", "bf16"])
-@pytest.mark.parametrize("rows", [50, 200, 330])
+@pytest.mark.parametrize("rows", [50, 200, 410])
 def test_pairs_enough_for_each_size_of_tile(layer, up, down, kind, rows):
-    """25, 100 and 165 pairs an expert, on average, and one expert with a pair, one with 33, 65 and 97."""
+    """25, 100 and 205 pairs an expert, on average, and one expert with a pair, one with 33, 65 and 97."""
     l = layer(up, down, 6, 256, 256)
     x, ids, w = inputs(l, rows, 3, kind, seed=rows)
     check(l, x, ids, w, kind, apply(l, x, ids, w, kind))
-    if rows < 330:
+    if rows < 410:
         return
     for few in (1, 33, 65, 97):
         i = ids.copy()
