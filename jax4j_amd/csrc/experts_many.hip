@@ -31,16 +31,55 @@ using gw::wait_vm_lgkm0;
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef int32_t i32x4 __attribute__((ext_vector_type(4)));
 
-// W of 4 waves of two groups of 32 rows in LDS, a unit at a time: two stages.
+// W of 4 waves of two groups of 32 rows in LDS, a unit at a time: two stages. Of Q4_K and Q6_K the codes; the scales of a superblock of
+// four stages come with its first unit and lie apart, 16 bytes a row and Q6_K's d, once: a row's are read into registers before the
+// next ones arrive. (What costs is the lines that a load touches, and each of these touches one a row.)
 template <int FMT>
 struct Unit : gt::WUnit<FMT, 8> {
-    static constexpr int kStages = 2;
+    static constexpr int kStages = 2, kScales = 0;
 };
+template <int FMT>
+struct SuperUnit : gt::WUnit<FMT, 8> {
+    using Base = gt::WUnit<FMT, 8>;
+    static constexpr int kStages = 2, kLoads = Base::kLoads - (FMT == Q6_K ? 2 : 1), kBytes = Base::kS, kSlot = FMT == Q6_K ? 768 : 1024, kScales = 8 * kSlot;
+    uint32_t soff[FMT == Q6_K ? 2 : 1];
+    __device__ __forceinline__ void init(const QMat &w, int nw, int wave_, int lane) {
+        Base::init(w, nw, wave_, lane);
+        // Q4_K: lane r < 32: row r's 16 bytes (the other lanes write zeros behind). Q6_K, for which LDS is short: dword L % 4 of 16 rows, twice.
+#pragma unroll
+        for (int j = 0; j < (FMT == Q6_K ? 2 : 1); j++) {
+            const int n = nw + (FMT == Q6_K ? 16 * j + (lane >> 2) : lane);
+            soff[j] = (FMT == Q6_K || lane < 32) && n < (int)w.rows ? (uint32_t)n * (uint32_t)(w.cols / 16) + (FMT == Q6_K ? 4u * (uint32_t)(lane & 3) : 0u) : kOob;
+        }
+    }
+    __device__ __forceinline__ void load(int u, bool live, uint8_t *wb) const {
+        const uint32_t uu = live ? (uint32_t)u : 0u;
+#pragma unroll
+        for (int j = 0; j < Base::QL; j++) dma16(this->qr, wb + (this->wave * Base::QL + j) * 1024, live ? this->qoff[j] : kOob, uu * (uint32_t)Base::QR);
+        if constexpr (FMT == Q6_K) dma16(this->hr, wb + Base::kH + this->wave * 1024, live ? this->hoff : kOob, uu * 32u);
+    }
+    // The scales of unit u's superblock, u even.
+    __device__ __forceinline__ void load_scales(int u, bool live, uint8_t *scales) const {
+        uint8_t *const slot = scales + this->wave * kSlot;
+        const uint32_t sb = live ? (uint32_t)u >> 1 : 0u;
+        if constexpr (FMT == Q4_K) {
+            dma16(this->sr, slot, live ? soff[0] : kOob, sb * 16u);
+        } else {
+            gw::dma4s(this->sr, slot, live ? soff[0] : kOob, sb * 16u);
+            gw::dma4s(this->sr, slot + 256, live ? soff[1] : kOob, sb * 16u);
+            gw::dma4(this->sr, slot + 512, live && this->doff != kOob ? (this->doff + sb * 2u) & ~3u : kOob);
+        }
+    }
+};
+template <>
+struct Unit<Q4_K> : SuperUnit<Q4_K> {};
+template <>
+struct Unit<Q6_K> : SuperUnit<Q6_K> {};
 // Q8_0: one stage, 64 bytes of codes a row (chunk c of row r at slot c ^ ((r / 4) % 4)) and a dword of scales; units of two stages
 // would leave room for one workgroup a CU.
 template <>
 struct Unit<Q8_0> {
-    static constexpr int kStages = 1, QR = 64, QL = 2, kLoads = 3, kS = 8 * 32 * QR, kSlot = 256, kBytes = kS + 8 * kSlot;
+    static constexpr int kStages = 1, kScales = 0, QR = 64, QL = 2, kLoads = 3, kS = 8 * 32 * QR, kSlot = 256, kBytes = kS + 8 * kSlot;
     __amdgpu_buffer_rsrc_t qr, sr;
     uint32_t qoff[QL], soff;
     int wave;
@@ -93,7 +132,12 @@ template <int FMT>
 struct Block {
     u32x4 q[FMT == Q8_0 ? 2 : 1];
     u32x2 hi;
+    uint32_t s;
+};
+// The scales of a row's superblock.
+struct Super {
     u32x4 s;
+    uint32_t d;
 };
 struct Scale {
     float s[2], o[2];
@@ -108,10 +152,11 @@ struct Lds {
 // The products of one team of 4 waves; first and count: its pairs of the tile.
 template <int FMT, bool HL, int TM, bool DOWN, int TEAMS>
 __device__ __forceinline__ void run(const Weights &w, const Call &c, int expert, int first, int count, int chunk, int team, uint8_t *xs0, uint8_t *xs1, uint8_t *ws0,
-                                    uint8_t *ws1, uint8_t *team_place) {
+                                    uint8_t *ws1, uint8_t *scales, uint8_t *team_place) {
     using U = Unit<FMT>;
     using L = Lds<FMT, HL, TM>;
-    constexpr int G = 2 / TEAMS, WL = G * U::kLoads,  // groups of W that a wave loads: its two, or one of the two it shares with the other team's
+    constexpr bool super = U::kScales != 0;
+    constexpr int G = 2 / TEAMS, WL = G * U::kLoads, WS = WL + (FMT == Q4_K ? G : FMT == Q6_K ? 3 * G : 0),  // with scales; G: groups of W that a wave loads: its two, or one of the two it shares with the other team's
                    XL = (HL ? 2 : 1) * TM, QR = U::QR;
     const int lane = (int)threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6) & 3;
     const int r32 = lane & 31, h = lane >> 5;
@@ -163,45 +208,57 @@ __device__ __forceinline__ void run(const Weights &w, const Call &c, int expert,
 #pragma unroll
         for (int g = 0; g < G; g++) unit[g].load(u, U::kStages * u < ns, wb);
     };
+    auto load_scales = [&](int u) __attribute__((always_inline)) {
+        if constexpr (super) {
+#pragma unroll
+            for (int g = 0; g < G; g++) unit[g].load_scales(u, U::kStages * u < ns, scales);
+        }
+    };
+    Super sup[2];
+    auto read_super = [&](int group) __attribute__((always_inline)) {
+        const uint8_t *const slot = scales + (2 * wave + group) * U::kSlot;
+        sup[group].s = *reinterpret_cast<const u32x4 *>(slot + r32 * 16);
+        if constexpr (FMT == Q6_K) sup[group].d = *reinterpret_cast<const uint32_t *>(slot + 512 + r32 * 4);
+    };
 
     auto read_block = [&](int j, int group, const uint8_t *wb, Block<FMT> &o) __attribute__((always_inline)) {
         const int swz = U::swz(r32), blk = U::kStages == 2 ? 2 * (j & 1) + h : h, unit_row = 32 * (2 * wave + group) + r32;
-        const uint8_t *const row = wb + unit_row * QR, *const slot = wb + U::kS + (2 * wave + group) * U::kSlot;
+        const uint8_t *const row = wb + unit_row * QR;
 #pragma unroll
         for (int k = 0; k < (FMT == Q8_0 ? 2 : 1); k++) o.q[k] = *reinterpret_cast<const u32x4 *>(row + ((((FMT == Q8_0 ? 2 : 1) * blk + k) ^ swz) << 4));
-        if constexpr (FMT == Q4_K) o.s = *reinterpret_cast<const u32x4 *>(slot + r32 * 16);
-        else o.s[0] = *reinterpret_cast<const uint16_t *>(slot + r32 * (4 * U::kStages) + blk * 2);
-        if constexpr (FMT == Q6_K) {
-            o.hi = *reinterpret_cast<const u32x2 *>(wb + U::kH + unit_row * 32 + blk * 8);
-            o.s[1] = *reinterpret_cast<const uint32_t *>(slot + 256 + r32 * 4);
-        }
+        if constexpr (!super) o.s = *reinterpret_cast<const uint16_t *>(wb + U::kS + (2 * wave + group) * U::kSlot + r32 * (4 * U::kStages) + blk * 2);
+        if constexpr (FMT == Q6_K) o.hi = *reinterpret_cast<const u32x2 *>(wb + U::kH + unit_row * 32 + blk * 8);
     };
-    auto decode_scale = [&](int j, int group, const Block<FMT> &b) __attribute__((always_inline)) -> Scale {
+    // Of block j, the Q-th stage of its superblock.
+    auto decode_scale = [&](auto Q_, int j, int group, const Block<FMT> &b) __attribute__((always_inline)) -> Scale {
         constexpr float k24 = gt::kTwo24, k20 = gt::kTwo20;
+        constexpr int Q = decltype(Q_)::value;
         const float pw = power[group];
+        const Super &p = sup[group];
         Scale c;
         if constexpr (FMT == Q8_0) {
-            const float d = half_bits_to_float(b.s[0]) * pw;
+            const float d = half_bits_to_float(b.s) * pw;
             c.s[0] = c.s[1] = d * k24;
             c.o[0] = c.o[1] = -128.f * d;
         } else if constexpr (FMT == Q4_0) {
-            const float d = half_bits_to_float(b.s[0]) * pw;
+            const float d = half_bits_to_float(b.s) * pw;
             c.s[0] = d * k24;
             c.s[1] = d * k20;
             c.o[0] = c.o[1] = -8.f * d;
         } else if constexpr (FMT == Q4_K) {
-            const int jsb = 2 * (j & 3) + h;
-            const uint32_t sc = __builtin_amdgcn_ubfe(b.s[1], 4 * jsb, 4) | (__builtin_amdgcn_ubfe(b.s[3], 2 * jsb, 2) << 4);
-            const uint32_t mn = __builtin_amdgcn_ubfe(b.s[2], 4 * jsb, 4) | (__builtin_amdgcn_ubfe(b.s[3], 16 + 2 * jsb, 2) << 4);
-            const float d = half_bits_to_float(b.s[0] & 0xFFFFu) * pw * (float)sc;
+            const int jsb = 2 * Q + h;
+            const uint32_t sc = __builtin_amdgcn_ubfe(p.s[1], 4 * jsb, 4) | (__builtin_amdgcn_ubfe(p.s[3], 2 * jsb, 2) << 4);
+            const uint32_t mn = __builtin_amdgcn_ubfe(p.s[2], 4 * jsb, 4) | (__builtin_amdgcn_ubfe(p.s[3], 16 + 2 * jsb, 2) << 4);
+            const float d = half_bits_to_float(p.s[0] & 0xFFFFu) * pw * (float)sc;
             c.s[0] = d * k24;
             c.s[1] = d * k20;
-            c.o[0] = c.o[1] = -(half_bits_to_float(b.s[0] >> 16) * pw * (float)mn);
+            c.o[0] = c.o[1] = -(half_bits_to_float(p.s[0] >> 16) * pw * (float)mn);
         } else {
             const int n = (group ? n1 : n0) + r32;
             const uint32_t odd = ((uint32_t)n * (uint32_t)nsb + (uint32_t)(j >> 2)) & 1u;  // an expert's rows are a multiple of 64
-            const float d = half_bits_to_float(odd ? b.s[1] >> 16 : b.s[1] & 0xFFFFu) * pw;
-            const float da = d * (float)(int8_t)(b.s[0] & 0xFFu), db = d * (float)(int8_t)(b.s[0] >> 8);
+            const float d = half_bits_to_float(odd ? p.d >> 16 : p.d & 0xFFFFu) * pw;
+            const uint32_t two = h ? p.s[Q] >> 16 : p.s[Q];
+            const float da = d * (float)(int8_t)(two & 0xFFu), db = d * (float)(int8_t)(two >> 8 & 0xFFu);
             c.s[0] = da * k24;
             c.o[0] = -32.f * da;
             c.s[1] = db * k20;
@@ -265,26 +322,32 @@ __device__ __forceinline__ void run(const Weights &w, const Call &c, int expert,
     auto stage = [&](auto S_, int i) __attribute__((always_inline)) {
         constexpr int S = decltype(S_)::value, cur = S & 1;
         uint8_t *const xb = cur ? xs1 : xs0, *const xn = cur ? xs0 : xs1;
+        using Next = std::integral_constant<int, (S + 1) % 4>;
         constexpr bool pairs = U::kStages == 2;
         constexpr int ur = pairs ? (S + 1) / 2 % 2 : (S + 1) % 2, un = pairs ? (S + 3) / 2 % 2 : S % 2;
         uint8_t *const wc = ur ? ws1 : ws0, *const wn = un ? ws1 : ws0;
-        wait_vm_lgkm0<pairs && S % 2 == 0 ? WL : 0>();
+        wait_vm_lgkm0<!pairs || S % 2 ? 0 : S == 0 ? WL : WS>();  // the newest unit of W, at stage 2 with its scales, is under way
         lds_barrier();
         Operand<HL> a[2][TM];
         read_x(xb, 0, a[0]);
         read_block(i + 1, 0, wc, blk[cur ^ 1][0]);
         read_block(i + 1, 1, wc, blk[cur ^ 1][1]);
+        if constexpr (super && S == 3) {
+            read_super(0);
+            read_super(1);
+        }
         load_x(i + 1, xn);
         load_order();  // X first: the wait at an even stage leaves the newest unit of W outstanding
         if constexpr (!pairs) load_w(i + 2, wn);
         else if constexpr (S % 2 == 1) load_w((i + 3) / 2, wn);
+        if constexpr (S == 1) load_scales((i + 3) / 2);
         __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int p = 0; p < 4; p++) {
             if (p < 3) read_x(xb, p + 1, a[(p + 1) & 1]);
             if (p == 1) {
-                sc[cur ^ 1][0] = decode_scale(i + 1, 0, blk[cur ^ 1][0]);
-                sc[cur ^ 1][1] = decode_scale(i + 1, 1, blk[cur ^ 1][1]);
+                sc[cur ^ 1][0] = decode_scale(Next{}, i + 1, 0, blk[cur ^ 1][0]);
+                sc[cur ^ 1][1] = decode_scale(Next{}, i + 1, 1, blk[cur ^ 1][1]);
             }
 #pragma unroll
             for (int g = 0; g < 2; g++) {
@@ -311,6 +374,7 @@ __device__ __forceinline__ void run(const Weights &w, const Call &c, int expert,
     };
 
     load_w(0, ws0);
+    load_scales(0);
     load_order();
     load_x(0, xs0);
     load_order();
@@ -321,7 +385,8 @@ __device__ __forceinline__ void run(const Weights &w, const Call &c, int expert,
 #pragma unroll
     for (int g = 0; g < 2; g++) {
         read_block(0, g, ws0, blk[0][g]);
-        sc[0][g] = decode_scale(0, g, blk[0][g]);
+        if constexpr (super) read_super(g);
+        sc[0][g] = decode_scale(std::integral_constant<int, 0>{}, 0, g, blk[0][g]);
         operand(blk[0][g], sc[0][g], 0, b[0][g]);
     }
 #define J4Q_STAGE(S) stage(std::integral_constant<int, S>{}, i + S);
@@ -418,12 +483,13 @@ __device__ __forceinline__ void run(const Weights &w, const Call &c, int expert,
 template <int FMT, bool HL, int TM, bool DOWN, int TEAMS>
 __global__ void __launch_bounds__(256 * TEAMS, 2)
 experts_many(Weights w, Call c) {
-    constexpr int kX = Lds<FMT, HL, TM>::kX, kW = Unit<FMT>::kBytes;
-    static_assert(2 * (TEAMS * kX + kW) * (2 / TEAMS) <= 163840, "a CU's LDS");
+    constexpr int kX = Lds<FMT, HL, TM>::kX, kW = Unit<FMT>::kBytes, kS = Unit<FMT>::kScales;
+    static_assert((2 * (TEAMS * kX + kW) + kS) * (2 / TEAMS) <= 163840, "a CU's LDS");
     static_assert(TEAMS == 2 ? kX >= 16384 : kW >= 16384, "room for the waves' results");
     // arrays of their own: what tells the compiler that a read of one need not wait for loads into another
     __shared__ __attribute__((aligned(1024))) uint8_t xs0[TEAMS * kX], xs1[TEAMS * kX];
     __shared__ __attribute__((aligned(1024))) uint8_t ws0[kW], ws1[kW];
+    __shared__ __attribute__((aligned(1024))) uint8_t scales[kS ? kS : 16];
     const int N = DOWN ? w.dim : w.ffn, chunks = DOWN ? (N + 255) / 256 : (N + 127) / 128, tiles = (DOWN ? c.down : c.up).count[0];
     // Workgroup b runs on XCD b % 8, and each XCD takes a contiguous range, down groups of 4 tiles of pairs: most often of one
     // expert, whose rows of W they share in the XCD's L2.
@@ -438,7 +504,7 @@ experts_many(Weights w, Call c) {
     const int left = all - skip < 0 ? 0 : all - skip, count = left < 32 * groups ? left : 32 * groups;
     const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
     uint8_t *const place = (wave < 4 ? xs0 : xs1) + (wave & 3) * 8192;
-#define J4Q_RUN(T) run<FMT, HL, (TM < T ? TM : T), DOWN, TEAMS>(w, c, expert, first, count, chunk, team, xs0 + team * kX, xs1 + team * kX, ws0, ws1, place)
+#define J4Q_RUN(T) run<FMT, HL, (TM < T ? TM : T), DOWN, TEAMS>(w, c, expert, first, count, chunk, team, xs0 + team * kX, xs1 + team * kX, ws0, ws1, scales, place)
     if (groups >= TM) J4Q_RUN(TM);
     else if (TM > 3 && groups == 3) J4Q_RUN(3);
     else if (TM > 2 && groups == 2) J4Q_RUN(2);
