@@ -54,6 +54,11 @@ def _addresses(*ps) -> list:
     return [p if p is None else index(p) for p in ps]
 
 
+def _plain_addresses(*ps) -> list:
+    """The same, with 0 for None: what is checked together, and passed on, as plain integers."""
+    return [0 if p is None else index(p) for p in ps]
+
+
 def _int32(v) -> int:
     """A number as the library takes it: ctypes would hand over its low bits, whatever the others are."""
     v = index(v)
@@ -327,9 +332,10 @@ class Mi355xBackend:
         ``out_ptr``. Every part but one input and one output may be absent (0, None). ``gate``: [dim], or with ``gate_every`` a row
         for so many rows. Strides in values, 0: dim."""
         if not type(residual_ptr) is type(out_ptr) is type(block_ptr) is type(gate_ptr) is type(residual_out_ptr) is type(stream) is int:
-            residual_ptr, out_ptr, block_ptr, gate_ptr, residual_out_ptr, stream = _addresses(residual_ptr, out_ptr, block_ptr, gate_ptr, residual_out_ptr, stream)
-        if dim >> 31 or (rows | gate_every | residual_stride | block_stride | gate_stride | residual_out_stride | out_stride) >> 63:
-            raise IllegalArgumentException(f"norm_into: {rows} rows of {dim} values, or a stride, are negative or do not fit")
+            residual_ptr, out_ptr, block_ptr, gate_ptr, residual_out_ptr, stream = _plain_addresses(residual_ptr, out_ptr, block_ptr, gate_ptr, residual_out_ptr, stream)
+        if dim >> 31 or (rows | gate_every | residual_stride | block_stride | gate_stride | residual_out_stride | out_stride) >> 63 or (
+                residual_ptr | out_ptr | block_ptr | gate_ptr | residual_out_ptr | stream) >> 64:
+            raise IllegalArgumentException(f"norm_into: {rows} rows of {dim} values, a stride or an address are negative or do not fit")
         a = N.NormArgs(residual_ptr, block_ptr, gate_ptr, residual_out_ptr, out_ptr, rows, gate_every, residual_stride, block_stride, gate_stride,
                        residual_out_stride, out_stride, dim, _kind(residual_type), _kind(block_type), _kind(gate_type), _kind(out_type), scale,
                        after.ref if after else None, before.ref if before else None)
@@ -345,9 +351,10 @@ class Mi355xBackend:
         if s is None:
             raise IllegalArgumentException(f"unknown score {score!r} (softmax or sigmoid)")
         if not type(logits_ptr) is type(ids_ptr) is type(weights_ptr) is type(bias_ptr) is type(stream) is int:
-            logits_ptr, ids_ptr, weights_ptr, bias_ptr, stream = _addresses(logits_ptr, ids_ptr, weights_ptr, bias_ptr, stream)
-        if (experts | top_k | groups | top_groups | group_best) >> 31 or (rows | stride) >> 63:
-            raise IllegalArgumentException(f"route_into: {rows} rows, {top_k} of {experts} experts in {groups} groups")
+            logits_ptr, ids_ptr, weights_ptr, bias_ptr, stream = _plain_addresses(logits_ptr, ids_ptr, weights_ptr, bias_ptr, stream)
+        if (experts | top_k | groups | top_groups | group_best) >> 31 or (rows | stride) >> 63 or (
+                logits_ptr | ids_ptr | weights_ptr | bias_ptr) >> 64 or stream >> 64:
+            raise IllegalArgumentException(f"route_into: {rows} rows, {top_k} of {experts} experts in {groups} groups, or an address, do not fit")
         a = N.RouteArgs(logits_ptr, bias_ptr, ids_ptr, weights_ptr, rows, stride, _kind(dtype), experts, top_k, s, groups, top_groups, group_best,
                         int(bool(renormalize)), scale)
         check(self._lib().j4q_route_into(C.byref(a), stream), "route_into")

@@ -17,7 +17,7 @@ from __future__ import annotations
 import ctypes as C
 
 from . import _native as N
-from .backend import Mi355xBackend, _addresses, _int32, _int64, _kind, check
+from .backend import Mi355xBackend, _int32, _int64, _kind, _plain_addresses, check
 from .tensor import DeviceBuffer, DType, IllegalArgumentException
 
 _ACTIVATIONS = {"silu": N.ACT_SILU, "gelu": N.ACT_GELU, "relu": N.ACT_RELU}
@@ -31,7 +31,9 @@ class Norm:
         k = {"rms": N.NORM_RMS, "layer": N.NORM_LAYER}.get(kind)
         if k is None:
             raise IllegalArgumentException(f"unknown norm {kind!r} (rms or layer)")
-        w, b = _addresses(weight_ptr, bias_ptr)
+        w, b = _plain_addresses(weight_ptr, bias_ptr)
+        if (w | b) >> 64:
+            raise IllegalArgumentException("norm: an address does not fit 64 bits")
         self.args = N.NormKind(k, eps, w or None, b or None, weight_add)
         self.ref = C.pointer(self.args)
 
@@ -72,8 +74,8 @@ class Experts:
         expert's index). x and out [rows, dim], F32 or BF16; strides in values, 0: dim. ``workspace``: the caller's, for calls that are
         captured into a graph; 0: the engine's."""
         if not type(x_ptr) is type(ids_ptr) is type(weights_ptr) is type(out_ptr) is type(workspace_ptr) is type(stream) is int:
-            x_ptr, ids_ptr, weights_ptr, out_ptr, workspace_ptr, stream = _addresses(x_ptr, ids_ptr, weights_ptr, out_ptr, workspace_ptr, stream)
-        if top_k >> 31 or (rows | x_stride | out_stride) >> 63 or workspace_bytes >> 64:
-            raise IllegalArgumentException(f"experts apply: {rows} rows of {top_k} experts, or a stride, are negative or do not fit")
+            x_ptr, ids_ptr, weights_ptr, out_ptr, workspace_ptr, stream = _plain_addresses(x_ptr, ids_ptr, weights_ptr, out_ptr, workspace_ptr, stream)
+        if top_k >> 31 or (rows | x_stride | out_stride) >> 63 or (workspace_bytes | x_ptr | ids_ptr | weights_ptr | out_ptr | workspace_ptr | stream) >> 64:
+            raise IllegalArgumentException(f"experts apply: {rows} rows of {top_k} experts, a stride or an address are negative or do not fit")
         a = N.ExpertsArgs(x_ptr, ids_ptr, weights_ptr, out_ptr, rows, x_stride, out_stride, top_k, _kind(dtype), workspace_ptr, workspace_bytes)
         check(self._be._lib().j4q_experts_apply(self.handle, C.byref(a), stream), "experts apply")
