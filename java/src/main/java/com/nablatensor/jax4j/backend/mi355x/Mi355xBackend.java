@@ -74,6 +74,7 @@ public final class Mi355xBackend implements ComputeBackend, QuantizedOps {
   private static void drainPending() {
     Mi355xDecodePlan.drainPending();
     Mi355xKvCache.drainPending();
+    Mi355xExperts.drainPending();
     Mi355xBuffer.drainPending();
   }
 
@@ -273,6 +274,68 @@ public final class Mi355xBackend implements ComputeBackend, QuantizedOps {
     try (Arena a = Arena.ofConfined()) {
       Mi355xNative.call("rope", Mi355xNative.ROPE_INTO, MemorySegment.ofAddress(x), MemorySegment.ofAddress(out), Mi355xNative.KIND_F32, rows, heads,
           headDim, 0L, 0L, rope.segment(a), MemorySegment.NULL);
+    }
+  }
+
+  /** The matrices of a layer of experts (see {@link Mi355xExperts}); they stay the caller's. */
+  public Mi355xExperts experts(DeviceBuffer gate, DeviceBuffer up, DeviceBuffer down, int experts, Mi355xExperts.Activation activation) {
+    Mi355xBuffer g = quant(gate), u = quant(up), d = quant(down);
+    try (Arena a = Arena.ofConfined()) {
+      long h = newHandle("experts", Mi355xNative.EXPERTS_CREATE, Mi355xExperts.config(a, g.handle, u.handle, d.handle, experts, activation));
+      return new Mi355xExperts(h, List.of(g, u, d));
+    }
+  }
+
+  /**
+   * h = residual + scale * after(block), written to residualOut (the residual itself, or apart; 0: nowhere); out = before(h).
+   * F32 [rows, dim], dense, but with outBf16 out; block 0: none; after and before may be null, out 0 where before is. Device addresses.
+   */
+  public void norm(long residual, long block, Mi355xExperts.Norm after, float scale, long residualOut, Mi355xExperts.Norm before, long out,
+      boolean outBf16, long rows, int dim) {
+    ensureInitialized();
+    try (Arena a = Arena.ofConfined()) {
+      MemorySegment s = a.allocate(136, 8);  // without a gate; strides 0: dense
+      s.set(JAVA_LONG, 0, residual);
+      s.set(JAVA_LONG, 8, block);
+      s.set(JAVA_LONG, 24, residualOut);
+      s.set(JAVA_LONG, 32, out);
+      s.set(JAVA_LONG, 40, rows);
+      s.set(JAVA_INT, 96, dim);
+      s.set(JAVA_INT, 100, Mi355xNative.KIND_F32);
+      s.set(JAVA_INT, 104, Mi355xNative.KIND_F32);
+      s.set(JAVA_INT, 108, Mi355xNative.KIND_F32);
+      s.set(JAVA_INT, 112, outBf16 ? Mi355xNative.KIND_BF16 : Mi355xNative.KIND_F32);
+      s.set(JAVA_FLOAT, 116, scale);
+      s.set(JAVA_LONG, 120, after == null ? 0 : after.segment(a).address());
+      s.set(JAVA_LONG, 128, before == null ? 0 : before.segment(a).address());
+      Mi355xNative.call("norm", Mi355xNative.NORM_INTO, s, MemorySegment.NULL);
+    }
+  }
+
+  /**
+   * The topK experts of every row of logits F32 [rows, experts] into ids (int32) and weights (F32), [rows, topK]; softmax over all
+   * experts, or sigmoid scores with a bias (F32 [experts], 0: none) for the choice; groups 1: no groups. Device addresses.
+   */
+  public void route(long logits, long bias, boolean sigmoid, int groups, int topGroups, int groupBest, boolean renormalize, float scale, long ids,
+      long weights, long rows, int experts, int topK) {
+    ensureInitialized();
+    try (Arena a = Arena.ofConfined()) {
+      MemorySegment s = a.allocate(88, 8);
+      s.set(JAVA_LONG, 0, logits);
+      s.set(JAVA_LONG, 8, bias);
+      s.set(JAVA_LONG, 16, ids);
+      s.set(JAVA_LONG, 24, weights);
+      s.set(JAVA_LONG, 32, rows);
+      s.set(JAVA_INT, 48, Mi355xNative.KIND_F32);
+      s.set(JAVA_INT, 52, experts);
+      s.set(JAVA_INT, 56, topK);
+      s.set(JAVA_INT, 60, sigmoid ? Mi355xNative.ROUTE_SIGMOID : Mi355xNative.ROUTE_SOFTMAX);
+      s.set(JAVA_INT, 64, groups);
+      s.set(JAVA_INT, 68, topGroups);
+      s.set(JAVA_INT, 72, groupBest);
+      s.set(JAVA_INT, 76, renormalize ? 1 : 0);
+      s.set(JAVA_FLOAT, 80, scale);
+      Mi355xNative.call("route", Mi355xNative.ROUTE_INTO, s, MemorySegment.NULL);
     }
   }
 

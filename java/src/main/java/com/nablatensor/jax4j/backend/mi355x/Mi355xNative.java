@@ -29,6 +29,8 @@ final class Mi355xNative {
   static final int GEMV_MATRIX_CORES = 0, GEMV_FP32 = 1;
   /** Kinds of values in caller memory (enum j4q_kind). */
   static final int KIND_F32 = 2, KIND_BF16 = 3;
+  /** Norms (enum j4q_norm_kind) and scores of experts (enum j4q_route_score). */
+  static final int NORM_RMS = 1, NORM_LAYER = 2, ROUTE_SOFTMAX = 0, ROUTE_SIGMOID = 1;
   /** j4q_buffer_desc: 48 bytes; dims at 16 and 24, device_ptr at 40. */
   static final long BUFFER_DESC_BYTES = 48, DESC_DIM0 = 16, DESC_DIM1 = 24, DESC_DEVICE_PTR = 40;
 
@@ -114,6 +116,13 @@ final class Mi355xNative {
       FunctionDescriptor.of(JAVA_INT, JAVA_LONG, JAVA_INT, ADDRESS, ADDRESS, JAVA_LONG, JAVA_INT, ADDRESS, ADDRESS, ADDRESS));
   static final MethodHandle ROPE_INTO = fn("j4q_rope_into",
       FunctionDescriptor.of(JAVA_INT, ADDRESS, ADDRESS, JAVA_INT, JAVA_LONG, JAVA_INT, JAVA_INT, JAVA_LONG, JAVA_LONG, ADDRESS, ADDRESS));
+
+  // A block of experts (j4q_norm_into, j4q_route_into, j4q_experts_*): argument structs in host memory, the stream last.
+  static final MethodHandle NORM_INTO = fn("j4q_norm_into", FunctionDescriptor.of(JAVA_INT, ADDRESS, ADDRESS));
+  static final MethodHandle ROUTE_INTO = fn("j4q_route_into", FunctionDescriptor.of(JAVA_INT, ADDRESS, ADDRESS));
+  static final MethodHandle EXPERTS_CREATE = fn("j4q_experts_create", FunctionDescriptor.of(JAVA_INT, ADDRESS, ADDRESS));
+  static final MethodHandle EXPERTS_DESTROY = fn("j4q_experts_destroy", FunctionDescriptor.of(JAVA_INT, JAVA_LONG));
+  static final MethodHandle EXPERTS_APPLY = fn("j4q_experts_apply", FunctionDescriptor.of(JAVA_INT, JAVA_LONG, ADDRESS, ADDRESS));
 
   /** Status to the reference's exception types (HipRuntime.java:129-141; CpuBackend.java:698-714). */
   static void check(int status, String op) {
