@@ -26,9 +26,12 @@ namespace ex {
 using gmf::h2;
 using gmf::h4;
 using gmf::h8;
+using gemv::Chunk;
 using gemv::f32x4;
 using gemv::kOob;
 using gemv::make_rsrc;
+using gemv::Offs;
+using gemv::Rsrc;
 using gemv::u32x2;
 using gemv::u32x4;
 
@@ -129,6 +132,27 @@ __device__ __forceinline__ QMat expert_of(const QMat &m, int fmt, int e, int64_t
         break;
     }
     return o;
+}
+
+// Rows of W as whole waves read them, a lane the 32 columns of a chunk.
+// Byte offsets of chunk c of a row.
+template <int FMT>
+__device__ __forceinline__ Offs chunk_at(uint32_t c) {
+    switch (FMT) {
+    case Q4_0: return {16 * c, 0, 2 * c, 0};
+    case Q8_0: return {32 * c, 0, 2 * c, 0};
+    case Q4_K: return {16 * c, 0, (c >> 3) * 16, 0};
+    default: return {16 * c, 8 * c, 2 * c, (c >> 3) * 2};
+    }
+}
+// ... of a row of K columns.
+template <int FMT>
+__device__ __forceinline__ Offs row_bytes(uint32_t K) {
+    switch (FMT) {
+    case Q8_0: return {K, 0, K / 16, 0};
+    case Q6_K: return {K / 2, K / 4, K / 16, K / 128};
+    default: return {K / 2, 0, K / 16, 0};
+    }
 }
 
 // The products of every tile: of up to 16 pairs (fp32: 8), or of rows_many(), by the type of the matrix.

@@ -274,30 +274,94 @@ experts_combine(Weights w, Call c) {
 
 // ---- what is known of the weights -----------------------------------------------------------
 
-// Of rows [row0, row0 + gridDim.x) of a matrix, dequantized at v: max |w| 2^pow in [2^13, 2^14) and the exponent of the norm.
+// Largest magnitude and sum of squares of a chunk's 32 values. (Squares of weights lie within fp32 by the types alone: |w| < 2^26.)
+template <int FMT>
+__device__ __forceinline__ void chunk_stats(const Chunk<FMT> &c, int j, float &top, float &sum) {
+    uint32_t part[16];
+    float s[2], o[2];
+    if constexpr (FMT == Q8_0) {
+#pragma unroll
+        for (int p = 0; p < 8; p++) {
+            const uint32_t u = (p < 4 ? c.qa[p & 3] : c.qb[p & 3]) ^ 0x80808080u;
+            part[2 * p] = u & 0x00FF00FFu;
+            part[2 * p + 1] = u >> 8 & 0x00FF00FFu;
+        }
+        const float d = half_bits_to_float(c.d);
+        s[0] = s[1] = d * 0x1p24f;
+        o[0] = o[1] = -128.f * d;
+    } else {
+#pragma unroll
+        for (int p = 0; p < 4; p++) {
+            const uint32_t v = c.q[p], t = v >> 8;
+            part[2 * p] = v & 0x000F000Fu;
+            part[2 * p + 1] = t & 0x000F000Fu;
+            part[8 + 2 * p] = v & 0x00F000F0u;
+            part[9 + 2 * p] = t & 0x00F000F0u;
+            if constexpr (FMT == Q6_K) {
+                const uint32_t raw = c.h[p >> 1], hw = p & 1 ? __builtin_amdgcn_alignbit(raw, raw, 8) : raw, u = hw >> 2;
+                part[2 * p] |= hw & 0x00300030u;
+                part[2 * p + 1] |= u & 0x00300030u;
+                part[8 + 2 * p] |= hw & 0x03000300u;
+                part[9 + 2 * p] |= u & 0x03000300u;
+            }
+        }
+        if constexpr (FMT == Q4_0) {
+            const float d = half_bits_to_float(c.d);
+            s[0] = d * 0x1p24f;
+            s[1] = d * 0x1p20f;
+            o[0] = o[1] = -8.f * d;
+        } else if constexpr (FMT == Q4_K) {
+            const uint32_t sc = __builtin_amdgcn_ubfe(c.meta.y, 4 * j, 4) | (__builtin_amdgcn_ubfe(c.meta.w, 2 * j, 2) << 4);
+            const uint32_t mn = __builtin_amdgcn_ubfe(c.meta.z, 4 * j, 4) | (__builtin_amdgcn_ubfe(c.meta.w, 16 + 2 * j, 2) << 4);
+            const float d = half_bits_to_float(c.meta.x & 0xFFFFu) * (float)sc;
+            s[0] = d * 0x1p24f;
+            s[1] = d * 0x1p20f;
+            o[0] = o[1] = -(half_bits_to_float(c.meta.x >> 16) * (float)mn);
+        } else {
+            const float d = half_bits_to_float(c.d), da = d * (float)(int8_t)(c.s & 0xFFu), db = d * (float)(int8_t)(c.s >> 8 & 0xFFu);
+            s[0] = da * 0x1p24f;
+            s[1] = db * 0x1p20f;
+            o[0] = -32.f * da;
+            o[1] = -32.f * db;
+        }
+    }
+    top = sum = 0.f;
+#pragma unroll
+    for (int p = 0; p < 16; p++) {
+        const h2 v = __builtin_bit_cast(h2, part[p]);
+        const float a = __builtin_fmaf((float)v.x, s[p >> 3], o[p >> 3]), b = __builtin_fmaf((float)v.y, s[p >> 3], o[p >> 3]);
+        top = fmaxf(top, fmaxf(fabsf(a), fabsf(b)));
+        sum = __builtin_fmaf(a, a, __builtin_fmaf(b, b, sum));
+    }
+}
+
+// Of every row of a matrix of `experts` x rows: max |w| 2^pow in [2^13, 2^14) and the exponent of the norm. A wave per row, straight
+// from the codes: what it reads is what bounds it. grid: (rows / 4, experts).
+template <int FMT>
 __global__ void __launch_bounds__(256)
-row_stats(const float *__restrict__ v, int cols, int64_t row0, int32_t *__restrict__ pow, int32_t *__restrict__ norm) {
-    __shared__ float most[4];
-    __shared__ double squares[4];
-    const int t = (int)threadIdx.x;
-    const float *const row = v + (int64_t)blockIdx.x * cols;
+row_stats(QMat all, int rows, int32_t *__restrict__ pow, int32_t *__restrict__ norm) {
+    const int lane = (int)threadIdx.x & 63, row = __builtin_amdgcn_readfirstlane(4 * (int)blockIdx.x + ((int)threadIdx.x >> 6)), expert = (int)blockIdx.y;
+    if (row >= rows) return;
+    const Rsrc r = gemv::rsrc_of(expert_of(all, FMT, expert, rows), FMT);
+    const uint32_t K = (uint32_t)all.cols;
+    const Offs rb = row_bytes<FMT>(K), so{rb.qs * (uint32_t)row, rb.qh * (uint32_t)row, rb.sc * (uint32_t)row, rb.d * (uint32_t)row};
     float top = 0.f;
     double sum = 0.;
-    for (int i = t; i < cols; i += 256) {
-        top = fmaxf(top, fabsf(row[i]));
-        sum += (double)row[i] * (double)row[i];
+    for (uint32_t c = (uint32_t)lane; c < K / 32; c += 64) {
+        Chunk<FMT> v;
+        v.load(r, chunk_at<FMT>(c), so);
+        float t, q;
+        chunk_stats<FMT>(v, (int)(c & 7), t, q);
+        top = fmaxf(top, t);
+        sum += (double)q;
     }
 #pragma unroll
     for (int o = 32; o > 0; o /= 2) {
         top = fmaxf(top, __shfl_xor(top, o));
         sum += __shfl_xor(sum, o);
     }
-    if ((t & 63) == 0) most[t >> 6] = top, squares[t >> 6] = sum;
-    __syncthreads();
-    if (t) return;
+    if (lane) return;
     int p = 0, q = kNothing;
-    top = fmaxf(fmaxf(most[0], most[1]), fmaxf(most[2], most[3]));
-    sum = (squares[0] + squares[1]) + (squares[2] + squares[3]);
     if (top > 0.f && top <= 3.402823466e38f) {
         (void)frexpf(top, &p);
         p = 14 - p;
@@ -310,8 +374,8 @@ row_stats(const float *__restrict__ v, int cols, int64_t row0, int32_t *__restri
             q = 0;
         }
     }
-    pow[row0 + blockIdx.x] = p;
-    norm[row0 + blockIdx.x] = q;
+    pow[(int64_t)expert * rows + row] = p;
+    norm[(int64_t)expert * rows + row] = q;
 }
 
 // bound[e] = the largest of gate's exponents of expert e (of `rows` rows) + the largest of up's, or + add where there are none.
@@ -378,18 +442,17 @@ bool type_ok(int type, int64_t cols) {
     }
 }
 
-// The powers of a matrix's rows and the exponents of their norms. scratch: room for `chunk` dequantized rows.
-hipError_t stats(int type, const QMat &m, float *scratch, int64_t chunk, int32_t *pow, int32_t *norm, hipStream_t s) {
-    hipError_t e = hipSuccess;
-    for (int64_t r = 0; r < m.rows && e == hipSuccess; r += chunk) {
-        const int64_t n = m.rows - r < chunk ? m.rows - r : chunk;
-        e = launch_dequant_rows(type, m, r, n, scratch, s);
-        if (e == hipSuccess) {
-            row_stats<<<(unsigned)n, 256, 0, s>>>(scratch, (int)m.cols, r, pow, norm);
-            e = hipGetLastError();
-        }
+// The powers of a matrix's rows and the exponents of their norms, `rows` of each expert.
+hipError_t stats(int type, const QMat &m, int experts, int rows, int32_t *pow, int32_t *norm, hipStream_t s) {
+    const dim3 grid((unsigned)((rows + 3) / 4), (unsigned)experts);
+    switch (type) {
+    case Q8_0: row_stats<Q8_0><<<grid, 256, 0, s>>>(m, rows, pow, norm); break;
+    case Q4_0: row_stats<Q4_0><<<grid, 256, 0, s>>>(m, rows, pow, norm); break;
+    case Q4_K: row_stats<Q4_K><<<grid, 256, 0, s>>>(m, rows, pow, norm); break;
+    case Q6_K: row_stats<Q6_K><<<grid, 256, 0, s>>>(m, rows, pow, norm); break;
+    default: return hipErrorInvalidValue;
     }
-    return e;
+    return hipGetLastError();
 }
 
 int create(const j4q_experts_config &c, j4q_experts *out) {
@@ -415,45 +478,39 @@ int create(const j4q_experts_config &c, j4q_experts *out) {
     if (slot == g_experts.size()) g_experts.emplace_back(new Experts);
     Experts &k = *g_experts[slot];
     const uint64_t words = (uint64_t)(4 * E * ffn + 2 * E * dim + 2 * E);  // bounds; powers and norms of gate, up, down
-    const int64_t wide = dim > ffn ? dim : ffn, chunk = (16 << 20) / wide;
     void *dev = nullptr;
     hipError_t e = abi::malloc_locked(&dev, words * 4);
     if (e != hipSuccess) return report_hip("experts", e);
-    Workspace ws;
     const hipStream_t s = abi::stream();
-    e = abi::workspace_begin_locked(s, (uint64_t)(chunk * wide) * 4, &ws);
+    int32_t *const at = (int32_t *)dev;
+    k.w = Weights{};
+    k.w.gate = gate.m;
+    k.w.up = up.m;
+    k.w.down = down.m;
+    k.w.up_type = gate.qtype;
+    k.w.down_type = down.qtype;
+    k.w.experts = (int)E;
+    k.w.dim = (int)dim;
+    k.w.ffn = (int)ffn;
+    k.w.act = c.activation;
+    int32_t *const gate_pow = at + 2 * E, *const up_pow = gate_pow + E * ffn, *const gate_norm = up_pow + E * ffn, *const up_norm = gate_norm + E * ffn,
+                  *const down_pow = up_norm + E * ffn, *const down_norm = down_pow + E * dim;
+    int root = 0;  // 4^root >= ffn
+    while (1ll << (2 * root) < ffn) root++;
+    k.w.bound = at;
+    k.w.bound_down = at + E;
+    k.w.gate_pow = gate_pow;
+    k.w.up_pow = up_pow;
+    k.w.down_pow = down_pow;
+    e = stats(gate.qtype, gate.m, (int)E, (int)ffn, gate_pow, gate_norm, s);
+    if (e == hipSuccess) e = stats(up.qtype, up.m, (int)E, (int)ffn, up_pow, up_norm, s);
+    if (e == hipSuccess) e = stats(down.qtype, down.m, (int)E, (int)dim, down_pow, down_norm, s);
     if (e == hipSuccess) {
-        int32_t *const at = (int32_t *)dev;
-        k.w = Weights{};
-        k.w.gate = gate.m;
-        k.w.up = up.m;
-        k.w.down = down.m;
-        k.w.up_type = gate.qtype;
-        k.w.down_type = down.qtype;
-        k.w.experts = (int)E;
-        k.w.dim = (int)dim;
-        k.w.ffn = (int)ffn;
-        k.w.act = c.activation;
-        int32_t *const gate_pow = at + 2 * E, *const up_pow = gate_pow + E * ffn, *const gate_norm = up_pow + E * ffn, *const up_norm = gate_norm + E * ffn,
-                      *const down_pow = up_norm + E * ffn, *const down_norm = down_pow + E * dim;
-        int root = 0;  // 4^root >= ffn
-        while (1ll << (2 * root) < ffn) root++;
-        k.w.bound = at;
-        k.w.bound_down = at + E;
-        k.w.gate_pow = gate_pow;
-        k.w.up_pow = up_pow;
-        k.w.down_pow = down_pow;
-        e = stats(gate.qtype, gate.m, ws.ptr, chunk, gate_pow, gate_norm, s);
-        if (e == hipSuccess) e = stats(up.qtype, up.m, ws.ptr, chunk, up_pow, up_norm, s);
-        if (e == hipSuccess) e = stats(down.qtype, down.m, ws.ptr, chunk, down_pow, down_norm, s);
-        if (e == hipSuccess) {
-            expert_bound<<<(unsigned)E, 256, 0, s>>>(gate_norm, up_norm, 0, (int)ffn, at);
-            expert_bound<<<(unsigned)E, 256, 0, s>>>(down_norm, nullptr, root, (int)dim, at + E);
-            e = hipGetLastError();
-        }
-        abi::workspace_end_locked(s, ws, e == hipSuccess);
-        if (e == hipSuccess) e = hipStreamSynchronize(s);
+        expert_bound<<<(unsigned)E, 256, 0, s>>>(gate_norm, up_norm, 0, (int)ffn, at);
+        expert_bound<<<(unsigned)E, 256, 0, s>>>(down_norm, nullptr, root, (int)dim, at + E);
+        e = hipGetLastError();
     }
+    if (e == hipSuccess) e = hipStreamSynchronize(s);
     if (e != hipSuccess) {
         (void)hipFree(dev);
         return report_hip("experts", e);

@@ -14,10 +14,7 @@ namespace j4q {
 namespace ex {
 namespace {
 
-using gemv::Chunk;
 using gemv::f32x2;
-using gemv::Offs;
-using gemv::Rsrc;
 using gemv::XChunk;
 
 constexpr int kWaves = 8, kPairs = 2;  // rows of gate and of up a wave
@@ -36,26 +33,6 @@ __device__ __forceinline__ void get(const f32x4 *xs, const float *s16, int NP, i
 #pragma unroll
     for (int j = 0; j < 8; j++) x.v[j] = xs[j * NP + c];
     sums = reinterpret_cast<const f32x2 *>(s16)[c];
-}
-
-// Byte offsets of chunk c of a row.
-template <int FMT>
-__device__ __forceinline__ Offs chunk_at(uint32_t c) {
-    switch (FMT) {
-    case Q4_0: return {16 * c, 0, 2 * c, 0};
-    case Q8_0: return {32 * c, 0, 2 * c, 0};
-    case Q4_K: return {16 * c, 0, (c >> 3) * 16, 0};
-    default: return {16 * c, 8 * c, 2 * c, (c >> 3) * 2};
-    }
-}
-// ... of a row of K columns.
-template <int FMT>
-__device__ __forceinline__ Offs row_bytes(uint32_t K) {
-    switch (FMT) {
-    case Q8_0: return {K, 0, K / 16, 0};
-    case Q6_K: return {K / 2, K / 4, K / 16, K / 128};
-    default: return {K / 2, 0, K / 16, 0};
-    }
 }
 
 // grid: (ffn / 16, slots). NP >= dim / 32.
