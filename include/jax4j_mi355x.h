@@ -461,9 +461,9 @@ typedef struct j4q_route_args {
 int j4q_route_into(const j4q_route_args *args, void *stream);
 
 /* The matrices of a layer of experts: gate and up [experts * ffn, dim] of one type, down [experts * dim, ffn], expert after expert, as
- * j4q_gguf_upload gives GGUF's three-dimensional tensors. Types Q8_0 (columns a multiple of 64), Q4_0 (of 128), Q4_K and Q6_K. The
- * handle keeps the buffers from being released, and holds a power of two for each row and a bound for each expert, which
- * j4q_experts_create computes once. */
+ * j4q_gguf_upload gives GGUF's three-dimensional tensors. Types Q8_0 (columns a multiple of 64), Q4_0 (of 128), Q4_K and Q6_K; at
+ * most 65536 columns, and fewer than 2^31 values of an expert in a matrix. The handle keeps the buffers from being released, and holds
+ * a power of two for each row and two bounds for each expert, which j4q_experts_create computes once. */
 typedef uint64_t j4q_experts; /* 0 is never a valid handle */
 enum j4q_activation { J4Q_ACT_SILU = 0, J4Q_ACT_GELU = 1 /* the tanh form */, J4Q_ACT_RELU = 2 };
 typedef struct j4q_experts_config {

@@ -2,16 +2,17 @@
 // reference has no experts.
 //
 // What a row needs is small (a read of its logits); what it costs is the choice, so a team of 16 lanes has a row of up to 128
-// experts (four rows a wave) and of 64 lanes the others, each lane J experts l + L j in registers, and a choice is a maximum over the
-// lane's own keys and log2(L) exchanges. Keys are whole numbers in the order of the values they stand for, 0 where nothing may be
-// chosen:
-//  - without bias and groups the choice goes by the logits themselves: 32 bits of the logit above 32 of the index turned round,
-//    so that one maximum finds the largest and of equals the lowest index;
-//  - else by score + bias (or the logit) in 64 bits, where rounding cannot exchange two sums that 32 bits would not tell apart, and the
-//    index apart.
+// experts (four rows a wave) and of 64 lanes the others, each lane J experts l + L j in registers. Keys are whole numbers in the order
+// of the values they stand for, 0 where nothing may be chosen: without bias and groups the logits' own 32 bits, else 64 bits of score
+// + bias (or the logit), where rounding cannot exchange two sums that 32 bits would not tell apart. A choice is the maximum of the keys'
+// 32 bits (of 64: of the upper ones, then of the lower ones where the upper are that) and the lowest index that has it, each over the
+// lane's own and then over the team. Instructions bound it, and
+// where rows are few the chain of maxima: 8 of 128 experts, 16381 rows 7.8 us (9.8 with keys of 64 bits and exchanges through LDS), 8 of 256 in groups, 61
+// rows 9.3 (12.7).
 // Lane s of the team then has slot s, reads that expert's logit once more and computes its weight.
 #include "arguments.h"
 #include "engine.h"
+#include "teams.h"
 
 namespace j4q {
 namespace {
@@ -39,22 +40,6 @@ __device__ __forceinline__ uint64_t order64(double v) {
     return u >> 63 ? ~u : u | 0x8000000000000000ull;
 }
 __device__ __forceinline__ double unorder64(uint64_t k) { return __builtin_bit_cast(double, k >> 63 ? k & 0x7fffffffffffffffull : ~k); }
-
-template <int L, class T>
-__device__ __forceinline__ T team_max(T v) {
-#pragma unroll
-    for (int o = 1; o < L; o *= 2) {
-        const T w = __shfl_xor(v, o, L);
-        v = w > v ? w : v;
-    }
-    return v;
-}
-template <int L>
-__device__ __forceinline__ float team_sum(float v) {
-#pragma unroll
-    for (int o = 1; o < L; o *= 2) v += __shfl_xor(v, o, L);
-    return v;
-}
 
 __device__ __forceinline__ float logit_of(const RouteP &p, int64_t row, int i) {
     const uint8_t *const at = p.logits + row * p.stride;
@@ -87,7 +72,6 @@ route_kernel(RouteP p) {
     uint64_t key[J];
 #pragma unroll
     for (int j = 0; j < J; j++) {
-        const int i = t + L * j;
         if constexpr (WIDE) {
             double c = x[j];
             if (p.bias && x[j] > -kInf) {
@@ -96,7 +80,7 @@ route_kernel(RouteP p) {
             }
             key[j] = __builtin_bit_cast(uint64_t, c);
         } else {
-            key[j] = x[j] > -kInf ? (uint64_t)order32(x[j]) << 32 | (uint32_t)~i : 0;
+            key[j] = x[j] > -kInf ? (uint64_t)order32(x[j]) << 32 : 0;
         }
     }
     if constexpr (WIDE) {
@@ -105,8 +89,7 @@ route_kernel(RouteP p) {
             total = 0.;
 #pragma unroll
             for (int j = 0; j < J; j++) total += x[j] > -kInf ? __builtin_bit_cast(double, key[j]) : 0.;
-#pragma unroll
-            for (int o = 1; o < L; o *= 2) total += __shfl_xor(total, o, L);
+            total = team_sum<L>(total);
         }
 #pragma unroll
         for (int j = 0; j < J; j++) {
@@ -145,29 +128,35 @@ route_kernel(RouteP p) {
         }
     }
     // Slot s of the row goes to lane s.
+    uint32_t upper[J], lower[WIDE ? J : 1];
+#pragma unroll
+    for (int j = 0; j < J; j++) {
+        upper[j] = (uint32_t)(key[j] >> 32);
+        if constexpr (WIDE) lower[j] = (uint32_t)key[j];
+    }
     int mine = -1;
     for (int s = 0; s < p.top; s++) {
-        uint64_t best = 0;
-        int at = 0;
+        uint32_t best = 0, low = 0;
 #pragma unroll
-        for (int j = 0; j < J; j++)
-            if (key[j] > best) best = key[j], at = t + L * j;  // of equals the first: the lowest index of the lane
+        for (int j = 0; j < J; j++) best = upper[j] > best ? upper[j] : best;
+        best = team_max<L>(best);
+        if (best == 0) break;  // the same in the whole team; no key above 0 has upper bits of 0
         if constexpr (WIDE) {
 #pragma unroll
-            for (int o = 1; o < L; o *= 2) {
-                const uint64_t k = __shfl_xor(best, o, L);
-                const int i = __shfl_xor(at, o, L);
-                if (k > best || (k == best && i < at)) best = k, at = i;
-            }
-        } else {
-            best = team_max<L>(best);
-            at = (int)~(uint32_t)best;
+            for (int j = 0; j < J; j++) low = upper[j] == best && lower[j] > low ? lower[j] : low;
+            low = team_max<L>(low);
         }
-        if (best == 0) break;  // the same in the whole team
+        int at = L * J;
+#pragma unroll
+        for (int j = J - 1; j >= 0; j--) {
+            bool is = upper[j] == best;
+            if constexpr (WIDE) is = is && lower[j] == low;
+            at = is ? t + L * j : at;
+        }
+        at = team_min<L>(at);
         if (t == s) mine = at;
 #pragma unroll
-        for (int j = 0; j < J; j++)
-            if (t + L * j == at) key[j] = 0;
+        for (int j = 0; j < J; j++) upper[j] = t + L * j == at ? 0 : upper[j];
     }
     float w = 0.f, part = 0.f;
     const float own = mine >= 0 ? logit_of(p, row, mine) : -kInf;
