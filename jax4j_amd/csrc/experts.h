@@ -70,7 +70,7 @@ struct Call {
     int rows, top, pairs;
     uint32_t top_inverse;  // ceil(2^32 / top); not used for 1
     bool half;      // bf16 x and out; x' and h' have no lo part
-    bool one;       // a single row on its own kernels
+    bool one;       // a row, or very few, on their own kernels
     bool few;       // tiles of up to 16 pairs
     int splits;     // of down's K, whose partial results are added too
     Tiles up, down;
@@ -160,7 +160,7 @@ int rows_many(int type, bool half, int each);
 int splits_few(const Weights &w, int tiles);
 hipError_t launch_few(const Weights &w, const Call &c, bool down, hipStream_t s);
 hipError_t launch_many(const Weights &w, const Call &c, bool down, hipStream_t s);
-// All of a call of one row, whose c.part is [top][ffn]; `done` as launch_with_event takes it.
+// All of a call of very few rows, whose c.part is [pairs][ffn]; `done` as launch_with_event takes it.
 bool one_fits(const Weights &w, int top);
 hipError_t launch_one(const Weights &w, const Call &c, hipEvent_t done, hipStream_t s);
 

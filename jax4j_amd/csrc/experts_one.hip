@@ -1,13 +1,13 @@
-// One row (experts.h): the experts of a single token, in two launches, without an order of pairs and in fp32 throughout.
+// One row, or very few (experts.h): the experts of a token or three, in two launches, without an order of pairs and in fp32 throughout.
 //
 // A call of a few microseconds: what bounds it is what waits for what, and then the stream of W. As in the batch-1 GEMV (gemv_impl.h,
 // whose loads and dot products these are) a wave has whole rows of W, a lane the 32 columns of a chunk, so that its loads are
 // contiguous kilobytes, and x lies in LDS; the matrix cores, of whose 16 operand rows one row would use one, gain nothing here
-// (with them, 8 of 64 Q4_K / Q6_K experts 2048 x 1024: 8.5 and 12.9 us; this way 9.6 and 8.3, 16.9 a call). All weights of a wave are on their way before
-// it waits for x.
-//  - experts_one_up: a workgroup has a slot and 16 rows of gate and of up, a wave two of each.
-//  - experts_one_down: a wave has a row of the result for all slots, its chunks running over slots and ffn; h, times the slot's weight, lies in
-//    LDS. No partial results and no further launch.
+// (with them, 8 of 64 Q4_K / Q6_K experts 2048 x 1024: 8.5 and 12.9 us beside the launches around them; this way 9.3 and 8.3, 16.8 a
+// call). All weights of a wave are on their way before it waits for x.
+//  - experts_one_up: a workgroup has a pair and 16 rows of gate and of up, a wave two of each.
+//  - experts_one_down: a wave has a column of a row's result for all slots, its chunks running over slots and ffn; h, times the slot's
+//    weight, lies in LDS. No partial results and no further launch.
 #include "experts.h"
 
 namespace j4q {
@@ -35,7 +35,7 @@ __device__ __forceinline__ void get(const f32x4 *xs, const float *s16, int NP, i
     sums = reinterpret_cast<const f32x2 *>(s16)[c];
 }
 
-// grid: (ffn / 16, slots). NP >= dim / 32.
+// grid: (ffn / 16, pairs). NP >= dim / 32.
 template <int FMT, bool HALF, int NP>
 __global__ void __launch_bounds__(kWaves * 64)
 experts_one_up(Weights w, Call c, float *__restrict__ h) {
@@ -43,9 +43,9 @@ experts_one_up(Weights w, Call c, float *__restrict__ h) {
     __shared__ __attribute__((aligned(8))) float s16[2 * NP];
     constexpr int XU = (8 * NP + kWaves * 64 - 1) / (kWaves * 64);
     const int t = (int)threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6);
-    const int K = w.dim, N = w.ffn, chunks = K / 32, steps = (chunks + 63) / 64, slot = (int)blockIdx.y;
+    const int K = w.dim, N = w.ffn, chunks = K / 32, steps = (chunks + 63) / 64, pair = (int)blockIdx.y;
     // x first: its values come back before the weights'
-    const __amdgpu_buffer_rsrc_t xr = make_rsrc(c.x, (uint64_t)K * (HALF ? 2u : 4u));
+    const __amdgpu_buffer_rsrc_t xr = make_rsrc((const uint8_t *)c.x + (int64_t)row_of(c, pair) * c.x_stride * (HALF ? 2 : 4), (uint64_t)K * (HALF ? 2u : 4u));
     u32x4 x[XU];
 #pragma unroll
     for (int u = 0; u < XU; u++) {
@@ -57,7 +57,7 @@ experts_one_up(Weights w, Call c, float *__restrict__ h) {
             x[u] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(xr, i < (uint32_t)K / 4u ? 16u * i : kOob, 0, 0));
         }
     }
-    const int expert = __builtin_amdgcn_readfirstlane(c.ids[slot]);
+    const int expert = __builtin_amdgcn_readfirstlane(c.ids[pair]);
     if (expert < 0 || expert >= w.experts) return;  // the workgroup as one
     const Rsrc rs[2] = {gemv::rsrc_of(expert_of(w.gate, FMT, expert, N), FMT), gemv::rsrc_of(expert_of(w.up, FMT, expert, N), FMT)};
     Offs ln, rowb, stepb;
@@ -110,11 +110,11 @@ experts_one_up(Weights w, Call c, float *__restrict__ h) {
 #pragma unroll
     for (int p = 0; p < kPairs; p++) {
         const float a = gemv::wave_sum(acc[p][0]), b = gemv::wave_sum(acc[p][1]);
-        if (lane == 0) h[(int64_t)slot * N + row0 + p] = activate(a, w.act) * b;
+        if (lane == 0) h[(int64_t)pair * N + row0 + p] = activate(a, w.act) * b;
     }
 }
 
-// grid: dim / WAVES. Dynamic LDS: image() bytes; NP = slots * ffn / 32.
+// grid: (dim / WAVES, rows). Dynamic LDS: image() bytes; NP = slots * ffn / 32.
 template <int FMT, bool HALF, int WAVES>
 __global__ void __launch_bounds__(WAVES * 64)
 experts_one_down(Weights w, Call c, const float *__restrict__ h, int NP) {
@@ -123,7 +123,9 @@ experts_one_down(Weights w, Call c, const float *__restrict__ h, int NP) {
     float *const s16 = reinterpret_cast<float *>(xs + 8 * NP);
     const int t = (int)threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6);
     const int K = w.ffn, N = w.dim, per = K / 32, steps = (NP + 63) / 64;
-    if (t < c.top) ids[t] = c.ids[t];
+    const int64_t first_pair = (int64_t)blockIdx.y * c.top;
+    h += first_pair * K;
+    if (t < c.top) ids[t] = c.ids[first_pair + t];
     __syncthreads();
     const Rsrc rs = gemv::rsrc_of(w.down, FMT);
     const Offs rowb = row_bytes<FMT>((uint32_t)K);
@@ -148,7 +150,7 @@ experts_one_down(Weights w, Call c, const float *__restrict__ h, int NP) {
     for (int i0 = 0; i0 < 8 * NP; i0 += WAVES * 64) {
         const int i = i0 + t, slot = i < 8 * NP ? i / (K / 4) : 0, e = ids[slot];
         f32x4 v = {};
-        if (i < 8 * NP && e >= 0 && e < w.experts) v = reinterpret_cast<const f32x4 *>(h)[i] * c.weights[slot];
+        if (i < 8 * NP && e >= 0 && e < w.experts) v = reinterpret_cast<const f32x4 *>(h)[i] * c.weights[first_pair + slot];
         put(xs, s16, NP, i, 8 * NP, v);
     }
     __syncthreads();
@@ -168,15 +170,16 @@ experts_one_down(Weights w, Call c, const float *__restrict__ h, int NP) {
     }
     const float y = gemv::wave_sum(acc);
     if (lane) return;
-    if constexpr (HALF) ((uint16_t *)c.out)[row] = __builtin_bit_cast(uint16_t, (__bf16)y);
-    else ((float *)c.out)[row] = y;
+    const int64_t at = (int64_t)blockIdx.y * c.out_stride + row;
+    if constexpr (HALF) ((uint16_t *)c.out)[at] = __builtin_bit_cast(uint16_t, (__bf16)y);
+    else ((float *)c.out)[at] = y;
 }
 
 constexpr int64_t image(int64_t chunks) { return chunks * (8 * 16 + 8); }
 
 template <int FMT, bool HALF>
 hipError_t launch_up(const Weights &w, const Call &c, float *h, hipStream_t s) {
-    const dim3 grid((unsigned)(w.ffn / (kWaves * kPairs)), (unsigned)c.top);
+    const dim3 grid((unsigned)(w.ffn / (kWaves * kPairs)), (unsigned)c.pairs);
     if (w.dim <= 2048) experts_one_up<FMT, HALF, 64><<<grid, kWaves * 64, 0, s>>>(w, c, h);
     else if (w.dim <= 4096) experts_one_up<FMT, HALF, 128><<<grid, kWaves * 64, 0, s>>>(w, c, h);
     else experts_one_up<FMT, HALF, 256><<<grid, kWaves * 64, 0, s>>>(w, c, h);
@@ -188,11 +191,11 @@ template <int FMT, bool HALF>
 hipError_t launch_down(const Weights &w, const Call &c, const float *h, hipEvent_t done, hipStream_t s) {
     const int NP = c.top * (w.ffn / 32), lds = (int)image(NP);
     if (lds > 64 * 1024) {
-        if (done) hipExtLaunchKernelGGL((experts_one_down<FMT, HALF, 16>), dim3((unsigned)(w.dim / 16)), dim3(1024), lds, s, nullptr, done, 0, w, c, h, NP);
-        else experts_one_down<FMT, HALF, 16><<<(unsigned)(w.dim / 16), 1024, lds, s>>>(w, c, h, NP);
+        if (done) hipExtLaunchKernelGGL((experts_one_down<FMT, HALF, 16>), dim3((unsigned)(w.dim / 16), (unsigned)c.rows), dim3(1024), lds, s, nullptr, done, 0, w, c, h, NP);
+        else experts_one_down<FMT, HALF, 16><<<dim3((unsigned)(w.dim / 16), (unsigned)c.rows), 1024, lds, s>>>(w, c, h, NP);
     } else {
-        if (done) hipExtLaunchKernelGGL((experts_one_down<FMT, HALF, 8>), dim3((unsigned)(w.dim / 8)), dim3(512), lds, s, nullptr, done, 0, w, c, h, NP);
-        else experts_one_down<FMT, HALF, 8><<<(unsigned)(w.dim / 8), 512, lds, s>>>(w, c, h, NP);
+        if (done) hipExtLaunchKernelGGL((experts_one_down<FMT, HALF, 8>), dim3((unsigned)(w.dim / 8), (unsigned)c.rows), dim3(512), lds, s, nullptr, done, 0, w, c, h, NP);
+        else experts_one_down<FMT, HALF, 8><<<dim3((unsigned)(w.dim / 8), (unsigned)c.rows), 512, lds, s>>>(w, c, h, NP);
     }
     return hipGetLastError();
 }

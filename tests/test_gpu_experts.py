@@ -225,6 +225,21 @@ def test_a_row_of_more_than_the_kernel_of_one_holds(layer, kind):
     check(l, x, ids, w, kind, apply(l, x, ids, w, kind))
 
 
+@pytest.mark.parametrize("up,down", PAIRS)
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+def test_few_rows_of_many_experts(layer, up, down, kind):
+    """Up to three rows with few pairs take the kernels of one row: as each row alone, bit for bit."""
+    l = layer(up, down, 16, 512, 256)
+    for rows, top in ((2, 4), (3, 2)):
+        x, ids, w = inputs(l, rows, top, kind, seed=rows)
+        ids[1] = ids[0]
+        ids[-1, 0] = -1
+        got = apply(l, x, ids, w, kind, x_stride=520, out_stride=528)
+        check(l, x, ids, w, kind, got)
+        for r in range(rows):
+            assert np.array_equal(got[r:r + 1], apply(l, x[r:r + 1], ids[r:r + 1], w[r:r + 1], kind))
+
+
 def some_rows(l, x, ids, w, kind, got, rows):
     check(l, x[rows].cpu(), ids[rows], w[rows], kind, got[rows])
 
