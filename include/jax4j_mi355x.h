@@ -496,9 +496,10 @@ int j4q_experts_destroy(j4q_experts experts);
 int j4q_experts_info(j4q_experts experts, j4q_experts_desc *out);
 /* out[r] = sum over the slots s of a row of weights[r][s] * down_e (act(gate_e x_r) * (up_e x_r)), e = ids[r][s]; a row without experts is
  * zeros, the same expert twice counts twice. fp32: as j4q_quant_matvec_into's batches, x and the inner activations in 22 bits, weights as
- * they are or in 22 bits, sums in 32. bf16: the inner activations in 11 bits, and in a prompt the weights too. A row of x with a value
- * that is not finite gives a row of NaN where it has an expert. Bit for bit the same on every call with the same arguments. The engine's
- * workspace is as j4q_quant_matvec_into's: under stream capture two memory nodes, which a caller's own workspace saves. */
+ * they are or in 22 bits, sums in 32 (up to three rows all in 32). bf16: the inner activations in 11 bits, and in a prompt the weights
+ * and each expert's share of a result too. A row of x with a value that is not finite gives a row of NaN where it has an expert. Bit for
+ * bit the same on every call with the same arguments. The engine's workspace is as j4q_quant_matvec_into's: under stream capture two
+ * memory nodes, which a caller's own workspace saves. */
 int j4q_experts_apply(j4q_experts experts, const j4q_experts_args *args, void *stream);
 /* Bytes of workspace that a call of so many rows takes. */
 int j4q_experts_workspace(j4q_experts experts, int64_t rows, int32_t top_k, int type, uint64_t *bytes);
