@@ -491,7 +491,7 @@ typedef struct j4q_experts_args {
 } j4q_experts_args;
 /* Waits for the device. */
 int j4q_experts_create(const j4q_experts_config *config, j4q_experts *out);
-/* Waits for the device. 0 is a no-op. */
+/* Waits for the device. 0 is a no-op. A graph that captured calls of these experts is not replayed afterwards. */
 int j4q_experts_destroy(j4q_experts experts);
 int j4q_experts_info(j4q_experts experts, j4q_experts_desc *out);
 /* out[r] = sum over the slots s of a row of weights[r][s] * down_e (act(gate_e x_r) * (up_e x_r)), e = ids[r][s]; a row without experts is

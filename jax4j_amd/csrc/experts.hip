@@ -653,7 +653,7 @@ int apply(const Experts &k, const j4q_experts_args &a, hipStream_t s) {
     c.half = a.type == J4Q_KIND_BF16;
     const int64_t e = dense_size(a.type), dim = k.w.dim;
     for (int64_t st : {c.x_stride, c.out_stride})
-        if (st < dim || st > 1ll << 40 || st * e % 16) return report_error(J4Q_EINVAL, "experts apply: rows of %lld values %lld apart, a multiple of 16 bytes", (long long)dim, (long long)st);
+        if (st < dim || st > 1ll << 36 || st * e % 16) return report_error(J4Q_EINVAL, "experts apply: rows of %lld values %lld apart, a multiple of 16 bytes", (long long)dim, (long long)st);
     if (!aligned(a.x, 16) || !aligned(a.out, 16) || !aligned(a.ids, 4) || !aligned(a.weights, 4))
         return report_error(J4Q_EINVAL, "experts apply: x and out must be 16-byte aligned, ids and weights 4-byte aligned");
     const uint64_t out_bytes = (uint64_t)(((c.rows - 1) * c.out_stride + dim) * e), x_bytes = (uint64_t)(((c.rows - 1) * c.x_stride + dim) * e),

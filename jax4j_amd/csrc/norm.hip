@@ -6,8 +6,8 @@
 // 256 or 1024 threads has a row, 8 values a thread and pass: 16 bytes of bf16, or twice 16 of fp32, where addresses and strides
 // allow, else value after value across the team. Sums of values and squares are in 64 bits: they neither overflow nor lose
 // what a mean far from 0 hides, and cost nothing beside the memory. 16381 rows of 4096, a norm on either side of the residual and a gate:
-// 163 us, 5.0 TB/s. Few rows wait for their sums, so these take no LDS within a wave and no division (1021 rows of 1152, two norms with
-// means: 8.8 us with them, 7.5 without; all loads of a row ahead of its first sum: no faster).
+// 162 us, 5.0 TB/s. Few rows wait for their sums, so these take no LDS within a wave and no division (1021 rows of 1152, two norms with
+// means: 8.8 us with them, 7.6 without; all loads of a row ahead of its first sum: no faster).
 #include "arguments.h"
 #include "engine.h"
 #include "teams.h"
@@ -141,7 +141,7 @@ __device__ __forceinline__ double row_sum(double v, double *slot, int t) {
 }
 
 template <int T, int C, bool VEC>
-__device__ __forceinline__ void apply(const NormK &k, f32x8 (&x)[C], double *slot, int t, int dim, double inv_dim) {
+__device__ __forceinline__ void apply(const NormK &k, f32x8 (&x)[C], Raw (&w)[C], Raw (&b)[C], double *slot, int t, int dim, double inv_dim) {
     double mean = 0;
     if (k.kind == J4Q_NORM_LAYER) {
 #pragma unroll
@@ -149,7 +149,9 @@ __device__ __forceinline__ void apply(const NormK &k, f32x8 (&x)[C], double *slo
 #pragma unroll
             for (int j = 0; j < 8; j++)
                 if (At<T, VEC>::of(t, c, j) < dim) mean += (double)x[c][j];
-        mean = row_sum<T>(mean, slot, t) * inv_dim;
+        mean = row_sum<T>(mean, slot, t);
+        const double near = mean * inv_dim;
+        mean = fma(fma(-near, (double)dim, mean), inv_dim, near);  // the quotient itself where it is exact: rows of equal values have no rest
     }
     double sum = 0;
 #pragma unroll
@@ -164,17 +166,18 @@ __device__ __forceinline__ void apply(const NormK &k, f32x8 (&x)[C], double *slo
     const float inv = inverse_root(fma(row_sum<T>(sum, slot, t), inv_dim, (double)k.eps));
 #pragma unroll
     for (int c = 0; c < C; c++) {
-        Raw w, b;
-        if (k.weight) load<T, VEC>(w, (const uint8_t *)k.weight, false, t, c, dim);
-        if (k.bias) load<T, VEC>(b, (const uint8_t *)k.bias, false, t, c, dim);
+        if (k.weight) load<T, VEC>(w[c], (const uint8_t *)k.weight, false, t, c, dim);
+        if (k.bias) load<T, VEC>(b[c], (const uint8_t *)k.bias, false, t, c, dim);
+    }
+#pragma unroll
+    for (int c = 0; c < C; c++)
 #pragma unroll
         for (int j = 0; j < 8; j++) {
             float v = x[c][j] * inv;
-            if (k.weight) v *= as_float(w.v[j >> 2][j & 3]) + k.add;
-            if (k.bias) v += as_float(b.v[j >> 2][j & 3]);
+            if (k.weight) v *= as_float(w[c].v[j >> 2][j & 3]) + k.add;
+            if (k.bias) v += as_float(b[c].v[j >> 2][j & 3]);
             x[c][j] = v;
         }
-    }
 }
 
 // G teams of T threads a workgroup, a row each; C passes of 8 T values.
@@ -186,7 +189,9 @@ norm_kernel(NormP p) {
     const int t = (int)threadIdx.x % T;
     const int64_t row = ((int64_t)blockIdx.y * gridDim.x + blockIdx.x) * G + threadIdx.x / T;
     if (row >= p.rows) return;  // teams of more than a wave have a workgroup each: whole workgroups leave
-    Raw res[C], blk[C];
+    const uint8_t *const g = p.gate + (p.gate_every ? (uint32_t)row / p.gate_every : 0) * p.gate_stride;
+    // Registers of each part's own, which the compiler then loads a pass ahead (16381 rows of 4096: 165 -> 162 us).
+    Raw res[C], blk[C], gate[C], w[2][C], b[2][C];
     if (p.block) {
 #pragma unroll
         for (int c = 0; c < C; c++) load<T, VEC>(blk[c], p.block + row * p.block_stride, p.block16, t, c, p.dim);
@@ -199,14 +204,12 @@ norm_kernel(NormP p) {
     if (p.block) {
 #pragma unroll
         for (int c = 0; c < C; c++) x[c] = values<VEC>(blk[c], p.block16);
-        if (p.after.kind) apply<T, C, VEC>(p.after, x, slots, t, p.dim, p.inv_dim);
+        if (p.after.kind) apply<T, C, VEC>(p.after, x, w[0], b[0], slots, t, p.dim, p.inv_dim);
         if (p.gate) {
-            const uint8_t *const g = p.gate + (p.gate_every ? (uint32_t)row / p.gate_every : 0) * p.gate_stride;
 #pragma unroll
             for (int c = 0; c < C; c++) {
-                Raw r;
-                load<T, VEC>(r, g, p.gate16, t, c, p.dim);
-                x[c] *= values<VEC>(r, p.gate16);
+                load<T, VEC>(gate[c], g, p.gate16, t, c, p.dim);
+                x[c] *= values<VEC>(gate[c], p.gate16);
             }
         }
 #pragma unroll
@@ -224,7 +227,7 @@ norm_kernel(NormP p) {
         for (int c = 0; c < C; c++) store<T, VEC>(x[c], p.residual_out + row * p.residual_out_stride, p.residual16, t, c, p.dim);
     }
     if (!p.before.kind) return;
-    apply<T, C, VEC>(p.before, x, slots, t, p.dim, p.inv_dim);
+    apply<T, C, VEC>(p.before, x, w[1], b[1], slots, t, p.dim, p.inv_dim);
 #pragma unroll
     for (int c = 0; c < C; c++) store<T, VEC>(x[c], p.out + row * p.out_stride, p.out16, t, c, p.dim);
 }

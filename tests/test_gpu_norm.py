@@ -172,3 +172,15 @@ def test_refusals_leave_memory_alone(backend):
         backend.norm_into(x.data_ptr(), x.data_ptr() + 64, 4, 64, Norm())
     with pytest.raises(IllegalArgumentException, match="together"):
         backend.norm_into(x.data_ptr(), x.data_ptr() + 1024, 4, 64)
+
+
+@pytest.mark.parametrize("dim", [7, 48, 100, 1000, 1152, 3000, 5001])
+def test_rows_of_equal_values(backend, dim):
+    """Less their mean nothing is left, whatever dim is, with an eps far below what a mean off in its last bit would leave."""
+    value = torch.tensor([[0.1], [1e6 / 3], [-7e-20], [3e30]], dtype=torch.float32)
+    x = value.expand(4, dim).contiguous().cuda()
+    out = torch.full((4, dim), 5.0, device="cuda")
+    torch.cuda.synchronize()
+    backend.norm_into(x.data_ptr(), out.data_ptr(), 4, dim, Norm(kind="layer", eps=1e-30))
+    torch.cuda.synchronize()
+    assert (out == 0).all()
