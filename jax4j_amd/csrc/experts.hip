@@ -11,6 +11,7 @@
 #include "engine.h"
 #include "experts.h"
 #include "kept_memory.h"
+#include "teams.h"
 
 namespace j4q {
 namespace ex {
@@ -125,12 +126,18 @@ __device__ void order_pairs(const Weights &w, const Call &c, int e) {
     }
 }
 
-// Row r of x as x' in the block layout, its power and its norm's exponent.
-__device__ void convert_row(const Weights &w, const Call &c, int r) {
+// The waves of a team that has a row, so that a lane's values are 4 passes of 8 at most where that can be.
+__host__ __device__ inline int row_waves(int K) { return K <= 2048 ? 1 : K <= 4096 ? 2 : K <= 8192 ? 4 : 8; }
+
+// Rows of x as x' in the block layout, their powers and their norms' exponents; 8 / row_waves() of them. Read once, up to 16384
+// columns (a workgroup a row, and each read twice: 509 rows of 2048 in fp32 1.5 us more of 175).
+__device__ void convert_rows(const Weights &w, const Call &c, int block) {
     __shared__ float most[kPlanThreads / 64], squares[kPlanThreads / 64];
-    const int t = (int)threadIdx.x, K = w.dim;
+    static_assert(kPlanThreads == 512, "8 waves");
+    const int K = w.dim, W = row_waves(K), lane = (int)threadIdx.x & 63, wave = (int)threadIdx.x >> 6, t = wave % W * 64 + lane, T = 64 * W;
+    const int row = block * (8 / W) + wave / W, chunks = row < c.rows ? K / 8 : 0, r = row < c.rows ? row : 0;
     const uint8_t *const x = (const uint8_t *)c.x + (int64_t)r * c.x_stride * (c.half ? 2 : 4);
-    // thread t and pass p: the 8 elements of chunk g = i % 4 of block i / 4, i = t + threads * p
+    // thread t and pass p: the 8 elements of chunk g = i % 4 of block i / 4, i = t + T p
     auto load = [&](int i, float (&v)[8]) __attribute__((always_inline)) {
         const int at = (i >> 2) * 32 + 4 * (i & 3);
         if (c.half) {
@@ -150,22 +157,35 @@ __device__ void convert_row(const Weights &w, const Call &c, int r) {
     };
     float top = 0.f;
     bool finite = true;
-    for (int i = t; i < K / 8; i += kPlanThreads) {
-        float v[8];
-        load(i, v);
+    auto look = [&](const float (&v)[8]) __attribute__((always_inline)) {
 #pragma unroll
         for (int j = 0; j < 8; j++) {
             top = fmaxf(top, fabsf(v[j]));
             finite &= fabsf(v[j]) <= 3.402823466e38f;
         }
+    };
+    float held[4][8];
+    const bool holds = K <= 2048 * W;
+    if (holds) {
+#pragma unroll
+        for (int p = 0; p < 4; p++)
+            if (t + T * p < chunks) load(t + T * p, held[p]);
+#pragma unroll
+        for (int p = 0; p < 4; p++)
+            if (t + T * p < chunks) look(held[p]);
+    } else {
+        for (int i = t; i < chunks; i += T) {
+            float v[8];
+            load(i, v);
+            look(v);
+        }
     }
-    top = finite ? top : __builtin_inff();
-#pragma unroll
-    for (int o = 32; o > 0; o /= 2) top = fmaxf(top, __shfl_xor(top, o));
-    if ((t & 63) == 0) most[t >> 6] = top;
-    __syncthreads();
-#pragma unroll
-    for (int v = 0; v < kPlanThreads / 64; v++) top = fmaxf(top, most[v]);
+    top = team_max<64>(finite ? top : __builtin_inff());
+    if (W > 1) {
+        if (lane == 0) most[wave] = top;
+        __syncthreads();
+        for (int v = 0; v < W; v++) top = fmaxf(top, most[wave / W * W + v]);
+    }
     finite = top <= 3.402823466e38f;
     int e = 0;
     if (finite && top > 0.f) {
@@ -175,9 +195,7 @@ __device__ void convert_row(const Weights &w, const Call &c, int r) {
     float sum = 0.f;
     const int64_t lo = (int64_t)c.rows * K;
     _Float16 *const out = c.xa + (int64_t)r * K;
-    for (int i = t; i < K / 8; i += kPlanThreads) {
-        float v[8];
-        load(i, v);
+    auto convert = [&](int i, const float (&v)[8]) __attribute__((always_inline)) {
         h8 h, l;
 #pragma unroll
         for (int j = 0; j < 8; j++) {
@@ -189,28 +207,40 @@ __device__ void convert_row(const Weights &w, const Call &c, int r) {
         }
         *reinterpret_cast<h8 *>(out + 8 * i) = h;
         if (!c.half) *reinterpret_cast<h8 *>(out + lo + 8 * i) = l;
-    }
+    };
+    if (holds) {
 #pragma unroll
-    for (int o = 32; o > 0; o /= 2) sum += __shfl_xor(sum, o);
-    if ((t & 63) == 0) squares[t >> 6] = sum;
-    __syncthreads();
-    if (t) return;
-    sum = 0.f;
-    for (int v = 0; v < kPlanThreads / 64; v++) sum += squares[v];
+        for (int p = 0; p < 4; p++)
+            if (t + T * p < chunks) convert(t + T * p, held[p]);
+    } else {
+        for (int i = t; i < chunks; i += T) {
+            float v[8];
+            load(i, v);
+            convert(i, v);
+        }
+    }
+    sum = team_sum<64>(sum);
+    if (W > 1) {
+        if (lane == 0) squares[wave] = sum;
+        __syncthreads();
+        sum = 0.f;
+        for (int v = 0; v < W; v++) sum += squares[wave / W * W + v];
+    }
+    if (t || !chunks) return;
     int norm = kNothing;
     if (finite && sum > 0.f) {
         (void)frexpf(sum * 1.0001f, &norm);  // above what the sum was rounded by
         norm = ((norm + 1) >> 1) - e;
     }
-    c.x_pow[r] = e;
-    c.x_norm[r] = finite ? norm : 0;
+    c.x_pow[row] = e;
+    c.x_norm[row] = finite ? norm : 0;
 }
 
-// grid: experts workgroups, and one for each row.
+// grid: experts workgroups, and those of the rows.
 __global__ void __launch_bounds__(kPlanThreads)
 experts_plan(Weights w, Call c) {
     if ((int)blockIdx.x < w.experts) order_pairs(w, c, (int)blockIdx.x);
-    else convert_row(w, c, (int)blockIdx.x - w.experts);
+    else convert_rows(w, c, (int)blockIdx.x - w.experts);
 }
 
 // ---- the sums -------------------------------------------------------------------------------
@@ -576,7 +606,8 @@ int check_size(const char *op, int64_t rows, int32_t top, int type) {
 
 hipError_t launch(const Weights &w, const Call &c, hipEvent_t done, hipStream_t s) {
     if (c.one) return launch_one(w, c, done, s);
-    experts_plan<<<(unsigned)(w.experts + c.rows), kPlanThreads, 0, s>>>(w, c);
+    const int rows = 8 / row_waves(w.dim);
+    experts_plan<<<(unsigned)(w.experts + (c.rows + rows - 1) / rows), kPlanThreads, 0, s>>>(w, c);
     hipError_t e = hipGetLastError();
     const auto products = c.few ? launch_few : launch_many;
     if (e == hipSuccess) e = products(w, c, false, s);
