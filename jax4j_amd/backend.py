@@ -9,7 +9,8 @@ same argument meaning and error types. Every operation runs the engine's HIP ker
 
 Engine-local extensions (no SPI counterpart): batched ``quant_matvec`` over x [B, K],
 ``quant_matmul`` (prefill GEMM, Q8_0 / Q4_0 / Q4_K / Q6_K weights x bf16 activations), ``quantize_act``,
-``dequantize`` and ``export_quantized``.
+``dequantize`` and ``export_quantized``; ``rope_into``, ``norm_into`` and ``route_into`` on device addresses, beside the
+``KvCache`` and ``Experts`` of ``kv.py`` and ``experts.py``.
 """
 from __future__ import annotations
 
