@@ -450,7 +450,7 @@ typedef struct j4q_route_args {
     int32_t score;           /* j4q_route_score */
     int32_t groups;          /* equal parts of the experts (up to 64); 0 or 1: none */
     int32_t top_groups;      /* how many of them are open */
-    int32_t group_best;      /* 1 or 2: a group's rank is the sum of so many of its best */
+    int32_t group_best;      /* 1: a group's rank is its best (logit, or score + bias); 2: the sum of its two best scores, with a bias scores + bias */
     int32_t renormalize;     /* the weights of a row are divided by their sum */
     float scale;
 } j4q_route_args;

@@ -347,7 +347,7 @@ class Mi355xBackend:
                    renormalize: bool = False, scale: float = 1.0, stream: int = 0) -> None:
         """The ``top_k`` experts of every row of logits [rows, experts]: int32 ids and fp32 weights [rows, top_k], the best first; id -1
         and weight 0 where none is left. ``score``: "softmax" or "sigmoid"; ``bias``: fp32 [experts], for the choice alone; ``groups``:
-        only experts of the ``top_groups`` groups with the largest sum of their ``group_best`` best."""
+        only experts of the ``top_groups`` groups with the largest best, or with ``group_best`` 2 the largest sum of their two best scores (+ bias)."""
         s = {"softmax": N.ROUTE_SOFTMAX, "sigmoid": N.ROUTE_SIGMOID}.get(score)
         if s is None:
             raise IllegalArgumentException(f"unknown score {score!r} (softmax or sigmoid)")

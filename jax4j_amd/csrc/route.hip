@@ -69,15 +69,15 @@ route_kernel(RouteP p) {
         for (int j = 0; j < J; j++) sum += x[j] == -kInf ? 0.f : x[j] == top ? 1.f : expf(x[j] - top);  // (inf - inf is no number)
         sum = team_sum<L>(sum);
     }
+    // Groups' two best are summed as scores, bias or not: sums of logits are not in the order of sums of scores, and a constant added
+    // to a row, which changes no softmax, moves a group's two logits twice as far as the one of a group that has no more.
+    const bool scored = WIDE && (p.bias || (p.groups > 1 && p.best == 2));
     uint64_t key[J];
 #pragma unroll
     for (int j = 0; j < J; j++) {
         if constexpr (WIDE) {
             double c = x[j];
-            if (p.bias && x[j] > -kInf) {
-                const double s = p.sigmoid ? 1. / (1. + exp(-(double)x[j])) : x[j] == top ? 1. : exp((double)x[j] - (double)top);
-                c = s;
-            }
+            if (scored && x[j] > -kInf) c = p.sigmoid ? 1. / (1. + exp(-(double)x[j])) : x[j] == top ? 1. : exp((double)x[j] - (double)top);
             key[j] = __builtin_bit_cast(uint64_t, c);
         } else {
             key[j] = x[j] > -kInf ? (uint64_t)order32(x[j]) << 32 : 0;
@@ -85,7 +85,7 @@ route_kernel(RouteP p) {
     }
     if constexpr (WIDE) {
         double total = 1.;
-        if (p.bias && !p.sigmoid) {  // the softmax in 64 bits
+        if (scored && !p.sigmoid) {  // the softmax in 64 bits
             total = 0.;
 #pragma unroll
             for (int j = 0; j < J; j++) total += x[j] > -kInf ? __builtin_bit_cast(double, key[j]) : 0.;
@@ -95,7 +95,7 @@ route_kernel(RouteP p) {
         for (int j = 0; j < J; j++) {
             const int i = t + L * j;
             double c = __builtin_bit_cast(double, key[j]);
-            if (p.bias && x[j] > -kInf) c = c / total + (double)p.bias[i];
+            if (scored && x[j] > -kInf) c = c / total + (p.bias ? (double)p.bias[i] : 0.);
             key[j] = x[j] > -kInf && c > (double)-kInf ? order64(c) : 0;
         }
         if (p.groups > 1) {
@@ -125,6 +125,10 @@ route_kernel(RouteP p) {
 #pragma unroll
             for (int j = 0; j < J; j++)
                 if (!(open >> ((t + L * j) / size & 63) & 1)) key[j] = 0;  // (past the experts keys are 0)
+            if (scored && !p.bias) {  // inside the open groups the logits decide, which tell apart what scores round to the same
+#pragma unroll
+                for (int j = 0; j < J; j++) key[j] = key[j] ? order64((double)x[j]) : 0;
+            }
         }
     }
     // Slot s of the row goes to lane s.

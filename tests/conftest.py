@@ -26,3 +26,14 @@ def backend():
     info = be.device_info()
     assert info["arch"].startswith("gfx950"), info
     return be
+
+
+# Their reference ranks groups by sums of two logits. Those are not in the order of sums of scores, and change with a constant added to a
+# row, which no softmax does: {3, -inf | 2, 2} gives 3 < 4, the same less 20 gives -17 > -36. test_gpu_route_groups.py holds the sums of scores.
+SUMS_OF_LOGITS = [f"test_gpu_route.py::test_groups[False-{groups}]" for groups in ("4-2-2", "8-4-2", "16-3-2")]
+
+
+def pytest_collection_modifyitems(items):
+    for item in items:
+        if item.nodeid.endswith(tuple(SUMS_OF_LOGITS)):
+            item.add_marker(pytest.mark.xfail(reason="the reference ranks groups by sums of logits", strict=True))
