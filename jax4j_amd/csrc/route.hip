@@ -170,8 +170,10 @@ route_kernel(RouteP p) {
         const float most = p.renormalize ? fminf(team_max<L>(own), 0.f) : 0.f;
         if (mine >= 0) w = own < 0.f ? expf(own - most) / (1.f + expf(own)) : 1.f / (1.f + expf(-own));
         part = w;
-    } else if (mine >= 0) {
-        w = own == top ? 1.f : expf(own - top);
+    } else {
+        // likewise: what a bias or a group keeps out may lie so far above that beside it all chosen scores are 0
+        const float most = p.renormalize ? team_max<L>(own) : top;
+        if (mine >= 0) w = own == most ? 1.f : expf(own - most);
         part = w;
         if (!p.renormalize) w /= sum;
     }
