@@ -12,6 +12,11 @@
 // the largest norms of the expert's gate and up rows, so h' = h 2^(14 - ceil(log2 of that)) cannot overflow. Where the vectors are no
 // worse than random the bound is about `dim` times what is typical: 2^12 of fp16's 2^29 normal binades at dim 4096.
 //
+// bf16 results of many pairs: a pair's partial result is fp16 on its way to a row's sum (11 bits before a rounding to 8), 64 columns at a
+// power that takes the largest of them into [2^13, 2^14), known once they are computed, so that 11 bits reach down to 2^-28 of it whatever
+// the sizes of the weights' rows. (At a power from bounds, as h' has it, one row of gate, up and down 32 times the others left up
+// to 7 % of error in all other columns.) Half of fp32's bytes: 32744 pairs of dim 2048, 643 -> 574 us of the whole; the powers take 7 of them.
+//
 // Layout of x' and h' (block layout): of every 32 values, 16-byte chunk g = 0..3 holds elements 4 g + {0, 2, 1, 3} and then
 // 16 + 4 g + {0, 2, 1, 3}: what masking dword g of a block of codes yields, for every type alike, so that a lane of the matrix core reads
 // its 8 values with one load and codes are never reordered.
@@ -56,7 +61,6 @@ struct Weights {
     int up_type, down_type;
     int experts, dim, ffn, act;
     const int32_t *bound;                       // ceil(log2(G U)) of each expert
-    const int32_t *bound_down;                  // the exponent of the largest norm of its down rows, times the root of ffn
     const int32_t *gate_pow, *up_pow, *down_pow;  // of each row: max |w| 2^pow in [2^13, 2^14)
 };
 
@@ -78,16 +82,12 @@ struct Call {
     int32_t *order;
     _Float16 *xa, *ha;         // hi; lo behind all of hi
     int32_t *x_pow, *x_norm;   // of each row: e, and an exponent with |x| <= 2^it
-    float *part;               // [splits][pairs][dim], times the weights; `small`: fp16 [pairs][dim] at part_pow(), without them
+    float *part;               // [splits][pairs][dim], times the weights; `small`: fp16 [pairs][dim] at powers part_pow, without them
+    int32_t *part_pow;         // [pairs][dim / 64]: `small`: of each 64 columns of a pair
     bool small;
 };
 
 __device__ __forceinline__ int h_pow(const Weights &w, int expert, int x_norm) { return kBound - (2 * x_norm + w.bound[expert]); }
-
-// The power at which a pair's partial result is kept as fp16 on its way to a row's sum in bf16: |down h| <= |h| D <= sqrt(ffn) |x|^2 G U D,
-// D the largest norm of the expert's down rows, so it is 2^14 at most, and a rounding to 11 bits before one to 8. Typical values lie a
-// further root of ffn below h's, 2^6 at 4096. Half of fp32's bytes: 32744 pairs of dim 2048, 643 -> 574 us of the whole.
-__device__ __forceinline__ int part_pow(const Weights &w, int expert, int x_norm) { return h_pow(w, expert, x_norm) - w.bound_down[expert]; }
 
 // pair / top: the inverse is above by less than top / 2^32 of itself, and pair * top < 2^32.
 __device__ __forceinline__ int row_of(const Call &c, int pair) { return c.top == 1 ? pair : (int)__umulhi((uint32_t)pair, c.top_inverse); }

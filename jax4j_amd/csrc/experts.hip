@@ -258,7 +258,6 @@ experts_combine(Weights w, Call c) {
     float s[V] = {};
     const int64_t first = (int64_t)r * c.top;
     if constexpr (SMALL) {
-        const int norm = c.x_norm[r];
         for (int k0 = 0; k0 < c.top; k0 += 4) {
             h8 v[4];
             float weight[4];
@@ -269,9 +268,12 @@ experts_combine(Weights w, Call c) {
                 const int k = k0 + u < c.top ? k0 + u : k0, id = c.ids[first + k];
                 is[u] = k0 + u < c.top && id >= 0 && id < w.experts;
                 weight[u] = c.weights[first + k];
-                pow[u] = is[u] ? -part_pow(w, id, norm) : 0;
+                pow[u] = 0;
                 v[u] = h8{};
-                if (is[u]) v[u] = *reinterpret_cast<const h8 *>((const _Float16 *)c.part + (first + k) * w.dim + col);
+                if (is[u]) {
+                    pow[u] = c.part_pow[(first + k) * (w.dim / 64) + col / 64];
+                    v[u] = *reinterpret_cast<const h8 *>((const _Float16 *)c.part + (first + k) * w.dim + col);
+                }
             }
 #pragma unroll
             for (int u = 0; u < 4; u++)
@@ -367,8 +369,8 @@ __device__ __forceinline__ void chunk_stats(const Chunk<FMT> &c, int j, float &t
     }
 }
 
-// Of every row of a matrix of `experts` x rows: max |w| 2^pow in [2^13, 2^14) and the exponent of the norm. A wave per row, straight
-// from the codes: what it reads is what bounds it. grid: (rows / 4, experts).
+// Of every row of a matrix of `experts` x rows: max |w| 2^pow in [2^13, 2^14) and the exponent of the norm (NULL: not asked for). A wave per
+// row, straight from the codes: what it reads is what bounds it. grid: (rows / 4, experts).
 template <int FMT>
 __global__ void __launch_bounds__(256)
 row_stats(QMat all, int rows, int32_t *__restrict__ pow, int32_t *__restrict__ norm) {
@@ -407,19 +409,19 @@ row_stats(QMat all, int rows, int32_t *__restrict__ pow, int32_t *__restrict__ n
         }
     }
     pow[(int64_t)expert * rows + row] = p;
-    norm[(int64_t)expert * rows + row] = q;
+    if (norm) norm[(int64_t)expert * rows + row] = q;
 }
 
-// bound[e] = the largest of gate's exponents of expert e (of `rows` rows) + the largest of up's, or + add where there are none.
+// bound[e] = the largest of gate's exponents of expert e (of `rows` rows) + the largest of up's.
 __global__ void __launch_bounds__(256)
-expert_bound(const int32_t *__restrict__ gate, const int32_t *__restrict__ up, int add, int rows, int32_t *__restrict__ bound) {
+expert_bound(const int32_t *__restrict__ gate, const int32_t *__restrict__ up, int rows, int32_t *__restrict__ bound) {
     __shared__ int most[2][4];
     const int t = (int)threadIdx.x;
     const int64_t first = (int64_t)blockIdx.x * rows;
-    int a = 2 * kNothing, b = up ? 2 * kNothing : add;
+    int a = 2 * kNothing, b = 2 * kNothing;
     for (int i = t; i < rows; i += 256) {
         a = a > gate[first + i] ? a : gate[first + i];
-        if (up) b = b > up[first + i] ? b : up[first + i];
+        b = b > up[first + i] ? b : up[first + i];
     }
 #pragma unroll
     for (int o = 32; o > 0; o /= 2) {
@@ -474,7 +476,7 @@ bool type_ok(int type, int64_t cols) {
     }
 }
 
-// The powers of a matrix's rows and the exponents of their norms, `rows` of each expert.
+// The powers of a matrix's rows and, but for NULL, the exponents of their norms, `rows` of each expert.
 hipError_t stats(int type, const QMat &m, int experts, int rows, int32_t *pow, int32_t *norm, hipStream_t s) {
     const dim3 grid((unsigned)((rows + 3) / 4), (unsigned)experts);
     switch (type) {
@@ -509,7 +511,7 @@ int create(const j4q_experts_config &c, j4q_experts *out) {
     while (slot < g_experts.size() && g_experts[slot]->live) slot++;
     if (slot == g_experts.size()) g_experts.emplace_back(new Experts);
     Experts &k = *g_experts[slot];
-    const uint64_t words = (uint64_t)(4 * E * ffn + 2 * E * dim + 2 * E);  // bounds; powers and norms of gate, up, down
+    const uint64_t words = (uint64_t)(4 * E * ffn + 2 * E * dim + 2 * E);  // bounds; powers and norms of gate and up; powers of down (E dim and E words are to spare)
     void *dev = nullptr;
     hipError_t e = abi::malloc_locked(&dev, words * 4);
     if (e != hipSuccess) return report_hip("experts", e);
@@ -526,20 +528,16 @@ int create(const j4q_experts_config &c, j4q_experts *out) {
     k.w.ffn = (int)ffn;
     k.w.act = c.activation;
     int32_t *const gate_pow = at + 2 * E, *const up_pow = gate_pow + E * ffn, *const gate_norm = up_pow + E * ffn, *const up_norm = gate_norm + E * ffn,
-                  *const down_pow = up_norm + E * ffn, *const down_norm = down_pow + E * dim;
-    int root = 0;  // 4^root >= ffn
-    while (1ll << (2 * root) < ffn) root++;
+                  *const down_pow = up_norm + E * ffn;
     k.w.bound = at;
-    k.w.bound_down = at + E;
     k.w.gate_pow = gate_pow;
     k.w.up_pow = up_pow;
     k.w.down_pow = down_pow;
     e = stats(gate.qtype, gate.m, (int)E, (int)ffn, gate_pow, gate_norm, s);
     if (e == hipSuccess) e = stats(up.qtype, up.m, (int)E, (int)ffn, up_pow, up_norm, s);
-    if (e == hipSuccess) e = stats(down.qtype, down.m, (int)E, (int)dim, down_pow, down_norm, s);
+    if (e == hipSuccess) e = stats(down.qtype, down.m, (int)E, (int)dim, down_pow, nullptr, s);
     if (e == hipSuccess) {
-        expert_bound<<<(unsigned)E, 256, 0, s>>>(gate_norm, up_norm, 0, (int)ffn, at);
-        expert_bound<<<(unsigned)E, 256, 0, s>>>(down_norm, nullptr, root, (int)dim, at + E);
+        expert_bound<<<(unsigned)E, 256, 0, s>>>(gate_norm, up_norm, (int)ffn, at);
         e = hipGetLastError();
     }
     if (e == hipSuccess) e = hipStreamSynchronize(s);
@@ -582,6 +580,7 @@ uint64_t lay_out(const Weights &w, Call *c, uint8_t *base) {
     c->xa = (_Float16 *)take(2 * planes * T * (uint64_t)w.dim);
     c->ha = (_Float16 *)take(2 * planes * P * (uint64_t)w.ffn);
     c->part = (float *)take((c->small ? 2 : 4 * (uint64_t)c->splits) * P * (uint64_t)w.dim);
+    c->part_pow = (int32_t *)take(c->small ? 4 * P * (uint64_t)(w.dim / 64) : 0);
     return at;
 }
 

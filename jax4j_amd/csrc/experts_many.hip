@@ -153,6 +153,26 @@ struct Lds {
     static constexpr int kPlane = 32 * TM * 128, kX = (HL ? 2 : 1) * kPlane;
 };
 
+// e with |v| < 2^e for the 64 values of a pair, acc at its rows' powers, whose halves lanes r and r + 32 have; values that are not finite
+// do not count.
+__device__ __forceinline__ int top_exponent(const f32x16 &a, const f32x16 &b, const i32x4 (&pa)[4], const i32x4 (&pb)[4]) {
+    auto most = [&](bool finite) __attribute__((always_inline)) -> float {
+        float top = 0.f;
+#pragma unroll
+        for (int v = 0; v < 16; v++) {
+            const float x = fabsf(__builtin_ldexpf(a[v], -pa[v >> 2][v & 3])), y = fabsf(__builtin_ldexpf(b[v], -pb[v >> 2][v & 3]));
+            top = fmaxf(top, finite && !(x < __builtin_inff()) ? 0.f : x);
+            top = fmaxf(top, finite && !(y < __builtin_inff()) ? 0.f : y);
+        }
+        const uint32_t u = __builtin_bit_cast(uint32_t, top);
+        const auto two = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+        return fmaxf(__builtin_bit_cast(float, (uint32_t)two[0]), __builtin_bit_cast(float, (uint32_t)two[1]));
+    };
+    float top = most(false);
+    if (__builtin_amdgcn_ballot_w64(!(top < __builtin_inff()))) top = most(true);  // the wave as one
+    return __builtin_amdgcn_frexp_expf(top);  // 0 of 0
+}
+
 // The products of one team of 4 waves; first and count: its pairs of the tile.
 template <int FMT, bool HL, int TM, bool DOWN, int TEAMS>
 __device__ __forceinline__ void run(const Weights &w, const Call &c, int expert, int first, int count, int chunk, int team, uint8_t *xs0, uint8_t *xs1, uint8_t *ws0,
@@ -432,9 +452,14 @@ __device__ __forceinline__ void run(const Weights &w, const Call &c, int expert,
 #pragma unroll
         for (int t = 0; t < TM; t++) {
             const int m = 32 * t + r32;
-            const int pair = c.order[first + (m < count ? m : 0)], token = row_of(c, pair), norm = c.x_norm[token];
+            const int pair = c.order[first + (m < count ? m : 0)], token = row_of(c, pair), hp = h_pow(w, expert, c.x_norm[token]);
             const float weight = HL ? c.weights[pair] : 1.f;
-            const int up = HL ? -h_pow(w, expert, norm) : part_pow(w, expert, norm) - h_pow(w, expert, norm);
+            int up = -hp;
+            if constexpr (!HL) {
+                const int e = 14 - top_exponent(acc[0][t], acc[1][t], p0, p1);
+                if (h == 0 && m < count && n0 < N) c.part_pow[(int64_t)pair * (N / 64) + n0 / 64] = -hp - e;
+                up = e;
+            }
 #pragma unroll
             for (int g = 0; g < 2; g++)
 #pragma unroll
