@@ -7,10 +7,12 @@
 //  3. down of every tile, a weighted partial result for each pair.   4. experts_combine: the sums of a row's pairs, slot by slot.
 //
 // Activations enter the matrix cores as fp16: x' = x 2^e, e a power for each row that brings its largest magnitude into
-// [2^14, 2^15), as one value (bf16 x: exact down to 2^-28 of the largest) or as hi + lo (fp32 x: 22 bits down to 2^-18). The inner
-// activations are stored the same way, at a power that is known before they are: |g u| <= |x|^2 G U, with G and U
-// the largest norms of the expert's gate and up rows, so h' = h 2^(14 - ceil(log2 of that)) cannot overflow. Where the vectors are no
-// worse than random the bound is about `dim` times what is typical: 2^12 of fp16's 2^29 normal binades at dim 4096.
+// [2^14, 2^15), as one value (bf16 x: exact down to 2^-28 of the largest) or as hi + lo 2^-11 (fp32 x: 22 bits down to 2^-28; lo lies
+// beside hi in size, and so in fp16's range where hi does). The inner activations are stored the same way, at a power that is known before
+// they are: |g u| <= |x|^2 max(G U), with G and U the norms of a gate row and of the same up row, so h' = h 2^(14 - ceil(log2 of that))
+// cannot overflow. Where the vectors are no worse than random the bound is about `dim` times what is typical: 2^12 of fp16's 2^29
+// normal binades at dim 4096, which leaves 2^16 for rows larger than the others: 256 times in gate and up at once. (With lo at hi's
+// own power, 22 bits ended 2^5 below what is typical: with such rows 32 times the others fp32 lost 5 bits, 256 times 11.)
 //
 // bf16 results of many pairs: a pair's partial result is fp16 on its way to a row's sum (11 bits before a rounding to 8), 64 columns at a
 // power that takes the largest of them into [2^13, 2^14), known once they are computed, so that 11 bits reach down to 2^-28 of it whatever
@@ -42,6 +44,7 @@ using gemv::u32x4;
 
 constexpr int kBound = 14;       // |h'| <= 2^kBound
 constexpr int kNothing = -4096;  // exponent of a norm of 0
+constexpr float kLow = 2048.f;   // lo times this is stored
 
 // A tile: pairs [first, first + count) of the order, all of one expert.
 struct Tile {
@@ -60,7 +63,7 @@ struct Weights {
     QMat gate, up, down;
     int up_type, down_type;
     int experts, dim, ffn, act;
-    const int32_t *bound;                       // ceil(log2(G U)) of each expert
+    const int32_t *bound;                       // ceil(log2(max(G U))) of each expert
     const int32_t *gate_pow, *up_pow, *down_pow;  // of each row: max |w| 2^pow in [2^13, 2^14)
 };
 
@@ -80,7 +83,7 @@ struct Call {
     Tiles up, down;
     // workspace
     int32_t *order;
-    _Float16 *xa, *ha;         // hi; lo behind all of hi
+    _Float16 *xa, *ha;         // hi; lo 2^11 behind all of hi
     int32_t *x_pow, *x_norm;   // of each row: e, and an exponent with |x| <= 2^it
     float *part;               // [splits][pairs][dim], times the weights; `small`: fp16 [pairs][dim] at powers part_pow, without them
     int32_t *part_pow;         // [pairs][dim / 64]: `small`: of each 64 columns of a pair
@@ -100,8 +103,8 @@ __device__ __forceinline__ int slot_of(int c) {
 
 // e^x, within 3 steps: v_exp_f32 of the product with log2 e, and what the product's rounding left.
 __device__ __forceinline__ float exp_of(float x) {
-    constexpr float kLog2e = 1.44269504f, kLow = 1.92596303e-8f, kLn2 = 0.693147181f;
-    const float t = x * kLog2e, e = __builtin_amdgcn_exp2f(t), rest = __builtin_fmaf(x, kLow, __builtin_fmaf(x, kLog2e, -t));
+    constexpr float kLog2e = 1.44269504f, kRest = 1.92596303e-8f, kLn2 = 0.693147181f;
+    const float t = x * kLog2e, e = __builtin_amdgcn_exp2f(t), rest = __builtin_fmaf(x, kRest, __builtin_fmaf(x, kLog2e, -t));
     return fabsf(t) < 128.f ? __builtin_fmaf(e, rest * kLn2, e) : e;
 }
 

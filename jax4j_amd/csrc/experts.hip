@@ -204,7 +204,7 @@ __device__ void convert_rows(const Weights &w, const Call &c, int block) {
             const float s = finite ? __builtin_ldexpf(v[from], e) : __builtin_nanf("");
             sum = __builtin_fmaf(s, s, sum);
             h[j] = (_Float16)s;
-            l[j] = (_Float16)(s - (float)h[j]);
+            l[j] = (_Float16)((s - (float)h[j]) * kLow);
         }
         *reinterpret_cast<h8 *>(out + 8 * i) = h;
         if (!c.half) *reinterpret_cast<h8 *>(out + lo + 8 * i) = l;
@@ -412,31 +412,27 @@ row_stats(QMat all, int rows, int32_t *__restrict__ pow, int32_t *__restrict__ n
     if (norm) norm[(int64_t)expert * rows + row] = q;
 }
 
-// bound[e] = the largest of gate's exponents of expert e (of `rows` rows) + the largest of up's.
+// bound[e] = the largest sum of the exponents of a gate row of expert e (of `rows`) and of the same up row.
 __global__ void __launch_bounds__(256)
 expert_bound(const int32_t *__restrict__ gate, const int32_t *__restrict__ up, int rows, int32_t *__restrict__ bound) {
-    __shared__ int most[2][4];
+    __shared__ int most[4];
     const int t = (int)threadIdx.x;
     const int64_t first = (int64_t)blockIdx.x * rows;
-    int a = 2 * kNothing, b = 2 * kNothing;
+    int a = 2 * kNothing;
     for (int i = t; i < rows; i += 256) {
-        a = a > gate[first + i] ? a : gate[first + i];
-        b = b > up[first + i] ? b : up[first + i];
+        const int v = gate[first + i] + up[first + i];
+        a = a > v ? a : v;
     }
 #pragma unroll
     for (int o = 32; o > 0; o /= 2) {
-        const int x = __shfl_xor(a, o), y = __shfl_xor(b, o);
-        a = a > x ? a : x;
-        b = b > y ? b : y;
+        const int v = __shfl_xor(a, o);
+        a = a > v ? a : v;
     }
-    if ((t & 63) == 0) most[0][t >> 6] = a, most[1][t >> 6] = b;
+    if ((t & 63) == 0) most[t >> 6] = a;
     __syncthreads();
     if (t) return;
-    for (int v = 1; v < 4; v++) {
-        a = a > most[0][v] ? a : most[0][v];
-        b = b > most[1][v] ? b : most[1][v];
-    }
-    bound[blockIdx.x] = a + b;
+    for (int v = 1; v < 4; v++) a = a > most[v] ? a : most[v];
+    bound[blockIdx.x] = a;
 }
 
 // ---- handles --------------------------------------------------------------------------------

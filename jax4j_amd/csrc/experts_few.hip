@@ -196,7 +196,7 @@ experts_few(Weights w, Call c) {
     __syncthreads();
     auto value = [&](int tile16, int o) __attribute__((always_inline)) -> float {
         const float *const v = red + tile16 * 256 + o;
-        return HL ? v[0] + v[128] : v[0];
+        return HL ? __builtin_fmaf(v[128], 1.f / kLow, v[0]) : v[0];
     };
     constexpr int kOut = HL ? 128 : 256, COLS = DOWN ? kWaves : kWaves / 2;
     for (int o = (int)threadIdx.x; o < COLS * kOut; o += kWaves * 64) {
@@ -211,7 +211,7 @@ experts_few(Weights w, Call c) {
             const _Float16 hi = (_Float16)h;
             _Float16 *const out = c.ha + (int64_t)(first + q) * w.ffn + slot_of(col);
             *out = hi;
-            if constexpr (HL) out[(int64_t)c.pairs * w.ffn] = (_Float16)(h - (float)hi);
+            if constexpr (HL) out[(int64_t)c.pairs * w.ffn] = (_Float16)((h - (float)hi) * kLow);
         }
     }
 }

@@ -88,7 +88,7 @@ def results(l, x, ids, kind):
 
 
 @pytest.mark.parametrize("up,down", [("Q8_0", "Q8_0"), ("Q4_0", "Q4_0"), ("Q4_K", "Q6_K"), ("Q6_K", "Q4_K")])
-@pytest.mark.parametrize("kind", ["bf16"])
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
 @pytest.mark.parametrize("inner,outer", [(1, 1), (32, 32), (256, 1), (256, 256)])
 def test_other_rows_keep_their_digits(layer, up, down, kind, inner, outer):
     l = layer(up, down, 2, 1024, 512, inner, outer)
