@@ -289,9 +289,16 @@ public final class Mi355xBackend implements ComputeBackend, QuantizedOps {
   /**
    * h = residual + scale * after(block), written to residualOut (the residual itself, or apart; 0: nowhere); out = before(h).
    * F32 [rows, dim], dense, but with outBf16 out; block 0: none; after and before may be null, out 0 where before is. Device addresses.
+   * A bf16 block (what {@link Mi355xExperts#applyBf16} writes) is the other method's, with blockBf16.
    */
   public void norm(long residual, long block, Mi355xExperts.Norm after, float scale, long residualOut, Mi355xExperts.Norm before, long out,
       boolean outBf16, long rows, int dim) {
+    norm(residual, block, false, after, scale, residualOut, before, out, outBf16, rows, dim);
+  }
+
+  /** The same; with blockBf16 the block is bf16, else F32. */
+  public void norm(long residual, long block, boolean blockBf16, Mi355xExperts.Norm after, float scale, long residualOut, Mi355xExperts.Norm before,
+      long out, boolean outBf16, long rows, int dim) {
     ensureInitialized();
     try (Arena a = Arena.ofConfined()) {
       MemorySegment s = a.allocate(136, 8);  // without a gate; strides 0: dense
@@ -302,7 +309,7 @@ public final class Mi355xBackend implements ComputeBackend, QuantizedOps {
       s.set(JAVA_LONG, 40, rows);
       s.set(JAVA_INT, 96, dim);
       s.set(JAVA_INT, 100, Mi355xNative.KIND_F32);
-      s.set(JAVA_INT, 104, Mi355xNative.KIND_F32);
+      s.set(JAVA_INT, 104, blockBf16 ? Mi355xNative.KIND_BF16 : Mi355xNative.KIND_F32);
       s.set(JAVA_INT, 108, Mi355xNative.KIND_F32);
       s.set(JAVA_INT, 112, outBf16 ? Mi355xNative.KIND_BF16 : Mi355xNative.KIND_F32);
       s.set(JAVA_FLOAT, 116, scale);

@@ -88,7 +88,10 @@ public final class Mi355xExperts implements AutoCloseable {
     apply(x, xStride, ids, weights, out, outStride, rows, topK, Mi355xNative.KIND_F32);
   }
 
-  /** The same with bf16 x and out, as prompts have them: a third of the matrix instructions. */
+  /**
+   * The same with bf16 x and out, as prompts have them: a third of the matrix instructions. The norm that adds its result takes it
+   * as a bf16 block ({@link Mi355xBackend#norm} with blockBf16).
+   */
   public void applyBf16(long x, long xStride, long ids, long weights, long out, long outStride, long rows, int topK) {
     apply(x, xStride, ids, weights, out, outStride, rows, topK, Mi355xNative.KIND_BF16);
   }
