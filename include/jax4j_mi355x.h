@@ -462,8 +462,9 @@ int j4q_route_into(const j4q_route_args *args, void *stream);
 
 /* The matrices of a layer of experts: gate and up [experts * ffn, dim] of one type, down [experts * dim, ffn], expert after expert, as
  * j4q_gguf_upload gives GGUF's three-dimensional tensors. Types Q8_0 (columns a multiple of 64), Q4_0 (of 128), Q4_K and Q6_K; at
- * most 65536 columns, and fewer than 2^31 values of an expert in a matrix. The handle keeps the buffers from being released, and holds
- * a power of two for each row and two bounds for each expert, which j4q_experts_create computes once. */
+ * most 65536 columns, and fewer than 2^31 values of an expert in a matrix; all experts of a matrix lie in one buffer, so within 2 GiB of
+ * codes, as j4q_upload_quantized takes it. The handle keeps the buffers from being released, and holds
+ * a power of two for each row and a bound for each expert, which j4q_experts_create computes once. */
 typedef uint64_t j4q_experts; /* 0 is never a valid handle */
 enum j4q_activation { J4Q_ACT_SILU = 0, J4Q_ACT_GELU = 1 /* the tanh form */, J4Q_ACT_RELU = 2 };
 typedef struct j4q_experts_config {
@@ -497,11 +498,13 @@ int j4q_experts_info(j4q_experts experts, j4q_experts_desc *out);
 /* out[r] = sum over the slots s of a row of weights[r][s] * down_e (act(gate_e x_r) * (up_e x_r)), e = ids[r][s]; a row without experts is
  * zeros, the same expert twice counts twice. fp32: as j4q_quant_matvec_into's batches, x and the inner activations in 22 bits, weights as
  * they are or in 22 bits, sums in 32 (up to three rows all in 32). bf16: the inner activations in 11 bits, and in a prompt the weights
- * and each expert's share of a result too. A row of x with a value that is not finite gives a row of NaN where it has an expert. Bit for
+ * and each expert's share of a result too. The inner activations have these bits down to 2^-28 of a bound on them, |x|^2 times the largest
+ * product of the norms of a gate row and of the same up row: at dim 4096 down to some 2^-16 of what is typical. A row of x with a value that is not finite gives a row of NaN where it has an expert. Bit for
  * bit the same on every call with the same arguments. The engine's workspace is as j4q_quant_matvec_into's: under stream capture two
  * memory nodes, which a caller's own workspace saves. */
 int j4q_experts_apply(j4q_experts experts, const j4q_experts_args *args, void *stream);
-/* Bytes of workspace that a call of so many rows takes. */
+/* Bytes of workspace that a call of so many rows takes. A call of fewer rows may take more (other kernels, other partial results): for
+ * calls of several sizes the largest of what each of them is said to take. */
 int j4q_experts_workspace(j4q_experts experts, int64_t rows, int32_t top_k, int type, uint64_t *bytes);
 
 /* ---- GGUF files (the step before uploadQuantized; engine-local) ---------------------- */

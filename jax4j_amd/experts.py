@@ -63,7 +63,7 @@ class Experts:
         return {"experts": d.config.experts, "dim": d.dim, "ffn": d.ffn, "weight_bytes": d.weight_bytes, "bytes": d.bytes}
 
     def workspace(self, rows: int, top_k: int, dtype: DType = DType.F32) -> int:
-        """Bytes of workspace that a call of so many rows takes."""
+        """Bytes of workspace that a call of so many rows takes; a call of fewer rows may take more, so ask for each size of call."""
         n = C.c_uint64()
         check(N.load().j4q_experts_workspace(self.handle, _int64(rows), _int32(top_k), _kind(dtype), C.byref(n)), "experts workspace")
         return n.value

@@ -141,3 +141,20 @@ def test_an_engine_stream_that_is_captured(shim):  # noqa: F811
         assert [l.split()[0] for l in lines] == ["launch"] * 4, lines
         fake.fake_capture(C.c_void_p(engine), 0)
     """)
+
+
+def test_a_workspace_is_of_a_call_s_own_rows(shim):  # noqa: F811
+    """Where calls go from few pairs an expert to many, shares take fewer bytes: a workspace for more rows may be short for fewer, which is refused."""
+    run(shim, MORE + """
+        e = Experts(be, *matrices(QuantType.Q4_K, QuantType.Q6_K, 64, 256, 256), experts=64)
+        sizes = {rows: e.workspace(rows, 8, B) for rows in (1, 2, 8, 100, 191, 192, 300)}
+        assert sizes[192] < sizes[191], sizes
+        x, ids, weights, out, space = (1 << 40 | i << 36 for i in range(5))
+        def call(rows, n):
+            return lambda: e.apply(x, ids, weights, out, rows, 8, B, workspace_ptr=space, workspace_bytes=n)
+        quiet([(call(191, sizes[192]), "workspace")])
+        for rows, n in sizes.items():
+            call(rows, n)()
+            call(rows, max(sizes.values()))()
+            quiet([(call(rows, n - 1), "workspace")])
+    """)
