@@ -131,13 +131,6 @@ template <>
 struct Operand<false> {
     h8 hi;
 };
-// Of W; HL: hi over kLow too, which x's lo is multiplied by: four packed products for 8 weights, 11 bits down to 2^-16 of the row's largest.
-template <bool HL>
-struct Weight : Operand<HL> {
-    h8 over;
-};
-template <>
-struct Weight<false> : Operand<false> {};
 
 // One block of a row of W as it lies in LDS; scales s and offsets o of its elements 0..15 and 16..31.
 template <int FMT>
@@ -301,7 +294,7 @@ __device__ __forceinline__ void run(const Weights &w, const Call &c, int expert,
     float minus = -1.f;
     asm("" : "+v"(minus));
     // Operand p of a block.
-    auto operand = [&](const Block<FMT> &b, const Scale &c, int p, Weight<HL> &out) __attribute__((always_inline)) {
+    auto operand = [&](const Block<FMT> &b, const Scale &c, int p, Operand<HL> &out) __attribute__((always_inline)) {
         uint32_t part[4];
         if constexpr (FMT == Q8_0) {
             const uint32_t u = b.q[0][p] ^ 0x80808080u, v = b.q[1][p] ^ 0x80808080u;
@@ -332,10 +325,7 @@ __device__ __forceinline__ void run(const Weights &w, const Call &c, int expert,
             lo[k] = y;
         }
         out.hi = __builtin_bit_cast(h8, hi);
-        if constexpr (HL) {
-            out.lo = __builtin_bit_cast(h8, lo);
-            out.over = out.hi * (_Float16)(1.f / kLow);
-        }
+        if constexpr (HL) out.lo = __builtin_bit_cast(h8, lo);
     };
 
     f32x16 acc[2][TM];
@@ -350,10 +340,11 @@ __device__ __forceinline__ void run(const Weights &w, const Call &c, int expert,
             if constexpr (HL) a[t].lo = *reinterpret_cast<const h8 *>(at + L::kPlane);
         }
     };
-    constexpr int kShadow = HL ? 7 : TM >= 4 ? 5 : TM == 3 ? 7 : TM == 2 ? 9 : 18;
+    // vector instructions behind an MFMA; two teams' down spills with 8 (8192 pairs of Q6_K gate and up, fp32: 866 us with 7, 843 with 8)
+    constexpr int kShadow = HL ? (TEAMS == 2 && !DOWN ? 8 : 7) : TM >= 4 ? 5 : TM == 3 ? 7 : TM == 2 ? 9 : 18;
     Block<FMT> blk[2][2];  // [stage parity][group]
     Scale sc[2][2];
-    Weight<HL> b[2][2];    // of MFMA p and p + 1
+    Operand<HL> b[2][2];   // of MFMA p and p + 1
     auto stage = [&](auto S_, int i) __attribute__((always_inline)) {
         constexpr int S = decltype(S_)::value, cur = S & 1;
         uint8_t *const xb = cur ? xs1 : xs0, *const xn = cur ? xs0 : xs1;
@@ -386,11 +377,13 @@ __device__ __forceinline__ void run(const Weights &w, const Call &c, int expert,
             }
 #pragma unroll
             for (int g = 0; g < 2; g++) {
+                h8 over;  // x's lo is stored kLow larger: 11 bits of W down to 2^-16 of the row's largest
+                if constexpr (HL) over = b[p & 1][g].hi * (_Float16)(1.f / kLow);
 #pragma unroll
                 for (int t = 0; t < TM; t++) {
                     if constexpr (HL) {
                         acc[g][t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(b[p & 1][g].lo, a[p & 1][t].hi, acc[g][t], 0, 0, 0);
-                        acc[g][t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(b[p & 1][g].over, a[p & 1][t].lo, acc[g][t], 0, 0, 0);
+                        acc[g][t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(over, a[p & 1][t].lo, acc[g][t], 0, 0, 0);
                     }
                     acc[g][t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(b[p & 1][g].hi, a[p & 1][t].hi, acc[g][t], 0, 0, 0);
                 }
