@@ -2,9 +2,9 @@
 //   h = residual + scale gate after(block),  out = before(h),
 // each norm x / sqrt(mean(x^2) + eps) w + b, or of x - mean(x). Engine-local; the reference has no norms on this path.
 //
-// Bound by memory: a row is read once, kept in registers from the first sum to the last product, and written once. A team of 64,
-// 256 or 1024 threads has a row, 8 values a thread and pass: 16 bytes of bf16, or twice 16 of fp32, where addresses and strides
-// allow, else value after value across the team. Sums of values and squares are in 64 bits: they neither overflow nor lose
+// Bound by memory: a row is read once, kept in registers (beyond 16384 values in LDS) from the first sum to the last product, and written
+// once. A team of 64, 256 or 1024 threads has a row, 8 values a thread and pass: 16 bytes of bf16, or twice 16 of fp32, where addresses and
+// strides allow, else value after value across the team. Sums of values and squares are in 64 bits: they neither overflow nor lose
 // what a mean far from 0 hides, and cost nothing beside the memory. 16381 rows of 4096, a norm on either side of the residual and a gate:
 // 162 us, 5.0 TB/s. Few rows wait for their sums, so these take no LDS within a wave and no division (1021 rows of 1152, two norms with
 // means: 8.8 us with them, 7.6 without; all loads of a row ahead of its first sum: no faster).
@@ -140,6 +140,12 @@ __device__ __forceinline__ double row_sum(double v, double *slot, int t) {
     return v;
 }
 
+// The quotient itself where it is exact: rows of equal values have no rest.
+__device__ __forceinline__ double mean_of(double sum, int dim, double inv_dim) {
+    const double near = sum * inv_dim;
+    return fma(fma(-near, (double)dim, sum), inv_dim, near);
+}
+
 template <int T, int C, bool VEC>
 __device__ __forceinline__ void apply(const NormK &k, f32x8 (&x)[C], Raw (&w)[C], Raw (&b)[C], double *slot, int t, int dim, double inv_dim) {
     double mean = 0;
@@ -149,9 +155,7 @@ __device__ __forceinline__ void apply(const NormK &k, f32x8 (&x)[C], Raw (&w)[C]
 #pragma unroll
             for (int j = 0; j < 8; j++)
                 if (At<T, VEC>::of(t, c, j) < dim) mean += (double)x[c][j];
-        mean = row_sum<T>(mean, slot, t);
-        const double near = mean * inv_dim;
-        mean = fma(fma(-near, (double)dim, mean), inv_dim, near);  // the quotient itself where it is exact: rows of equal values have no rest
+        mean = mean_of(row_sum<T>(mean, slot, t), dim, inv_dim);
     }
     double sum = 0;
 #pragma unroll
@@ -232,18 +236,103 @@ norm_kernel(NormP p) {
     for (int c = 0; c < C; c++) store<T, VEC>(x[c], p.out + row * p.out_stride, p.out16, t, c, p.dim);
 }
 
+// Rows beyond 16384, 32 values of 1024 threads: they lie in LDS, of which each thread has its own, and go through registers 8 at a time. (In
+// registers, 128 a thread, they spilled 142 of them: 2000 rows of 20000, two norms and the residual, 470 us; here 115, 2.8 TB/s, and of
+// 20001, value by value, 203.) The sums' order is that of norm_kernel.
+template <bool VEC>
+__global__ void __launch_bounds__(1024)
+norm_long_kernel(NormP p) {
+    constexpr int T = 1024, C = 4;
+    __shared__ float held[C * 8 * T];
+    __shared__ double slots[T / 64];
+    const int t = (int)threadIdx.x, dim = p.dim, passes = (dim + 8 * T - 1) / (8 * T);
+    const int64_t row = (int64_t)blockIdx.y * gridDim.x + blockIdx.x;
+    if (row >= p.rows) return;
+    const uint8_t *const g = p.gate + (p.gate_every ? (uint32_t)row / p.gate_every : 0) * p.gate_stride;
+    auto put = [&](int c, const f32x8 &x) __attribute__((always_inline)) {
+#pragma unroll
+        for (int j = 0; j < 8; j++) held[(8 * c + j) * T + t] = x[j];
+    };
+    auto get = [&](int c) __attribute__((always_inline)) {
+        f32x8 x;
+#pragma unroll
+        for (int j = 0; j < 8; j++) x[j] = held[(8 * c + j) * T + t];
+        return x;
+    };
+    auto read = [&](const uint8_t *at, bool half, int c) __attribute__((always_inline)) {
+        Raw r;
+        load<T, VEC>(r, at, half, t, c, dim);
+        return values<VEC>(r, half);
+    };
+    auto apply = [&](const NormK &k) __attribute__((always_inline)) {
+        double mean = 0;
+        if (k.kind == J4Q_NORM_LAYER) {
+#pragma unroll 1
+            for (int c = 0; c < passes; c++) {
+                const f32x8 x = get(c);
+#pragma unroll
+                for (int j = 0; j < 8; j++)
+                    if (At<T, VEC>::of(t, c, j) < dim) mean += (double)x[j];
+            }
+            mean = mean_of(row_sum<T>(mean, slots, t), dim, p.inv_dim);
+        }
+        double sum = 0;
+#pragma unroll 1
+        for (int c = 0; c < passes; c++) {
+            f32x8 x = get(c);
+#pragma unroll
+            for (int j = 0; j < 8; j++)
+                if (At<T, VEC>::of(t, c, j) < dim) {
+                    const double d = (double)x[j] - mean;
+                    sum = fma(d, d, sum);
+                    x[j] = (float)d;
+                }
+            if (k.kind == J4Q_NORM_LAYER) put(c, x);
+        }
+        const float inv = inverse_root(fma(row_sum<T>(sum, slots, t), p.inv_dim, (double)k.eps));
+#pragma unroll 1
+        for (int c = 0; c < passes; c++) {
+            f32x8 x = get(c);
+            x *= inv;
+            if (k.weight) x *= read((const uint8_t *)k.weight, false, c) + k.add;
+            if (k.bias) x += read((const uint8_t *)k.bias, false, c);
+            put(c, x);
+        }
+    };
+    if (p.block) {
+#pragma unroll 1
+        for (int c = 0; c < passes; c++) put(c, read(p.block + row * p.block_stride, p.block16, c));
+        if (p.after.kind) apply(p.after);
+    }
+#pragma unroll 1
+    for (int c = 0; c < passes; c++) {
+        f32x8 x = {};
+        if (p.block) {
+            x = get(c);
+            if (p.gate) x *= read(g, p.gate16, c);
+            x *= p.scale;
+        }
+        if (p.residual) x += read(p.residual + row * p.residual_stride, p.residual16, c);
+        if (p.residual_out) store<T, VEC>(x, p.residual_out + row * p.residual_out_stride, p.residual16, t, c, dim);
+        put(c, x);
+    }
+    if (!p.before.kind) return;
+    apply(p.before);
+#pragma unroll 1
+    for (int c = 0; c < passes; c++) store<T, VEC>(get(c), p.out + row * p.out_stride, p.out16, t, c, dim);
+}
+
+template <int G>
+dim3 grid_of(const NormP &p) {
+    const int64_t groups = (p.rows + G - 1) / G, x = groups < 1 << 20 ? groups : 1 << 20;  // a grid's threads are counted in 32 bits
+    return dim3((unsigned)x, (unsigned)((groups + x - 1) / x));
+}
+
 template <int T, int C>
 hipError_t launch(const NormP &p, bool vec, hipStream_t s) {
     constexpr int G = T < 256 ? 256 / T : 1;
-    const int64_t groups = (p.rows + G - 1) / G, x = groups < 1 << 20 ? groups : 1 << 20;  // a grid's threads are counted in 32 bits
-    const dim3 grid((unsigned)x, (unsigned)((groups + x - 1) / x));
-    if constexpr (T * C < 4096) {
-        if (vec) {
-            norm_kernel<T, C, true><<<grid, T * G, 0, s>>>(p);
-            return hipGetLastError();
-        }
-    }
-    norm_kernel<T, C, false><<<grid, T * G, 0, s>>>(p);
+    if (vec) norm_kernel<T, C, true><<<grid_of<G>(p), T * G, 0, s>>>(p);
+    else norm_kernel<T, C, false><<<grid_of<G>(p), T * G, 0, s>>>(p);
     return hipGetLastError();
 }
 
@@ -254,7 +343,9 @@ hipError_t launch_norm(const NormP &p, bool vec, hipStream_t s) {
     if (p.dim <= 4096) return launch<256, 2>(p, vec, s);
     if (p.dim <= 8192) return launch<256, 4>(p, vec, s);
     if (p.dim <= 16384) return launch<1024, 2>(p, vec, s);
-    return launch<1024, 4>(p, false, s);  // 128 registers a thread: the wide loads would not fit them
+    if (vec) norm_long_kernel<true><<<grid_of<1>(p), 1024, 0, s>>>(p);
+    else norm_long_kernel<false><<<grid_of<1>(p), 1024, 0, s>>>(p);
+    return hipGetLastError();
 }
 
 int check_norm(const char *which, const j4q_norm *n, NormK *out) {
