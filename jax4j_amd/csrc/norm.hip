@@ -120,10 +120,14 @@ __device__ __forceinline__ void store(const f32x8 &x, uint8_t *row, bool half, i
 }
 
 // 1 / sqrt(v): v_rsq_f64, good to some 24 bits, and a step of Newton's.
-__device__ __forceinline__ float inverse_root(double v) {
+__device__ __forceinline__ double inverse_root(double v) {
     const double y = __builtin_amdgcn_rsq(v), e = fma(-v * y, y, 1.0);
-    return (float)(e == e ? fma(0.5 * y, e, y) : y);  // not of 0 or infinity
+    return e == e ? fma(0.5 * y, e, y) : y;  // not of 0 or infinity
 }
+
+// A root's inverse y beyond 32 bits, or with fewer of them, and the power of two that the values take of it first. The same in a whole team.
+__device__ __forceinline__ bool far(double y) { return y > 0x1p126 || y < 0x1p-126; }
+__device__ __forceinline__ int far_power(double y) { return y > 1. ? 100 : -64; }
 
 // Sum over the team's T threads, in the same order whichever row of the workgroup the team has. `slot`: T / 64 doubles of the team.
 template <int T>
@@ -167,7 +171,14 @@ __device__ __forceinline__ void apply(const NormK &k, f32x8 (&x)[C], Raw (&w)[C]
                 sum = fma(d, d, sum);
                 x[c][j] = (float)d;
             }
-    const float inv = inverse_root(fma(row_sum<T>(sum, slot, t), inv_dim, (double)k.eps));
+    double root = inverse_root(fma(row_sum<T>(sum, slot, t), inv_dim, (double)k.eps));
+    if (far(root)) {
+        const int power = far_power(root);
+        root = ldexp(root, -power);
+#pragma unroll
+        for (int c = 0; c < C; c++) x[c] *= ldexpf(1.f, power);
+    }
+    const float inv = (float)root;
 #pragma unroll
     for (int c = 0; c < C; c++) {
         if (k.weight) load<T, VEC>(w[c], (const uint8_t *)k.weight, false, t, c, dim);
@@ -289,10 +300,13 @@ norm_long_kernel(NormP p) {
                 }
             if (k.kind == J4Q_NORM_LAYER) put(c, x);
         }
-        const float inv = inverse_root(fma(row_sum<T>(sum, slots, t), p.inv_dim, (double)k.eps));
+        const double root = inverse_root(fma(row_sum<T>(sum, slots, t), p.inv_dim, (double)k.eps));
+        const int power = far(root) ? far_power(root) : 0;
+        const float first = ldexpf(1.f, power), inv = (float)ldexp(root, -power);
 #pragma unroll 1
         for (int c = 0; c < passes; c++) {
             f32x8 x = get(c);
+            x *= first;
             x *= inv;
             if (k.weight) x *= read((const uint8_t *)k.weight, false, c) + k.add;
             if (k.bias) x += read((const uint8_t *)k.bias, false, c);
