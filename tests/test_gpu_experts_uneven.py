@@ -106,3 +106,24 @@ def test_other_rows_keep_their_digits(layer, up, down, kind, inner, outer):
             assert error <= bound or not some.any(), (rows, error, bound)
             own = np.abs(got - want)[some][:, COLUMN]
             assert np.linalg.norm(own) <= 4 * np.linalg.norm(off[some][:, COLUMN]), rows  # few values: four times the root mean square
+
+
+@pytest.mark.parametrize("up,down", [("Q8_0", "Q8_0"), ("Q4_0", "Q4_0"), ("Q4_K", "Q6_K"), ("Q6_K", "Q4_K")])
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+@pytest.mark.parametrize("value", [np.inf, np.nan])
+def test_a_row_of_down_that_is_not_finite_stays_alone(backend, up, down, kind, value):
+    with np.errstate(invalid="ignore"):  # inf times 0
+        l = Uneven(backend, up, down, 2, 256, 512, 1, value)
+    try:
+        others = np.arange(l.dim) != COLUMN
+        l.plain[2] = tuple(np.where(others[None, :, None], v, 0.0) for v in l.plain[2])
+        for rows in (1, 20, 120):
+            rng = np.random.default_rng(rows)
+            x = torch.from_numpy(rng.standard_normal((rows, l.dim)).astype(np.float32)).to(TYPES[kind][1])
+            ids = (np.arange(rows, dtype=np.int32) % 2)[:, None]
+            got = apply(l, x, ids, np.ones((rows, 1), np.float32), kind)
+            assert not np.isfinite(got[:, COLUMN]).any()
+            want, off, _ = results(l, x.float().numpy(), ids, kind)
+            assert np.linalg.norm((got - want)[:, others]) <= np.linalg.norm(off[:, others]), rows
+    finally:
+        l.close()
