@@ -154,23 +154,26 @@ struct Lds {
     static constexpr int kPlane = 32 * TM * 128, kX = (HL ? 2 : 1) * kPlane;
 };
 
-// e with |v| < 2^e for the 64 values of a pair, acc at its rows' powers, whose halves lanes r and r + 32 have; values that are not finite
-// do not count.
-__device__ __forceinline__ int top_exponent(const f32x16 &a, const f32x16 &b, const i32x4 (&pa)[4], const i32x4 (&pb)[4]) {
-    auto most = [&](bool finite) __attribute__((always_inline)) -> float {
-        float top = 0.f;
-#pragma unroll
-        for (int v = 0; v < 16; v++) {
-            const float x = fabsf(__builtin_ldexpf(a[v], -pa[v >> 2][v & 3])), y = fabsf(__builtin_ldexpf(b[v], -pb[v >> 2][v & 3]));
-            top = fmaxf(top, finite && !(x < __builtin_inff()) ? 0.f : x);
-            top = fmaxf(top, finite && !(y < __builtin_inff()) ? 0.f : y);
-        }
-        const uint32_t u = __builtin_bit_cast(uint32_t, top);
+// e with |v| < 2^e for the 64 values of a pair, whose halves lanes r and r + 32 have; values that are not finite do not count.
+__device__ __forceinline__ int top_exponent(const f32x16 &a, const f32x16 &b) {
+    auto both = [](float v) __attribute__((always_inline)) -> float {
+        const uint32_t u = __builtin_bit_cast(uint32_t, v);
         const auto two = __builtin_amdgcn_permlane32_swap(u, u, false, false);
         return fmaxf(__builtin_bit_cast(float, (uint32_t)two[0]), __builtin_bit_cast(float, (uint32_t)two[1]));
     };
-    float top = most(false);
-    if (__builtin_amdgcn_ballot_w64(!(top < __builtin_inff()))) top = most(true);  // the wave as one
+    float top = 0.f;
+#pragma unroll
+    for (int v = 0; v < 16; v++) top = fmaxf(fmaxf(top, fabsf(a[v])), fabsf(b[v]));
+    top = both(top);
+    if (__builtin_amdgcn_ballot_w64(!(top < __builtin_inff()))) {  // the wave as one
+        top = 0.f;
+#pragma unroll
+        for (int v = 0; v < 16; v++) {
+            top = fabsf(a[v]) < __builtin_inff() ? fmaxf(top, fabsf(a[v])) : top;
+            top = fabsf(b[v]) < __builtin_inff() ? fmaxf(top, fabsf(b[v])) : top;
+        }
+        top = both(top);
+    }
     return __builtin_amdgcn_frexp_expf(top);  // 0 of 0
 }
 
@@ -460,9 +463,13 @@ __device__ __forceinline__ void run(const Weights &w, const Call &c, int expert,
             const float weight = HL ? c.weights[pair] : 1.f;
             int up = -hp;
             if constexpr (!HL) {
-                const int e = 14 - top_exponent(acc[0][t], acc[1][t], p0, p1);
-                if (h == 0 && m < count && n0 < N) c.part_pow[(int64_t)pair * (N / 64) + n0 / 64] = -hp - e;
-                up = e;
+#pragma unroll
+                for (int v = 0; v < 16; v++) {
+                    acc[0][t][v] = __builtin_ldexpf(acc[0][t][v], -p0[v >> 2][v & 3]);
+                    acc[1][t][v] = __builtin_ldexpf(acc[1][t][v], -p1[v >> 2][v & 3]);
+                }
+                up = 14 - top_exponent(acc[0][t], acc[1][t]);
+                if (h == 0 && m < count && n0 < N) c.part_pow[(int64_t)pair * (N / 64) + n0 / 64] = -hp - up;
             }
 #pragma unroll
             for (int g = 0; g < 2; g++)
@@ -470,7 +477,7 @@ __device__ __forceinline__ void run(const Weights &w, const Call &c, int expert,
                 for (int q = 0; q < 4; q++) {
                     f32x4 v;
 #pragma unroll
-                    for (int j = 0; j < 4; j++) v[j] = __builtin_ldexpf(HL ? acc[g][t][4 * q + j] * weight : acc[g][t][4 * q + j], up - (g ? p1[q][j] : p0[q][j]));
+                    for (int j = 0; j < 4; j++) v[j] = HL ? __builtin_ldexpf(acc[g][t][4 * q + j] * weight, up - (g ? p1[q][j] : p0[q][j])) : __builtin_ldexpf(acc[g][t][4 * q + j], up);
                     if constexpr (HL) *reinterpret_cast<f32x4 *>(place + r32 * 256 + (((8 * g + 2 * q + h) ^ (r32 & 7)) << 4)) = v;
                     else *reinterpret_cast<h4 *>(place + r32 * 128 + (((4 * g + q) ^ (r32 & 7)) << 4) + 8 * h) = __builtin_convertvector(v, h4);
                 }
