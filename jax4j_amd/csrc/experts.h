@@ -17,7 +17,7 @@
 // bf16 results of many pairs: a pair's partial result is fp16 on its way to a row's sum (11 bits before a rounding to 8), 64 columns at a
 // power that takes the largest of them into [2^13, 2^14), known once they are computed, so that 11 bits reach down to 2^-28 of it whatever
 // the sizes of the weights' rows. (At a power from bounds, as h' has it, one row of gate, up and down 32 times the others left up
-// to 7 % of error in all other columns.) Half of fp32's bytes: 32744 pairs of dim 2048, 643 -> 574 us of the whole; the powers take 7 of them.
+// to 7 % of error in all other columns.) Half of fp32's bytes: 32744 pairs of dim 2048, 643 -> 574 us of the whole; the powers take 5 of them.
 //
 // Layout of x' and h' (block layout): of every 32 values, 16-byte chunk g = 0..3 holds elements 4 g + {0, 2, 1, 3} and then
 // 16 + 4 g + {0, 2, 1, 3}: what masking dword g of a block of codes yields, for every type alike, so that a lane of the matrix core reads

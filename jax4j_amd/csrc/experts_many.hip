@@ -18,8 +18,8 @@
 // x's lo is stored 2^11 larger and meets W's hi 2^11 smaller (169 -> 174 us, 509 tokens of 32 Q4_0 experts).
 //
 // What bounds it are the matrix cores and the vector instructions that unpack W, whose times add, and the lines of W. 32744 pairs of 64
-// experts 2048 x 1024, bf16: gate|up (Q4_K, tiles of 128) 288 us, 955 TFLOP/s, down (Q6_K, tiles of 96) 203 us, 676; 4086 pairs of 8 experts
-// 4096 x 14336: 945 us, 1015 TFLOP/s, and 654 us, 734.
+// experts 2048 x 1024, bf16: gate|up (Q4_K, tiles of 128) 287 us, 960 TFLOP/s, down (Q6_K, tiles of 96) 215 us, 640; 4086 pairs of 8 experts
+// 4096 x 14336: 929 us, 1033 TFLOP/s, and 666 us, 721.
 #include <type_traits>
 
 #include "experts.h"

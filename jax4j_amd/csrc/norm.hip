@@ -7,7 +7,7 @@
 // strides allow, else value after value across the team. Sums of values and squares are in 64 bits: they neither overflow nor lose
 // what a mean far from 0 hides, and cost nothing beside the memory. 16381 rows of 4096, a norm on either side of the residual and a gate:
 // 162 us, 5.0 TB/s. Few rows wait for their sums, so these take no LDS within a wave and no division (1021 rows of 1152, two norms with
-// means: 8.8 us with them, 7.6 without; all loads of a row ahead of its first sum: no faster).
+// means: 8.8 us with them, 7.7 without; all loads of a row ahead of its first sum: no faster).
 #include "arguments.h"
 #include "engine.h"
 #include "teams.h"

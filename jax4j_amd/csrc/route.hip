@@ -8,7 +8,7 @@
 // 32 bits (of 64: of the upper ones, then of the lower ones where the upper are that) and the lowest index that has it, each over the
 // lane's own and then over the team. Instructions bound it, and
 // where rows are few the chain of maxima: 8 of 128 experts, 16381 rows 7.8 us (9.8 with keys of 64 bits and exchanges through LDS), 8 of 256 in groups, 61
-// rows 9.3 (12.7).
+// rows 9.5 (12.7).
 // Lane s of the team then has slot s, reads that expert's logit once more and computes its weight.
 #include "arguments.h"
 #include "engine.h"
